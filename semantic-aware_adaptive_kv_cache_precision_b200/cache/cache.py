@@ -10,6 +10,8 @@ a cache) are sorted into groups by what they need:
   blocks back as soon as every position in them has fallen out of the window.
 * every entry with a `StateNeed` has a tensor [slots, *shape]: state of fixed
   size per sequence, zeroed when a slot is taken.
+* a sequence that is forked (`SequenceCache.fork`) shares its full blocks with the new ones: a
+  block goes back to its pool when the last sequence that lists it lets go of it.
 * an entry with a `MultiNeed` holds one of the above for each of its parts (an attention
   layer that also keeps a little running state beside its keys and values).
 
@@ -27,6 +29,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
+from .. import ops
 from ..errors import allocate
 from .allocator import CacheFull, Pool
 from .needs import KVNeed, MultiNeed, StateNeed
@@ -53,23 +56,32 @@ class KVGroup:
                  max_slots: int, dtype: torch.dtype, device):
         self.need, self.entries = need, entries
         self.pool = Pool(blocks, "cache block")
+        self.holders = np.zeros(blocks, dtype=np.int32)     # sequences that list each block
         if need.dtype is not None:
             if need.dtype not in _DTYPES:
                 raise TypeError(f"{need!r}: dtype must be one of {sorted(_DTYPES)} or None")
             dtype = _DTYPES[need.dtype]
-        lead = (len(entries), max(blocks, 1), need.kv_heads, BLOCK)
-        def zeros(width):
-            shape = lead + (width,)
-            count = int(np.prod(shape))
-            return allocate(lambda: torch.zeros(shape, dtype=dtype, device=device),
-                            f"a cache of {blocks} blocks of {BLOCK} positions for "
-                            f"{len(entries)} layer(s)", count * dtype.itemsize)
-
-        self.keys = zeros(need.head_dim)
-        self.values = None if need.value_width == 0 else zeros(need.value_width)
+        self.dtype, self.device = dtype, device
+        self.keys, self.values = self.storage(blocks)
         self.max_blocks_per_seq = max_blocks_per_seq
         # host copy of every slot's block list; -1 = no block
         self.tables = np.full((max_slots, max_blocks_per_seq), -1, dtype=np.int32)
+
+    def storage(self, blocks: int):
+        """Zeroed (keys, values) of `blocks` blocks; values None where the need has none."""
+        def zeros(width):
+            shape = (len(self.entries), max(blocks, 1), self.need.kv_heads, BLOCK, width)
+            count = int(np.prod(shape))
+            return allocate(lambda: torch.zeros(shape, dtype=self.dtype, device=self.device),
+                            f"a cache of {blocks} blocks of {BLOCK} positions for "
+                            f"{len(self.entries)} layer(s)", count * self.dtype.itemsize)
+
+        return zeros(self.need.head_dim), (None if self.need.value_width == 0
+                                           else zeros(self.need.value_width))
+
+    @property
+    def tensors(self) -> list:
+        return [t for t in (self.keys, self.values) if t is not None]
 
 
 class SequenceCache:
@@ -82,6 +94,7 @@ class SequenceCache:
         self.dtype, self.device = dtype, torch.device(device)
         self.blocks = -(-max_tokens // BLOCK)
         self.max_tokens = self.blocks * BLOCK
+        self.max_positions = max_positions
         self.max_seq_len = min(max_positions, self.max_tokens)
         self.max_blocks_per_seq = -(-self.max_seq_len // BLOCK)
         self.max_slots = max_slots if max_slots is not None else min(self.blocks, 1024)
@@ -118,6 +131,10 @@ class SequenceCache:
                                        self.max_slots, dtype, device))
             for i, entry in enumerate(entries):
                 self.entry_group[entry] = (g, i)
+        # holders beyond the first, over all blocks (0: no block is listed twice), and a number that
+        # moves whenever the sequences that share blocks may have changed
+        self._shared = 0
+        self.sharing = 0
         # first position whose block a window group still holds, per (group, slot)
         self._front = [np.zeros(self.max_slots, dtype=np.int64) for _ in self.groups]
 
@@ -160,14 +177,121 @@ class SequenceCache:
         self.slots.give_back(slots)
 
     def _release(self, group: KVGroup, blocks: list[int]) -> None:
+        """A sequence lets go of `blocks`; those that no other sequence lists go back to the pool."""
         if not blocks:
             return
+        group.holders[blocks] -= 1
+        if self._shared:
+            self._shared -= sum(1 for b in blocks if group.holders[b] > 0)
+            self.sharing += 1
+            blocks = [b for b in blocks if group.holders[b] == 0]
+            if not blocks:
+                return
         if self.poison_freed and group.keys.is_floating_point():
             index = torch.as_tensor(blocks, dtype=torch.long, device=self.device)
             group.keys.index_fill_(1, index, float("nan"))
             if group.values is not None:
                 group.values.index_fill_(1, index, float("nan"))
         group.pool.give_back(blocks)
+
+    # -- forks ----------------------------------------------------------------
+
+    @property
+    def shares_blocks(self) -> bool:
+        """Whether some block is listed by more than one sequence."""
+        return self._shared > 0
+
+    def _copy(self, tensors, src, dst, **how) -> None:
+        if self.device.type == "cuda":
+            ops.copy_blocks(tensors, src, dst, **how)
+            return
+        # (a cache whose tensors lie on the host: the bookkeeping's tests)
+        into = how.get("into") or tensors
+        for t, u in zip(tensors, into):
+            if how.get("axis", 1) == 0:
+                u[dst] = t[src]
+            else:
+                u[:, dst, :, :how.get("rows") or BLOCK] = t[:, src, :, :how.get("rows") or BLOCK]
+
+    def fork(self, slot: int, count: int = 1) -> list[int]:
+        """`count` new sequences that begin with everything the sequence in `slot` has: its length, its
+        blocks and its state. Blocks whose 64 positions are all filled are shared (a sequence writes
+        behind its length only), the last, partly filled one and the state are copied. All or nothing: if
+        slots or blocks are lacking, nothing changes."""
+        if slot not in self.slots._held:
+            raise RuntimeError(f"slot {slot} is not held (closed, or never opened)")
+        if count < 0:
+            raise ValueError(f"cannot fork {count} sequences")
+        length = int(self.lengths[slot])
+        full, rows = divmod(length, BLOCK)
+        for group in self.groups:
+            if rows and group.pool.free < count:
+                raise CacheFull(f"{count} cache block(s) of {BLOCK} positions needed, {group.pool.free} of "
+                                f"{group.pool.size} free; nothing was taken")
+        new = self.slots.take(count)
+        if not count:
+            return new
+        for g, group in enumerate(self.groups):
+            row = group.tables[slot]
+            common = row[:full]
+            listed = common[common >= 0]
+            group.holders[listed] += count
+            self._shared += count * len(listed)
+            group.tables[new] = -1
+            group.tables[new, :full] = common
+            self._front[g][new] = self._front[g][slot]
+            if rows:
+                own = group.pool.take(count)
+                group.holders[own] = 1
+                group.tables[new, full] = own
+                self._copy(group.tensors, [int(row[full])] * count, own, rows=rows)
+        self.lengths[new] = length
+        self.sharing += 1
+        if self.states:
+            by_type = list(self.states.values())
+            self._copy(by_type, [slot] * count, new, axis=0)
+        return new
+
+    # -- another size ---------------------------------------------------------
+
+    def resize(self, max_tokens: int) -> None:
+        """Give every pool room for `max_tokens` positions (rounded up to blocks) while sequences live:
+        held blocks are moved into new storage, one behind the other in the order of their numbers, and the
+        old storage is given up. The number of slots stays. All or nothing: `CacheFull` where the held
+        blocks, or a sequence's length, do not fit; `OutOfDeviceMemory` where the device has no room for
+        old and new storage together."""
+        if max_tokens <= 0:
+            raise ValueError(f"max_tokens must be positive, got {max_tokens}")
+        blocks = -(-max_tokens // BLOCK)
+        longest = min(self.max_positions, blocks * BLOCK)
+        width = -(-longest // BLOCK)
+        for group in self.groups:
+            if group.pool.held > blocks:
+                raise CacheFull(f"{group.pool.held} cache blocks are held, {blocks} would not hold them; "
+                                "nothing was changed")
+        for s in self.slots._held:
+            if self.lengths[s] > longest or any((group.tables[s, width:] >= 0).any() for group in self.groups):
+                raise CacheFull(f"a sequence of {int(self.lengths[s])} positions does not fit a cache of "
+                                f"{longest} per sequence; nothing was changed")
+        storage = [group.storage(blocks) for group in self.groups]
+        for group, (keys, values) in zip(self.groups, storage):
+            held = sorted(group.pool._held)
+            self._copy(group.tensors, held, list(range(len(held))),
+                       into=[t for t in (keys, values) if t is not None])
+            place = np.full(group.pool.size + 1, -1, dtype=np.int32)       # (the last: -1 stays -1)
+            place[held] = np.arange(len(held), dtype=np.int32)
+            tables = np.full((self.max_slots, width), -1, dtype=np.int32)
+            kept = min(width, group.max_blocks_per_seq)
+            tables[:, :kept] = place[group.tables[:, :kept]]
+            holders = np.zeros(blocks, dtype=np.int32)
+            holders[:len(held)] = group.holders[held]
+            group.pool = Pool(blocks, "cache block")
+            group.pool.take(len(held))
+            group.keys, group.values = keys, values
+            group.tables, group.holders, group.max_blocks_per_seq = tables, holders, width
+        self.blocks, self.max_tokens = blocks, blocks * BLOCK
+        self.max_seq_len, self.max_blocks_per_seq = longest, width
+        self.sharing += 1
 
     # -- growth -------------------------------------------------------------
 
@@ -197,6 +321,7 @@ class SequenceCache:
             for s, missing in want:
                 for b, block in zip(missing, group.pool.take(len(missing))):
                     group.tables[s, b] = block
+                    group.holders[block] = 1
 
     def advance(self, slots, new_lengths) -> None:
         """Record the new lengths after a step; window groups give back the blocks
@@ -247,7 +372,16 @@ class SequenceCache:
         for group in self.groups:
             group.pool.check()
             listed = group.tables[group.tables >= 0].tolist()
-            if len(set(listed)) != len(listed):
+            counts = np.bincount(np.asarray(listed, dtype=np.int64), minlength=len(group.holders))
+            if (counts != group.holders).any():
+                raise RuntimeError("a cache block is listed for more or fewer places than it counts")
+            for s in range(self.max_slots):
+                row = group.tables[s][group.tables[s] >= 0]
+                if len(np.unique(row)) != len(row):
+                    raise RuntimeError("a cache block is listed for two places")
+            # (a block that sequences share holds the same positions of each)
+            if len(np.unique(np.argwhere(group.tables >= 0)[:, 1] * (len(group.holders) + 1)
+                             + group.tables[group.tables >= 0])) != len(set(listed)):
                 raise RuntimeError("a cache block is listed for two places")
             if set(listed) != group.pool._held:
                 raise RuntimeError("held blocks and listed blocks differ: "
@@ -255,3 +389,5 @@ class SequenceCache:
             for s in range(self.max_slots):
                 if s not in self.slots._held and (group.tables[s] >= 0).any():
                     raise RuntimeError(f"free slot {s} still lists blocks")
+        if self._shared != sum(int(np.maximum(g.holders - 1, 0).sum()) for g in self.groups):
+            raise RuntimeError("the count of shared blocks is wrong")

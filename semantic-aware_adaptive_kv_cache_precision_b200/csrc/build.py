@@ -61,6 +61,9 @@ LIBRARIES = {
     "recurrent_scan": "recurrent_scan.cu",
     "chunk_scan": "chunk_scan.cu",
     "gated_delta": "gated_delta.cu",
+    "copy_blocks": "copy_blocks.cu",
+    "attention_shared": "attention_shared.cu",
+    "logprobs": "logprobs.cu",
 }
 
 #: extra flags of single libraries (libraries that need the driver API, for instance)

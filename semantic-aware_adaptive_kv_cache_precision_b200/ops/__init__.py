@@ -20,10 +20,13 @@ from .recurrent import delta_rule, gated_delta
 from .scan import causal_conv, decay_attention, dual_scan, norm_gate, run_length, selective_scan, step_size
 from . import mixture
 from .mixture import latent_prepare, rotate_heads
+from .blocks import copy_blocks
 from .attention import (attention_decode, attention_prefill, attention_prefill_tc, decode_splits,
                         forget_descriptors,
                         fast_path_takes, kernel_errors, plan_token_blocks, plan_wide_tiles, tc_prefill_takes, upload_query_tiles,
                         upload_wide_plan)
+from .logprobs import token_logprobs
+from .shared import SharedPlan, plan_shared, shared_decode_attention
 
 __all__ = ["CACHE_BLOCK", "KernelError", "embed", "rms_norm", "rope_store", "attention_plain",
            "attention_decode", "attention_prefill", "attention_prefill_tc", "tc_prefill_takes", "plan_wide_tiles", "upload_wide_plan",
@@ -32,7 +35,9 @@ __all__ = ["CACHE_BLOCK", "KernelError", "embed", "rms_norm", "rope_store", "att
            "kernel_errors", "gated_silu", "gelu_tanh", "relu_squared", "dense_up", "embed_pairs", "gated_delta", "streams_step", "streams_spread", "token_shift",
            "delta_rule", "kv_store", "layer_norm", "cached_attention", "mixture", "latent_prepare",
            "rotate_heads", "distance_attention", "rms_update", "rms_join", "qk_prepare", "causal_conv",
-           "decay_attention", "dual_scan", "norm_gate", "run_length", "selective_scan", "step_size", "gated_up", "gemm_tc", "add_into", "scale_cap_", "linear", "per_head", "choose", "Deferred", "aside", "goes_aside"]
+           "decay_attention", "dual_scan", "norm_gate", "run_length", "selective_scan", "step_size", "gated_up", "gemm_tc", "add_into", "scale_cap_", "linear", "per_head", "choose", "Deferred", "aside", "goes_aside",
+           "copy_blocks", "SharedPlan", "plan_shared", "shared_decode_attention",
+           "token_logprobs"]
 
 
 def _check(cond: bool, message: str) -> None:

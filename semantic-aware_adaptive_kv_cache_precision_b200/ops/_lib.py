@@ -98,6 +98,11 @@ SIGNATURES = {
     "sakv_gemm_few": ("gemm_few", [P, L, P, I, I, I, I, I, I, P, I, P, L, L, F, F, F, P]),
     "sakv_gemm_wide": ("gemm_wide", [P, P, I, I, I, I, P, L, P]),
     "sakv_gemm_pair": ("gemm_pair", [P, P, I, I, I, I, P, L, I, F, F, F, P]),
+    "sakv_copy_blocks": ("copy_blocks", [P, I, P, I, P]),
+    "sakv_shared_attention": ("attention_shared", [P, P, P, L, P, P, I, P, I, I, I, I, P, P, P, I, I, I, I, I, F, P]),
+    "sakv_logprob_pieces": ("logprobs", [P, P, I, I, I, P, P, P, P, I, F, F, P]),
+    "sakv_logprob_fold": ("logprobs", [P, L, I, I, I, I, P, P, P, P, I, F, F, P]),
+    "sakv_logprob_join": ("logprobs", [P, P, P, P, P, I, I, I, P]),
     "sakv_lib_accumulate": ("gemm_lib", [P, L, P, P, L, I, I, I, P, L, P]),
 }
 
@@ -110,6 +115,12 @@ PLAIN_SIGNATURES = {
     "sakv_decode_attention_map": ("attention_decode", [P, P, L, I, I]),
     "sakv_decode_attention_error": ("attention_decode", [P]),
     "sakv_decode_attention_max_cluster": ("attention_decode", [I]),
+    "sakv_logprob_tile": ("logprobs", []),
+    "sakv_logprob_fold_columns": ("logprobs", []),
+    "sakv_logprob_resident": ("logprobs", []),
+    "sakv_logprob_map": ("logprobs", [P, P, L, L, L]),
+    "sakv_logprob_error": ("logprobs", [P]),
+    "sakv_shared_attention_error": ("attention_shared", [P]),
     "sakv_prefill_attention_error": ("attention_prefill", [P]),
     "sakv_prefill_attention_tc_error": ("attention_prefill_tc", [P]),
     "sakv_prefill_attention_tc_qmap": ("attention_prefill_tc", [P, P, L, L, L]),
@@ -188,6 +199,25 @@ def sm_count(device=None) -> int:
     if index not in _sm_counts:
         _sm_counts[index] = torch.cuda.get_device_properties(index).multi_processor_count
     return _sm_counts[index]
+
+
+class _Nothing:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(t: torch.Tensor):
+    """A context in which `t`'s device is the current one (nothing to do where it is already: asking
+    costs a microsecond less than switching)."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return _NOTHING
+    return torch.cuda.device(t.device)
 
 
 def require_cuda(*tensors) -> None:

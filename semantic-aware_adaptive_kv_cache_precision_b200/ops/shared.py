@@ -1,0 +1,209 @@
+"""Decode attention over blocks that several sequences list (`csrc/attention_shared.cu`), and the plan
+that says which. The plan is worked out on the host from the block lists, when sequences are forked or
+end, and serves every layer of every step until the next such change."""
+
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import CACHE_BLOCK, KernelError, call, on_device, ptr, require_cuda, sm_count
+from .attention import fast_path_takes, tensor_map
+
+UNIT_ROWS = 64            # most rows (sequences x query heads of one KV head) of a unit of work
+UNIT_WORDS = 8
+
+
+def common_runs(tables: np.ndarray, lengths: np.ndarray, reach: np.ndarray) -> list:
+    """The block lists cut into runs that one set of sequences lists: [(sequences, first column, end)],
+    each column of a sequence below its reach in exactly one. A column counts as shared where it is filled
+    (below `lengths`) and names the same block; what it is preceded by does not matter, a sum over
+    positions can be cut anywhere."""
+    count, width = tables.shape
+    full = lengths // CACHE_BLOCK
+    columns = -(-reach // CACHE_BLOCK)
+    runs = []
+    shared_to = np.zeros(count, dtype=np.int64)
+    if count > 1 and full.max(initial=0) > 0:
+        used = int(full.max())
+        # (numbers below every block's for columns that are not filled: each its own)
+        ids = tables[:, :used].astype(np.int64)
+        filled = np.arange(used)[None, :] < full[:, None]
+        ids[~filled] = -1 - np.broadcast_to(np.arange(count)[:, None], ids.shape)[~filled]
+        order = np.argsort(ids, axis=0, kind="stable")
+        ranked = np.take_along_axis(ids, order, axis=0)
+        begins = np.ones_like(ranked, dtype=bool)
+        begins[1:] = ranked[1:] != ranked[:-1]
+        # the first sequence of each group of equal numbers, given to all of the group
+        at = np.maximum.accumulate(np.where(begins, np.arange(count)[:, None], 0), axis=0)
+        lead = np.empty_like(order)
+        np.put_along_axis(lead, order, np.take_along_axis(order, at, axis=0), axis=0)
+        alone = np.arange(count)[:, None] == lead
+        crowd = np.zeros_like(alone)                      # whether anyone else is in the sequence's group
+        np.logical_or.at(crowd, (lead, np.broadcast_to(np.arange(used), lead.shape)), ~alone)
+        crowd = np.take_along_axis(crowd, lead, axis=0)
+        changes = [0] + (1 + np.flatnonzero((lead[:, 1:] != lead[:, :-1]).any(axis=0))).tolist() + [used]
+        open_runs = {}
+        for c0, c1 in zip(changes, changes[1:]):
+            now = {}
+            together = np.flatnonzero(crowd[:, c0])
+            for first in np.unique(lead[together, c0]):
+                members = tuple(together[lead[together, c0] == first].tolist())
+                now[members] = open_runs.pop(members, c0)
+            for members, begin in open_runs.items():
+                runs.append((members, begin, c0))
+            open_runs = now
+        for members, begin in open_runs.items():
+            runs.append((members, begin, used))
+    # what is left of each sequence: its columns outside the runs it belongs to
+    own = [[] for _ in range(count)]
+    for members, c0, c1 in runs:
+        for b in members:
+            own[b].append((c0, c1))
+    for b in range(count):
+        at = 0
+        for c0, c1 in sorted(own[b]) + [(int(columns[b]), int(columns[b]))]:
+            if c0 > at:
+                runs.append(((b,), at, c0))
+            at = max(at, c1)
+    return runs
+
+
+def choose_piece(runs: list, group: int, kv_heads: int, slots: int) -> int:
+    """Into pieces of how many blocks the runs are cut: the fewest with which the units of work do not
+    outnumber `slots`, the thread blocks that run at one time."""
+    per = max(1, UNIT_ROWS // group)
+    sizes = np.array([c1 - c0 for _, c0, c1 in runs], dtype=np.int64)
+    tiles = np.array([-(-len(m) // per) for m, _, _ in runs], dtype=np.int64) * kv_heads
+    longest = int(sizes.max(initial=1))
+    piece = max(1, int((sizes * tiles).sum()) // max(1, slots))
+    while piece < longest and int((-(-sizes // piece) * tiles).sum()) > slots:
+        piece += max(1, piece // 16)
+    return min(piece, longest)
+
+
+class SharedPlan:
+    """Which pieces of the block lists are read for which sequences: int32 words on the device, and their
+    layout. Right for every step until `lengths` pass `reach` or the sharing changes."""
+
+    __slots__ = ("words", "sequences", "heads", "kv_heads", "units", "unit_at", "unit_capacity", "member_at",
+                 "first_at", "partials", "reach", "width", "saved")
+
+    def on(self, words: torch.Tensor) -> "SharedPlan":
+        """The same plan with its words at `words` (int32, on the device)."""
+        other = SharedPlan()
+        for name in SharedPlan.__slots__:
+            setattr(other, name, getattr(self, name))
+        other.words = words
+        return other
+
+
+def _round_up(n: int, to: int) -> int:
+    return -(-n // to) * to
+
+
+def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reach=None,
+                slots: int | None = None, roomy: bool = False) -> SharedPlan:
+    """The plan of `shared_decode_attention` for sequences whose block lists are `tables` (host integers
+    [B, width], -1 for none) and which hold `lengths` positions (`reach`: how far they may grow before the
+    plan is made again; default: as they are). `device` None leaves the words on the host (`words`: a
+    numpy array); `roomy` rounds the layout's sizes up, so that plans of like shape have the same."""
+    tables = np.asarray(tables)
+    lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    reach = lengths if reach is None else np.asarray(reach, dtype=np.int64).reshape(-1)
+    if tables.ndim != 2 or tables.shape[0] != len(lengths) or len(reach) != len(lengths):
+        raise KernelError(f"plan_shared: block lists {tables.shape} for {len(lengths)} lengths, {len(reach)} reaches")
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or heads // kv_heads > UNIT_ROWS:
+        raise KernelError(f"plan_shared: {heads} heads over {kv_heads} (at most {UNIT_ROWS} a KV head)")
+    count, width = tables.shape
+    if count and (lengths.min() < 0 or (reach < lengths).any() or reach.max() > width * CACHE_BLOCK):
+        raise KernelError(f"plan_shared: lengths and reaches must lie in [0, {width * CACHE_BLOCK}], reach >= length")
+    listed = np.arange(width)[None, :] < -(-lengths // CACHE_BLOCK)[:, None]
+    if (tables[listed] < 0).any():
+        raise KernelError("plan_shared: a sequence has positions without a block")
+    group = heads // kv_heads
+    runs = common_runs(tables, lengths, reach)
+    piece = choose_piece(runs, group, kv_heads, slots or 2 * sm_count(device)) if runs else 1
+    per = max(1, UNIT_ROWS // group)
+    pieces = []                                            # (members, first column, columns)
+    for members, c0, c1 in runs:
+        n = -(-(c1 - c0) // piece)
+        for i in range(n):                                 # (even pieces)
+            a, z = c0 + (c1 - c0) * i // n, c0 + (c1 - c0) * (i + 1) // n
+            pieces.append((members, a, z - a))
+    # a sequence's partials in the order of its positions
+    pieces.sort(key=lambda p: p[1])
+    counts = np.zeros(count, dtype=np.int64)
+    place = []
+    for members, _, _ in pieces:
+        place.append([int(counts[b]) for b in members])
+        counts[list(members)] += 1
+    first = np.concatenate([[0], np.cumsum(counts)])
+    units, pairs = [], []
+    for (members, c0, n), where in zip(pieces, place):
+        for i in range(0, len(members), per):
+            some = members[i:i + per]
+            units.append((some[0], c0, n, len(pairs), len(some), 0, 0, 0))
+            pairs += [(b, int(first[b]) + w) for b, w in zip(some, where[i:i + per])]
+    units.sort(key=lambda u: -u[2] * (1 + u[4] * group // 16))        # the heaviest start first
+    plan = SharedPlan()
+    plan.sequences, plan.heads, plan.kv_heads, plan.width = count, heads, kv_heads, width
+    plan.units, plan.reach = len(units), reach
+    plan.unit_capacity = _round_up(len(units), 64) if roomy else len(units)
+    members_room = _round_up(len(pairs), 256) if roomy else len(pairs)
+    plan.partials = members_room                           # (a member is a partial)
+    plan.unit_at = 8
+    plan.member_at = plan.unit_at + UNIT_WORDS * plan.unit_capacity
+    plan.first_at = plan.member_at + 2 * members_room
+    plan.saved = int(sum((len(m) - 1) * (c1 - c0) for m, c0, c1 in runs))
+    words = np.zeros(_round_up(plan.first_at + count + 1, 4), dtype=np.int32)
+    words[0], words[1] = len(units), count
+    if units:
+        words[8:8 + UNIT_WORDS * len(units)] = np.asarray(units, dtype=np.int32).reshape(-1)
+        words[plan.member_at:plan.member_at + 2 * len(pairs)] = np.asarray(pairs, dtype=np.int32).reshape(-1)
+    words[plan.first_at:plan.first_at + count + 1] = first
+    plan.words = words if device is None else torch.from_numpy(words).to(device)
+    return plan
+
+
+def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            seq_lens: torch.Tensor, block_table: torch.Tensor, plan: SharedPlan, heads: int,
+                            kv_heads: int, head_dim: int, scale: float) -> torch.Tensor:
+    """One query token per sequence over its cached keys and values, like `attention_decode` (bfloat16,
+    head sizes 64 and 128, no window; `qkv`'s rows begin with the rotated queries, the newest key and value
+    are in the cache), reading a block that `plan` found in several sequences' lists once for all of them.
+    `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros."""
+    if not fast_path_takes(qkv.dtype, heads, kv_heads, head_dim):
+        raise KernelError("shared_decode_attention: sizes not taken; use the plain kernel")
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < heads * head_dim or qkv.stride(0) % 2 \
+            or qkv.data_ptr() % 4:
+        raise KernelError("shared_decode_attention: qkv must be [B, >= heads * head_dim], rows contiguous")
+    for cache in (k_cache, v_cache):
+        if cache.dim() != 4 or tuple(cache.shape[1:]) != (kv_heads, CACHE_BLOCK, head_dim) \
+                or cache.shape != k_cache.shape:
+            raise KernelError(f"shared_decode_attention: cache entries must be [blocks, {kv_heads}, {CACHE_BLOCK}, "
+                              f"{head_dim}]")
+    sequences = qkv.shape[0]
+    for t, shape in ((seq_lens, (sequences,)), (block_table, (sequences, plan.width))):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise KernelError(f"shared_decode_attention: lengths and block lists must be contiguous int32, {shape}")
+    if (plan.sequences, plan.heads, plan.kv_heads) != (sequences, heads, kv_heads):
+        raise KernelError(f"shared_decode_attention: the plan is for {plan.sequences} sequences, {plan.heads} heads "
+                          f"over {plan.kv_heads}")
+    require_cuda(qkv, k_cache, v_cache, seq_lens, block_table)
+    if any(t.device != qkv.device for t in (k_cache, v_cache, seq_lens, block_table, plan.words)):
+        raise KernelError("shared_decode_attention: tensors on different devices")
+    out = torch.empty((sequences, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
+    if sequences == 0:
+        return out
+    part = torch.empty(plan.partials * heads * (head_dim + 2), dtype=torch.float32, device=qkv.device)
+    with on_device(qkv):
+        call("sakv_shared_attention", tensor_map(k_cache), tensor_map(v_cache), ptr(qkv), qkv.stride(0),
+             ptr(seq_lens), ptr(block_table), block_table.shape[1], ptr(plan.words), plan.unit_at,
+             plan.unit_capacity, plan.member_at, plan.first_at, ptr(out), ptr(part),
+             part.data_ptr() + 4 * plan.partials * heads * head_dim, plan.partials, sequences, heads, kv_heads,
+             head_dim, float(scale))
+    if plan.unit_capacity:
+        _lib.launches += 1          # the call launched the join too
+    return out

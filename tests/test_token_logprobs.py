@@ -1,0 +1,154 @@
+"""Log-probabilities of given tokens without keeping the logits, against float64."""
+
+import math
+
+import pytest
+import torch
+
+from semantic_aware_adaptive_kv_cache_precision_b200 import ops
+from semantic_aware_adaptive_kv_cache_precision_b200.ops import KernelError, logprobs
+
+
+def test_refusals():
+    x, w, t = torch.zeros(3, 16), torch.zeros(50, 16), torch.zeros(3, dtype=torch.int32)
+    call = ops.token_logprobs
+    for args, how in (((x, w[:, :8], t), {}), ((x, w.to(torch.bfloat16), t), {}), ((x, w[::2], t), {}),
+                      ((x[:, ::2], w[:, :8].contiguous(), t), {}), ((x, w, t.long()), {}), ((x, w, t[:2]), {}),
+                      ((x, w, t, torch.zeros(49)), {}), ((x, w, t, torch.zeros(50).double()), {}),
+                      ((x, w[:0], t), {}), ((x[:, :0], w[:, :0], t), {}), ((x, w, t), {"softcap": -1.0}),
+                      ((x, w, t), {"softcap": math.inf}), ((x, w, t), {"softcap": math.nan}),
+                      ((x.double(), w.double(), t), {})):
+        with pytest.raises(KernelError):
+            call(*args, **how)
+    with pytest.raises(KernelError, match="CUDA device only"):
+        call(x, w, t)
+
+
+def reference(x, w, targets, bias, scale, softcap):
+    z = x.double() @ w.double().t()
+    size = x.double().abs() @ w.double().abs().t()          # of the products whose sum a logit is
+    if bias is not None:
+        z, size = z + bias.double(), size + bias.double().abs().nan_to_num(0, 0, 0)
+    z, size = z * scale, size * abs(scale)
+    if softcap:
+        z = softcap * torch.tanh(z / softcap)
+    lse = torch.logsumexp(z, 1)
+    picked = z.gather(1, targets.long().clamp(0, w.shape[0] - 1)[:, None])[:, 0]
+    # a logit is a sum of K products in fp32, every addition off by a step at most (2^-23 of what it adds up:
+    # the tensor cores cut off), then the cap's tanh by 2^-21 of the cap; lse moves by no more than the largest
+    # of them, and its own sum of V positive terms in runs of at most 512 by 512 2^-23, its logarithm by 2^-21
+    k = x.shape[1]
+    dz = ((k + 4) * 2.0 ** -23 * size).amax(1) + 2.0 ** -21 * softcap
+    return picked - lse, lse, 2 * dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (1 + lse.abs()) + 2.0 ** -22 * picked.abs()
+
+
+def check(rows, k, vocab, dtype, bias=None, scale=1.0, softcap=0.0, seed=0, x_pad=0, spread=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((rows, k + x_pad), generator=g, device="cuda").to(dtype)[:, :k]
+    w = (torch.randn((vocab, k), generator=g, device="cuda") * spread / math.sqrt(k)).to(dtype)
+    b = None if bias is None else torch.randn(vocab, generator=g, device="cuda").to(bias)
+    targets = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    targets[0], targets[-1] = vocab - 1, 0
+    got, lse = ops.token_logprobs(x, w, targets, b, scale=scale, softcap=softcap)
+    want, want_lse, bound = reference(x, w, targets, b, scale, softcap)
+    assert ((lse.double() - want_lse).abs() <= bound).all(), ((lse.double() - want_lse).abs() / bound).max()
+    assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() / bound).max()
+    return x, w, targets, got, lse
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows, k, vocab", [(1, 8, 1), (1, 64, 255), (5, 96, 256), (31, 72, 257), (127, 128, 1000),
+                                            (129, 192, 4095), (256, 64, 4097), (257, 200, 8193), (600, 256, 70001)])
+def test_against_float64(dtype, rows, k, vocab):
+    check(rows, k, vocab, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale, softcap", [(1.0, 0.0), (0.25, 0.0), (1.0, 5.0), (-0.5, 30.0)])
+def test_bias_scale_and_cap(dtype, bias, scale, softcap):
+    check(70, 104, 1333, dtype, bias, scale, softcap)
+    check(3, 104, 1333, dtype, bias, scale, softcap, spread=40.0)
+
+
+@pytest.mark.gpu
+def test_operands_that_the_copies_do_not_take():
+    check(20, 37, 500, torch.bfloat16)                     # rows of the head at odd addresses
+    check(20, 37, 500, torch.float32)
+    check(33, 64, 500, torch.bfloat16, x_pad=3)            # rows of x likewise
+    check(33, 64, 500, torch.bfloat16, x_pad=24)           # rows a multiple of 16 bytes apart
+    check(40, 64, 500, torch.float32, x_pad=3)
+
+
+@pytest.mark.gpu
+def test_pieces_of_rows_where_logits_lie_in_memory(monkeypatch):
+    x, w, targets, got, lse = check(50, 48, 9000, torch.float32, seed=5)
+    monkeypatch.setattr(logprobs, "PIECE_ELEMENTS", 17 * 4096)
+    again, lse2 = ops.token_logprobs(x, w, targets)
+    assert torch.equal(got, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_targets_that_ask_for_nothing_and_masked_tokens(dtype):
+    rows, k, vocab = 9, 64, 700
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((rows, k), generator=g, device="cuda").to(dtype)
+    w = torch.randn((vocab, k), generator=g, device="cuda").mul_(0.3).to(dtype)
+    bias = torch.zeros(vocab, device="cuda")
+    bias[300:] = -math.inf                                   # whole pieces of the vocabulary
+    bias[::2] = -math.inf
+    targets = torch.tensor([1, 299, 3, 2, 500, -1, -2 ** 31, vocab, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    got, lse = ops.token_logprobs(x, w, targets, bias)
+    want, want_lse, bound = reference(x, w, targets, bias, 1.0, 0.0)
+    assert ((lse.double() - want_lse).abs() <= bound).all()
+    assert ((got.double() - want)[:3].abs() <= bound[:3]).all()
+    assert (got[3:5] == -math.inf).all() and (got[5:7] == 0).all() and got[7:].isnan().all()
+    lowest = torch.finfo(torch.float32).min                  # a mask of the type's lowest value does the same
+    same, lse2 = ops.token_logprobs(x, w, targets, bias.clamp(min=lowest))
+    assert torch.equal(lse, lse2) and torch.equal(got[:3], same[:3]) and (same[3:5] < -1e38).all()
+    bias[:] = -math.inf
+    got, lse = ops.token_logprobs(x, w, targets, bias)
+    assert (lse == -math.inf).all() and got[:5].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_rows_that_are_not_finite_stay_their_own(dtype, softcap):
+    x = torch.randn(40, 64, device="cuda").to(dtype)
+    w = torch.randn(900, 64, device="cuda").mul_(0.3).to(dtype)
+    targets = torch.arange(40, dtype=torch.int32, device="cuda")
+    good, _ = ops.token_logprobs(x, w, targets, softcap=softcap)
+    x[7] = math.nan
+    got, lse = ops.token_logprobs(x, w, targets, softcap=softcap)
+    assert got[7].isnan() and lse[7].isnan()
+    rest = [i for i in range(40) if i != 7]
+    assert torch.equal(got[rest], good[rest])
+
+
+@pytest.mark.gpu
+def test_no_rows_rows_alone_streams_and_graphs():
+    x, w, targets, got, lse = check(300, 128, 3001, torch.bfloat16, seed=9)
+    none, none_lse = ops.token_logprobs(x[:0], w, targets[:0])
+    assert none.shape == none_lse.shape == (0,)
+    # a row's sums do not depend on the rows beside it
+    for i in (0, 130, 299):
+        alone, _ = ops.token_logprobs(x[i:i + 1], w, targets[i:i + 1])
+        assert torch.equal(alone, got[i:i + 1])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        again, _ = ops.token_logprobs(x, w, targets)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, _ = ops.token_logprobs(x, w, targets)
+    graph.replay()
+    assert torch.equal(again, got) and torch.equal(held, got)
+    x.copy_(x.flip(0))
+    graph.replay()
+    fresh, _ = ops.token_logprobs(x, w, targets)
+    assert torch.equal(held, fresh) and not torch.equal(held, got)
