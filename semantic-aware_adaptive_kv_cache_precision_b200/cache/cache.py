@@ -182,9 +182,11 @@ class SequenceCache:
             return
         group.holders[blocks] -= 1
         if self._shared:
-            self._shared -= sum(1 for b in blocks if group.holders[b] > 0)
-            self.sharing += 1
+            kept = len(blocks)
             blocks = [b for b in blocks if group.holders[b] == 0]
+            kept -= len(blocks)
+            self._shared -= kept
+            self.sharing += kept > 0
             if not blocks:
                 return
         if self.poison_freed and group.keys.is_floating_point():

@@ -6,6 +6,9 @@
         --prompt-ids 1,2,3 --prompt-ids 4,5 --new-tokens 16 [--temperature 0.8 --seed 1]
     python -m semantic_aware_adaptive_kv_cache_precision_b200 throughput --model DIR \
         --lengths 512 2048 --repeat 3 --warmup 1
+    python -m semantic_aware_adaptive_kv_cache_precision_b200 generate ... --samples 8 --temperature 0.8
+    python -m semantic_aware_adaptive_kv_cache_precision_b200 score --model DIR --prompt-ids 1,2,3 \
+        --continuation-ids 4,5 --continuation-ids 6
     python -m semantic_aware_adaptive_kv_cache_precision_b200 random-model --config config.json \
         --seed 0 --out DIR
 
@@ -47,13 +50,26 @@ def cmd_generate(args) -> int:
         except RuntimeError as exc:             # no tokenizer.json, or no `tokenizers` package
             raise SystemExit(f"{exc}; give token ids with --prompt-ids") from None
     out = engine.generate(prompts, args.new_tokens, stop_at_eos=not args.ignore_eos,
-                          temperature=args.temperature, seed=args.seed)
+                          temperature=args.temperature, seed=args.seed, samples=args.samples)
+    if args.samples is not None:
+        out = [tokens for of_prompt in out for tokens in of_prompt]
     for i, (tokens, ending) in enumerate(zip(out, engine.endings)):
         record = {"request": i, "tokens": tokens.tolist(), "ending": ending.state,
                   "reason": ending.reason, "positions": ending.positions}
         if args.prompt:
             record["text"] = engine.decode(tokens.tolist())
         print(json.dumps(record))
+    return 0
+
+
+def cmd_score(args) -> int:
+    """Log-probabilities of a prompt's tokens, or of continuations behind it."""
+    engine = _engine(args)
+    prompt = _ids(args.prompt_ids)
+    scores = engine.score(prompt, [_ids(c) for c in args.continuation_ids] if args.continuation_ids else None)
+    for i, s in enumerate(scores if args.continuation_ids else [scores]):
+        print(json.dumps({"continuation" if args.continuation_ids else "prompt": i, "tokens": len(s),
+                          "logprob": float(s.sum(dtype="float64")), "logprobs": [float(v) for v in s]}))
     return 0
 
 
@@ -117,7 +133,15 @@ def main(argv=None) -> int:
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--ignore-eos", action="store_true", help="do not stop at end-of-sequence ids")
+    g.add_argument("--samples", type=int, default=None, help="continuations of every prompt, which is "
+                   "prefilled once; they are requests samples * i, samples * i + 1, ... of prompt i")
     g.set_defaults(run=cmd_generate)
+
+    c = sub.add_parser("score", help="log-probabilities of a prompt's tokens, or of continuations behind it")
+    common(c)
+    c.add_argument("--prompt-ids", required=True, help="token ids, comma or space separated")
+    c.add_argument("--continuation-ids", action="append", help="token ids behind the prompt; repeat for several")
+    c.set_defaults(run=cmd_score)
 
     t = sub.add_parser("throughput", help="prefill and decode tokens a second on random ids")
     common(t)

@@ -21,10 +21,10 @@ from ..ops import _lib
 from ..cache import BLOCK, CacheFull, SequenceCache
 from ..config import config_from_dict, config_from_folder
 from .generate import (decode_ahead, COMPLETE, DECODING, EXHAUSTED, PREFILLING, Ending, RequestState,
-                       check_prompt, check_window, plan_batches, plan_prefill, positions_needed,
+                       check_prompt, check_window, plan_batches, plan_prefill, plan_samples, positions_needed,
                        stop_ids_of_folder)
 from .model import DecoderModel
-from .step import StepStager
+from .step import StepStager, table_width
 
 DEFAULT_MAX_TOKENS = 16384
 DEFAULT_MAX_BATCH = 64
@@ -74,6 +74,11 @@ class Engine:
         self._decode_ran_eagerly = False
         self.graph_failure = None
         self._prefill_graphs = {}
+        #: decode steps of sequences that share blocks read them once for all of them where that saves
+        #: at least this many blocks a layer (None: never)
+        self.shared_blocks_worth = 1
+        self._shared_now = None        # (what the plans below are right for, how far, the plans)
+        self._shared_buffers: dict = {}
         #: steps of up to this many tokens are captured when their shape repeats (0: never);
         #: at most `prefill_graph_count` of them are kept
         self.prefill_graph_tokens = 8192
@@ -104,9 +109,16 @@ class Engine:
         the TMA descriptors that were kept for both (a later tensor at one of their addresses
         then gets a descriptor of its own). The weights stay; the next step builds a new
         cache. Called when the engine is dropped."""
+        self._forget_storage()
+        self.cache = None
+
+    def _forget_storage(self) -> None:
+        """Drop what was captured or made over the cache's storage and over the weights."""
         from .. import ops
         self._graphs.clear()
         self._prefill_graphs.clear()
+        self._shared_now = None
+        self._shared_buffers.clear()
         held = [] if self.model.arena is None else [self.model.arena.buffer]
         if self.cache is not None:
             for group in self.cache.groups:
@@ -115,7 +127,6 @@ class Engine:
             ops.forget_descriptors(*held)
         except Exception:            # the interpreter may be shutting down
             pass
-        self.cache = None
 
     def __del__(self):
         try:
@@ -193,6 +204,68 @@ class Engine:
         """End sequences; what they hold goes back to the cache."""
         self._need_cache().close(slots)
 
+    def fork(self, slot: int, count: int = 1) -> list[int]:
+        """`count` new sequences that go on from where the one in `slot` is: its whole blocks are shared, its
+        last block and its state are copied (`SequenceCache.fork`; all or nothing, `CacheFull` if slots or
+        blocks are lacking). Decode steps over such sequences read a shared block once for all of them."""
+        with torch.cuda.device(self.device):
+            return self._need_cache().fork(slot, count)
+
+    def resize_cache(self, max_tokens: int) -> None:
+        """Give the cache room for `max_tokens` positions, more or fewer, while sequences live: what they
+        hold is moved together into new storage and the old is given up (`SequenceCache.resize`; nothing
+        changes where it raises `CacheFull` or `OutOfDeviceMemory`). The number of slots stays. Steps
+        captured over the old storage are captured again when their shape comes up."""
+        if max_tokens <= 0:
+            raise ValueError(f"max_tokens must be positive, got {max_tokens}")
+        if self.cache is not None:
+            old = [t for group in self.cache.groups for t in group.tensors]
+            with torch.cuda.device(self.device):
+                self.cache.resize(max_tokens)
+                self._forget_storage()
+                ops.forget_descriptors(*old)
+                self.model.prepare(self.cache.max_seq_len)
+        self.max_tokens = int(max_tokens)
+
+    def _shared_plans(self, slots, ends, cache) -> dict:
+        """The plans of a decode step over sequences some of which share blocks: {(cache group, query heads):
+        ops.SharedPlan}, at device addresses that stay the same for plans of one layout (captured steps read
+        them there). Worked out when the sequences, what they share or the width of the block lists change,
+        or a sequence outgrows them."""
+        if self.shared_blocks_worth is None or not cache.shares_blocks:
+            return {}
+        width = min(table_width(ends), cache.max_blocks_per_seq)
+        key = (tuple(slots), cache.sharing, width)
+        if self._shared_now is not None:
+            known, reach, plans = self._shared_now
+            if known == key and all(e <= r for e, r in zip(ends, reach)):
+                return plans
+        if len(self._shared_buffers) >= 64:       # layouts come and go; captured steps go with them
+            self._graphs.clear()
+            self._shared_buffers.clear()
+        # (eight blocks further: a decode loop asks again after 512 steps at the earliest)
+        reach = [min(width * BLOCK, e + 8 * BLOCK) for e in ends]
+        tables = cache.tables_for(slots)
+        plans = {}
+        for need, heads in self.model.shared_readers():
+            for g, group in enumerate(cache.groups):
+                if group.need != need:
+                    continue
+                plan = ops.plan_shared(tables[g][:, :width], ends, heads, need.kv_heads, None, reach=reach,
+                                       roomy=True, slots=2 * _lib.sm_count(self.device))
+                if plan.saved < self.shared_blocks_worth:
+                    continue
+                place = (g, heads, plan.layout)
+                buffer = self._shared_buffers.get(place)
+                words = torch.from_numpy(plan.words)
+                if buffer is None:
+                    buffer = self._shared_buffers[place] = torch.empty(words.shape, dtype=torch.int32,
+                                                                       device=self.device)
+                buffer.copy_(words.pin_memory(), non_blocking=True)
+                plans[g, heads] = plan.on(buffer)
+        self._shared_now = (key, reach, plans)
+        return plans
+
     def next_tokens(self, slots: list, device_tokens: torch.Tensor) -> torch.Tensor:
         """One greedy decode step: feed `device_tokens[i]` (int32 [len(slots)], on the device)
         to the sequence in `slots[i]` and return the token each sequence chooses next, int32
@@ -205,7 +278,8 @@ class Engine:
 
     def step(self, slots: list, new_tokens: list | None = None, want: list | None = None, *,
              device_tokens: torch.Tensor | None = None,
-             hidden_states: list | None = None, _greedy: bool = False) -> torch.Tensor:
+             hidden_states: list | None = None, targets: list | None = None,
+             _greedy: bool = False) -> torch.Tensor:
         """Feed `new_tokens[i]` to the sequence in `slots[i]`, after what its cache
         already holds, all sequences as one batch. Returns fp32 logits
         [wanted, vocab] on the device for `want[i]`, the places among
@@ -223,7 +297,11 @@ class Engine:
         `hidden_states` (a list): fp32 copies [tokens, hidden] of the residual stream are
         appended to it, after the embedding, after every layer call but the last, and after
         the final norm (the reference's order, `src/microinfer/model.py:355-364, 398-402`);
-        such a step runs kernel by kernel."""
+        such a step runs kernel by kernel.
+
+        `targets` (lists of token ids, one for each wanted place): returns fp32 [wanted], the
+        log-probability of each under the logits at its place, instead of the logits, which are
+        not kept; such a step runs kernel by kernel too."""
         cache = self._need_cache()
         if device_tokens is not None:
             if new_tokens is not None:
@@ -250,11 +328,24 @@ class Engine:
                     raise ValueError(f"wanted place {p} is outside the {c} tokens brought")
                 rows.append(base + p)
             base += c
+        if targets is not None:
+            if hidden_states is not None or [len(t) for t in targets] != [len(w) for w in want]:
+                raise ValueError("targets: one token id for each wanted place, without hidden_states")
+            flat = [int(t) for of in targets for t in of]
+            if flat and not 0 <= min(flat) <= max(flat) < self.spec.vocab_size:
+                raise ValueError(f"targets must lie in [0, {self.spec.vocab_size})")
         with torch.cuda.device(self.device):
             cache.reserve(slots, ends)
             ctx = self._stager.build(slots, new_tokens, starts, rows, cache.tables_for(slots),
                                      device_tokens)
-            if hidden_states is not None:
+            if ctx.is_decode:
+                ctx.shared = self._shared_plans(slots, ends, cache)
+            if targets is not None:
+                x = self.model.hidden(ctx, cache)
+                wanted = torch.tensor(flat, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+                logits = self.model.logprobs(x, ctx.want, wanted) if rows else torch.empty(
+                    0, dtype=torch.float32, device=self.device)
+            elif hidden_states is not None:
                 x = self.model.hidden(ctx, cache, capture=hidden_states)
                 hidden_states.append(self.model.final_states(x))
                 logits = self.model.logits(x, ctx.want) if rows else torch.empty(
@@ -302,7 +393,8 @@ class Engine:
             self._decode_ran_eagerly = True
             return run()
         key = (ctx.sequences, tuple(tuple(t.shape) for t in ctx.tables), self._stager.generation,
-               self._slots_in_key(ctx, cache), greedy)
+               self._slots_in_key(ctx, cache), greedy,
+               tuple((k, plan.layout) for k, plan in sorted(ctx.shared.items())))
         entry = self._graphs.get(key)
         if entry is None:
             if len(self._graphs) >= 64:                 # shapes come and go; keep the table small
@@ -449,10 +541,91 @@ class Engine:
         finally:
             self.close([slot])
 
+    def score(self, prompt, continuations=None):
+        """How probable given tokens are, without keeping logits. With `prompt` alone: fp32
+        (len(prompt) - 1,), the log-probability of every token of it but the first, given those before it.
+        With `continuations` (lists of ids, or text where the folder has a tokenizer.json): a list of fp32
+        arrays, the log-probability of each continuation's tokens behind the prompt; the prompt runs once and
+        its sequence is forked for them."""
+        self._need_loaded()
+
+        def ids_of(what, name):
+            return check_prompt(self.encode(what) if isinstance(what, str) else what, self.spec.vocab_size, name)
+
+        ids = ids_of(prompt, "token_ids")
+        rest = None
+        if continuations is not None:
+            rest = [np.empty(0, np.int32) if len(c) == 0 else ids_of(c, f"continuation {i}")
+                    for i, c in enumerate(continuations)]
+        # (the last token of a sequence is never fed)
+        check_window(len(ids) + max((len(c) - 1 for c in rest or () if len(c)), default=0), self.spec.max_positions)
+        if rest is None and len(ids) == 1:
+            return np.empty(0, np.float32)
+        out, first = [], {}
+        (slot,) = self.open(1)
+        try:
+            # the prompt: every token's successor within it, or the continuations' first tokens behind it
+            fed = ids[:-1] if rest is None else ids
+            for begin in range(0, len(fed), self.max_step_tokens):
+                chunk = fed[begin:begin + self.max_step_tokens]
+                if rest is None:
+                    want, targets = list(range(len(chunk))), ids[begin + 1:begin + 1 + len(chunk)]
+                elif begin + len(chunk) == len(fed):
+                    targets = [int(c[0]) for c in rest if len(c)]
+                    want = [len(chunk) - 1] * len(targets)
+                else:
+                    want, targets = [], []
+                out.append(self.step([slot], [chunk], [want], targets=[targets]))
+            if rest is None:
+                return torch.cat(out).cpu().numpy()
+            heads = iter(out[-1].split(1))
+            parts = [[next(heads)] if len(c) else [] for c in rest]
+            todo = [i for i, c in enumerate(rest) if len(c) > 1]
+            while todo:
+                group = self._score_group(slot, [rest[i] for i in todo])
+                for i, scores in zip(todo, group):
+                    parts[i].append(scores)
+                todo = todo[len(group):]
+            joined = [torch.cat(p) if p else torch.empty(0, device=self.device) for p in parts]
+            flat = torch.cat(joined).cpu().numpy() if joined else np.empty(0, np.float32)
+            at = np.cumsum([0] + [len(c) for c in rest])
+            return [flat[a:z] for a, z in zip(at, at[1:])]
+        finally:
+            self.close([slot])
+
+    def _score_group(self, slot, continuations) -> list:
+        """Log-probabilities of all tokens but the first of as many of `continuations`, in order, as the batch
+        and the cache's free blocks take (at least one), each on a fork of `slot`."""
+        cache = self._need_cache()
+        length = int(cache.lengths[slot])
+        free = min([group.pool.free for group in cache.groups], default=None)
+        count = 0
+        for c in continuations[:min(self.max_batch, max(1, cache.slots.free))]:
+            need = -(-(length + len(c) - 1) // BLOCK) - length // BLOCK
+            if free is not None:
+                if count and need > free:
+                    break
+                free -= need
+            count += 1
+        fed = [c[:-1] for c in continuations[:count]]
+        slots = self.fork(slot, count)
+        try:
+            got = [[] for _ in fed]
+            for plan in plan_prefill([len(c) for c in fed], self.max_step_tokens):
+                scores = self.step([slots[i] for i, _, _ in plan], [fed[i][a:a + n] for i, a, n in plan],
+                                   [list(range(n)) for _, _, n in plan],
+                                   targets=[continuations[i][a + 1:a + 1 + n] for i, a, n in plan])
+                for (i, _, _), some in zip(plan, scores.split([n for _, _, n in plan])):
+                    got[i].append(some)
+            return [torch.cat(g) for g in got]
+        finally:
+            self.close(slots)
+
     # -- generation -------------------------------------------------------------------------
 
     def generate(self, prompt, max_new_tokens: int = 64, *, stop_at_eos: bool = True,
-                 report=None, temperature: float = 0.0, seed: int = 0, stop_token_ids=None):
+                 report=None, temperature: float = 0.0, seed: int = 0, stop_token_ids=None,
+                 samples: int | None = None):
         """New token ids for one prompt (a 1-D sequence of ids, or text if the model folder
         has a tokenizer.json: returns one int32 array) or for a list of prompts (returns a
         list of int32 arrays).
@@ -466,6 +639,11 @@ class Engine:
         None and after each decoded token; for a list of prompts it gets the
         request's number as a fourth argument. `self.ending` (one prompt) or
         `self.endings` say how each request ended.
+
+        `samples` n: n continuations of every prompt, each prompt prefilled once and its sequence
+        forked; every prompt's result is a list of n arrays. They are requests n * i, n * i + 1, ... of
+        prompt i (draws at a temperature go by that number, as in a list that names the prompt n times),
+        in `report` and in `self.endings`; `self.ending` is None.
         """
         self._need_loaded()
         if isinstance(prompt, str):                    # text, if the folder has a tokenizer
@@ -475,13 +653,24 @@ class Engine:
         prompts = [self.encode(p) if isinstance(p, str) else p for p in prompts]
         if max_new_tokens < 0:
             raise ValueError(f"max_new_tokens must not be negative, got {max_new_tokens}")
+        if samples is not None and samples <= 0:
+            raise ValueError(f"samples must be positive, got {samples}")
+        each = samples or 1
+
+        def result():
+            tokens = [e.tokens for e in self.endings]
+            if samples is not None:
+                tokens = [tokens[i:i + each] for i in range(0, len(tokens), each)]
+            self.ending = self.endings[0] if single and samples is None else None
+            return tokens[0] if single else tokens
+
         ids = [check_prompt(p, self.spec.vocab_size, f"prompt {i}" if not single else "token_ids")
                for i, p in enumerate(prompts)]
         params = sampling.SamplingParams(float(temperature), int(seed))
         if max_new_tokens == 0:
-            self.endings = [Ending(COMPLETE, 0, np.empty(0, np.int32), "length") for _ in ids]
-            self.ending = self.endings[0] if single else None
-            return self.endings[0].tokens if single else [e.tokens for e in self.endings]
+            self.endings = [Ending(COMPLETE, 0, np.empty(0, np.int32), "length")
+                            for _ in ids for _ in range(each)]
+            return result()
         for p in ids:
             check_window(positions_needed(len(p), max_new_tokens), self.spec.max_positions)
         if stop_token_ids is not None:
@@ -490,26 +679,34 @@ class Engine:
             stops = self.eos_token_ids if stop_at_eos else frozenset()
         if report is None:
             tell = lambda *a: None
-        elif single:
+        elif single and samples is None:
             tell = lambda phase, positions, token, request: report(phase, positions, token)
         else:
             tell = report
 
         cache = self._need_cache()
-        batches = plan_batches([len(p) for p in ids], max_new_tokens, self.max_batch,
-                               cache.max_tokens)
+        lengths = [len(p) for p in ids]
+        if samples is None:
+            batches = [[(i, 0, 1) for i in batch] for batch in
+                       plan_batches(lengths, max_new_tokens, self.max_batch, cache.max_tokens)]
+        else:
+            batches = plan_samples(lengths, samples, max_new_tokens, min(self.max_batch, cache.max_slots),
+                                   cache.max_tokens)
         endings: dict[int, Ending] = {}
         for batch in batches:
-            self._run_batch([RequestState(i, ids[i]) for i in batch], max_new_tokens, stops,
-                            params, tell, endings)
-        self.endings = [endings[i] for i in range(len(ids))]
-        self.ending = self.endings[0] if single else None
-        return self.endings[0].tokens if single else [e.tokens for e in self.endings]
+            self._run_batch([[RequestState(i * each + s, ids[i]) for s in range(first, first + n)]
+                             for i, first, n in batch], max_new_tokens, stops, params, tell, endings)
+        self.endings = [endings[i] for i in range(len(ids) * each)]
+        return result()
 
-    def _run_batch(self, requests, max_new_tokens, stops, params, tell, endings) -> None:
+    def _run_batch(self, groups, max_new_tokens, stops, params, tell, endings) -> None:
+        """`groups`: lists of requests of one prompt each; the first of a group is prefilled, the others
+        are forked from it."""
         cache = self._need_cache()
-        slots = cache.open(len(requests))
-        slot_of = {r.index: s for r, s in zip(requests, slots)}
+        requests = [r for group in groups for r in group]
+        heads = [group[0] for group in groups]
+        slots = cache.open(len(groups))
+        slot_of = {r.index: s for r, s in zip(heads, slots)}
         live = list(requests)
 
         def positions(r):           # what its cache holds: the last new token is never fed
@@ -523,12 +720,12 @@ class Engine:
         try:
             # prefill: every prompt whole, in one step unless the batch is too large
             try:
-                plans = plan_prefill([len(r.prompt) for r in requests], self.max_step_tokens)
+                plans = plan_prefill([len(r.prompt) for r in heads], self.max_step_tokens)
                 logits = {}
                 for plan in plans:
                     step_slots = [slots[i] for i, _, _ in plan]
-                    tokens = [requests[i].prompt[a:a + n] for i, a, n in plan]
-                    ends = [a + n == len(requests[i].prompt) for i, a, n in plan]
+                    tokens = [heads[i].prompt[a:a + n] for i, a, n in plan]
+                    ends = [a + n == len(heads[i].prompt) for i, a, n in plan]
                     want = [[n - 1] if last else [] for (_, _, n), last in zip(plan, ends)]
                     out = self.step(step_slots, tokens, want)
                     row = 0
@@ -536,13 +733,18 @@ class Engine:
                         if last:
                             logits[i] = out[row]
                             row += 1
+                for slot, group in zip(slots, groups):
+                    if len(group) > 1:
+                        for r, s in zip(group[1:], self.fork(slot, len(group) - 1)):
+                            slot_of[r.index] = s
             except CacheFull as exc:
-                for r in live:
-                    endings[r.index] = Ending(EXHAUSTED, int(cache.lengths[slot_of[r.index]]),
-                                              np.asarray(r.out, np.int32), str(exc))
-                    cache.close([slot_of[r.index]])
+                for slot, group in zip(slots, groups):
+                    for r in group:
+                        endings[r.index] = Ending(EXHAUSTED, int(cache.lengths[slot]),
+                                                  np.asarray(r.out, np.int32), str(exc))
+                cache.close(slot_of.values())
                 return
-            first = self._choose(torch.stack([logits[i] for i in range(len(requests))]),
+            first = self._choose(torch.stack([logits[i] for i, group in enumerate(groups) for _ in group]),
                                  params, live)
             for r, token in zip(live, self._read(first)):
                 r.drawn = 1
@@ -571,7 +773,7 @@ class Engine:
                          on_finish=finish,
                          on_exhausted=lambda r, why: finish(r, EXHAUSTED, why))
         except BaseException:
-            held = [slot_of[r.index] for r in requests if r.index not in endings]
+            held = [slot_of[r.index] for r in requests if r.index in slot_of and r.index not in endings]
             cache.close(held)
             raise
 

@@ -66,6 +66,38 @@ def plan_batches(prompt_lens: list, max_new_tokens: int, max_batch: int,
     return batches
 
 
+def plan_samples(prompt_lens: list, samples: int, max_new_tokens: int, max_batch: int,
+                 max_tokens: int) -> list[list[tuple]]:
+    """The same for `samples` continuations of every prompt, which share the prompt's whole blocks: batches of
+    (prompt, first sample, count), in order, at most `max_batch` sequences each; a prompt's samples go to
+    several batches where one does not take them."""
+    if max_batch <= 0:
+        raise ValueError(f"max_batch must be positive, got {max_batch}")
+    budget = max_tokens // BLOCK
+    batches, current, taken, used = [], [], 0, 0
+    for i, n in enumerate(prompt_lens):
+        common = n // BLOCK
+        own = blocks_needed(n, max_new_tokens) - common
+        # (a prompt that ends with a block has nothing of its own before its first new token)
+        if common + own > budget:
+            raise ValueError(f"request {i} needs {(common + own) * BLOCK} cache positions ({n} prompt + "
+                             f"{max_new_tokens} new), the cache holds {budget * BLOCK}")
+        done = 0
+        while done < samples:
+            room = budget - used - common
+            fit = min(samples - done, max_batch - taken, samples if own <= 0 and room >= 0 else
+                      room // max(own, 1))
+            if fit <= 0:
+                batches.append(current)
+                current, taken, used = [], 0, 0
+                continue
+            current.append((i, done, fit))
+            done, taken, used = done + fit, taken + fit, used + common + fit * own
+    if current:
+        batches.append(current)
+    return batches
+
+
 def plan_prefill(prompt_lens: list, max_step_tokens: int) -> list[list[tuple]]:
     """Cut the prefill of a batch into steps of at most `max_step_tokens` tokens.
     Each step is a list of (sequence index, first token, count). Normally one

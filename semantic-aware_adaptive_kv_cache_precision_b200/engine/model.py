@@ -105,6 +105,11 @@ class DecoderModel:
         for block in self.blocks:
             block.prepare(self.device, max_positions)
 
+    def shared_readers(self) -> list:
+        """[(cache need, query heads)], each once: see `Part.shared_readers`."""
+        return list(dict.fromkeys(reader for b in self.blocks
+                                  for reader in getattr(b, "shared_readers", list)()))
+
     # -- the forward pass ---------------------------------------------------------
 
     def hidden(self, step, cache, capture: list | None = None) -> torch.Tensor:
@@ -195,6 +200,15 @@ class DecoderModel:
         if self.spec.logit_scale != 1.0 or self.spec.logit_softcap:
             ops.scale_cap_(out, self.spec.logit_scale, self.spec.logit_softcap)
         return out
+
+    def logprobs(self, x: torch.Tensor, rows: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        """fp32 [len(rows)]: the log-probability of token `targets[i]` (int32) behind the token row
+        `rows[i]` of `x`, under the softmax of `logits`, which are not kept."""
+        normed = self.final_norm.forward(x, rows=rows)
+        if normed.dtype != self.head.dtype:          # (a head stored in 32 bits beside 16-bit activations)
+            normed = normed.to(self.head.dtype)
+        return ops.token_logprobs(normed, self.head, targets, self.head_bias, scale=self.spec.logit_scale,
+                                  softcap=self.spec.logit_softcap or 0.0)[0]
 
 
 def _settle(x, pending) -> None:

@@ -44,6 +44,14 @@ class StepContext:
     max_len_bound: int = 0            # a bound on max_len that changes rarely (block-list width)
     plans: dict = field(default_factory=dict)   # what a part worked out for this step, for its
                                                 # other layers to use again (key chosen by the part)
+    # decode steps of sequences that share blocks: (cache group, query heads) -> ops.SharedPlan
+    shared: dict = field(default_factory=dict)
+
+
+def table_width(ends) -> int:
+    """Columns of a step's block lists: as many as its longest sequence needs, rounded up to a multiple
+    of 8, so that a decode loop keeps one shape for 512 steps and its captured graph can be replayed."""
+    return -(-max(1, -(-max(ends, default=1) // BLOCK)) // 8) * 8
 
 
 class StepStager:
@@ -112,9 +120,7 @@ class StepStager:
         W = want_rows.size
         # block lists only as wide as the longest sequence of the step needs
         ends = [s + c for s, c in zip(starts, counts)]
-        # (rounded up to a multiple of 8 blocks, so that a decode loop keeps one shape for
-        # 512 steps and its captured graph can be replayed)
-        width = -(-max(1, -(-max(ends, default=1) // BLOCK)) // 8) * 8
+        width = table_width(ends)
         tables = [np.ascontiguousarray(t[:, :min(width, t.shape[1])]) for t in tables]
         offsets, total, views, dev_tables = self._layout(T, B, W, tuple(t.shape for t in tables))
         turn = self.turn = 1 - self.turn

@@ -90,6 +90,11 @@ class SharedPlan:
     __slots__ = ("words", "sequences", "heads", "kv_heads", "units", "unit_at", "unit_capacity", "member_at",
                  "first_at", "partials", "reach", "width", "saved")
 
+    @property
+    def layout(self) -> tuple:
+        """What a captured call keeps of a plan besides its words' address."""
+        return (self.sequences, self.width, self.unit_capacity, self.member_at, self.first_at, self.partials)
+
     def on(self, words: torch.Tensor) -> "SharedPlan":
         """The same plan with its words at `words` (int32, on the device)."""
         other = SharedPlan()

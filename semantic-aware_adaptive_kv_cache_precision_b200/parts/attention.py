@@ -74,6 +74,12 @@ class GQAAttention(Part):
     def cache_need(self):
         return KVNeed(self.spec.kv_heads, self.spec.head_dim, self.spec.window)
 
+    def shared_readers(self):
+        s = self.spec
+        if s.window or not ops.fast_path_takes(self.act_dtype, s.heads, s.kv_heads, s.head_dim):
+            return []
+        return [(self.cache_need(), s.heads)]
+
     # -- the step ---------------------------------------------------------------
 
     can_defer = True
@@ -82,14 +88,20 @@ class GQAAttention(Part):
         s = self.spec
         qkv = ops.linear(h, self.w_qkv, self.b_qkv, out_dtype=self.act_dtype)
         rotary = None
-        if step.is_decode and ops.fast_path_takes(qkv.dtype, s.heads, s.kv_heads, s.head_dim) \
+        shared = step.shared.get((view.group, s.heads)) if step.is_decode else None
+        if shared is None and step.is_decode and ops.fast_path_takes(qkv.dtype, s.heads, s.kv_heads, s.head_dim) \
                 and hasattr(self.position, "tables"):
             # one token a sequence: the attention kernel rotates and stores on its own way
             rotary = self.position.tables(step, s.head_dim)
         if rotary is None:
             self.position.rotate_store(qkv, step, view, s.heads, s.kv_heads, s.head_dim,
                                        write_cache)
-        attended = self.attend(qkv, step, view, rotary, write_cache)
+        if shared is not None:       # sequences forked from one another: common blocks are read once
+            attended = ops.shared_decode_attention(qkv, view.keys, view.values, step.seq_lens,
+                                                   view.block_table, shared, s.heads, s.kv_heads,
+                                                   s.head_dim, s.scale)
+        else:
+            attended = self.attend(qkv, step, view, rotary, write_cache)
         out = ops.linear(attended, self.w_o, self.b_o, accumulate_into=residual, may_defer=defer)
         return out.delta if isinstance(out, ops.Deferred) else None
 

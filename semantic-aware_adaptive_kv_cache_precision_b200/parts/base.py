@@ -74,6 +74,12 @@ class Part:
     def tensor_decls(self) -> list[TensorDecl]:
         return []
 
+    def shared_readers(self) -> list:
+        """[(cache need, query heads)] of the mixers here that read blocks which several sequences list
+        once for all of them, in steps whose `step.shared` has a plan for their cache group and heads."""
+        inner = tuple(getattr(self, "parts", ())) + tuple(getattr(self, "branches", ()))
+        return [reader for part in inner for reader in getattr(part, "shared_readers", list)()]
+
     def bind(self, arena) -> None:
         """Pick up this part's tensors from the loaded arena."""
 
