@@ -8,11 +8,15 @@
 // pieces that the same set of sequences lists (ops/shared.py); a unit of work is a piece, up to 64 rows of
 // queries (sequences of the piece x query heads of one KV head) and that KV head.
 //
-//   grid  = units x KV heads, heaviest first; block = 4 warps
+//   grid  = units x KV heads, heaviest first; block = 6 warps, two blocks an SM
 //   tile  = one cache block: 64 keys x head_dim by TMA (128-byte swizzle) into a ring of stages
-//   NR    = groups of 16 rows the unit has (1, 2 or 4): warp w takes rows 16 (w % NR) .. + 15 and 16 NR keys
-//           of every tile from 16 NR (w / NR) on, so that four warps have work however few the rows; warps of
-//           the same rows are merged at the end.
+// and a unit's rows of queries are worked on in one of two ways:
+//   wide   (more than kNarrowRows rows, up to 128) on tcgen05: S = Q K^T with the rows on tensor memory's lanes,
+//          one thread a row for the softmax, P written over S as the A operand of P V, O in tensor memory; the
+//          next tile's S is computed under this tile's softmax.
+//   narrow (up to kNarrowRows rows) on mma.sync: NR = groups of 16 rows (1, 2 or 4); warp w of four takes rows
+//          16 (w % NR) .. + 15 and 16 NR keys of every tile from 16 NR (w / NR) on, so that four warps have
+//          work however few the rows; warps of the same rows are merged at the end.
 //
 // Every unit leaves a partial (m, l, o) for each of its (sequence, head); a sequence's partials lie side by
 // side, in the order of its positions, and `join_kernel` merges them. Scores, maxima, exponentials and sums
@@ -21,22 +25,32 @@
 // The reference reads a sequence's cache for every sequence (`src/core_kernels/attention.cu:754-815`).
 #include "common.cuh"
 #include "mma.cuh"
+#include "tcgen05.cuh"
 #include "tma.cuh"
 
 namespace {
 
 constexpr int KT = kCacheBlock;
 constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;
-constexpr int kRows = 64;            // most rows of a unit
+constexpr int kThreads = 192;        // 6 warps; four of them in a narrow unit and in the join
+constexpr int kNarrowThreads = kWarps * 32;
+constexpr int kStages = 3;           // of a narrow unit
+constexpr int kWideRows = 128, kNarrowRows = 64;
+constexpr int kWideStages = 2;
+constexpr int kMembers = kWideRows + 2;
+constexpr uint32_t kTmemCols = 256;  // wide: S 2 x 64 (P over the first 32 of each), O from 128 on
+constexpr uint32_t kOCol = 128;
+constexpr float kLazy = 8.f;         // O is rescaled when a row's maximum has grown by 2^8
 
 template <int D>
 struct Smem {
   static constexpr int kBoxes = D / 64;
   static constexpr int kTileBytes = KT * D * 2;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kBytes = kStages * kStageBytes + 1024 + 256;
+  static constexpr int kQBytes = kWideRows * D * 2;
+  static constexpr int kNarrow = kStages * kStageBytes, kWide = kQBytes + kWideStages * kStageBytes;
+  static constexpr int kBarriers = kNarrow > kWide ? kNarrow : kWide;     // where they lie
+  static constexpr int kBytes = kBarriers + 1024 + 256;
 };
 
 // What the host's plan holds (int32 words, offsets in words): see ops/shared.py.
@@ -62,22 +76,37 @@ struct Params {
 };
 
 // Words 0-1 of the plan: units, sequences. A unit's words: the sequence whose block list is read, its first
-// block, blocks, first member, members, 0, 0, 0. A member: (sequence, its partial).
+// block, blocks, first member, first row of that member, rows, 0, 0; rows are (member, query head of the KV
+// head), heads fastest. A member: (sequence, its partial).
+struct Unit {
+  int sequence, column, columns, member, row, rows, pad0, pad1;
+};
+
+// Row r of the unit: its query, and where its partial goes.
+struct Row {
+  const __nv_bfloat16* q;
+  long long slot;
+};
+__device__ __forceinline__ Row row_at(const Params& p, const int2* member, const Unit& u, int g, int r, int d) {
+  const int group = p.heads / p.kv_heads;
+  const int j = (u.row + r) / group, h = g * group + u.row + r - j * group;
+  return Row{p.q + (long long)member[j].x * p.q_stride + (long long)h * d, (long long)member[j].y * p.heads + h};
+}
+
 template <int D, int NR>
 __device__ __forceinline__ void
-attend(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint8_t* smem, uint64_t* full,
-       uint64_t* empty, const int* listed, int g, int row_seq, int col0, int n_tiles, int kv_len,
-       const int2* member, int members) {
+attend_narrow(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint8_t* smem, uint64_t* full,
+              uint64_t* empty, int* failed, const int* listed, int g, const Unit& u, int n_tiles, int kv_len,
+              const int2* member) {
   using S = Smem<D>;
   constexpr int KW = 16 * NR;          // keys of a tile that a warp takes
-  const int group = p.heads / p.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rg = warp % NR, kp = warp / NR;
-  const int rows = members * group;
+  const int rows = u.rows, col0 = u.column;
 
   auto request = [&](int i) {
     const int stage = i % kStages;
-    const int block = i < kThreads ? listed[i] : p.block_table[(long long)row_seq * p.max_blocks + col0 + i];
+    const int block = i < kThreads ? listed[i] : p.block_table[(long long)u.sequence * p.max_blocks + col0 + i];
     const int row0 = (block * p.kv_heads + g) * KT;
     uint8_t* dst = smem + stage * S::kStageBytes;
     tma::mbar_expect_tx(&full[stage], S::kStageBytes);
@@ -97,11 +126,7 @@ attend(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = rg * 16 + (lane >> 2) + 8 * i;
-      at[i] = nullptr;
-      if (r < rows) {
-        const int j = r / group;
-        at[i] = p.q + (long long)member[j].x * p.q_stride + (long long)(g * group + r - j * group) * D + c;
-      }
+      at[i] = r < rows ? row_at(p, member, u, g, r, D).q + c : nullptr;
     }
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
@@ -220,12 +245,12 @@ attend(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
   }
-  alive = __syncthreads_and(alive);
-  if (!alive) {                  // (a copy did not come: see the others land before the memory is given back)
+  if (!alive) *failed = 1;
+  asm volatile("bar.sync 1, %0;" ::"n"(kNarrowThreads) : "memory");
+  if (*failed) {                  // (a copy did not come: see the others land before the memory is given back)
     if (threadIdx.x == 0)
       for (int i = max(0, n_tiles - kStages); i < n_tiles; ++i)
         tma::mbar_wait(&full[i % kStages], (i / kStages) & 1, p.error, 153);
-    __syncthreads();
     return;
   }
   constexpr int kRow = D + 8;
@@ -245,7 +270,7 @@ attend(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint
       sm_l[warp * 16 + r0] = l[0]; sm_l[warp * 16 + r0 + 8] = l[1];
     }
   }
-  __syncthreads();
+  asm volatile("bar.sync 1, %0;" ::"n"(kNarrowThreads) : "memory");
   // a warp takes rows warp, warp + 4, ...; a lane four sizes of the head
 #pragma unroll 2
   for (int r = warp; r < rows; r += kWarps) {
@@ -263,8 +288,7 @@ attend(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint
       weight[w] = sum == 0.f ? 0.f : mma::exp2_fast(mine - big);
       total += weight[w] * sum;
     }
-    const int j = r / group;
-    const long long to = (long long)member[j].y * p.heads + g * group + r - j * group;
+    const long long to = row_at(p, member, u, g, r, D).slot;
     if (lane < D / 4) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -279,74 +303,315 @@ attend(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint
   }
 }
 
+// V tile as the B operand of P V: N (head dims) contiguous, 64 per 128-byte row, the next 64 dims one box
+// further; 8 keys per 1024-byte swizzle group.
+__device__ __forceinline__ uint64_t desc_values(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>((KT * 128) >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+struct WideBarriers {
+  uint64_t q_full;
+  uint64_t k_full[kWideStages], k_empty[kWideStages];     // keys: free again as soon as S_j is done
+  uint64_t v_full[kWideStages], v_empty[kWideStages];     // values: free once P_j V_j is done
+  uint64_t s_full[2];
+  uint64_t p_full;       // P_j lies in tensor memory over S_j
+  uint64_t pv_done;      // P_j V_j has been added to O
+};
+
+// Up to 128 rows on tcgen05: warp 0 copies, lane 0 of warp 1 issues the products, warps 2-5 hold a row a thread.
 template <int D>
-__global__ void __launch_bounds__(kThreads)
+__device__ __forceinline__ void
+attend_wide(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map, uint8_t* smem, WideBarriers* bar,
+            uint32_t tmem, const int* listed, int g, const Unit& u, int n, int kv_len, const int2* member) {
+  using S = Smem<D>;
+  uint8_t* q_s = smem;
+  uint8_t* kv_s = q_s + S::kQBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    if (lane == 0) {
+      int j = 0, v_sent = 0;
+      for (; j < n; ++j) {
+        const int stage = j % kWideStages;
+        const int block = j < kThreads ? listed[j]
+                                       : p.block_table[(long long)u.sequence * p.max_blocks + u.column + j];
+        const int row0 = (block * p.kv_heads + g) * KT;
+        uint8_t* dst = kv_s + stage * S::kStageBytes;
+        if (j >= kWideStages &&
+            !tma::mbar_wait(&bar->k_empty[stage], ((j / kWideStages) - 1) & 1, p.error, 161))
+          break;
+        tma::mbar_expect_tx(&bar->k_full[stage], S::kTileBytes);
+        for (int x = 0; x < S::kBoxes; ++x)
+          tma::load_2d(dst + x * (KT * 128), k_map, x * 64, row0, &bar->k_full[stage]);
+        if (j >= kWideStages &&
+            !tma::mbar_wait(&bar->v_empty[stage], ((j / kWideStages) - 1) & 1, p.error, 162)) {
+          ++j;
+          break;
+        }
+        tma::mbar_expect_tx(&bar->v_full[stage], S::kTileBytes);
+        for (int x = 0; x < S::kBoxes; ++x)
+          tma::load_2d(dst + S::kTileBytes + x * (KT * 128), v_map, x * 64, row0, &bar->v_full[stage]);
+        v_sent = j + 1;
+      }
+      // the copies in flight land before the memory is given back (they have, unless a wait ran out)
+      for (int i = max(0, j - kWideStages); i < j; ++i)
+        tma::mbar_wait(&bar->k_full[i % kWideStages], (i / kWideStages) & 1, p.error, 163);
+      for (int i = max(0, v_sent - kWideStages); i < v_sent; ++i)
+        tma::mbar_wait(&bar->v_full[i % kWideStages], (i / kWideStages) & 1, p.error, 164);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kWideRows, KT);                   // K-major both
+      constexpr uint32_t idesc_pv = tc::idesc_bf16_f32(kWideRows, D) | (1u << 16);      // B MN-major
+      bool ok = tma::mbar_wait(&bar->q_full, 0, p.error, 165);
+      const uint32_t q_addr = tma::smem_u32(q_s);
+      auto issue_pv = [&](int i) {
+        const int stage = i % kWideStages;
+        if (!tma::mbar_wait(&bar->p_full, i & 1, p.error, 166)) return false;
+        if (!tma::mbar_wait(&bar->v_full[stage], (i / kWideStages) & 1, p.error, 167)) return false;
+        tc::fence_after_sync();
+        const uint32_t v_addr = tma::smem_u32(kv_s + stage * S::kStageBytes + S::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k)
+          tc::mma_ts(tmem + kOCol, tmem + (i & 1) * KT + k * 8, desc_values(v_addr + k * 2048), idesc_pv,
+                     i > 0 || k > 0);
+        tc::commit(&bar->pv_done);
+        tc::commit(&bar->v_empty[stage]);
+        return true;
+      };
+      for (int j = 0; j < n && ok; ++j) {
+        const int stage = j % kWideStages;
+        // (S_j goes where S_{j-2} and then P_{j-2} lay: P_{j-2} V_{j-2} was issued before this, and one
+        // thread's products run in the order it issued them)
+        ok = tma::mbar_wait(&bar->k_full[stage], (j / kWideStages) & 1, p.error, 168);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const uint32_t k_addr = tma::smem_u32(kv_s + stage * S::kStageBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc::mma_ss(tmem + (j & 1) * KT,
+                     tc::smem_desc_k_major_sw128(q_addr + (k >> 2) * (kWideRows * 128) + (k & 3) * 32),
+                     tc::smem_desc_k_major_sw128(k_addr + (k >> 2) * (KT * 128) + (k & 3) * 32), idesc_s, k > 0);
+        tc::commit(&bar->s_full[j & 1]);
+        tc::commit(&bar->k_empty[stage]);
+        if (j >= 1) ok = issue_pv(j - 1);
+      }
+      if (ok && n > 0) issue_pv(n - 1);
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;                         // row of the unit = tensor-memory lane
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    Row row{nullptr, 0};
+    if (r < u.rows) row = row_at(p, member, u, g, r, D);
+    // this thread's query into the swizzled tile (zeros for rows that the unit does not have)
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row.q) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(row.q + c * 8);      // (rows begin at 4 bytes)
+        v = make_uint4(src[0], src[1], src[2], src[3]);
+      }
+      *reinterpret_cast<uint4*>(q_s + (c >> 3) * (kWideRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+    }
+    tma::fence_proxy_async();
+    tma::mbar_arrive(&bar->q_full);
+    float m_true = -INFINITY;      // running maximum of the scaled scores
+    float m_ref = -INFINITY;       // what the exponentials, the row's sum and O are relative to
+    float l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int bj = j & 1;
+      if (!tma::mbar_wait(&bar->s_full[bj], (j >> 1) & 1, p.error, 169)) { ok = false; break; }
+      tc::fence_after_sync();
+      float s[KT];
+      tc::ld_32x32b_x64(lane_base + bj * KT, s);
+      const int valid = kv_len - (u.column + j) * KT;          // keys of the tile that exist
+      if (valid < KT) {
+#pragma unroll
+        for (int c = 0; c < KT; ++c) s[c] = c < valid ? s[c] : -INFINITY;
+      }
+      float big4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < KT; c += 8) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) big4[q] = mma::max3(big4[q], s[c + 2 * q], s[c + 2 * q + 1]);
+      }
+      const float big = fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3]));
+      m_true = fmaxf(m_true, big * p.scale_log2e);
+      bool waited = j == 0;          // whether P_{j-1} V_{j-1} is known to be done
+      const bool move = m_true > m_ref + kLazy;      // (also true the first time a key is seen)
+      if (__any_sync(0xffffffffu, move)) {
+        const float factor = move ? mma::exp2_fast(m_ref - m_true) : 1.f;   // 0 when m_ref = -inf
+        if (j >= 1) {
+          if (!tma::mbar_wait(&bar->pv_done, (j - 1) & 1, p.error, 170)) { ok = false; break; }
+          waited = true;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            float v[16];
+            tc::ld_32x32b_x16(lane_base + kOCol + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) mma::mul2(v[i], v[i + 1], factor);
+            tc::st_32x32b_x16(lane_base + kOCol + c, v);
+          }
+          tc::fence_before_sync();
+        }
+        if (move) {
+          l *= factor;
+          m_ref = m_true;
+        }
+      }
+      const float minus_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
+      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t packed[KT / 2];
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) {
+        float e0, e1;
+        mma::fma2(e0, e1, s[2 * i], s[2 * i + 1], p.scale_log2e, minus_m);
+        const float p0 = mma::exp2_fast(e0), p1 = mma::exp2_fast(e1);
+        mma::add2(sum4[(i & 1) * 2], sum4[(i & 1) * 2 + 1], p0, p1);
+        packed[i] = mma::pack_bf16(p0, p1);
+      }
+      tc::st_32x32b_x32(lane_base + bj * KT, packed);
+      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      if (valid < KT) {
+        // value rows behind the sequence's end are stale: zero them, so that 0 x garbage is 0
+        if (!tma::mbar_wait(&bar->v_full[j % kWideStages], (j / kWideStages) & 1, p.error, 171)) { ok = false; break; }
+        uint8_t* vt = kv_s + (j % kWideStages) * S::kStageBytes + S::kTileBytes;
+        for (int i = r; i < (KT - valid) * (D / 8); i += kWideRows) {
+          const int key = valid + i / (D / 8), c = i % (D / 8);
+          *reinterpret_cast<uint4*>(vt + (c >> 3) * (KT * 128) + key * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        tma::fence_proxy_async();
+      }
+      // (every product is waited for once, in order: a barrier's phases are told apart by one bit)
+      if (!waited && !tma::mbar_wait(&bar->pv_done, (j - 1) & 1, p.error, 172)) { ok = false; break; }
+      tc::fence_before_sync();
+      tma::mbar_arrive(&bar->p_full);
+    }
+    if (ok && tma::mbar_wait(&bar->pv_done, (n - 1) & 1, p.error, 173)) {
+      tc::fence_after_sync();
+      float* po = p.part_o + row.slot * D;
+#pragma unroll
+      for (int c = 0; c < D; c += 16) {
+        float v[16];
+        tc::ld_32x32b_x16(lane_base + kOCol + c, v);
+        if (row.q) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(po + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+      }
+      if (row.q) p.part_ml[row.slot] = make_float2(m_ref, l);
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2)
 shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                         const __grid_constant__ Params p) {
   using S = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * S::kStageBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBarriers);       // narrow: kStages full, kStages empty
   uint64_t* empty = full + kStages;
+  WideBarriers* wide = reinterpret_cast<WideBarriers*>(smem + S::kBarriers);
   __shared__ int listed[kThreads];
-  __shared__ int2 member[kRows];
+  __shared__ int2 member[kMembers];
+  __shared__ int failed;
+  __shared__ uint32_t tmem_at;
 
-  let_next_kernel_start();
-  const int unit = blockIdx.x / p.kv_heads, g = blockIdx.x - unit * p.kv_heads;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      tma::mbar_init(&full[s], 1);
-      tma::mbar_init(&empty[s], kWarps);
-    }
-    tma::fence_barrier_init();
-    tma::prefetch_map(&k_map);
-    tma::prefetch_map(&v_map);
-  }
   // (the plan, the block lists and the lengths are the step's inputs: they were written before the kernel
   // before this one began; what that one wrote, queries, keys and values, is read behind the wait)
+  const int unit = blockIdx.x / p.kv_heads, g = blockIdx.x - unit * p.kv_heads;
+  const int group = p.heads / p.kv_heads;
   const bool live = unit < min(p.plan.words[0], p.plan.unit_capacity);
-  int4 what = make_int4(0, 0, 0, 0);
-  int members = 0, n_tiles = 0, kv_len = 0;
+  Unit u{};
+  int n_tiles = 0, kv_len = 0;
   if (live) {
-    what = *reinterpret_cast<const int4*>(p.plan.words + p.plan.unit_at + unit * 8);
-    members = p.plan.words[p.plan.unit_at + unit * 8 + 4];
-    const int given = p.seq_lens[what.x];
+    const int4* words = reinterpret_cast<const int4*>(p.plan.words + p.plan.unit_at + unit * 8);
+    const int4 a = words[0], b = words[1];
+    u = Unit{a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
+    const int given = p.seq_lens[u.sequence];
     kv_len = given < 0 || given > p.max_blocks * KT ? 0 : given;
-    n_tiles = min((kv_len + KT - 1) / KT - what.y, what.z);
+    n_tiles = min((kv_len + KT - 1) / KT - u.column, u.columns);
+    const int members = (u.row + u.rows + group - 1) / group;
     if (threadIdx.x < members)
       member[threadIdx.x] = *reinterpret_cast<const int2*>(p.plan.words + p.plan.member_at +
-                                                           2 * (what.w + threadIdx.x));
+                                                           2 * (u.member + threadIdx.x));
     if (threadIdx.x < n_tiles)
-      listed[threadIdx.x] = p.block_table[(long long)what.x * p.max_blocks + what.y + threadIdx.x];
+      listed[threadIdx.x] = p.block_table[(long long)u.sequence * p.max_blocks + u.column + threadIdx.x];
   }
+  const bool is_wide = u.rows > kNarrowRows && n_tiles > 0;
+  if (threadIdx.x == 0) {
+    failed = 0;
+    tma::prefetch_map(&k_map);
+    tma::prefetch_map(&v_map);
+    if (is_wide) {
+      tma::mbar_init(&wide->q_full, kWideRows);
+      for (int s = 0; s < kWideStages; ++s) {
+        tma::mbar_init(&wide->k_full[s], 1);
+        tma::mbar_init(&wide->k_empty[s], 1);
+        tma::mbar_init(&wide->v_full[s], 1);
+        tma::mbar_init(&wide->v_empty[s], 1);
+      }
+      for (int i = 0; i < 2; ++i) tma::mbar_init(&wide->s_full[i], 1);
+      tma::mbar_init(&wide->p_full, kWideRows);
+      tma::mbar_init(&wide->pv_done, 1);
+    } else {
+      for (int s = 0; s < kStages; ++s) {
+        tma::mbar_init(&full[s], 1);
+        tma::mbar_init(&empty[s], kWarps);
+      }
+    }
+    tma::fence_barrier_init();
+  }
+  if (is_wide && (threadIdx.x >> 5) == 1) tc::tmem_alloc(&tmem_at, kTmemCols);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  let_next_kernel_start();       // (with its shared and tensor memory in hand)
   wait_for_previous_kernel();
   if (!live) return;
-  __syncthreads();
-  const int group = p.heads / p.kv_heads;
-  const int rows = members * group;
   if (n_tiles <= 0) {            // a piece that the sequence has not reached yet: it counts for nothing
-    for (int r = threadIdx.x; r < rows; r += kThreads) {
-      const int j = r / group;
-      p.part_ml[(long long)member[j].y * p.heads + g * group + r - j * group] = make_float2(-INFINITY, 0.f);
+    for (int r = threadIdx.x; r < u.rows; r += kThreads)
+      p.part_ml[row_at(p, member, u, g, r, D).slot] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  if (is_wide) {
+    attend_wide<D>(p, &k_map, &v_map, smem, wide, tmem_at, listed, g, u, n_tiles, kv_len, member);
+    tc::fence_before_sync();
+    __syncthreads();
+    if ((threadIdx.x >> 5) == 1) {
+      tc::fence_after_sync();
+      tc::tmem_dealloc(tmem_at, kTmemCols);
     }
     return;
   }
-#define SAKV_ATTEND(NR) \
-  attend<D, NR>(p, &k_map, &v_map, smem, full, empty, listed, g, what.x, what.y, n_tiles, kv_len, member, members)
-  if (rows <= 16) SAKV_ATTEND(1);
-  else if (rows <= 32) SAKV_ATTEND(2);
-  else SAKV_ATTEND(4);
-#undef SAKV_ATTEND
+  if (threadIdx.x >= kNarrowThreads) return;
+#define SAKV_NARROW(NR) \
+  attend_narrow<D, NR>(p, &k_map, &v_map, smem, full, empty, &failed, listed, g, u, n_tiles, kv_len, member)
+  if (u.rows <= 16) SAKV_NARROW(1);
+  else if (u.rows <= 32) SAKV_NARROW(2);
+  else SAKV_NARROW(4);
+#undef SAKV_NARROW
 }
 
 // out[b, h] = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m), over the sequence's partials. A block a
 // (sequence, head): D / 4 threads hold four sizes each, the block's groups of them take partials s, s + groups,
 // ... with kRound reads in flight, and are merged through shared memory in their order.
 template <int D>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kNarrowThreads)
 join_kernel(const Plan plan, const float* __restrict__ part_o, const float2* __restrict__ part_ml,
             __nv_bfloat16* __restrict__ out, int heads) {
-  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kRound = 4;
+  constexpr int kLanes = D / 4, kGroups = kNarrowThreads / kLanes, kRound = 4;
   let_next_kernel_start();
   const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
   const int first = plan.words[plan.first_at + b], end = plan.words[plan.first_at + b + 1];
@@ -426,7 +691,7 @@ int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_b
                                     dim3(kThreads), Smem<D>::kBytes, stream, 1, k_map, v_map, p);
     if (e) return e;
   }
-  return launch_overlapped(join_kernel<D>, dim3((unsigned)(p.sequences * p.heads)), dim3(kThreads), 0, stream, 1,
+  return launch_overlapped(join_kernel<D>, dim3((unsigned)(p.sequences * p.heads)), dim3(kNarrowThreads), 0, stream, 1,
                            p.plan, p.part_o, p.part_ml, out, p.heads);
 }
 
@@ -441,9 +706,9 @@ SAKV_EXPORT int sakv_shared_attention(const void* k_map, const void* v_map, cons
                                       int first_at, void* out, float* part_o, float* part_ml, int partials,
                                       int sequences, int heads, int kv_heads, int head_dim, float scale,
                                       cudaStream_t stream) {
-  if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kRows ||
+  if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kNarrowRows ||
       max_blocks <= 0 || max_blocks > (1 << 24) || unit_capacity < 0 || partials < 0 || (q_stride & 1) ||
-      (unit_at & 3) || (member_at & 1) || (reinterpret_cast<uintptr_t>(q) & 3) ||
+      (unit_at & 7) || (member_at & 1) || (reinterpret_cast<uintptr_t>(q) & 3) ||
       (reinterpret_cast<uintptr_t>(plan) & 15) || (long long)unit_capacity * kv_heads > 0x7fffffffLL ||
       (long long)sequences * heads > 0x7fffffffLL)
     return cudaErrorInvalidValue;

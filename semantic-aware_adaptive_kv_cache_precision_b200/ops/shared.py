@@ -11,7 +11,8 @@ from . import _lib
 from ._lib import CACHE_BLOCK, KernelError, call, on_device, ptr, require_cuda, sm_count
 from .attention import fast_path_takes, tensor_map
 
-UNIT_ROWS = 64            # most rows (sequences x query heads of one KV head) of a unit of work
+UNIT_ROWS = 128           # most rows (sequences x query heads of one KV head) of a unit of work
+MOST_GROUP = 64           # most query heads of one KV head
 UNIT_WORDS = 8
 
 
@@ -73,9 +74,8 @@ def common_runs(tables: np.ndarray, lengths: np.ndarray, reach: np.ndarray) -> l
 def choose_piece(runs: list, group: int, kv_heads: int, slots: int) -> int:
     """Into pieces of how many blocks the runs are cut: the fewest with which the units of work do not
     outnumber `slots`, the thread blocks that run at one time."""
-    per = max(1, UNIT_ROWS // group)
     sizes = np.array([c1 - c0 for _, c0, c1 in runs], dtype=np.int64)
-    tiles = np.array([-(-len(m) // per) for m, _, _ in runs], dtype=np.int64) * kv_heads
+    tiles = np.array([-(-len(m) * group // UNIT_ROWS) for m, _, _ in runs], dtype=np.int64) * kv_heads
     longest = int(sizes.max(initial=1))
     piece = max(1, int((sizes * tiles).sum()) // max(1, slots))
     while piece < longest and int((-(-sizes // piece) * tiles).sum()) > slots:
@@ -119,8 +119,8 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     reach = lengths if reach is None else np.asarray(reach, dtype=np.int64).reshape(-1)
     if tables.ndim != 2 or tables.shape[0] != len(lengths) or len(reach) != len(lengths):
         raise KernelError(f"plan_shared: block lists {tables.shape} for {len(lengths)} lengths, {len(reach)} reaches")
-    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or heads // kv_heads > UNIT_ROWS:
-        raise KernelError(f"plan_shared: {heads} heads over {kv_heads} (at most {UNIT_ROWS} a KV head)")
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or heads // kv_heads > MOST_GROUP:
+        raise KernelError(f"plan_shared: {heads} heads over {kv_heads} (at most {MOST_GROUP} a KV head)")
     count, width = tables.shape
     if count and (lengths.min() < 0 or (reach < lengths).any() or reach.max() > width * CACHE_BLOCK):
         raise KernelError(f"plan_shared: lengths and reaches must lie in [0, {width * CACHE_BLOCK}], reach >= length")
@@ -130,7 +130,6 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     group = heads // kv_heads
     runs = common_runs(tables, lengths, reach)
     piece = choose_piece(runs, group, kv_heads, slots or 2 * sm_count(device)) if runs else 1
-    per = max(1, UNIT_ROWS // group)
     pieces = []                                            # (members, first column, columns)
     for members, c0, c1 in runs:
         n = -(-(c1 - c0) // piece)
@@ -147,11 +146,11 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     first = np.concatenate([[0], np.cumsum(counts)])
     units, pairs = [], []
     for (members, c0, n), where in zip(pieces, place):
-        for i in range(0, len(members), per):
-            some = members[i:i + per]
-            units.append((some[0], c0, n, len(pairs), len(some), 0, 0, 0))
-            pairs += [(b, int(first[b]) + w) for b, w in zip(some, where[i:i + per])]
-    units.sort(key=lambda u: -u[2] * (1 + u[4] * group // 16))        # the heaviest start first
+        rows = len(members) * group
+        for r in range(0, rows, UNIT_ROWS):
+            units.append((members[0], c0, n, len(pairs) + r // group, r % group, min(UNIT_ROWS, rows - r), 0, 0))
+        pairs += [(b, int(first[b]) + w) for b, w in zip(members, where)]
+    units.sort(key=lambda u: -u[2] * (1 + u[5] // 16))                # the heaviest start first
     plan = SharedPlan()
     plan.sequences, plan.heads, plan.kv_heads, plan.width = count, heads, kv_heads, width
     plan.units, plan.reach = len(units), reach

@@ -46,19 +46,24 @@ def covered(plan, tables, reach):
     count, read = len(reach), []
     first = w[plan.first_at:plan.first_at + count + 1]
     seen, partials = [set() for _ in reach], set()
-    per = max(1, 64 // (plan.heads // plan.kv_heads))
+    group = plan.heads // plan.kv_heads
+    heads_of = {}
     assert w[0] == plan.units <= plan.unit_capacity and w[1] == count
     for unit in w[plan.unit_at:plan.unit_at + 8 * plan.units].reshape(-1, 8):
-        row, c0, n, begin, members = unit[:5]
-        assert n > 0 and 0 < members <= per
-        for b, p in w[plan.member_at + 2 * begin:plan.member_at + 2 * (begin + members)].reshape(-1, 2):
-            assert first[b] <= p < first[b + 1] <= plan.partials and p not in partials
-            partials.add(p)
-            for c in range(c0, c0 + n):
-                assert c not in seen[b] and tables[b, c] == tables[row, c]
-                seen[b].add(c)
+        row, c0, n, begin, first_row, rows = unit[:6]
+        assert n > 0 and 0 < rows <= 128 and 0 <= first_row < group
+        for r in range(first_row, first_row + rows):
+            b, p = w[plan.member_at + 2 * (begin + r // group):][:2]
+            assert first[b] <= p < first[b + 1] <= plan.partials
+            heads_of.setdefault((b, p), []).append(r % group)
+            if r % group == 0:
+                assert p not in partials
+                partials.add(p)
+                for c in range(c0, c0 + n):
+                    assert c not in seen[b] and tables[b, c] == tables[row, c]
+                    seen[b].add(c)
         read += [(row, c) for c in range(c0, c0 + n)]
-    assert len(partials) == first[-1]
+    assert len(partials) == first[-1] and all(sorted(h) == list(range(group)) for h in heads_of.values())
     assert all(s == set(range(-(-int(r) // BLOCK))) for s, r in zip(seen, reach))
     return read
 
@@ -81,7 +86,7 @@ def test_a_plan_reads_every_column_once(name, heads, kv_heads, slots):
     tables, lengths, blocks = lists_of(CASES[name])
     plan = ops.plan_shared(tables, lengths, heads, kv_heads, slots=slots)
     read = covered(plan, tables, lengths)
-    if heads == 8:                                   # (all sequences fit a unit: nothing is read twice)
+    if heads == 8:                                   # (all rows fit a unit: nothing is read twice)
         assert len({tables[r, c] for r, c in read}) == len(read) == len({b for b in tables.reshape(-1) if b >= 0})
     grown = np.minimum(lengths + 100, tables.shape[1] * BLOCK)
     for roomy in (False, True):
@@ -107,7 +112,7 @@ def test_a_last_block_that_is_not_filled_is_nobody_elses():
 def test_pieces_fill_the_slots():
     runs = [(tuple(range(64)), 0, 500)] + [((b,), 500, 508) for b in range(64)]
     piece = choose_piece(runs, 6, 2, 296)
-    units = sum(-(-(z - a) // piece) * -(-len(m) // 10) * 2 for m, a, z in runs)
+    units = sum(-(-(z - a) // piece) * -(-len(m) * 6 // 128) * 2 for m, a, z in runs)
     assert units <= 296 or piece == 500
 
 
