@@ -70,7 +70,6 @@ struct Params {
   int heads, kv_heads;
   float* part_o;                       // [partials][heads][D]
   float2* part_ml;                     // [partials][heads]: (maximum in base 2, sum)
-  int partials;
   float scale_log2e;
   int* error;
 };
@@ -697,28 +696,33 @@ int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_b
 
 }  // namespace
 
-// `plan`: int32 words on the device (see ops/shared.py for their order), of which `unit_capacity` units at
-// word `unit_at`, the members at `member_at` and the sequences' first partials at `first_at`; `partials`: how
-// many the scratch holds ([partials][heads][head_dim] and [partials][heads][2] floats).
+// A plan's numbers (ops/shared.py): width of the block lists, words where units, members and the sequences'
+// first partials begin, units, partials that the scratch holds.
+struct SakvSharedPlan {
+  int width, unit_at, unit_capacity, member_at, first_at, partials, sequences, heads, kv_heads;
+};
+
+// `plan`: int32 words on the device, laid out as the numbers `n` (on the host) say; `part`: scratch of
+// partials x heads x (head_dim + 2) floats.
 SAKV_EXPORT int sakv_shared_attention(const void* k_map, const void* v_map, const void* q, long long q_stride,
-                                      const int32_t* seq_lens, const int32_t* block_table, int max_blocks,
-                                      const int32_t* plan, int unit_at, int unit_capacity, int member_at,
-                                      int first_at, void* out, float* part_o, float* part_ml, int partials,
-                                      int sequences, int heads, int kv_heads, int head_dim, float scale,
+                                      const int32_t* seq_lens, const int32_t* block_table, const int32_t* plan,
+                                      const SakvSharedPlan* n, void* out, float* part, int head_dim, float scale,
                                       cudaStream_t stream) {
+  const int sequences = n->sequences, heads = n->heads, kv_heads = n->kv_heads, max_blocks = n->width;
   if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kNarrowRows ||
-      max_blocks <= 0 || max_blocks > (1 << 24) || unit_capacity < 0 || partials < 0 || (q_stride & 1) ||
-      (unit_at & 7) || (member_at & 1) || (reinterpret_cast<uintptr_t>(q) & 3) ||
-      (reinterpret_cast<uintptr_t>(plan) & 15) || (long long)unit_capacity * kv_heads > 0x7fffffffLL ||
-      (long long)sequences * heads > 0x7fffffffLL)
+      max_blocks <= 0 || max_blocks > (1 << 24) || n->unit_capacity < 0 || n->partials < 0 || (q_stride & 1) ||
+      (n->unit_at & 7) || (n->member_at & 1) || (reinterpret_cast<uintptr_t>(q) & 3) ||
+      (reinterpret_cast<uintptr_t>(plan) & 15) || (reinterpret_cast<uintptr_t>(part) & 15) ||
+      (long long)n->unit_capacity * kv_heads > 0x7fffffffLL || (long long)sequences * heads > 0x7fffffffLL)
     return cudaErrorInvalidValue;
   if (sequences == 0) return 0;
   Params p;
-  p.plan = Plan{plan, unit_at, member_at, first_at, unit_capacity};
+  p.plan = Plan{plan, n->unit_at, n->member_at, n->first_at, n->unit_capacity};
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.q_stride = q_stride;
   p.seq_lens = seq_lens; p.block_table = block_table; p.max_blocks = max_blocks; p.sequences = sequences;
   p.heads = heads; p.kv_heads = kv_heads;
-  p.part_o = part_o; p.part_ml = reinterpret_cast<float2*>(part_ml); p.partials = partials;
+  p.part_o = part;
+  p.part_ml = reinterpret_cast<float2*>(part + (long long)n->partials * heads * head_dim);
   p.scale_log2e = scale * 1.4426950408889634f;
   p.error = nullptr;
   if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p.error), g_error) != cudaSuccess) return cudaErrorInvalidValue;

@@ -7,13 +7,21 @@
 // target's column leaves z_target; `join_kernel` merges the pieces. 2,048 tokens over 151,936 logits would be
 // 1.2 GB written and read again; the pieces are 10 MB.
 //
-// Two ways to a piece. bfloat16 operands: tcgen05 on PAIRS of SMs (`cta_group::2`), a tile of 256 tokens x 256
-// rows of the head, the softmax's sums in the epilogue, thread = token row, so that no sum crosses a thread.
-//   warp 0     TMA: boxes of x [128 tokens x 64] and of the head [128 rows x 64] into a ring of six 32 KB
-//              stages (each block of the pair fetches its own half of both; no multicast),
+// Two ways to a piece. bfloat16 operands: tcgen05 on PAIRS of SMs (`cta_group::2`), the softmax's sums in the
+// epilogue. A pair takes a tile of the head's rows (up to 128 a block) against
+//   256 tokens   tokens on tensor memory's lanes, the head's rows its columns: thread = token row, so that no sum
+//                crosses a thread, or
+//   the rest     (up to 255 tokens, all of them where there are fewer than 256) the other way round, the head's
+//                rows on the lanes and the tokens, rounded up to 32, the columns: a few tokens do not pay for 256.
+//                32 columns are reduced over 32 lanes in 31 exchanges (each step hands half of what is left to the
+//                neighbour), and a warp keeps its running sums for the whole kernel.
+//   warp 0     TMA: boxes of x and of the head (64 wide) into a ring of stages (each block of the pair fetches
+//              its own half of both; no multicast),
 //   warp 1     tensor memory; in the pair's first block lane 0 issues the products,
 //   warps 2-5  epilogue of a tile under the products of the next (two accumulators of 256 columns).
-// Up to 256 tokens the head is read once and that bounds it; above, the tensor cores do.
+// Tiles of one piece of the head lie side by side in time, so the head comes from memory once. Up to some 256
+// tokens its bytes bound the kernel, above the tensor cores. The tile's height is chosen so that the last round
+// of tiles is not nearly empty (see the launcher).
 // float32 operands (and rows that TMA cannot take): `fold_kernel` reads a piece of logits that a product of
 // its own left in a scratch.
 //
@@ -26,16 +34,13 @@
 
 namespace {
 
-constexpr int BM = 128;                          // tokens per block
-constexpr int BN = 256;                          // rows of the head a tile
+constexpr int BM = 128;                          // rows of an operand that a block holds at most
 constexpr int BK = 64;
-constexpr int kStages = 6;
-constexpr int kXBytes = BM * BK * 2;
-constexpr int kWBytes = (BN / 2) * BK * 2;
-constexpr int kStageBytes = kXBytes + kWBytes;
+constexpr int kMaxStages = 12;
+constexpr int kWBytes = BM * BK * 2;             // room for the head's rows in a stage
+constexpr int kMaxTokens = 256;                  // tokens of a tile
 constexpr int kEpilogueThreads = 128;
 constexpr int kThreads = 64 + kEpilogueThreads;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint16_t kBoth = 3;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -45,7 +50,7 @@ struct Shape {
   const void* bias;          // or null
   int bias_bf16;
   float scale;
-  float cap, two_over_cap;   // 0: none; 2 log2(e) / cap
+  float cap, over_cap;       // 0: none; 1 / cap
 };
 
 __device__ __forceinline__ float bias_at(const Shape& f, int v) {
@@ -53,32 +58,71 @@ __device__ __forceinline__ float bias_at(const Shape& f, int v) {
                      : reinterpret_cast<const float*>(f.bias)[v];
 }
 
-// tanh(y) = 1 - 2 / (e^2y + 1): off by a few 2^-24 of 1, so z by a few 2^-24 of the cap
-template <bool kCap>
-__device__ __forceinline__ float shaped(const Shape& f, float z) {
-  z *= f.scale;
-  if (kCap) {
-    const float y = z * f.two_over_cap;          // (kept below 2^126, where the quotient is still one; NaN stays)
-    z = f.cap - __fdividef(2.f * f.cap, 1.f + mma::exp2_fast(y > 125.f ? 125.f : y));
-  }
-  return z;
+// c tanh(z / c). tanh(y) = 1 - 2 / (e^2y + 1), and below 1/4, where that difference would cancel, the series
+// y - y^3/3 + 2 y^5/15 - 17 y^7/315 + 62 y^9/2835 (the next term is below 2^-26 of y there).
+__device__ __forceinline__ float capped(const Shape& f, float z) {
+  const float y = z * f.over_cap;
+  const float q = y * y;
+  const float near = fmaf(y * q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y);
+  // (2 log2(e) y is kept below 2^7, where the quotient is still one; NaN stays)
+  const float e = y > 40.f ? 40.f : y;
+  const float far = 1.f - __fdividef(2.f, 1.f + mma::exp2_fast(e * (2.f * kLog2e)));
+  return f.cap * (q < 0.0625f ? near : far);
 }
 
 struct Params {
   int M, N, K;               // tokens, vocabulary, inner size
-  int m_tiles, n_tiles;
+  int full, rest, rest_cols; // tiles of 256 tokens; tokens behind them, and those rounded up to 32
+  int w_rows;                // rows of the head a block takes of a tile
+  int n_tiles;               // tiles of 2 w_rows rows of the head
+  int stages, stage_bytes;
   const int32_t* targets;
-  float2* part;              // [n_tiles][M]
+  float2* part;              // [n_tiles][256 full], then [4 blocks][rest]: (maximum, sum) in base 2
   float* mine;               // [M]: the targets' logits
   Shape form;
   int* error;
 };
 
 struct Barriers {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem;
 };
+
+// Behind the ring: barriers, a tile's biases twice, the rest's targets, and the warps' running sums of the rest.
+struct Tail {
+  Barriers bar;
+  alignas(16) float bias[2][2 * BM];
+  alignas(16) int32_t target[kMaxTokens];
+  float2 run[kEpilogueThreads / 32][kMaxTokens];
+};
+constexpr int kSmemMost = 232448;                // 227 KB
+constexpr int kRingMost = kSmemMost - 1024 - static_cast<int>(sizeof(Tail));
+
+// Which tile a pair takes in a round. (Shifted by one a round: with an even number of pairs and of token tiles
+// each pair would otherwise meet the same kind of tile every time.)
+struct Tiles {
+  int per, total;
+  __device__ explicit Tiles(const Params& p) : per(p.full + (p.rest > 0)), total(per * p.n_tiles) {}
+  __device__ int at(int round, int pair, int pairs) const { return round * pairs + (pair + round) % pairs; }
+};
+
+__device__ __forceinline__ void ld_32x32b_x32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
+      "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
 
 // 64 columns of a row joined to the row's running (maximum, sum) in base 2. `z` in natural units.
 __device__ __forceinline__ void take_up(const float (&z)[64], float& top, float& sum) {
@@ -103,22 +147,40 @@ __device__ __forceinline__ void take_up(const float (&z)[64], float& top, float&
   sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
 }
 
+// 32 values a lane reduced over the lanes: lane i gets the i-th's. Each step a lane keeps half of its values and
+// gets its neighbour's share of them.
+template <bool kMax>
+__device__ __forceinline__ float over_lanes(float (&v)[32], int lane) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const bool upper = lane & s;
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      const float keep = upper ? v[i + s] : v[i], give = upper ? v[i] : v[i + s];
+      const float got = __shfl_xor_sync(0xffffffffu, give, s);
+      v[i] = kMax ? fmaxf(keep, got) : keep + got;
+    }
+  }
+  return v[0];
+}
+
 // kPlain: no bias, no scale, no cap
 template <bool kPlain, bool kCap>
 __global__ void __launch_bounds__(kThreads, 1)
-logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
-               const __grid_constant__ Params p) {
+logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap rest_map,
+               const __grid_constant__ CUtensorMap w_map, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Barriers* bar = reinterpret_cast<Barriers*>(smem + kStages * kStageBytes);
+  Tail* tail = reinterpret_cast<Tail*>(smem + p.stages * p.stage_bytes);
+  Barriers* bar = &tail->bar;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = tma::cluster_rank();
+  const int rank = static_cast<int>(tma::cluster_rank());
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = p.m_tiles * p.n_tiles;
+  const Tiles tiles(p);
   const int n_kb = (p.K + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       tma::mbar_init(&bar->full[s], 1);
       tma::mbar_init(&bar->empty[s], 1);
     }
@@ -138,36 +200,41 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
   wait_for_previous_kernel();
 
   if (warp == 0) {
-    // ---- TMA: this block's tokens and its half of the tile's rows -----------------------------
+    // ---- TMA: this block's half of the tile's tokens and of its rows of the head -----------------
     if (lane == 0) {
-      tma::prefetch_map(&x_map);
       tma::prefetch_map(&w_map);
       int stage = 0, phase = 0;
       bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        const int m_tile = tile % p.m_tiles, n_tile = tile / p.m_tiles;     // token tiles fastest
-        const int x_row = (m_tile * 2 + static_cast<int>(rank)) * BM;
-        const int w_row = n_tile * BN + static_cast<int>(rank) * (BN / 2);
+      for (int round = 0; round * pairs < tiles.total && ok; ++round) {
+        const int tile = tiles.at(round, pair, pairs);
+        if (tile >= tiles.total) continue;
+        const int m_tile = tile % tiles.per, n_tile = tile / tiles.per;     // tokens fastest
+        const bool rest = m_tile == p.full;
+        const int x_rows = rest ? p.rest_cols / 2 : BM;
+        const int x_row = m_tile * kMaxTokens + rank * x_rows;
+        const int w_row = (2 * n_tile + rank) * p.w_rows;
+        const CUtensorMap* xm = rest ? &rest_map : &x_map;
+        const uint32_t bytes = 2 * (x_rows + p.w_rows) * BK * 2;
         for (int kb = 0; kb < n_kb; ++kb) {
           if (!tma::mbar_wait(&bar->empty[stage], phase ^ 1, p.error, 801)) {
             ok = false;
             break;
           }
-          uint8_t* dst = smem + stage * kStageBytes;
+          uint8_t* dst = smem + stage * p.stage_bytes;
           const uint32_t full = tma::cluster_address(tma::smem_u32(&bar->full[stage]), 0);
-          if (rank == 0) tma::mbar_expect_tx(&bar->full[stage], 2 * kStageBytes);
-          tma::load_2d_pair(dst, &x_map, kb * BK, x_row, full);
-          tma::load_2d_pair(dst + kXBytes, &w_map, kb * BK, w_row, full);
-          if (++stage == kStages) {
+          if (rank == 0) tma::mbar_expect_tx(&bar->full[stage], bytes);
+          tma::load_2d_pair(dst, &w_map, kb * BK, w_row, full);
+          tma::load_2d_pair(dst + kWBytes, xm, kb * BK, x_row, full);
+          if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
       // before this block may leave: every stage it filled has been given back
-      for (int s = 0; s < kStages && ok; ++s) {
+      for (int s = 0; s < p.stages && ok; ++s) {
         ok = tma::mbar_wait(&bar->empty[stage], phase ^ 1, p.error, 805);
-        if (++stage == kStages) {
+        if (++stage == p.stages) {
           stage = 0;
           phase ^= 1;
         }
@@ -176,83 +243,152 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
   } else if (warp == 1) {
     // ---- MMA issue: one lane of the pair's first block ----------------------------------------
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = tc::idesc_bf16_f32(2 * BM, BN);
-      int stage = 0, phase = 0, round = 0;
+      int stage = 0, phase = 0, count = 0;
       bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs, ++round) {
-        const int buf = round & 1;
-        if (round >= 2 && !tma::mbar_wait(&bar->acc_empty[buf], ((round >> 1) - 1) & 1, p.error, 802)) break;
+      for (int round = 0; round * pairs < tiles.total && ok; ++round) {
+        const int tile = tiles.at(round, pair, pairs);
+        if (tile >= tiles.total) continue;
+        const bool rest = tile % tiles.per == p.full;
+        const uint32_t idesc = tc::idesc_bf16_f32(2 * BM, rest ? p.rest_cols : 2 * p.w_rows);
+        const int buf = count & 1;
+        if (count >= 2 && !tma::mbar_wait(&bar->acc_empty[buf], ((count >> 1) - 1) & 1, p.error, 802)) break;
         for (int kb = 0; kb < n_kb && ok; ++kb) {
           if (!tma::mbar_wait(&bar->full[stage], phase, p.error, 803)) {
             ok = false;
             break;
           }
           tc::fence_after_sync();
-          const uint32_t a = tma::smem_u32(smem + stage * kStageBytes);
-          const uint32_t b = a + kXBytes;
+          const uint32_t w = tma::smem_u32(smem + stage * p.stage_bytes), x = w + kWBytes;
+          const uint32_t a = rest ? w : x, b = rest ? x : w;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            tc::mma_ss_pair(tmem + buf * BN, tc::smem_desc_k_major_sw128(a + k * 32),
+            tc::mma_ss_pair(tmem + buf * kMaxTokens, tc::smem_desc_k_major_sw128(a + k * 32),
                             tc::smem_desc_k_major_sw128(b + k * 32), idesc, kb > 0 || k > 0);
           tc::commit_pair(&bar->empty[stage], kBoth);
-          if (++stage == kStages) {
+          if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (ok) tc::commit_pair(&bar->acc_full[buf], kBoth);
+        ++count;
       }
     }
   } else {
-    // ---- epilogue: thread = token row -----------------------------------------------------------
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
+    // ---- epilogue -------------------------------------------------------------------------------
+    const int quarter = warp & 3, thread = quarter * 32 + lane;      // thread = lane of tensor memory
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    int round = 0;
+    const int first_rest = p.full * kMaxTokens;
+    float2* run = tail->run[quarter];
+    for (int c = thread; c < kMaxTokens; c += kEpilogueThreads)
+      tail->target[c] = c < p.rest ? p.targets[first_rest + c] : -1;
+    for (int c = lane; c < kMaxTokens; c += 32) run[c] = make_float2(-INFINITY, 0.f);
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
+    int count = 0, wide = 0;       // tiles so far, and those of 256 tokens among them
     bool ok = true;
-    for (int tile = pair; tile < tiles; tile += pairs, ++round) {
-      const int m_tile = tile % p.m_tiles, n_tile = tile / p.m_tiles;
-      const int buf = round & 1;
-      const int m = (m_tile * 2 + static_cast<int>(rank)) * BM + row;
-      const int target = m < p.M ? p.targets[m] : -1;
-      ok = ok && tma::mbar_wait(&bar->acc_full[buf], (round >> 1) & 1, p.error, 804);
-      tc::fence_after_sync();
-      const int n0 = n_tile * BN;
-      float top = -INFINITY, sum = 0.f;
-      // (a warp whose rows are all beyond the last token has nothing to read)
-      const bool any = (m_tile * 2 + static_cast<int>(rank)) * BM + quarter * 32 < p.M;
+    for (int round = 0; round * pairs < tiles.total; ++round) {
+      const int tile = tiles.at(round, pair, pairs);
+      if (tile >= tiles.total) continue;
+      const int m_tile = tile % tiles.per, n_tile = tile / tiles.per;
+      const int buf = count & 1;
+      const int n0 = n_tile * 2 * p.w_rows;
+      const uint32_t acc = lane_base + buf * kMaxTokens;
+      if (m_tile < p.full) {
+        // tokens on the lanes: this thread's row against 2 w_rows rows of the head
+        const int cols = 2 * p.w_rows;
+        const int m = m_tile * kMaxTokens + rank * BM + thread;
+        const int target = p.targets[m];
+        // (a warp that comes here has seen every other one behind the barrier of the wide tile before, and so
+        // done with the one before that, whose biases these replace)
+        const float* biases = tail->bias[wide & 1];
+        if (!kPlain && p.form.bias) {
+          for (int c = thread; c < cols; c += kEpilogueThreads)
+            tail->bias[wide & 1][c] = n0 + c < p.N ? bias_at(p.form, n0 + c) : 0.f;
+          asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
+        }
+        ++wide;
+        ok = ok && tma::mbar_wait(&bar->acc_full[buf], (count >> 1) & 1, p.error, 804);
+        tc::fence_after_sync();
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < BN && ok && any && n0 + c < p.N; c += 64) {
-        float z[64];
-        tc::ld_32x32b_x64(lane_base + buf * BN + c, z);
-        if (!kPlain) {
-          if (p.form.bias) {
+        for (int c = 0; c < cols && ok && n0 + c < p.N; c += 64) {
+          float z[64];
+          tc::ld_32x32b_x64(acc + c, z);
+          if (!kPlain) {
+            if (p.form.bias) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (n0 + c + i < p.N) z[i] += bias_at(p.form, n0 + c + i);
+              for (int i = 0; i < 64; i += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(biases + c + i);
+                z[i] += b.x; z[i + 1] += b.y; z[i + 2] += b.z; z[i + 3] += b.w;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+              z[i] *= p.form.scale;
+              if (kCap) z[i] = capped(p.form, z[i]);
+            }
           }
+          const int real = min(cols, p.N - n0) - c;         // columns of the 64 that are tokens' of this tile
+          if (real < 64) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) z[i] = shaped<kCap>(p.form, z[i]);
-        }
-        if (n0 + c + 64 > p.N) {
+            for (int i = 0; i < 64; ++i) z[i] = i < real ? z[i] : -INFINITY;
+          }
+          const int at = target - (n0 + c);
+          const bool here = at >= 0 && at < min(real, 64);
+          if (__any_sync(0xffffffffu, here)) {
+            float found = 0.f;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (n0 + c + i >= p.N) z[i] = -INFINITY;
+            for (int i = 0; i < 64; ++i) found = at == i ? z[i] : found;
+            if (here) p.mine[m] = found;
+          }
+          take_up(z, top, sum);
         }
-        const int at = target - (n0 + c);
-        if (__any_sync(0xffffffffu, at >= 0 && at < 64)) {
-          float found = 0.f;
+        if (ok) p.part[(long long)n_tile * first_rest + m] = make_float2(top, sum);
+      } else {
+        // rows of the head on the lanes: this thread's row against the rest of the tokens
+        const int v = n0 + rank * p.w_rows + thread;
+        const bool real = thread < p.w_rows && v < p.N;
+        const float bias = !kPlain && p.form.bias && real ? bias_at(p.form, v) : 0.f;
+        ok = ok && tma::mbar_wait(&bar->acc_full[buf], (count >> 1) & 1, p.error, 806);
+        tc::fence_after_sync();
+#pragma unroll 1
+        for (int c = 0; c < p.rest_cols && ok; c += 32) {
+          float z[32];
+          ld_32x32b_x32(acc + c, z);
 #pragma unroll
-          for (int i = 0; i < 64; ++i) found = at == i ? z[i] : found;
-          if (at >= 0 && at < 64 && target < p.N) p.mine[m] = found;
+          for (int i = 0; i < 32; i += 4) {
+            const int4 t = *reinterpret_cast<const int4*>(&tail->target[c + i]);
+            const int of[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (!kPlain) {
+                z[i + j] = (z[i + j] + bias) * p.form.scale;
+                if (kCap) z[i + j] = capped(p.form, z[i + j]);
+              }
+              if (of[j] == v && real) p.mine[first_rest + c + i + j] = z[i + j];
+              z[i + j] = real ? z[i + j] * kLog2e : -INFINITY;
+            }
+          }
+          float most[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) most[i] = z[i];
+          const float2 old = run[c + lane];
+          const float top = fmaxf(old.x, over_lanes<true>(most, lane));
+          const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] = mma::exp2_fast(z[i] - __shfl_sync(0xffffffffu, base, i));
+          const float sum = over_lanes<false>(z, lane);
+          run[c + lane] = make_float2(top, (old.y == 0.f ? 0.f : old.y * mma::exp2_fast(old.x - top)) + sum);
         }
-        take_up(z, top, sum);
       }
-      if (ok && m < p.M) p.part[(long long)n_tile * p.M + m] = make_float2(top, sum);
       tc::fence_before_sync();
       // (given back whatever happened: the issuing lane counts 256 arrivals a tile)
       tma::mbar_arrive_cluster(tma::cluster_address(tma::smem_u32(&bar->acc_empty[buf]), 0));
+      ++count;
     }
+    __syncwarp();
+    float2* part = p.part + (long long)p.n_tiles * first_rest + (long long)(blockIdx.x * 4 + quarter) * p.rest;
+    for (int c = lane; c < p.rest; c += 32) part[c] = run[c];
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -287,7 +423,7 @@ fold_kernel(const float* __restrict__ z, long long ld, int M, int n, int first, 
     if (c < end) {
       if (form.bias) v[i] += bias_at(form, first + c);
       v[i] *= form.scale;
-      if (form.cap > 0.f) v[i] = form.cap * tanhf(v[i] / form.cap);
+      if (form.cap > 0.f) v[i] = form.cap * tanhf(v[i] * form.over_cap);
       if (c == target) mine[m] = v[i];
     }
     top = fmaxf(top, v[i]);
@@ -310,25 +446,30 @@ fold_kernel(const float* __restrict__ z, long long ld, int M, int n, int first, 
   part[(long long)blockIdx.y * M + m] = make_float2(top * kLog2e, sum);
 }
 
-// lse and log-probability of every row from its `pieces` partials [pieces][M]. A block has 32 rows, a warp takes
-// every eighth piece of all of them (lane = row: neighbouring rows' partials are neighbours in memory).
-constexpr int kJoinWarps = 8;
+// lse and log-probability of every row from its partials: rows below `full` have `pieces` of them, [pieces][full],
+// the others `rest_pieces`, [rest_pieces][M - full] behind them. A block has 32 rows, all of one kind; a warp takes
+// every 16th piece of all of them (lane = row: neighbouring rows' partials are neighbours in memory).
+constexpr int kJoinWarps = 16;
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, const int32_t* __restrict__ targets,
-            float* __restrict__ logprob, float* __restrict__ lse, int M, int N, int pieces) {
+            float* __restrict__ logprob, float* __restrict__ lse, int M, int N, int full, int pieces,
+            int rest_pieces) {
   constexpr int kRound = 8;
   let_next_kernel_start();
   wait_for_previous_kernel();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m = blockIdx.x * 32 + lane;
+  const bool in_full = m < full;               // (full is a multiple of 256, or M)
+  const int width = in_full ? full : M - full, count = in_full ? pieces : rest_pieces;
+  const float2* mine_part = part + (in_full ? (long long)m : (long long)pieces * full + m - full);
   float top = -INFINITY, sum = 0.f;
   if (m < M)
-    for (int s0 = warp; s0 < pieces; s0 += kJoinWarps * kRound) {
+    for (int s0 = warp; s0 < count; s0 += kJoinWarps * kRound) {
       float2 v[kRound];
 #pragma unroll
       for (int i = 0; i < kRound; ++i) {
         const int s = s0 + i * kJoinWarps;
-        v[i] = s < pieces ? part[(long long)s * M + m] : make_float2(-INFINITY, 0.f);
+        v[i] = s < count ? mine_part[(long long)s * width] : make_float2(-INFINITY, 0.f);
       }
       float big = top;
 #pragma unroll
@@ -364,13 +505,13 @@ int resident_pairs() {
   if (known[device]) return known[device] - 1;
   int clusters = 0;
   auto allow = [](auto kernel) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost) == cudaSuccess;
   };
   if (allow(logprob_kernel<true, false>) && allow(logprob_kernel<false, false>) && allow(logprob_kernel<false, true>)) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * sm_count());
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kSmemBytes;
+    config.dynamicSmemBytes = kSmemMost;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -388,53 +529,96 @@ int resident_pairs() {
 Shape shape_of(const void* bias, int bias_bf16, float scale, float cap) {
   Shape f;
   f.bias = bias; f.bias_bf16 = bias_bf16; f.scale = scale; f.cap = cap;
-  f.two_over_cap = cap > 0.f ? 2.f * kLog2e / cap : 0.f;
+  f.over_cap = cap > 0.f ? 1.f / cap : 0.f;
   return f;
 }
 
 }  // namespace
 
-// Rows of the head a piece of the tensor-core kernel has, and columns a piece of the fold has.
-SAKV_EXPORT int sakv_logprob_tile() { return BN; }
+// Columns a piece of the fold has.
 SAKV_EXPORT int sakv_logprob_fold_columns() { return kFoldColumns; }
 // Pairs of SMs that can hold the tensor-core kernel at one time (0: it cannot run here).
 SAKV_EXPORT int sakv_logprob_resident() { return resident_pairs(); }
 
-// A TMA descriptor of a row-major bf16 matrix read in boxes of [128 rows, 64 columns].
-SAKV_EXPORT int sakv_logprob_map(void* map, const void* base, long long rows, long long cols, long long row_stride) {
-  if (rows <= 0 || cols <= 0 || rows > 0x7fffffffLL || (cols % 8) || (row_stride % 8) || row_stride < cols)
-    return cudaErrorInvalidValue;
-  return tma::make_map_bf16_2d(reinterpret_cast<CUtensorMap*>(map), base, (uint64_t)rows, (uint64_t)cols,
-                               (uint64_t)row_stride * 2, BM, BK);
+// How M tokens against N rows of the head are cut, for `pairs` pairs of SMs:
+// shape = {tiles of 256 tokens, rows of the head a block takes of a tile, tiles of the head, pairs launched}.
+// A block takes 128 rows of the head, or fewer where that makes the last round of tiles fuller. Fewer than 256
+// tokens: bound by the head's bytes, so any height serves, the one that gives every block the same number of
+// rows in all. More: bound by the products, whose width (two blocks' rows) is a multiple of 32; a tile costs its
+// width and some 8 rows' worth besides.
+SAKV_EXPORT int sakv_logprob_shape(int M, int N, int pairs, int* shape) {
+  if (M <= 0 || N <= 0 || pairs <= 0 || N > 0x7fffffff - 512 || M > 0x7fffffff - 512) return cudaErrorInvalidValue;
+  const int full = M / kMaxTokens, per = full + (M % kMaxTokens > 0);
+  int rows = BM;
+  if (full == 0) {
+    const int rounds = (N + 2 * BM * pairs - 1) / (2 * BM * pairs);
+    rows = (N + 2 * pairs * rounds - 1) / (2 * pairs * rounds);
+  } else {
+    long long best = -1;
+    for (int r = BM; r >= 96; r -= 16) {
+      const long long tiles = (N + 2 * r - 1) / (2 * r) * (long long)per;
+      const long long cost = (tiles + pairs - 1) / pairs * (r + 8);
+      if (best < 0 || cost < best) {
+        best = cost;
+        rows = r;
+      }
+    }
+  }
+  const long long n_tiles = (N + 2LL * rows - 1) / (2 * rows);
+  if (n_tiles * per > 0x3fffffffLL) return cudaErrorInvalidValue;
+  shape[0] = full;
+  shape[1] = rows;
+  shape[2] = (int)n_tiles;
+  shape[3] = n_tiles * per < pairs ? (int)(n_tiles * per) : pairs;
+  return 0;
 }
 
-// part [ceil(N / 256)][M] and mine [M] for x [M, K] and the head [N, K] in bf16, by their tensor maps.
-SAKV_EXPORT int sakv_logprob_pieces(const void* x_map, const void* w_map, int M, int N, int K,
-                                    const int32_t* targets, float* part, float* mine, const void* bias,
-                                    int bias_bf16, float scale, float cap, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0 || (K % 8) || N > 0x7fffffff - BN || M > 0x7fffffff - 2 * BM || !(cap >= 0.f))
+// A TMA descriptor of a row-major bf16 matrix read in boxes of [box_rows, 64 columns].
+static int logprob_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long row_stride,
+                       int box_rows) {
+  if (rows <= 0 || cols <= 0 || rows > 0x7fffffffLL || (cols % 8) || (row_stride % 8) || row_stride < cols)
     return cudaErrorInvalidValue;
+  return tma::make_map_bf16_2d(map, base, (uint64_t)rows, (uint64_t)cols, (uint64_t)row_stride * 2,
+                               (uint32_t)box_rows, BK);
+}
+
+// The partials of x [M, K] against the head [N, K] in bf16 (rows of x `x_stride` apart; 16-byte aligned), cut as
+// `shape` (sakv_logprob_shape) says: part [shape[2]][256 shape[0]] and, behind it, [8 shape[3]][M - 256 shape[0]].
+SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const void* head, int M, int N, int K,
+                                    const int* shape, const int32_t* targets, float* part, float* mine,
+                                    const void* bias, int bias_bf16, float scale, float cap, cudaStream_t stream) {
+  int expect[4];
   const int here = resident_pairs();
+  if (K <= 0 || (K % 8) || !(cap >= 0.f)) return cudaErrorInvalidValue;
   if (here <= 0) return cudaErrorNotSupported;
+  const int bad = sakv_logprob_shape(M, N, here, expect);
+  if (bad) return bad;
+  for (int i = 0; i < 4; ++i)
+    if (shape[i] != expect[i]) return cudaErrorInvalidValue;
   Params p;
   p.M = M; p.N = N; p.K = K;
-  p.m_tiles = (M + 2 * BM - 1) / (2 * BM);
-  p.n_tiles = (N + BN - 1) / BN;
-  if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffLL - here) return cudaErrorInvalidValue;
+  p.full = shape[0]; p.w_rows = shape[1]; p.n_tiles = shape[2];
+  p.rest = M - p.full * kMaxTokens;
+  p.rest_cols = (p.rest + 31) / 32 * 32;
+  const int x_rows = p.full ? BM : p.rest_cols / 2;
+  p.stage_bytes = kWBytes + x_rows * BK * 2;
+  p.stages = kRingMost / p.stage_bytes < kMaxStages ? kRingMost / p.stage_bytes : kMaxStages;
   p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;
   p.form = shape_of(bias, bias_bf16, scale, cap);
   p.error = nullptr;
   if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p.error), g_error) != cudaSuccess) return cudaErrorInvalidValue;
-  const int tiles = p.m_tiles * p.n_tiles;
-  const dim3 grid(2 * (tiles < here ? tiles : here));
-  const CUtensorMap& xm = *reinterpret_cast<const CUtensorMap*>(x_map);
-  const CUtensorMap& wm = *reinterpret_cast<const CUtensorMap*>(w_map);
+  CUtensorMap x_map, rest_map, w_map;
+  int e = logprob_map(&w_map, head, N, K, K, p.w_rows);
+  if (!e) e = logprob_map(&x_map, x, M, K, x_stride, p.full ? BM : p.rest_cols / 2);
+  if (!e && p.full && p.rest) e = logprob_map(&rest_map, x, M, K, x_stride, p.rest_cols / 2);
+  else rest_map = x_map;
+  if (e) return e;
   auto kernel = cap > 0.f ? logprob_kernel<false, true>
                           : bias || scale != 1.f ? logprob_kernel<false, false> : logprob_kernel<true, false>;
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
+  config.gridDim = dim3(2 * shape[3]);
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = kSmemBytes;
+  config.dynamicSmemBytes = p.stages * p.stage_bytes + 1024 + sizeof(Tail);
   config.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -445,8 +629,8 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x_map, const void* w_map, int M,
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
   config.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, xm, wm, p);
-  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+  const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, x_map, rest_map, w_map, p);
+  return launched != cudaSuccess ? static_cast<int>(launched) : launch_status();
 }
 
 // The same partials of a piece of logits in memory: z [M, n], columns `first`, first + 1, ... of the vocabulary;
@@ -462,11 +646,15 @@ SAKV_EXPORT int sakv_logprob_fold(const float* z, long long ld, int M, int n, in
                         reinterpret_cast<float2*>(part), mine, shape_of(bias, bias_bf16, scale, cap));
 }
 
+// The join of `pieces` partials of rows below `full` and `rest_pieces` of the others (full: a multiple of 256, or M).
 SAKV_EXPORT int sakv_logprob_join(const float* part, const float* mine, const int32_t* targets, float* logprob,
-                                  float* lse, int M, int N, int pieces, cudaStream_t stream) {
-  if (M <= 0 || pieces < 0) return cudaErrorInvalidValue;
+                                  float* lse, int M, int N, int full, int pieces, int rest_pieces,
+                                  cudaStream_t stream) {
+  if (M <= 0 || pieces < 0 || rest_pieces < 0 || full < 0 || full > M || (full % 32 && full != M))
+    return cudaErrorInvalidValue;
   return launch_overlapped(join_kernel, dim3((M + 31) / 32), dim3(32 * kJoinWarps), 0, stream, 1,
-                           reinterpret_cast<const float2*>(part), mine, targets, logprob, lse, M, N, pieces);
+                           reinterpret_cast<const float2*>(part), mine, targets, logprob, lse, M, N, full, pieces,
+                           rest_pieces);
 }
 
 SAKV_EXPORT int sakv_logprob_error(int* value) {

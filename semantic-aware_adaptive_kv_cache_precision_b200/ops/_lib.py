@@ -99,10 +99,10 @@ SIGNATURES = {
     "sakv_gemm_wide": ("gemm_wide", [P, P, I, I, I, I, P, L, P]),
     "sakv_gemm_pair": ("gemm_pair", [P, P, I, I, I, I, P, L, I, F, F, F, P]),
     "sakv_copy_blocks": ("copy_blocks", [P, I, P, I, P]),
-    "sakv_shared_attention": ("attention_shared", [P, P, P, L, P, P, I, P, I, I, I, I, P, P, P, I, I, I, I, I, F, P]),
-    "sakv_logprob_pieces": ("logprobs", [P, P, I, I, I, P, P, P, P, I, F, F, P]),
+    "sakv_shared_attention": ("attention_shared", [P, P, P, L, P, P, P, P, P, P, I, F, P]),
+    "sakv_logprob_pieces": ("logprobs", [P, L, P, I, I, I, P, P, P, P, P, I, F, F, P]),
     "sakv_logprob_fold": ("logprobs", [P, L, I, I, I, I, P, P, P, P, I, F, F, P]),
-    "sakv_logprob_join": ("logprobs", [P, P, P, P, P, I, I, I, P]),
+    "sakv_logprob_join": ("logprobs", [P, P, P, P, P, I, I, I, I, I, P]),
     "sakv_lib_accumulate": ("gemm_lib", [P, L, P, P, L, I, I, I, P, L, P]),
 }
 
@@ -115,10 +115,9 @@ PLAIN_SIGNATURES = {
     "sakv_decode_attention_map": ("attention_decode", [P, P, L, I, I]),
     "sakv_decode_attention_error": ("attention_decode", [P]),
     "sakv_decode_attention_max_cluster": ("attention_decode", [I]),
-    "sakv_logprob_tile": ("logprobs", []),
+    "sakv_logprob_shape": ("logprobs", [I, I, I, P]),
     "sakv_logprob_fold_columns": ("logprobs", []),
     "sakv_logprob_resident": ("logprobs", []),
-    "sakv_logprob_map": ("logprobs", [P, P, L, L, L]),
     "sakv_logprob_error": ("logprobs", [P]),
     "sakv_shared_attention_error": ("attention_shared", [P]),
     "sakv_prefill_attention_error": ("attention_prefill", [P]),

@@ -3,9 +3,10 @@ pages belong to one sequence and are never copied (`src/core_kernels/kv_pages.cu
 
 from __future__ import annotations
 
+import array
 import ctypes
+import math
 
-import numpy as np
 import torch
 
 from ._lib import KernelError, call, on_device, require_cuda
@@ -22,7 +23,7 @@ def _span(t: torch.Tensor) -> tuple:
 
 
 def _ids(ids, size: int, what: str) -> list:
-    ids = [int(i) for i in ids]
+    ids = list(map(int, ids))
     if ids and (min(ids) < 0 or max(ids) >= size):
         raise KernelError(f"copy_blocks: {what} must lie in [0, {size}), got [{min(ids)}, {max(ids)}]")
     return ids
@@ -42,58 +43,82 @@ def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: 
     targets = tensors if into is None else list(into)
     if len(targets) != len(tensors):
         raise KernelError(f"copy_blocks: {len(tensors)} tensors into {len(targets)}")
-    if axis not in (0, 1):
+    if axis != 0 and axis != 1:
         raise KernelError(f"copy_blocks: axis must be 0 or 1, got {axis}")
     if not tensors:
         return
     table = (_Tensor * len(tensors))()
-    blocks, room = tensors[0].shape[axis] if tensors[0].dim() > axis else 0, None
+    device = tensors[0].get_device()
+    known, blocks, room, empty = None, -1, -1, False
+    spans = []
     for i, (t, u) in enumerate(zip(tensors, targets)):
-        if t.dim() <= axis or t.dim() != u.dim() or t.dtype != u.dtype or t.device != u.device \
-                or t.device != tensors[0].device or not t.is_contiguous() or not u.is_contiguous() \
-                or t.shape[:axis] != u.shape[:axis] or t.shape[axis + 1:] != u.shape[axis + 1:]:
-            raise KernelError(f"copy_blocks: {tuple(t.shape)} {t.dtype} into {tuple(u.shape)} {u.dtype}: contiguous "
-                              "tensors on one device, alike but for the number of blocks")
-        if t.shape[axis] != blocks or (room is not None and u.shape[axis] != room):
-            raise KernelError("copy_blocks: the tensors must have the same number of blocks")
-        room = u.shape[axis]
-        if rows is not None and (axis != 1 or t.dim() != 5 or not 0 < rows <= t.shape[3]):
-            raise KernelError(f"copy_blocks: rows = {rows} of {tuple(t.shape)}")
-        size = t.element_size()
-        entry = t.numel() // t.shape[0] * size if axis else 0       # (0 where there are no entries)
-        block = size
-        for n in t.shape[axis + 1:]:
-            block *= n
-        chunks, chunk, pitch = 1, block, block
-        if rows is not None and rows < t.shape[3]:
-            chunks, pitch = t.shape[2], t.shape[3] * t.shape[4] * size
-            chunk = pitch // t.shape[3] * rows
-        table[i] = _Tensor(t.data_ptr(), u.data_ptr(), entry, u.shape[1] * block if axis else 0, block,
-                           t.shape[0] if axis else 1, chunks, chunk, pitch)
+        shape = t.shape
+        alike = (shape, t.dtype, None if u is t else u.shape)
+        if alike != known:                 # (the keys' pool and the values' are mostly alike)
+            known = alike
+            geometry, blocks, room = _geometry(t, u, rows, axis, blocks, room)
+            empty = empty or t.numel() == 0
+        if not t.is_contiguous() or t.get_device() != device or u is not t and (
+                not u.is_contiguous() or u.get_device() != device or u.dtype != t.dtype):
+            raise KernelError(f"copy_blocks: {tuple(shape)} {t.dtype} into {tuple(u.shape)} {u.dtype}: contiguous "
+                              "tensors of one type on one device")
+        a, z = t.data_ptr(), u.data_ptr()
+        table[i] = (a, z) + geometry
+        spans.append((z, z + (geometry[1] or room * geometry[2]) * geometry[3]))
     src, dst = _ids(src, blocks, "sources"), _ids(dst, room, "targets")
-    if len(src) != len(dst):
-        raise KernelError(f"copy_blocks: {len(src)} sources, {len(dst)} targets")
-    if len(set(dst)) != len(dst):
+    count = len(src)
+    if count != len(dst):
+        raise KernelError(f"copy_blocks: {count} sources, {len(dst)} targets")
+    if len(set(dst)) != count:
         raise KernelError("copy_blocks: a target is named twice")
     if into is None:
         if not set(dst).isdisjoint(src):
             raise KernelError("copy_blocks: a target is a source too")
-        if _overlap([_span(t) for t in tensors]):
+        if _overlap(spans):
             raise KernelError("copy_blocks: tensors overlap")
-    elif _overlap([_span(t) for t in targets], [_span(t) for t in tensors]):
+    elif _overlap(spans, [_span(t) for t in tensors]):
         raise KernelError("copy_blocks: a target tensor overlaps another one")
-    require_cuda(*tensors, *targets)
-    if not src or any(t.numel() == 0 for t in tensors):
+    if device < 0:
+        require_cuda(*tensors)
+    if not count or empty:
         return
-    pairs = np.empty((len(src), 2), dtype=np.int32)
-    pairs[:, 0], pairs[:, 1] = src, dst
+    pairs = array.array("i", bytes(8 * count))
+    pairs[0::2], pairs[1::2] = array.array("i", src), array.array("i", dst)
     with on_device(tensors[0]):
-        call("sakv_copy_blocks", ctypes.addressof(table), len(tensors), pairs.ctypes.data, len(src))
+        call("sakv_copy_blocks", ctypes.addressof(table), len(tensors), pairs.buffer_info()[0], count)
+
+
+def _geometry(t, u, rows, axis, blocks, room) -> tuple:
+    """((bytes from entry to entry here and there, bytes of a block, entries, chunks, bytes copied of a chunk,
+    bytes from chunk to chunk), blocks here, blocks there) of tensors alike."""
+    shape, there = t.shape, u.shape
+    if len(shape) <= axis or len(shape) != len(there) or shape[:axis] != there[:axis] \
+            or shape[axis + 1:] != there[axis + 1:]:
+        raise KernelError(f"copy_blocks: {tuple(shape)} into {tuple(there)}: alike but for the number of blocks")
+    if blocks >= 0 and (shape[axis], there[axis]) != (blocks, room):
+        raise KernelError("copy_blocks: the tensors must have the same number of blocks")
+    if rows is not None and (axis != 1 or len(shape) != 5 or not 0 < rows <= shape[3]):
+        raise KernelError(f"copy_blocks: rows = {rows} of {tuple(shape)}")
+    block = t.element_size() * math.prod(shape[axis + 1:])
+    chunks, chunk, pitch = 1, block, block
+    if rows is not None and rows < shape[3]:
+        chunks, pitch = shape[2], block // max(1, shape[2])
+        chunk = pitch // shape[3] * rows
+    entry = (shape[1] * block, there[1] * block) if axis else (0, 0)       # (0: no entries)
+    return entry + (block, shape[0] if axis else 1, chunks, chunk, pitch), shape[axis], there[axis]
 
 
 def _overlap(spans: list, others: list = ()) -> bool:
     """Whether two of `spans` have bytes in common, or one of them with one of `others`."""
-    ordered = sorted(s for s in spans if s[0] < s[1])
-    if any(a[1] > b[0] for a, b in zip(ordered, ordered[1:])):
-        return True
-    return any(a[0] < b[1] and b[0] < a[1] for a in ordered for b in others if b[0] < b[1])
+    ordered = sorted(spans)
+    end = 0
+    for a, z in ordered:
+        if a < z:
+            if a < end:
+                return True
+            end = z
+    for a, z in others:
+        for b, y in ordered:
+            if a < z and b < y and a < y and b < z:
+                return True
+    return False

@@ -15,8 +15,15 @@ from .linear import linear
 PIECE_ELEMENTS = 8 << 20
 
 
-def _map(t: torch.Tensor):
-    return gemm_wide._make_map(t, "sakv_logprob_map")
+_resident: dict = {}
+
+
+def _pairs() -> int:
+    """Pairs of SMs that hold the tensor-core kernel at one time (74 on a B200; 0: not here)."""
+    device = torch.cuda.current_device()
+    if device not in _resident:
+        _resident[device] = int(plain_function("sakv_logprob_resident")())
+    return _resident[device]
 
 
 def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, bias: torch.Tensor | None = None,
@@ -45,17 +52,19 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
         raise KernelError("token_logprobs: tensors on different devices")
     require_cuda(x, head, targets, bias)
     with on_device(x):
-        logprob = torch.empty(rows, dtype=torch.float32, device=x.device)
-        lse, mine = torch.empty_like(logprob), torch.empty_like(logprob)
+        logprob = x.new_empty(rows, dtype=torch.float32)
+        lse, mine = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
         if rows == 0:
             return logprob, lse
         form = (ptr(bias), bias_code, float(scale), float(softcap))
-        if gemm_wide.takes(x, head) and plain_function("sakv_logprob_resident")() > 0:
-            pieces = -(-vocab // plain_function("sakv_logprob_tile")())
-            part = torch.empty((pieces, rows, 2), dtype=torch.float32, device=x.device)
-            x_raw, x_map = _map(x)
-            w_raw, w_map = _map(head)
-            call("sakv_logprob_pieces", x_map, w_map, rows, vocab, k, ptr(targets), ptr(part), ptr(mine), *form)
+        if gemm_wide.takes(x, head) and _pairs() > 0:
+            shape = (ctypes.c_int * 4)()
+            if plain_function("sakv_logprob_shape")(rows, vocab, _pairs(), shape) != 0:
+                raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
+            full, pieces, rest_pieces = shape[0] * 256, shape[2], 8 * shape[3]
+            part = x.new_empty(2 * (pieces * full + rest_pieces * (rows - full)), dtype=torch.float32)
+            call("sakv_logprob_pieces", ptr(x), x.stride(0), ptr(head), rows, vocab, k, shape, ptr(targets),
+                 ptr(part), ptr(mine), *form)
         else:
             columns = plain_function("sakv_logprob_fold_columns")()
             most = max(1, PIECE_ELEMENTS // columns)
@@ -64,11 +73,12 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
                                         softcap=softcap) for i in range(0, rows, most)]
                 return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
             piece = max(1, min(-(-vocab // columns), PIECE_ELEMENTS // (rows * columns))) * columns
-            pieces = -(-vocab // columns)
+            full, pieces, rest_pieces = rows, -(-vocab // columns), 0
             part = torch.empty((pieces, rows, 2), dtype=torch.float32, device=x.device)
             for first in range(0, vocab, piece):
                 z = linear(x, head[first:first + piece], out_dtype=torch.float32)
                 call("sakv_logprob_fold", ptr(z), z.stride(0), rows, z.shape[1], first, vocab, ptr(targets),
                      ptr(part[first // columns]), ptr(mine), *form)
-        call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, pieces)
+        call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, full, pieces,
+             rest_pieces)
     return logprob, lse

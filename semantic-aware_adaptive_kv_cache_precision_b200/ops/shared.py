@@ -4,11 +4,13 @@ end, and serves every layer of every step until the next such change."""
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import CACHE_BLOCK, KernelError, call, on_device, ptr, require_cuda, sm_count
+from ._lib import CACHE_BLOCK, KernelError, call, on_device, require_cuda, sm_count
 from .attention import fast_path_takes, tensor_map
 
 UNIT_ROWS = 128           # most rows (sequences x query heads of one KV head) of a unit of work
@@ -83,12 +85,18 @@ def choose_piece(runs: list, group: int, kv_heads: int, slots: int) -> int:
     return min(piece, longest)
 
 
+class _Numbers(ctypes.Structure):
+    """A plan's numbers as the launch takes them."""
+    _fields_ = [(name, ctypes.c_int) for name in ("width", "unit_at", "unit_capacity", "member_at", "first_at",
+                                                  "partials", "sequences", "heads", "kv_heads")]
+
+
 class SharedPlan:
     """Which pieces of the block lists are read for which sequences: int32 words on the device, and their
     layout. Right for every step until `lengths` pass `reach` or the sharing changes."""
 
     __slots__ = ("words", "sequences", "heads", "kv_heads", "units", "unit_at", "unit_capacity", "member_at",
-                 "first_at", "partials", "reach", "width", "saved")
+                 "first_at", "partials", "reach", "width", "saved", "numbers")
 
     @property
     def layout(self) -> tuple:
@@ -162,6 +170,7 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     plan.first_at = plan.member_at + 2 * members_room
     plan.saved = int(sum((len(m) - 1) * (c1 - c0) for m, c0, c1 in runs))
     words = np.zeros(_round_up(plan.first_at + count + 1, 4), dtype=np.int32)
+    plan.numbers = _Numbers(*(getattr(plan, name) for name, _ in _Numbers._fields_))
     words[0], words[1] = len(units), count
     if units:
         words[8:8 + UNIT_WORDS * len(units)] = np.asarray(units, dtype=np.int32).reshape(-1)
@@ -178,6 +187,38 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     head sizes 64 and 128, no window; `qkv`'s rows begin with the rotated queries, the newest key and value
     are in the cache), reading a block that `plan` found in several sequences' lists once for all of them.
     `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros."""
+    q_shape, k_shape, device = qkv.shape, k_cache.shape, qkv.get_device()
+    # (one expression for the calls that are right: a decode step outside a captured graph is bound by the
+    # host's work; `_refuse` says what is wrong with the others)
+    if not (qkv.dtype is torch.bfloat16 and (head_dim == 128 or head_dim == 64) and heads % kv_heads == 0
+            and heads <= 16 * kv_heads and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
+            and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
+            and k_shape == v_cache.shape and len(k_shape) == 4 and k_shape[1] == kv_heads
+            and k_shape[2] == CACHE_BLOCK and k_shape[3] == head_dim
+            and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32
+            and seq_lens.dim() == 1 and block_table.dim() == 2
+            and seq_lens.shape[0] == q_shape[0] and block_table.shape[0] == q_shape[0]
+            and block_table.shape[1] == plan.width and seq_lens.is_contiguous() and block_table.is_contiguous()
+            and plan.sequences == q_shape[0] and plan.heads == heads and plan.kv_heads == kv_heads
+            and device >= 0 and device == k_cache.get_device() == v_cache.get_device() == seq_lens.get_device()
+            == block_table.get_device() == plan.words.get_device()):
+        _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim)
+    sequences = q_shape[0]
+    out = qkv.new_empty((sequences, heads * head_dim))
+    if sequences == 0:
+        return out
+    part = qkv.new_empty(plan.partials * heads * (head_dim + 2), dtype=torch.float32)
+    with on_device(qkv):
+        call("sakv_shared_attention", tensor_map(k_cache), tensor_map(v_cache), qkv.data_ptr(), qkv.stride(0),
+             seq_lens.data_ptr(), block_table.data_ptr(), plan.words.data_ptr(), ctypes.addressof(plan.numbers), out.data_ptr(),
+             part.data_ptr(), head_dim, scale)
+    if plan.unit_capacity:
+        _lib.launches += 1          # the call launched the join too
+    return out
+
+
+def _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim) -> None:
+    """Says what is wrong with a call of `shared_decode_attention`."""
     if not fast_path_takes(qkv.dtype, heads, kv_heads, head_dim):
         raise KernelError("shared_decode_attention: sizes not taken; use the plain kernel")
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < heads * head_dim or qkv.stride(0) % 2 \
@@ -195,19 +236,5 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if (plan.sequences, plan.heads, plan.kv_heads) != (sequences, heads, kv_heads):
         raise KernelError(f"shared_decode_attention: the plan is for {plan.sequences} sequences, {plan.heads} heads "
                           f"over {plan.kv_heads}")
-    require_cuda(qkv, k_cache, v_cache, seq_lens, block_table)
-    if any(t.device != qkv.device for t in (k_cache, v_cache, seq_lens, block_table, plan.words)):
-        raise KernelError("shared_decode_attention: tensors on different devices")
-    out = torch.empty((sequences, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
-    if sequences == 0:
-        return out
-    part = torch.empty(plan.partials * heads * (head_dim + 2), dtype=torch.float32, device=qkv.device)
-    with on_device(qkv):
-        call("sakv_shared_attention", tensor_map(k_cache), tensor_map(v_cache), ptr(qkv), qkv.stride(0),
-             ptr(seq_lens), ptr(block_table), block_table.shape[1], ptr(plan.words), plan.unit_at,
-             plan.unit_capacity, plan.member_at, plan.first_at, ptr(out), ptr(part),
-             part.data_ptr() + 4 * plan.partials * heads * head_dim, plan.partials, sequences, heads, kv_heads,
-             head_dim, float(scale))
-    if plan.unit_capacity:
-        _lib.launches += 1          # the call launched the join too
-    return out
+    require_cuda(qkv, k_cache, v_cache, seq_lens, block_table, plan.words)
+    raise KernelError("shared_decode_attention: tensors on different devices")

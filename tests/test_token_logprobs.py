@@ -59,7 +59,8 @@ def check(rows, k, vocab, dtype, bias=None, scale=1.0, softcap=0.0, seed=0, x_pa
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows, k, vocab", [(1, 8, 1), (1, 64, 255), (5, 96, 256), (31, 72, 257), (127, 128, 1000),
-                                            (129, 192, 4095), (256, 64, 4097), (257, 200, 8193), (600, 256, 70001)])
+                                            (129, 192, 4095), (256, 64, 4097), (257, 200, 8193), (600, 256, 70001), (255, 64, 3000), (333, 136, 20000),
+                                            (511, 64, 128), (40, 1024, 40000)])
 def test_against_float64(dtype, rows, k, vocab):
     check(rows, k, vocab, dtype)
 
@@ -71,6 +72,27 @@ def test_against_float64(dtype, rows, k, vocab):
 def test_bias_scale_and_cap(dtype, bias, scale, softcap):
     check(70, 104, 1333, dtype, bias, scale, softcap)
     check(3, 104, 1333, dtype, bias, scale, softcap, spread=40.0)
+
+
+@pytest.mark.parametrize("pairs", [1, 7, 74])
+def test_tiles_cover_the_vocabulary(pairs):
+    """Host code of the launcher: every row of the head in one tile, tiles no higher than a block's rows, and no
+    more pairs than tiles. (Needs nvcc, not a GPU.)"""
+    import ctypes
+    from semantic_aware_adaptive_kv_cache_precision_b200.ops._lib import plain_function
+    shape = (ctypes.c_int * 4)()
+    for rows in (1, 31, 255, 256, 257, 333, 2047, 2048):
+        for vocab in (1, 2, 300, 4097, 50257, 151936):
+            assert plain_function("sakv_logprob_shape")(rows, vocab, pairs, shape) == 0
+            full, height, tiles, launched = shape
+            per = full + (rows % 256 > 0)
+            assert full == rows // 256 and 1 <= height <= 128 and (not full or height % 16 == 0)
+            assert (tiles - 1) * 2 * height < vocab <= tiles * 2 * height
+            assert launched == min(pairs, tiles * per)
+            if not full:                      # every block has the same number of rows in all, but for the last ones
+                assert -(-tiles // launched) * 2 * height * launched - vocab < 2 * launched * -(-tiles // launched)
+    for bad in ((0, 5, 1), (5, 0, 1), (5, 5, 0), (2 ** 31 - 1, 5, 1)):
+        assert plain_function("sakv_logprob_shape")(*bad, shape) != 0
 
 
 @pytest.mark.gpu
@@ -134,10 +156,12 @@ def test_no_rows_rows_alone_streams_and_graphs():
     x, w, targets, got, lse = check(300, 128, 3001, torch.bfloat16, seed=9)
     none, none_lse = ops.token_logprobs(x[:0], w, targets[:0])
     assert none.shape == none_lse.shape == (0,)
-    # a row's sums do not depend on the rows beside it
+    # in 32 bits a row's sums do not depend on the rows beside it
+    wide, head = x.float(), w.float()
+    whole, _ = ops.token_logprobs(wide, head, targets)
     for i in (0, 130, 299):
-        alone, _ = ops.token_logprobs(x[i:i + 1], w, targets[i:i + 1])
-        assert torch.equal(alone, got[i:i + 1])
+        alone, _ = ops.token_logprobs(wide[i:i + 1], head, targets[i:i + 1])
+        assert torch.equal(alone, whole[i:i + 1])
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
