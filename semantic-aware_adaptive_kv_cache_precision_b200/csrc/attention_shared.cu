@@ -14,7 +14,7 @@
 //   wide   (more than kNarrowRows rows, up to 128) on tcgen05: S = Q K^T with the rows on tensor memory's lanes,
 //          one thread a row for the softmax, P written over S as the A operand of P V, O in tensor memory; the
 //          next tile's S is computed under this tile's softmax.
-//   narrow (up to kNarrowRows rows) on mma.sync: NR = groups of 16 rows (1, 2 or 4); warp w of four takes rows
+//   narrow (up to kNarrowRows rows) on mma.sync: NR = groups of 16 rows (1 or 2); warp w of four takes rows
 //          16 (w % NR) .. + 15 and 16 NR keys of every tile from 16 NR (w / NR) on, so that four warps have
 //          work however few the rows; warps of the same rows are merged at the end.
 //
@@ -35,7 +35,9 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 192;        // 6 warps; four of them in a narrow unit and in the join
 constexpr int kNarrowThreads = kWarps * 32;
 constexpr int kStages = 3;           // of a narrow unit
-constexpr int kWideRows = 128, kNarrowRows = 64;
+// Rows up to which a unit is narrow. Measured, us of the kernel over 32,000 shared positions, two KV heads of 6
+// query heads: 12 rows 11.5 narrow; 24 rows 14.3 narrow, 14.1 wide; 60 rows 20.2 narrow, 14.1 wide.
+constexpr int kWideRows = 128, kNarrowRows = 32, kMostGroup = 64;
 constexpr int kWideStages = 2;
 constexpr int kMembers = kWideRows + 2;
 constexpr uint32_t kTmemCols = 256;  // wide: S 2 x 64 (P over the first 32 of each), O from 128 on
@@ -64,6 +66,7 @@ struct Params {
   Plan plan;
   const __nv_bfloat16* q;
   long long q_stride;
+  int q_aligned;                       // whether its rows begin at multiples of 16 bytes
   const int32_t* seq_lens;
   const int32_t* block_table;
   int max_blocks, sequences;
@@ -408,15 +411,32 @@ attend_wide(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     Row row{nullptr, 0};
     if (r < u.rows) row = row_at(p, member, u, g, r, D);
-    // this thread's query into the swizzled tile (zeros for rows that the unit does not have)
+    // this warp's 32 queries into the swizzled tile, 16 bytes a lane, neighbouring lanes along a row (zeros for
+    // rows that the unit does not have). A row a thread, 4 bytes at a time, took 5 to 8 us.
+    {
+      constexpr int kLanes = D / 8, kPer = 32 / kLanes;          // lanes of a row, rows at a time
+      const int c = lane % kLanes;
+      uint4 v[32 / kPer];
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row.q) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(row.q + c * 8);      // (rows begin at 4 bytes)
-        v = make_uint4(src[0], src[1], src[2], src[3]);
+      for (int i = 0; i < 32 / kPer; ++i) {
+        const int of = i * kPer + lane / kLanes;
+        const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row.q), of);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (at) {
+          const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(at) + c * 8;
+          if (p.q_aligned) {
+            v[i] = *reinterpret_cast<const uint4*>(src);
+          } else {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
+            v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
       }
-      *reinterpret_cast<uint4*>(q_s + (c >> 3) * (kWideRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+      for (int i = 0; i < 32 / kPer; ++i) {
+        const int of = quarter * 32 + i * kPer + lane / kLanes;
+        *reinterpret_cast<uint4*>(q_s + (c >> 3) * (kWideRows * 128) + of * 128 + (((c & 7) ^ (of & 7)) << 4)) = v[i];
+      }
     }
     tma::fence_proxy_async();
     tma::mbar_arrive(&bar->q_full);
@@ -496,18 +516,29 @@ attend_wide(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
     }
     if (ok && tma::mbar_wait(&bar->pv_done, (n - 1) & 1, p.error, 173)) {
       tc::fence_after_sync();
-      float* po = p.part_o + row.slot * D;
+      // through shared memory (every copy has landed and every product is done), so that a warp writes whole
+      // rows: a row a thread took 3 us
+      constexpr int kRow = D + 4;          // (padded: neighbouring rows' pieces lie in other banks)
+      float* mine = reinterpret_cast<float*>(smem) + quarter * 32 * kRow;
 #pragma unroll
       for (int c = 0; c < D; c += 16) {
         float v[16];
         tc::ld_32x32b_x16(lane_base + kOCol + c, v);
-        if (row.q) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(po + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        }
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(mine + lane * kRow + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       }
       if (row.q) p.part_ml[row.slot] = make_float2(m_ref, l);
+      __syncwarp();
+      constexpr int kLanes = D / 4, kPer = 32 / kLanes;
+      const int c = lane % kLanes * 4;
+#pragma unroll 8
+      for (int i = 0; i < 32; i += kPer) {
+        const int of = i + lane / kLanes;
+        const long long slot = __shfl_sync(0xffffffffu, row.slot, of);
+        if (quarter * 32 + of < u.rows)
+          *reinterpret_cast<float4*>(p.part_o + slot * D + c) = *reinterpret_cast<const float4*>(mine + of * kRow + c);
+      }
     }
   }
 }
@@ -527,16 +558,21 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   __shared__ int failed;
   __shared__ uint32_t tmem_at;
 
+  // First of all, and in narrow units too: until a block has given up its right to tensor memory, the SM starts no
+  // second block of a kernel that may ask for it (measured: the second ones started 8 to 15 us late).
+  if ((threadIdx.x >> 5) == 1) tc::tmem_alloc(&tmem_at, kTmemCols);
   // (the plan, the block lists and the lengths are the step's inputs: they were written before the kernel
   // before this one began; what that one wrote, queries, keys and values, is read behind the wait)
   const int unit = blockIdx.x / p.kv_heads, g = blockIdx.x - unit * p.kv_heads;
   const int group = p.heads / p.kv_heads;
-  const bool live = unit < min(p.plan.words[0], p.plan.unit_capacity);
+  // (the grid is as large as the plan has room for; a unit behind its last one reads words of no meaning, and
+  // nothing with them)
+  const int4* words = reinterpret_cast<const int4*>(p.plan.words + p.plan.unit_at + unit * 8);
+  const int4 a = words[0], b = words[1];
+  const bool live = unit < p.plan.words[0];
   Unit u{};
   int n_tiles = 0, kv_len = 0;
   if (live) {
-    const int4* words = reinterpret_cast<const int4*>(p.plan.words + p.plan.unit_at + unit * 8);
-    const int4 a = words[0], b = words[1];
     u = Unit{a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
     const int given = p.seq_lens[u.sequence];
     kv_len = given < 0 || given > p.max_blocks * KT ? 0 : given;
@@ -572,35 +608,29 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     }
     tma::fence_barrier_init();
   }
-  if (is_wide && (threadIdx.x >> 5) == 1) tc::tmem_alloc(&tmem_at, kTmemCols);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   let_next_kernel_start();       // (with its shared and tensor memory in hand)
   wait_for_previous_kernel();
-  if (!live) return;
   if (n_tiles <= 0) {            // a piece that the sequence has not reached yet: it counts for nothing
     for (int r = threadIdx.x; r < u.rows; r += kThreads)
       p.part_ml[row_at(p, member, u, g, r, D).slot] = make_float2(-INFINITY, 0.f);
-    return;
-  }
-  if (is_wide) {
+  } else if (is_wide) {
     attend_wide<D>(p, &k_map, &v_map, smem, wide, tmem_at, listed, g, u, n_tiles, kv_len, member);
-    tc::fence_before_sync();
-    __syncthreads();
-    if ((threadIdx.x >> 5) == 1) {
-      tc::fence_after_sync();
-      tc::tmem_dealloc(tmem_at, kTmemCols);
-    }
-    return;
-  }
-  if (threadIdx.x >= kNarrowThreads) return;
+  } else if (threadIdx.x < kNarrowThreads) {
 #define SAKV_NARROW(NR) \
   attend_narrow<D, NR>(p, &k_map, &v_map, smem, full, empty, &failed, listed, g, u, n_tiles, kv_len, member)
-  if (u.rows <= 16) SAKV_NARROW(1);
-  else if (u.rows <= 32) SAKV_NARROW(2);
-  else SAKV_NARROW(4);
+    if (u.rows <= 16) SAKV_NARROW(1);
+    else SAKV_NARROW(2);
 #undef SAKV_NARROW
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if ((threadIdx.x >> 5) == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem_at, kTmemCols);
+  }
 }
 
 // out[b, h] = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m), over the sequence's partials. A block a
@@ -709,7 +739,7 @@ SAKV_EXPORT int sakv_shared_attention(const void* k_map, const void* v_map, cons
                                       const SakvSharedPlan* n, void* out, float* part, int head_dim, float scale,
                                       cudaStream_t stream) {
   const int sequences = n->sequences, heads = n->heads, kv_heads = n->kv_heads, max_blocks = n->width;
-  if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kNarrowRows ||
+  if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kMostGroup ||
       max_blocks <= 0 || max_blocks > (1 << 24) || n->unit_capacity < 0 || n->partials < 0 || (q_stride & 1) ||
       (n->unit_at & 7) || (n->member_at & 1) || (reinterpret_cast<uintptr_t>(q) & 3) ||
       (reinterpret_cast<uintptr_t>(plan) & 15) || (reinterpret_cast<uintptr_t>(part) & 15) ||
@@ -719,6 +749,7 @@ SAKV_EXPORT int sakv_shared_attention(const void* k_map, const void* v_map, cons
   Params p;
   p.plan = Plan{plan, n->unit_at, n->member_at, n->first_at, n->unit_capacity};
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.q_stride = q_stride;
+  p.q_aligned = q_stride % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   p.seq_lens = seq_lens; p.block_table = block_table; p.max_blocks = max_blocks; p.sequences = sequences;
   p.heads = heads; p.kv_heads = kv_heads;
   p.part_o = part;
