@@ -11,10 +11,12 @@
 // epilogue. A pair takes a tile of the head's rows (up to 128 a block) against
 //   256 tokens   tokens on tensor memory's lanes, the head's rows its columns: thread = token row, so that no sum
 //                crosses a thread, or
-//   the rest     (up to 255 tokens, all of them where there are fewer than 256) the other way round, the head's
-//                rows on the lanes and the tokens, rounded up to 32, the columns: a few tokens do not pay for 256.
-//                32 columns are reduced over 32 lanes in 31 exchanges (each step hands half of what is left to the
-//                neighbour), and a warp keeps its running sums for the whole kernel.
+//   a rest       of up to 96 tokens the other way round, the head's rows on the lanes and the tokens, rounded up to
+//                32, the columns: a few tokens do not pay for 256. 32 columns are reduced over 32 lanes in 31
+//                exchanges (each step hands half of what is left to the neighbour), and a warp keeps its running
+//                sums for the whole kernel, or
+//   both         257 to 384 tokens: what comes of the head into shared memory serves both products (what L2 gives
+//                an SM bounds tiles of this size), at the price of one accumulator instead of two.
 //   warp 0     TMA: boxes of x and of the head (64 wide) into a ring of stages (each block of the pair fetches
 //              its own half of both; no multicast),
 //   warp 1     tensor memory; in the pair's first block lane 0 issues the products,
@@ -38,7 +40,18 @@ constexpr int BM = 128;                          // rows of an operand that a bl
 constexpr int BK = 64;
 constexpr int kMaxStages = 12;
 constexpr int kWBytes = BM * BK * 2;             // room for the head's rows in a stage
+constexpr int kXBytes = BM * BK * 2;
 constexpr int kMaxTokens = 256;                  // tokens of a tile
+// Tokens behind the last 256 up to which they are a rest; more are a tile of 256 that is not full. Measured
+// (us, rest / tile of 256; the sums over lanes cost the rest more where K is small): 97 tokens alone, vocabulary
+// x K 151936 x 1536 95 / 98, 50257 x 2048 62 / 52, 50257 x 768 35 / 33, 152064 x 3584 200 / 215; 129 100 / 100,
+// 54 / 52, 37 / 33, 232 / 218; 65 behind 512 tokens 291 / 263, 110 / 114, 52 / 51, 560 / 599; 140 behind them
+// 280 / 268, 118 / 116, 60 / 51, 658 / 645.
+constexpr int kRestMost = 96;
+// Tokens behind 256 up to which one tile takes both. Measured likewise (both / two tiles of 256): 32 170 / 178,
+// 70 / 84, 39 / 40, 375 / 394; 77 172 / 177, 76 / 84, 44 / 41, 380 / 394; 128 180 / 181, 79 / 85, 46 / 41, 367 /
+// 408; 160 189 / 182, 83 / 86, 49 / 41, 435 / 409.
+constexpr int kBothMost = 128;
 constexpr int kEpilogueThreads = 128;
 constexpr int kThreads = 64 + kEpilogueThreads;
 constexpr uint32_t kTmemCols = 512;
@@ -73,11 +86,12 @@ __device__ __forceinline__ float capped(const Shape& f, float z) {
 struct Params {
   int M, N, K;               // tokens, vocabulary, inner size
   int full, rest, rest_cols; // tiles of 256 tokens; tokens behind them, and those rounded up to 32
+  int both;                  // one tile takes 256 tokens AND the rest (full is 1)
   int w_rows;                // rows of the head a block takes of a tile
   int n_tiles;               // tiles of 2 w_rows rows of the head
   int stages, stage_bytes;
   const int32_t* targets;
-  float2* part;              // [n_tiles][256 full], then [4 blocks][rest]: (maximum, sum) in base 2
+  float2* part;              // [n_tiles][256 full], then [blocks][rest]: (maximum, sum) in base 2
   float* mine;               // [M]: the targets' logits
   Shape form;
   int* error;
@@ -103,7 +117,8 @@ constexpr int kRingMost = kSmemMost - 1024 - static_cast<int>(sizeof(Tail));
 // each pair would otherwise meet the same kind of tile every time.)
 struct Tiles {
   int per, total;
-  __device__ explicit Tiles(const Params& p) : per(p.full + (p.rest > 0)), total(per * p.n_tiles) {}
+  __device__ explicit Tiles(const Params& p)
+      : per(p.both ? 1 : p.full + (p.rest > 0)), total(per * p.n_tiles) {}
   __device__ int at(int round, int pair, int pairs) const { return round * pairs + (pair + round) % pairs; }
 };
 
@@ -209,12 +224,12 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         const int tile = tiles.at(round, pair, pairs);
         if (tile >= tiles.total) continue;
         const int m_tile = tile % tiles.per, n_tile = tile / tiles.per;     // tokens fastest
-        const bool rest = m_tile == p.full;
-        const int x_rows = rest ? p.rest_cols / 2 : BM;
-        const int x_row = m_tile * kMaxTokens + rank * x_rows;
+        const bool wide = m_tile < p.full, rest = !wide || p.both;
         const int w_row = (2 * n_tile + rank) * p.w_rows;
-        const CUtensorMap* xm = rest ? &rest_map : &x_map;
-        const uint32_t bytes = 2 * (x_rows + p.w_rows) * BK * 2;
+        const int x_row = m_tile * kMaxTokens + rank * BM;
+        const int rest_row = p.full * kMaxTokens + rank * (p.rest_cols / 2);
+        const int rest_at = kWBytes + (wide ? kXBytes : 0);
+        const uint32_t bytes = 2 * (p.w_rows + (wide ? BM : 0) + (rest ? p.rest_cols / 2 : 0)) * BK * 2;
         for (int kb = 0; kb < n_kb; ++kb) {
           if (!tma::mbar_wait(&bar->empty[stage], phase ^ 1, p.error, 801)) {
             ok = false;
@@ -224,7 +239,8 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           const uint32_t full = tma::cluster_address(tma::smem_u32(&bar->full[stage]), 0);
           if (rank == 0) tma::mbar_expect_tx(&bar->full[stage], bytes);
           tma::load_2d_pair(dst, &w_map, kb * BK, w_row, full);
-          tma::load_2d_pair(dst + kWBytes, xm, kb * BK, x_row, full);
+          if (wide) tma::load_2d_pair(dst + kWBytes, &x_map, kb * BK, x_row, full);
+          if (rest) tma::load_2d_pair(dst + rest_at, &rest_map, kb * BK, rest_row, full);
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
@@ -248,10 +264,13 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       for (int round = 0; round * pairs < tiles.total && ok; ++round) {
         const int tile = tiles.at(round, pair, pairs);
         if (tile >= tiles.total) continue;
-        const bool rest = tile % tiles.per == p.full;
-        const uint32_t idesc = tc::idesc_bf16_f32(2 * BM, rest ? p.rest_cols : 2 * p.w_rows);
-        const int buf = count & 1;
-        if (count >= 2 && !tma::mbar_wait(&bar->acc_empty[buf], ((count >> 1) - 1) & 1, p.error, 802)) break;
+        const bool wide = tile % tiles.per < p.full, rest = !wide || p.both;
+        const uint32_t wide_desc = tc::idesc_bf16_f32(2 * BM, 2 * p.w_rows);
+        const uint32_t rest_desc = tc::idesc_bf16_f32(2 * BM, p.rest_cols);
+        // (both: 256 tokens in the first half of tensor memory, the rest in the second, one tile at a time)
+        const int buf = p.both ? 0 : count & 1, use = p.both ? count : count >> 1;
+        const uint32_t wide_acc = tmem + buf * kMaxTokens, rest_acc = tmem + (p.both ? 1 : buf) * kMaxTokens;
+        if (use >= 1 && !tma::mbar_wait(&bar->acc_empty[buf], (use - 1) & 1, p.error, 802)) break;
         for (int kb = 0; kb < n_kb && ok; ++kb) {
           if (!tma::mbar_wait(&bar->full[stage], phase, p.error, 803)) {
             ok = false;
@@ -259,11 +278,19 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           }
           tc::fence_after_sync();
           const uint32_t w = tma::smem_u32(smem + stage * p.stage_bytes), x = w + kWBytes;
-          const uint32_t a = rest ? w : x, b = rest ? x : w;
+          const uint32_t xr = x + (wide ? kXBytes : 0);
+          if (wide) {
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            tc::mma_ss_pair(tmem + buf * kMaxTokens, tc::smem_desc_k_major_sw128(a + k * 32),
-                            tc::smem_desc_k_major_sw128(b + k * 32), idesc, kb > 0 || k > 0);
+            for (int k = 0; k < BK / 16; ++k)
+              tc::mma_ss_pair(wide_acc, tc::smem_desc_k_major_sw128(x + k * 32),
+                              tc::smem_desc_k_major_sw128(w + k * 32), wide_desc, kb > 0 || k > 0);
+          }
+          if (rest) {
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              tc::mma_ss_pair(rest_acc, tc::smem_desc_k_major_sw128(w + k * 32),
+                              tc::smem_desc_k_major_sw128(xr + k * 32), rest_desc, kb > 0 || k > 0);
+          }
           tc::commit_pair(&bar->empty[stage], kBoth);
           if (++stage == p.stages) {
             stage = 0;
@@ -290,14 +317,13 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       const int tile = tiles.at(round, pair, pairs);
       if (tile >= tiles.total) continue;
       const int m_tile = tile % tiles.per, n_tile = tile / tiles.per;
-      const int buf = count & 1;
+      const int buf = p.both ? 0 : count & 1, use = p.both ? count : count >> 1;
       const int n0 = n_tile * 2 * p.w_rows;
-      const uint32_t acc = lane_base + buf * kMaxTokens;
       if (m_tile < p.full) {
         // tokens on the lanes: this thread's row against 2 w_rows rows of the head
         const int cols = 2 * p.w_rows;
         const int m = m_tile * kMaxTokens + rank * BM + thread;
-        const int target = p.targets[m];
+        const int target = m < p.M ? p.targets[m] : -1;
         // (a warp that comes here has seen every other one behind the barrier of the wide tile before, and so
         // done with the one before that, whose biases these replace)
         const float* biases = tail->bias[wide & 1];
@@ -307,8 +333,9 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
         }
         ++wide;
-        ok = ok && tma::mbar_wait(&bar->acc_full[buf], (count >> 1) & 1, p.error, 804);
+        ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 804);
         tc::fence_after_sync();
+        const uint32_t acc = lane_base + buf * kMaxTokens;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
         for (int c = 0; c < cols && ok && n0 + c < p.N; c += 64) {
@@ -339,18 +366,22 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
             float found = 0.f;
 #pragma unroll
             for (int i = 0; i < 64; ++i) found = at == i ? z[i] : found;
-            if (here) p.mine[m] = found;
+            if (here) p.mine[m] = found;       // (a row behind the last token has no target)
           }
           take_up(z, top, sum);
         }
-        if (ok) p.part[(long long)n_tile * first_rest + m] = make_float2(top, sum);
-      } else {
+        if (ok && m < p.M) p.part[(long long)n_tile * first_rest + m] = make_float2(top, sum);
+      }
+      if (m_tile == p.full || p.both) {
         // rows of the head on the lanes: this thread's row against the rest of the tokens
         const int v = n0 + rank * p.w_rows + thread;
         const bool real = thread < p.w_rows && v < p.N;
         const float bias = !kPlain && p.form.bias && real ? bias_at(p.form, v) : 0.f;
-        ok = ok && tma::mbar_wait(&bar->acc_full[buf], (count >> 1) & 1, p.error, 806);
-        tc::fence_after_sync();
+        if (!p.both) {             // (else it has been waited for)
+          ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 806);
+          tc::fence_after_sync();
+        }
+        const uint32_t acc = lane_base + (p.both ? 1 : buf) * kMaxTokens;
 #pragma unroll 1
         for (int c = 0; c < p.rest_cols && ok; c += 32) {
           float z[32];
@@ -386,9 +417,20 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       tma::mbar_arrive_cluster(tma::cluster_address(tma::smem_u32(&bar->acc_empty[buf]), 0));
       ++count;
     }
-    __syncwarp();
-    float2* part = p.part + (long long)p.n_tiles * first_rest + (long long)(blockIdx.x * 4 + quarter) * p.rest;
-    for (int c = lane; c < p.rest; c += 32) part[c] = run[c];
+    // the warps' sums of the rest, joined
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
+    float2* part = p.part + (long long)p.n_tiles * first_rest + (long long)blockIdx.x * p.rest;
+    for (int c = thread; c < p.rest; c += kEpilogueThreads) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kEpilogueThreads / 32; ++w) top = fmaxf(top, tail->run[w][c].x);
+#pragma unroll
+      for (int w = 0; w < kEpilogueThreads / 32; ++w) {
+        const float2 v = tail->run[w][c];
+        sum += v.y == 0.f ? 0.f : v.y * mma::exp2_fast(v.x - top);
+      }
+      part[c] = make_float2(top, sum);
+    }
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -459,7 +501,7 @@ join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, con
   wait_for_previous_kernel();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m = blockIdx.x * 32 + lane;
-  const bool in_full = m < full;               // (full is a multiple of 256, or M)
+  const bool in_full = m < full;               // (full is a multiple of 256, past M where the last tile is not, or M)
   const int width = in_full ? full : M - full, count = in_full ? pieces : rest_pieces;
   const float2* mine_part = part + (in_full ? (long long)m : (long long)pieces * full + m - full);
   float top = -INFINITY, sum = 0.f;
@@ -526,6 +568,9 @@ int resident_pairs() {
   return clusters;
 }
 
+// Whether one tile takes the 256 tokens and the rest of M tokens.
+bool both_of(int M, int full) { return full == 1 && M > kMaxTokens; }
+
 Shape shape_of(const void* bias, int bias_bf16, float scale, float cap) {
   Shape f;
   f.bias = bias; f.bias_bf16 = bias_bf16; f.scale = scale; f.cap = cap;
@@ -542,22 +587,25 @@ SAKV_EXPORT int sakv_logprob_resident() { return resident_pairs(); }
 
 // How M tokens against N rows of the head are cut, for `pairs` pairs of SMs:
 // shape = {tiles of 256 tokens, rows of the head a block takes of a tile, tiles of the head, pairs launched}.
-// A block takes 128 rows of the head, or fewer where that makes the last round of tiles fuller. Fewer than 256
-// tokens: bound by the head's bytes, so any height serves, the one that gives every block the same number of
-// rows in all. More: bound by the products, whose width (two blocks' rows) is a multiple of 32; a tile costs its
-// width and some 8 rows' worth besides.
+// A block takes 128 rows of the head, or fewer where that makes the last round of tiles fuller. A few tokens: bound
+// by the head's bytes, so any height serves, the one that gives every block the same number of rows in all. More:
+// the height is a multiple of 16 (the products' width, two blocks' rows, is one of 32), and a round of tiles costs
+// what its operands' rows take from L2.
 SAKV_EXPORT int sakv_logprob_shape(int M, int N, int pairs, int* shape) {
   if (M <= 0 || N <= 0 || pairs <= 0 || N > 0x7fffffff - 512 || M > 0x7fffffff - 512) return cudaErrorInvalidValue;
-  const int full = M / kMaxTokens, per = full + (M % kMaxTokens > 0);
+  const int most = M > kMaxTokens && M < 2 * kMaxTokens ? kBothMost : kRestMost;
+  const int full = M / kMaxTokens + (M % kMaxTokens > most ? 1 : 0);
+  const int per = both_of(M, full) ? 1 : full + (M > full * kMaxTokens);
   int rows = BM;
   if (full == 0) {
     const int rounds = (N + 2 * BM * pairs - 1) / (2 * BM * pairs);
     rows = (N + 2 * pairs * rounds - 1) / (2 * pairs * rounds);
   } else {
+    const int beside = both_of(M, full) ? (M - kMaxTokens + 31) / 32 * 16 : 0;
     long long best = -1;
     for (int r = BM; r >= 96; r -= 16) {
       const long long tiles = (N + 2 * r - 1) / (2 * r) * (long long)per;
-      const long long cost = (tiles + pairs - 1) / pairs * (r + 8);
+      const long long cost = (tiles + pairs - 1) / pairs * (r + BM + beside);
       if (best < 0 || cost < best) {
         best = cost;
         rows = r;
@@ -583,7 +631,7 @@ static int logprob_map(CUtensorMap* map, const void* base, long long rows, long 
 }
 
 // The partials of x [M, K] against the head [N, K] in bf16 (rows of x `x_stride` apart; 16-byte aligned), cut as
-// `shape` (sakv_logprob_shape) says: part [shape[2]][256 shape[0]] and, behind it, [8 shape[3]][M - 256 shape[0]].
+// `shape` (sakv_logprob_shape) says: part [shape[2]][256 shape[0]] and, behind it, [2 shape[3]][M - 256 shape[0]].
 SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const void* head, int M, int N, int K,
                                     const int* shape, const int32_t* targets, float* part, float* mine,
                                     const void* bias, int bias_bf16, float scale, float cap, cudaStream_t stream) {
@@ -598,10 +646,10 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const voi
   Params p;
   p.M = M; p.N = N; p.K = K;
   p.full = shape[0]; p.w_rows = shape[1]; p.n_tiles = shape[2];
-  p.rest = M - p.full * kMaxTokens;
+  p.rest = M > p.full * kMaxTokens ? M - p.full * kMaxTokens : 0;
   p.rest_cols = (p.rest + 31) / 32 * 32;
-  const int x_rows = p.full ? BM : p.rest_cols / 2;
-  p.stage_bytes = kWBytes + x_rows * BK * 2;
+  p.both = both_of(M, p.full);
+  p.stage_bytes = kWBytes + (p.full ? kXBytes : 0) + (p.full == 0 || p.both ? p.rest_cols / 2 * BK * 2 : 0);
   p.stages = kRingMost / p.stage_bytes < kMaxStages ? kRingMost / p.stage_bytes : kMaxStages;
   p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;
   p.form = shape_of(bias, bias_bf16, scale, cap);
@@ -646,12 +694,12 @@ SAKV_EXPORT int sakv_logprob_fold(const float* z, long long ld, int M, int n, in
                         reinterpret_cast<float2*>(part), mine, shape_of(bias, bias_bf16, scale, cap));
 }
 
-// The join of `pieces` partials of rows below `full` and `rest_pieces` of the others (full: a multiple of 256, or M).
+// The join of `pieces` partials [pieces][full] of rows below `full` and `rest_pieces` [.][M - full] of the others, which
+// lie behind them (full: a multiple of 256, perhaps past M, or M).
 SAKV_EXPORT int sakv_logprob_join(const float* part, const float* mine, const int32_t* targets, float* logprob,
                                   float* lse, int M, int N, int full, int pieces, int rest_pieces,
                                   cudaStream_t stream) {
-  if (M <= 0 || pieces < 0 || rest_pieces < 0 || full < 0 || full > M || (full % 32 && full != M))
-    return cudaErrorInvalidValue;
+  if (M <= 0 || pieces < 0 || rest_pieces < 0 || full < 0 || (full % 32 && full != M)) return cudaErrorInvalidValue;
   return launch_overlapped(join_kernel, dim3((M + 31) / 32), dim3(32 * kJoinWarps), 0, stream, 1,
                            reinterpret_cast<const float2*>(part), mine, targets, logprob, lse, M, N, full, pieces,
                            rest_pieces);

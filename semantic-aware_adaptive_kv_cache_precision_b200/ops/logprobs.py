@@ -61,8 +61,8 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
             shape = (ctypes.c_int * 4)()
             if plain_function("sakv_logprob_shape")(rows, vocab, _pairs(), shape) != 0:
                 raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
-            full, pieces, rest_pieces = shape[0] * 256, shape[2], 8 * shape[3]
-            part = x.new_empty(2 * (pieces * full + rest_pieces * (rows - full)), dtype=torch.float32)
+            full, pieces, rest_pieces = shape[0] * 256, shape[2], 2 * shape[3]
+            part = x.new_empty(2 * (pieces * full + rest_pieces * max(0, rows - full)), dtype=torch.float32)
             call("sakv_logprob_pieces", ptr(x), x.stride(0), ptr(head), rows, vocab, k, shape, ptr(targets),
                  ptr(part), ptr(mine), *form)
         else:

@@ -60,7 +60,8 @@ def check(rows, k, vocab, dtype, bias=None, scale=1.0, softcap=0.0, seed=0, x_pa
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows, k, vocab", [(1, 8, 1), (1, 64, 255), (5, 96, 256), (31, 72, 257), (127, 128, 1000),
                                             (129, 192, 4095), (256, 64, 4097), (257, 200, 8193), (600, 256, 70001), (255, 64, 3000), (333, 136, 20000),
-                                            (511, 64, 128), (40, 1024, 40000)])
+                                            (511, 64, 128), (40, 1024, 40000), (96, 64, 5000), (97, 64, 5000),
+                                            (384, 72, 5000), (385, 72, 5000), (608, 64, 5000), (609, 64, 5000)])
 def test_against_float64(dtype, rows, k, vocab):
     check(rows, k, vocab, dtype)
 
@@ -70,7 +71,8 @@ def test_against_float64(dtype, rows, k, vocab):
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("scale, softcap", [(1.0, 0.0), (0.25, 0.0), (1.0, 5.0), (-0.5, 30.0)])
 def test_bias_scale_and_cap(dtype, bias, scale, softcap):
-    check(70, 104, 1333, dtype, bias, scale, softcap)
+    for rows in (70, 130, 300, 700):
+        check(rows, 104, 1333, dtype, bias, scale, softcap)
     check(3, 104, 1333, dtype, bias, scale, softcap, spread=40.0)
 
 
@@ -81,12 +83,13 @@ def test_tiles_cover_the_vocabulary(pairs):
     import ctypes
     from semantic_aware_adaptive_kv_cache_precision_b200.ops._lib import plain_function
     shape = (ctypes.c_int * 4)()
-    for rows in (1, 31, 255, 256, 257, 333, 2047, 2048):
+    for rows in (1, 31, 96, 97, 255, 256, 257, 333, 384, 385, 511, 513, 608, 609, 2047, 2048):
         for vocab in (1, 2, 300, 4097, 50257, 151936):
             assert plain_function("sakv_logprob_shape")(rows, vocab, pairs, shape) == 0
             full, height, tiles, launched = shape
-            per = full + (rows % 256 > 0)
-            assert full == rows // 256 and 1 <= height <= 128 and (not full or height % 16 == 0)
+            rest = rows - 256 * full
+            per = 1 if full == 1 and rest > 0 else full + (rest > 0)
+            assert rest <= 128 and rest > -256 and 1 <= height <= 128 and (not full or height % 16 == 0)
             assert (tiles - 1) * 2 * height < vocab <= tiles * 2 * height
             assert launched == min(pairs, tiles * per)
             if not full:                      # every block has the same number of rows in all, but for the last ones
