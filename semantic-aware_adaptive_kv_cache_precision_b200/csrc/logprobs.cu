@@ -20,7 +20,8 @@
 //   warp 0     TMA: boxes of x and of the head (64 wide) into a ring of stages (each block of the pair fetches
 //              its own half of both; no multicast),
 //   warp 1     tensor memory; in the pair's first block lane 0 issues the products,
-//   warps 2-5  epilogue of a tile under the products of the next (two accumulators of 256 columns).
+//   warps 2-9  epilogue of a tile under the products of the next (two accumulators of 256 columns): two warps for
+//              every 32 lanes of tensor memory, each with every other run of columns.
 // Tiles of one piece of the head lie side by side in time, so the head comes from memory once. Up to some 256
 // tokens its bytes bound the kernel, above the tensor cores. The tile's height is chosen so that the last round
 // of tiles is not nearly empty (see the launcher).
@@ -52,7 +53,7 @@ constexpr int kRestMost = 96;
 // 70 / 84, 39 / 40, 375 / 394; 77 172 / 177, 76 / 84, 44 / 41, 380 / 394; 128 180 / 181, 79 / 85, 46 / 41, 367 /
 // 408; 160 189 / 182, 83 / 86, 49 / 41, 435 / 409.
 constexpr int kBothMost = 128;
-constexpr int kEpilogueThreads = 128;
+constexpr int kEpilogueThreads = 256;            // two warps a quarter of tensor memory's lanes, each half the columns
 constexpr int kThreads = 64 + kEpilogueThreads;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint16_t kBoth = 3;
@@ -73,14 +74,35 @@ __device__ __forceinline__ float bias_at(const Shape& f, int v) {
 
 // c tanh(z / c). tanh(y) = 1 - 2 / (e^2y + 1), and below 1/4, where that difference would cancel, the series
 // y - y^3/3 + 2 y^5/15 - 17 y^7/315 + 62 y^9/2835 (the next term is below 2^-26 of y there).
+constexpr float kNear = 0.25f;
+__device__ __forceinline__ float capped_near(const Shape& f, float z) {
+  const float y = z * f.over_cap, q = y * y;
+  return f.cap * fmaf(y * q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y);
+}
 __device__ __forceinline__ float capped(const Shape& f, float z) {
   const float y = z * f.over_cap;
-  const float q = y * y;
-  const float near = fmaf(y * q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y);
   // (2 log2(e) y is kept below 2^7, where the quotient is still one; NaN stays)
   const float e = y > 40.f ? 40.f : y;
   const float far = 1.f - __fdividef(2.f, 1.f + mma::exp2_fast(e * (2.f * kLog2e)));
-  return f.cap * (q < 0.0625f ? near : far);
+  return fabsf(y) < kNear ? capped_near(f, z) : f.cap * far;
+}
+// The same for a run of logits, which are mostly all near zero or not.
+template <int N>
+__device__ __forceinline__ void cap_all(const Shape& f, float (&z)[N]) {
+  float big = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    big = fmaxf(big, fabsf(z[i]));
+    odd |= z[i] != z[i];
+  }
+  if (__any_sync(0xffffffffu, odd || !(big * f.over_cap < kNear))) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = capped(f, z[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = capped_near(f, z[i]);
+  }
 }
 
 struct Params {
@@ -108,7 +130,8 @@ struct Tail {
   Barriers bar;
   alignas(16) float bias[2][2 * BM];
   alignas(16) int32_t target[kMaxTokens];
-  float2 run[kEpilogueThreads / 32][kMaxTokens];
+  float2 run[4][kMaxTokens];
+  float2 share[BM];
 };
 constexpr int kSmemMost = 232448;                // 227 KB
 constexpr int kRingMost = kSmemMost - 1024 - static_cast<int>(sizeof(Tail));
@@ -303,13 +326,15 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     }
   } else {
     // ---- epilogue -------------------------------------------------------------------------------
-    const int quarter = warp & 3, thread = quarter * 32 + lane;      // thread = lane of tensor memory
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int thread = quarter * 32 + lane;                          // lane of tensor memory
+    const int worker = half * BM + thread;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const int first_rest = p.full * kMaxTokens;
-    float2* run = tail->run[quarter];
-    for (int c = thread; c < kMaxTokens; c += kEpilogueThreads)
+    float2* run = tail->run[quarter];        // (a warp's own columns of it)
+    for (int c = worker; c < kMaxTokens; c += kEpilogueThreads)
       tail->target[c] = c < p.rest ? p.targets[first_rest + c] : -1;
-    for (int c = lane; c < kMaxTokens; c += 32) run[c] = make_float2(-INFINITY, 0.f);
+    for (int c = half * 32 + lane; c < kMaxTokens; c += 64) run[c] = make_float2(-INFINITY, 0.f);
     asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
     int count = 0, wide = 0;       // tiles so far, and those of 256 tokens among them
     bool ok = true;
@@ -328,7 +353,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         // done with the one before that, whose biases these replace)
         const float* biases = tail->bias[wide & 1];
         if (!kPlain && p.form.bias) {
-          for (int c = thread; c < cols; c += kEpilogueThreads)
+          for (int c = worker; c < cols; c += kEpilogueThreads)
             tail->bias[wide & 1][c] = n0 + c < p.N ? bias_at(p.form, n0 + c) : 0.f;
           asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
         }
@@ -338,7 +363,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         const uint32_t acc = lane_base + buf * kMaxTokens;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-        for (int c = 0; c < cols && ok && n0 + c < p.N; c += 64) {
+        for (int c = half * 64; c < cols && ok && n0 + c < p.N; c += 128) {
           float z[64];
           tc::ld_32x32b_x64(acc + c, z);
           if (!kPlain) {
@@ -350,10 +375,8 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
               }
             }
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              z[i] *= p.form.scale;
-              if (kCap) z[i] = capped(p.form, z[i]);
-            }
+            for (int i = 0; i < 64; ++i) z[i] *= p.form.scale;
+            if (kCap) cap_all(p.form, z);
           }
           const int real = min(cols, p.N - n0) - c;         // columns of the 64 that are tokens' of this tile
           if (real < 64) {
@@ -370,7 +393,17 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           }
           take_up(z, top, sum);
         }
-        if (ok && m < p.M) p.part[(long long)n_tile * first_rest + m] = make_float2(top, sum);
+        // the second warp of the quarter hands its share to the first
+        if (half) tail->share[thread] = make_float2(top, sum);
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
+        if (!half) {
+          const float2 other = tail->share[thread];
+          const float big = fmaxf(top, other.x);
+          sum = (sum == 0.f ? 0.f : sum * mma::exp2_fast(top - big)) +
+                (other.y == 0.f ? 0.f : other.y * mma::exp2_fast(other.x - big));
+          if (ok && m < p.M) p.part[(long long)n_tile * first_rest + m] = make_float2(big, sum);
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
       }
       if (m_tile == p.full || p.both) {
         // rows of the head on the lanes: this thread's row against the rest of the tokens
@@ -383,19 +416,20 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         }
         const uint32_t acc = lane_base + (p.both ? 1 : buf) * kMaxTokens;
 #pragma unroll 1
-        for (int c = 0; c < p.rest_cols && ok; c += 32) {
+        for (int c = half * 32; c < p.rest_cols && ok; c += 64) {
           float z[32];
           ld_32x32b_x32(acc + c, z);
+          if (!kPlain) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = (z[i] + bias) * p.form.scale;
+            if (kCap) cap_all(p.form, z);
+          }
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             const int4 t = *reinterpret_cast<const int4*>(&tail->target[c + i]);
             const int of[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if (!kPlain) {
-                z[i + j] = (z[i + j] + bias) * p.form.scale;
-                if (kCap) z[i + j] = capped(p.form, z[i + j]);
-              }
               if (of[j] == v && real) p.mine[first_rest + c + i + j] = z[i + j];
               z[i + j] = real ? z[i + j] * kLog2e : -INFINITY;
             }
@@ -420,12 +454,12 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     // the warps' sums of the rest, joined
     asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
     float2* part = p.part + (long long)p.n_tiles * first_rest + (long long)blockIdx.x * p.rest;
-    for (int c = thread; c < p.rest; c += kEpilogueThreads) {
+    for (int c = worker; c < p.rest; c += kEpilogueThreads) {
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kEpilogueThreads / 32; ++w) top = fmaxf(top, tail->run[w][c].x);
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, tail->run[w][c].x);
 #pragma unroll
-      for (int w = 0; w < kEpilogueThreads / 32; ++w) {
+      for (int w = 0; w < 4; ++w) {
         const float2 v = tail->run[w][c];
         sum += v.y == 0.f ? 0.f : v.y * mma::exp2_fast(v.x - top);
       }
