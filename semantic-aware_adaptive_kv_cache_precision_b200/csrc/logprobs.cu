@@ -3,8 +3,8 @@
 //   z_v = cap(scale (x . w_v + b_v)),   cap(z) = c tanh(z / c) where c > 0
 //   lse = m + log sum_v e^(z_v - m),  m = max_v z_v;    logprob = z_target - lse
 //
-// The vocabulary is taken in pieces: a piece leaves (m, sum 2^(z - m)) a row, in base 2, and whoever meets the
-// target's column leaves z_target; `join_kernel` merges the pieces. 2,048 tokens over 151,936 logits would be
+// The vocabulary is taken in pieces: a piece leaves (m, sum e^(z - m)) a row (m in natural units: the type's lowest
+// value, a common mask, times log2(e) would be -inf), and whoever meets the target's column leaves z_target; `join_kernel` merges the pieces. 2,048 tokens over 151,936 logits would be
 // 1.2 GB written and read again; the pieces are 10 MB.
 //
 // Two ways to a piece. bfloat16 operands: tcgen05 on PAIRS of SMs (`cta_group::2`), the softmax's sums in the
@@ -25,8 +25,9 @@
 // Tiles of one piece of the head lie side by side in time, so the head comes from memory once. Up to some 256
 // tokens its bytes bound the kernel, above the tensor cores. The tile's height is chosen so that the last round
 // of tiles is not nearly empty (see the launcher).
-// float32 operands (and rows that TMA cannot take): `fold_kernel` reads a piece of logits that a product of
-// its own left in a scratch.
+// float32 operands: plain FFMA, each sum over k = 0, 1, 2, ... and each row's sums over the vocabulary in one order
+// whatever rows are beside it, as in the other 32-bit products. bfloat16 rows that TMA cannot take: `fold_kernel`
+// reads a piece of logits that a product of its own left in a scratch.
 //
 // Sums and maxima are fp32. Every mbarrier wait is bounded, and a pair leaves together.
 // The reference keeps all logits (`src/microinfer/model.py:388-402`).
@@ -57,7 +58,7 @@ constexpr int kEpilogueThreads = 256;            // two warps a quarter of tenso
 constexpr int kThreads = 64 + kEpilogueThreads;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint16_t kBoth = 3;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // What becomes of a product x . w before the softmax.
 struct Shape {
@@ -113,7 +114,7 @@ struct Params {
   int n_tiles;               // tiles of 2 w_rows rows of the head
   int stages, stage_bytes;
   const int32_t* targets;
-  float2* part;              // [n_tiles][256 full], then [blocks][rest]: (maximum, sum) in base 2
+  float2* part;              // [n_tiles][256 full], then [blocks][rest]: (maximum, sum)
   float* mine;               // [M]: the targets' logits
   Shape form;
   int* error;
@@ -162,19 +163,31 @@ __device__ __forceinline__ void ld_32x32b_x32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// 64 columns of a row joined to the row's running (maximum, sum) in base 2. `z` in natural units.
+// e^(z - top), right where the difference is; top may be -inf only beside z = -inf (0) or NaN (NaN)
+__device__ __forceinline__ float weight_of(float z, float top) {
+  return mma::exp2_fast((z - (top == -INFINITY ? 0.f : top)) * kLog2e);
+}
+// Below this a maximum's product with log2(e) leaves the type's range, or nearly.
+constexpr float kLow = -2e38f;
+
+// 64 columns of a row joined to the row's running (maximum, sum).
 __device__ __forceinline__ void take_up(const float (&z)[64], float& top, float& sum) {
   float big4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 64; c += 8)
 #pragma unroll
     for (int q = 0; q < 4; ++q) big4[q] = mma::max3(big4[q], z[c + 2 * q], z[c + 2 * q + 1]);
-  const float big = fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3])) * kLog2e;
+  const float big = fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3]));
   if (big > top) {
-    sum *= mma::exp2_fast(top - big);
+    sum = sum == 0.f ? 0.f : sum * weight_of(top, big);
     top = big;
   }
-  const float base = top == -INFINITY ? 0.f : top;
+  if (top < kLow) {                    // nothing so far, or values that a mask made the type's lowest
+#pragma unroll
+    for (int c = 0; c < 64; ++c) sum += weight_of(z[c], top);
+    return;
+  }
+  const float base = top * kLog2e;
   float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 64; c += 2) {
@@ -399,8 +412,8 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         if (!half) {
           const float2 other = tail->share[thread];
           const float big = fmaxf(top, other.x);
-          sum = (sum == 0.f ? 0.f : sum * mma::exp2_fast(top - big)) +
-                (other.y == 0.f ? 0.f : other.y * mma::exp2_fast(other.x - big));
+          sum = (sum == 0.f ? 0.f : sum * weight_of(top, big)) +
+                (other.y == 0.f ? 0.f : other.y * weight_of(other.x, big));
           if (ok && m < p.M) p.part[(long long)n_tile * first_rest + m] = make_float2(big, sum);
         }
         asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
@@ -431,7 +444,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               if (of[j] == v && real) p.mine[first_rest + c + i + j] = z[i + j];
-              z[i + j] = real ? z[i + j] * kLog2e : -INFINITY;
+              z[i + j] = real ? z[i + j] : -INFINITY;
             }
           }
           float most[32];
@@ -441,9 +454,9 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           const float top = fmaxf(old.x, over_lanes<true>(most, lane));
           const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = mma::exp2_fast(z[i] - __shfl_sync(0xffffffffu, base, i));
+          for (int i = 0; i < 32; ++i) z[i] = mma::exp2_fast((z[i] - __shfl_sync(0xffffffffu, base, i)) * kLog2e);
           const float sum = over_lanes<false>(z, lane);
-          run[c + lane] = make_float2(top, (old.y == 0.f ? 0.f : old.y * mma::exp2_fast(old.x - top)) + sum);
+          run[c + lane] = make_float2(top, (old.y == 0.f ? 0.f : old.y * weight_of(old.x, top)) + sum);
         }
       }
       tc::fence_before_sync();
@@ -461,7 +474,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float2 v = tail->run[w][c];
-        sum += v.y == 0.f ? 0.f : v.y * mma::exp2_fast(v.x - top);
+        sum += v.y == 0.f ? 0.f : v.y * weight_of(v.x, top);
       }
       part[c] = make_float2(top, sum);
     }
@@ -519,13 +532,132 @@ fold_kernel(const float* __restrict__ z, long long ld, int M, int n, int first, 
   if (threadIdx.x) return;
   sum = 0.f;
   for (int w = 0; w < kFoldThreads / 32; ++w) sum += sums[w];
-  part[(long long)blockIdx.y * M + m] = make_float2(top * kLog2e, sum);
+  part[(long long)blockIdx.y * M + m] = make_float2(top, sum);
+}
+
+// The product and its softmax in 32 bits. A block takes 8 TM rows of x and kCols rows of the head, K in steps of 16
+// through a ring copied with cp.async; thread (ty, tx) of 8 x 16 has rows ty + 8 i and columns tx + 16 j, so that
+// the column's threads, and with them the order of a row's sums, are the same for every TM. Bound by the FFMA pipe
+// from some 32 rows on (TM 8: 16 reads of 16 bytes for 256 multiply-adds a thread), by the head's bytes below.
+constexpr int kCols = 128, kF32Threads = 128, kF32K = 16, kF32Stages = 4, kLd = kF32K + 4;
+
+__device__ __forceinline__ void copy_f32(uint32_t dst, const float* src, bool real, bool wide) {
+  if (wide)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+
+template <int TM>
+__global__ void __launch_bounds__(kF32Threads, 3)
+f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restrict__ head, int M, int N, int K,
+           int m_tiles, int wide, const int32_t* __restrict__ targets, float2* __restrict__ part,
+           float* __restrict__ mine, const Shape form) {
+  constexpr int kRows = 8 * TM;
+  extern __shared__ __align__(16) float ring[];            // [stages][kRows + kCols][kLd]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int m0 = blockIdx.x % m_tiles * kRows, piece = blockIdx.x / m_tiles;      // tokens fastest
+  const long long n0 = (long long)piece * kCols;
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const int steps = (K + kF32K - 1) / kF32K;
+  auto fill = [&](int step) {
+    const int k0 = step * kF32K;
+    const uint32_t to = base + (step % kF32Stages) * (kRows + kCols) * kLd * 4;
+    const int per = wide ? kF32K / 4 : kF32K, width = kF32K / per;
+    for (int i = threadIdx.x; i < (kRows + kCols) * per; i += kF32Threads) {
+      const int r = i / per, c = i % per * width;
+      const bool in_x = r < kRows;
+      const bool real = k0 + c < K && (in_x ? m0 + r < M : n0 + r - kRows < N);
+      const float* from = in_x ? x + (m0 + r) * x_stride : head + (n0 + r - kRows) * K;
+      copy_f32(to + (r * kLd + c) * 4, real ? from + k0 + c : head, real, wide);
+    }
+  };
+  float acc[TM][8];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+  for (int s = 0; s < kF32Stages - 1; ++s) {
+    if (s < steps) fill(s);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kF32Stages - 2) : "memory");
+    __syncthreads();
+    if (step + kF32Stages - 1 < steps) fill(step + kF32Stages - 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const float* xs = ring + (step % kF32Stages) * (kRows + kCols) * kLd;
+    const float* ws = xs + kRows * kLd;
+#pragma unroll
+    for (int k = 0; k < kF32K; k += 4) {
+      float4 a[TM], w[8];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const float4*>(xs + (ty + 8 * i) * kLd + k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const float4*>(ws + (tx + 16 * j) * kLd + k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            acc[i][j] = fmaf(reinterpret_cast<const float*>(&a[i])[e], reinterpret_cast<const float*>(&w[j])[e],
+                             acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + ty + 8 * i;
+    const int target = m < M ? targets[m] : -1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const long long v = n0 + tx + 16 * j;
+      float z = -INFINITY;
+      if (v < N) {
+        z = acc[i][j];
+        if (form.bias) z += bias_at(form, static_cast<int>(v));
+        z *= form.scale;
+        if (form.cap > 0.f) z = form.cap * tanhf(z * form.over_cap);
+        if (v == target) mine[m] = z;
+      }
+      acc[i][j] = z;
+      top = fmaxf(top, z);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n0 + tx + 16 * j < N) sum += expf(acc[i][j] - from);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (tx == 0 && m < M) part[(long long)piece * M + m] = make_float2(top, sum);
+  }
+}
+
+template <int TM>
+int launch_f32(const float* x, long long x_stride, const float* head, int M, int N, int K, const int32_t* targets,
+               float2* part, float* mine, const Shape& form, cudaStream_t stream) {
+  constexpr int kSmem = kF32Stages * (8 * TM + kCols) * kLd * 4;
+  static PerDeviceOnce configured;
+  if (configured.needs()) {
+    const cudaError_t e = cudaFuncSetAttribute(f32_kernel<TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return (int)e;
+    configured.done();
+  }
+  const long long m_tiles = (M + 8 * TM - 1) / (8 * TM), pieces = ((long long)N + kCols - 1) / kCols;
+  if (m_tiles * pieces > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int wide = K % 4 == 0 && x_stride % 4 == 0 && !((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(head)) & 15);
+  return launch_ordered(f32_kernel<TM>, dim3((unsigned)(m_tiles * pieces)), dim3(kF32Threads), kSmem, stream, x,
+                        x_stride, head, M, N, K, (int)m_tiles, wide, targets, part, mine, form);
 }
 
 // lse and log-probability of every row from its partials: rows below `full` have `pieces` of them, [pieces][full],
 // the others `rest_pieces`, [rest_pieces][M - full] behind them. A block has 32 rows, all of one kind; a warp takes
-// every 16th piece of all of them (lane = row: neighbouring rows' partials are neighbours in memory).
-constexpr int kJoinWarps = 16;
+// every 32nd piece of all of them (lane = row: neighbouring rows' partials are neighbours in memory).
+constexpr int kJoinWarps = 32;
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, const int32_t* __restrict__ targets,
             float* __restrict__ logprob, float* __restrict__ lse, int M, int N, int full, int pieces,
@@ -550,10 +682,10 @@ join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, con
       float big = top;
 #pragma unroll
       for (int i = 0; i < kRound; ++i) big = fmaxf(big, v[i].x);
-      sum = sum == 0.f ? 0.f : sum * exp2f(top - big);
+      sum = sum == 0.f ? 0.f : sum * expf(top - big);
       top = big;
 #pragma unroll
-      for (int i = 0; i < kRound; ++i) sum += v[i].y == 0.f ? 0.f : v[i].y * exp2f(v[i].x - top);
+      for (int i = 0; i < kRound; ++i) sum += v[i].y == 0.f ? 0.f : v[i].y * expf(v[i].x - top);
     }
   __shared__ float2 all[kJoinWarps][32];
   all[warp][lane] = make_float2(top, sum);
@@ -564,8 +696,8 @@ join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, con
   sum = 0.f;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w)
-    sum += all[w][lane].y == 0.f ? 0.f : all[w][lane].y * exp2f(all[w][lane].x - top);
-  const float total = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    sum += all[w][lane].y == 0.f ? 0.f : all[w][lane].y * expf(all[w][lane].x - top);
+  const float total = sum == 0.f ? -INFINITY : top + logf(sum);
   const int target = targets[m];
   lse[m] = total;
   // (a row that asks for nothing: 0; a target that is no token: NaN)
@@ -616,6 +748,24 @@ Shape shape_of(const void* bias, int bias_bf16, float scale, float cap) {
 
 // Columns a piece of the fold has.
 SAKV_EXPORT int sakv_logprob_fold_columns() { return kFoldColumns; }
+// Rows of the head a piece of the 32-bit kernel has.
+SAKV_EXPORT int sakv_logprob_f32_columns() { return kCols; }
+
+// The partials of x [M, K] (rows `x_stride` apart) against the head [N, K] in float32: part [ceil(N / 128)][M].
+SAKV_EXPORT int sakv_logprob_f32(const float* x, long long x_stride, const float* head, int M, int N, int K,
+                                 const int32_t* targets, float* part, float* mine, const void* bias, int bias_bf16,
+                                 float scale, float cap, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || x_stride < K || M > 0x7fffffff - 64 || !(cap >= 0.f)) return cudaErrorInvalidValue;
+  const Shape form = shape_of(bias, bias_bf16, scale, cap);
+  float2* to = reinterpret_cast<float2*>(part);
+#define SAKV_F32(TM) return launch_f32<TM>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
+  if (M <= 8) SAKV_F32(1);
+  if (M <= 16) SAKV_F32(2);
+  if (M <= 32) SAKV_F32(4);
+  SAKV_F32(8);
+#undef SAKV_F32
+}
+
 // Pairs of SMs that can hold the tensor-core kernel at one time (0: it cannot run here).
 SAKV_EXPORT int sakv_logprob_resident() { return resident_pairs(); }
 

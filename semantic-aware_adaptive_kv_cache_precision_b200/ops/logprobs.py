@@ -65,6 +65,11 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
             part = x.new_empty(2 * (pieces * full + rest_pieces * max(0, rows - full)), dtype=torch.float32)
             call("sakv_logprob_pieces", ptr(x), x.stride(0), ptr(head), rows, vocab, k, shape, ptr(targets),
                  ptr(part), ptr(mine), *form)
+        elif x.dtype == torch.float32:
+            full, pieces, rest_pieces = rows, -(-vocab // plain_function("sakv_logprob_f32_columns")()), 0
+            part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
+            call("sakv_logprob_f32", ptr(x), x.stride(0), ptr(head), rows, vocab, k, ptr(targets), ptr(part),
+                 ptr(mine), *form)
         else:
             columns = plain_function("sakv_logprob_fold_columns")()
             most = max(1, PIECE_ELEMENTS // columns)
