@@ -25,7 +25,7 @@
 // Tiles of one piece of the head lie side by side in time, so the head comes from memory once. Up to some 256
 // tokens its bytes bound the kernel, above the tensor cores. The tile's height is chosen so that the last round
 // of tiles is not nearly empty (see the launcher).
-// float32 operands: plain FFMA, each sum over k = 0, 1, 2, ... and each row's sums over the vocabulary in one order
+// float32 operands: plain multiply-adds, each sum over k and each row's sums over the vocabulary in one order
 // whatever rows are beside it, as in the other 32-bit products. bfloat16 rows that TMA cannot take: `fold_kernel`
 // reads a piece of logits that a product of its own left in a scratch.
 //
@@ -537,74 +537,101 @@ fold_kernel(const float* __restrict__ z, long long ld, int M, int n, int first, 
 
 // The product and its softmax in 32 bits. A block takes 8 TM rows of x and kCols rows of the head, K in steps of 16
 // through a ring copied with cp.async; thread (ty, tx) of 8 x 16 has rows ty + 8 i and columns tx + 16 j, so that
-// the column's threads, and with them the order of a row's sums, are the same for every TM. Bound by the FFMA pipe
-// from some 32 rows on (TM 8: 16 reads of 16 bytes for 256 multiply-adds a thread), by the head's bytes below.
+// the column's threads, and with them the order of a row's sums, are the same for every TM. Two multiply-adds an
+// instruction: a sum is one over the even k's and one over the odd ones, whose operands lie side by side as they
+// are read. Bound by reads of shared memory (16 bytes a lane take four cycles whatever the lanes share) beside
+// the multiply-adds: 64 rows of 1,024 over 32,768 take 131 us, 58 us at the multiply-adds' rate; one to eight
+// rows 54 us, 21 us at the memory's.
 constexpr int kCols = 128, kF32Threads = 128, kF32K = 16, kF32Stages = 4, kLd = kF32K + 4;
 
-__device__ __forceinline__ void copy_f32(uint32_t dst, const float* src, bool real, bool wide) {
-  if (wide)
+// d += a * b in both halves
+__device__ __forceinline__ void fma_pair(uint64_t& d, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+
+template <bool kWide>
+__device__ __forceinline__ void copy_f32(uint32_t dst, const float* src, bool real) {
+  if (kWide)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
-template <int TM>
-__global__ void __launch_bounds__(kF32Threads, 3)
+// kWide: rows that begin at multiples of 16 bytes
+template <int TM, bool kWide>
+__global__ void __launch_bounds__(kF32Threads, TM == 8 ? 2 : 3)
 f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restrict__ head, int M, int N, int K,
-           int m_tiles, int wide, const int32_t* __restrict__ targets, float2* __restrict__ part,
+           int m_tiles, const int32_t* __restrict__ targets, float2* __restrict__ part,
            float* __restrict__ mine, const Shape form) {
-  constexpr int kRows = 8 * TM;
+  constexpr int kRows = 8 * TM, kStages = kF32Stages;
   extern __shared__ __align__(16) float ring[];            // [stages][kRows + kCols][kLd]
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int m0 = blockIdx.x % m_tiles * kRows, piece = blockIdx.x / m_tiles;      // tokens fastest
   const long long n0 = (long long)piece * kCols;
   const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   const int steps = (K + kF32K - 1) / kF32K;
+  // a thread copies one place of K (of a step) in rows kAt, kAt + kStep, ... of x and of the head
+  constexpr int kWidth = kWide ? 4 : 1, kPer = kF32K / kWidth, kStep = kF32Threads / kPer;
+  const int kc = threadIdx.x % kPer * kWidth, row = threadIdx.x / kPer;
+  const float* from_x = x + (m0 + row) * x_stride + kc;
+  const float* from_w = head + (n0 + row) * K + kc;
+  const uint32_t to0 = base + (row * kLd + kc) * 4;
   auto fill = [&](int step) {
-    const int k0 = step * kF32K;
-    const uint32_t to = base + (step % kF32Stages) * (kRows + kCols) * kLd * 4;
-    const int per = wide ? kF32K / 4 : kF32K, width = kF32K / per;
-    for (int i = threadIdx.x; i < (kRows + kCols) * per; i += kF32Threads) {
-      const int r = i / per, c = i % per * width;
-      const bool in_x = r < kRows;
-      const bool real = k0 + c < K && (in_x ? m0 + r < M : n0 + r - kRows < N);
-      const float* from = in_x ? x + (m0 + r) * x_stride : head + (n0 + r - kRows) * K;
-      copy_f32(to + (r * kLd + c) * 4, real ? from + k0 + c : head, real, wide);
+    const uint32_t to = to0 + (step % kStages) * ((kRows + kCols) * kLd * 4);
+    const bool in_k = step * kF32K + kc < K;
+#pragma unroll
+    for (int r = 0; r < kRows; r += kStep) {
+      if (kRows % kStep && r + row >= kRows) break;
+      const bool real = in_k && m0 + row + r < M;
+      copy_f32<kWide>(to + r * kLd * 4, real ? from_x + r * x_stride : head, real);
     }
+#pragma unroll
+    for (int r = 0; r < kCols; r += kStep) {
+      const bool real = in_k && n0 + row + r < N;
+      copy_f32<kWide>(to + (kRows + r) * kLd * 4, real ? from_w + (long long)r * K : head, real);
+    }
+    from_x += kF32K;
+    from_w += kF32K;
   };
-  float acc[TM][8];
+  uint64_t sums[TM][8];              // (sum over even k, sum over odd k)
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-  for (int s = 0; s < kF32Stages - 1; ++s) {
+    for (int j = 0; j < 8; ++j) sums[i][j] = 0;
+  for (int s = 0; s < kStages - 1; ++s) {
     if (s < steps) fill(s);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   for (int step = 0; step < steps; ++step) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kF32Stages - 2) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
-    if (step + kF32Stages - 1 < steps) fill(step + kF32Stages - 1);
+    if (step + kStages - 1 < steps) fill(step + kStages - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const float* xs = ring + (step % kF32Stages) * (kRows + kCols) * kLd;
+    const float* xs = ring + (step % kStages) * (kRows + kCols) * kLd;
     const float* ws = xs + kRows * kLd;
 #pragma unroll
     for (int k = 0; k < kF32K; k += 4) {
-      float4 a[TM], w[8];
+      ulonglong2 a[TM], w[8];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const float4*>(xs + (ty + 8 * i) * kLd + k);
+      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(xs + (ty + 8 * i) * kLd + k);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const float4*>(ws + (tx + 16 * j) * kLd + k);
+      for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const ulonglong2*>(ws + (tx + 16 * j) * kLd + k);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int j = 0; j < 8; ++j) fma_pair(sums[i][j], a[i].x, w[j].x);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            acc[i][j] = fmaf(reinterpret_cast<const float*>(&a[i])[e], reinterpret_cast<const float*>(&w[j])[e],
-                             acc[i][j]);
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fma_pair(sums[i][j], a[i].y, w[j].y);
     }
   }
+  float acc[TM][8];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      acc[i][j] = __uint_as_float(static_cast<uint32_t>(sums[i][j])) + __uint_as_float(static_cast<uint32_t>(sums[i][j] >> 32));
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int m = m0 + ty + 8 * i;
@@ -637,21 +664,20 @@ f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restr
   }
 }
 
-template <int TM>
+template <int TM, bool kWide>
 int launch_f32(const float* x, long long x_stride, const float* head, int M, int N, int K, const int32_t* targets,
                float2* part, float* mine, const Shape& form, cudaStream_t stream) {
   constexpr int kSmem = kF32Stages * (8 * TM + kCols) * kLd * 4;
   static PerDeviceOnce configured;
   if (configured.needs()) {
-    const cudaError_t e = cudaFuncSetAttribute(f32_kernel<TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(f32_kernel<TM, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return (int)e;
     configured.done();
   }
   const long long m_tiles = (M + 8 * TM - 1) / (8 * TM), pieces = ((long long)N + kCols - 1) / kCols;
   if (m_tiles * pieces > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const int wide = K % 4 == 0 && x_stride % 4 == 0 && !((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(head)) & 15);
-  return launch_ordered(f32_kernel<TM>, dim3((unsigned)(m_tiles * pieces)), dim3(kF32Threads), kSmem, stream, x,
-                        x_stride, head, M, N, K, (int)m_tiles, wide, targets, part, mine, form);
+  return launch_ordered(f32_kernel<TM, kWide>, dim3((unsigned)(m_tiles * pieces)), dim3(kF32Threads), kSmem, stream, x,
+                        x_stride, head, M, N, K, (int)m_tiles, targets, part, mine, form);
 }
 
 // lse and log-probability of every row from its partials: rows below `full` have `pieces` of them, [pieces][full],
@@ -758,7 +784,11 @@ SAKV_EXPORT int sakv_logprob_f32(const float* x, long long x_stride, const float
   if (M <= 0 || N <= 0 || K <= 0 || x_stride < K || M > 0x7fffffff - 64 || !(cap >= 0.f)) return cudaErrorInvalidValue;
   const Shape form = shape_of(bias, bias_bf16, scale, cap);
   float2* to = reinterpret_cast<float2*>(part);
-#define SAKV_F32(TM) return launch_f32<TM>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
+  const bool wide = K % 4 == 0 && x_stride % 4 == 0 &&
+                    !((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(head)) & 15);
+#define SAKV_F32(TM)                                                                                       \
+  return wide ? launch_f32<TM, true>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)           \
+              : launch_f32<TM, false>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
   if (M <= 8) SAKV_F32(1);
   if (M <= 16) SAKV_F32(2);
   if (M <= 32) SAKV_F32(4);
