@@ -29,6 +29,13 @@ from .step import StepStager, table_width
 DEFAULT_MAX_TOKENS = 16384
 DEFAULT_MAX_BATCH = 64
 DEFAULT_MAX_STEP_TOKENS = 16384
+# Bytes of keys and values a layer that a decode step must save by reading shared blocks once: below, the kernel
+# that reads every sequence's list for itself (rotating queries and keys on its way, one kernel fewer a layer) is
+# the faster. Measured (ms a step, each for itself / shared, MB saved): 28 layers of 12 heads over 2, 64 sequences
+# 1.548 / 1.647 (33), 1.665 / 1.673 (66), 1.894 / 1.723 (132); 16 sequences 1.336 / 1.353 (63), 1.538 / 1.487 (126);
+# 8 sequences 1.242 / 1.320 (59), 1.539 / 1.485 (115); 14 layers of 28 over 4, 64 sequences 1.617 / 1.731 (66),
+# 1.730 / 1.744 (132), 1.964 / 1.838 (264); 8 sequences 1.372 / 1.412 (29), 1.511 / 1.471 (59).
+SHARED_BYTES_WORTH = 80 << 20
 
 
 class Engine:
@@ -75,8 +82,8 @@ class Engine:
         self.graph_failure = None
         self._prefill_graphs = {}
         #: decode steps of sequences that share blocks read them once for all of them where that saves
-        #: at least this many blocks a layer (None: never)
-        self.shared_blocks_worth = 1
+        #: at least this many bytes a layer (None: never)
+        self.shared_bytes_worth = SHARED_BYTES_WORTH
         self._shared_now = None        # (what the plans below are right for, how far, the plans)
         self._shared_buffers: dict = {}
         #: steps of up to this many tokens are captured when their shape repeats (0: never);
@@ -232,7 +239,7 @@ class Engine:
         ops.SharedPlan}, at device addresses that stay the same for plans of one layout (captured steps read
         them there). Worked out when the sequences, what they share or the width of the block lists change,
         or a sequence outgrows them."""
-        if self.shared_blocks_worth is None or not cache.shares_blocks:
+        if self.shared_bytes_worth is None or not cache.shares_blocks:
             return {}
         width = min(table_width(ends), cache.max_blocks_per_seq)
         key = (tuple(slots), cache.sharing, width)
@@ -253,7 +260,8 @@ class Engine:
                     continue
                 plan = ops.plan_shared(tables[g][:, :width], ends, heads, need.kv_heads, None, reach=reach,
                                        roomy=True, slots=2 * _lib.sm_count(self.device))
-                if plan.saved < self.shared_blocks_worth:
+                block = sum(t.numel() // (t.shape[0] * t.shape[1]) * t.element_size() for t in group.tensors)
+                if plan.saved * block < self.shared_bytes_worth:
                     continue
                 place = (g, heads, plan.layout)
                 buffer = self._shared_buffers.get(place)

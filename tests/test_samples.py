@@ -162,7 +162,7 @@ def test_sixteen_bit_steps_over_shared_blocks(varied_folders, name, graphs):
     choice of tokens inside the captured step follows its own logits."""
     engine = engine_of(varied_folders(name, "bfloat16"), "bfloat16", cuda_graphs=graphs, max_tokens=8192)
     alone = engine_of(varied_folders(name, "bfloat16"), "bfloat16", cuda_graphs=graphs, max_tokens=8192)
-    alone.shared_blocks_worth = None
+    engine.shared_bytes_worth, alone.shared_bytes_worth = 0, None
     assert (len(engine.model.shared_readers()) > 0) == (name in "DC")
     rng = np.random.default_rng(4)
     vocab, prompt = engine.vocab_size, rng.integers(0, engine.vocab_size, 450).tolist()
@@ -196,6 +196,7 @@ def test_a_captured_step_reads_the_plan_of_the_moment(varied_folders):
     """The same batch shape with other sequences sharing: graphs are shared between plans of one layout, and
     every one reads its own."""
     engine = engine_of(varied_folders("D", "bfloat16"), "bfloat16", max_tokens=16384)
+    engine.shared_bytes_worth = 0
     rng = np.random.default_rng(5)
     prompts = [rng.integers(0, 400, 200).tolist() for _ in range(2)]
     heads = engine.open(2)
@@ -255,6 +256,7 @@ def test_a_cache_of_another_size_between_steps(varied_folders, dtype):
 @pytest_gpu
 def test_samples_that_end_and_a_full_cache(varied_folders):
     engine = engine_of(varied_folders("D", "bfloat16"), "bfloat16", max_tokens=40 * BLOCK)
+    engine.shared_bytes_worth = 0
     prompt = prompts_for("D", (300,))[0]
     free = engine.generate(prompt, 30, samples=12, temperature=1.0, seed=1, stop_at_eos=False)
     stops = {int(free[0][4]), int(free[5][9])}
