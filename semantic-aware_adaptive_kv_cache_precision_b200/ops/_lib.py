@@ -202,25 +202,6 @@ def sm_count(device=None) -> int:
     return _sm_counts[index]
 
 
-class _Nothing:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NOTHING = _Nothing()
-
-
-def on_device(t: torch.Tensor):
-    """A context in which `t`'s device is the current one (nothing to do where it is already: asking
-    costs a microsecond less than switching)."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return _NOTHING
-    return torch.cuda.device(t.device)
-
-
 def require_cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -236,6 +217,21 @@ def call(name: str, *args) -> None:
     global launches
     launches += 1
     code = function(name)(*args, stream())
+    if code != 0:
+        raise KernelError(f"{name} failed with CUDA error {code}"
+                          + (" (invalid value: a size this kernel does not take)" if code == 1 else ""))
+
+
+def call_on(device: int, name: str, *args) -> None:
+    """`call` on the device of number `device` and its current stream, whichever device is current."""
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            call(name, *args)
+        return
+    global launches
+    launches += 1
+    fn = _functions.get(name) or function(name)
+    code = fn(*args, stream() if _raw_stream is None else _raw_stream(device))
     if code != 0:
         raise KernelError(f"{name} failed with CUDA error {code}"
                           + (" (invalid value: a size this kernel does not take)" if code == 1 else ""))

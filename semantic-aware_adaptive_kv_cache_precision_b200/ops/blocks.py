@@ -9,7 +9,7 @@ import math
 
 import torch
 
-from ._lib import KernelError, call, on_device, require_cuda
+from ._lib import KernelError, call_on, require_cuda
 
 
 class _Tensor(ctypes.Structure):
@@ -84,8 +84,7 @@ def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: 
         return
     pairs = array.array("i", bytes(8 * count))
     pairs[0::2], pairs[1::2] = array.array("i", src), array.array("i", dst)
-    with on_device(tensors[0]):
-        call("sakv_copy_blocks", ctypes.addressof(table), len(tensors), pairs.buffer_info()[0], count)
+    call_on(device, "sakv_copy_blocks", ctypes.addressof(table), len(tensors), pairs.buffer_info()[0], count)
 
 
 def _geometry(t, u, rows, axis, blocks, room) -> tuple:

@@ -8,7 +8,7 @@ import ctypes
 import torch
 
 from . import gemm_wide
-from ._lib import F32, KernelError, call, dtype_code, on_device, plain_function, ptr, require_cuda
+from ._lib import F32, KernelError, call, dtype_code, plain_function, ptr, require_cuda
 from .linear import linear
 
 #: logits that lie in memory at one time where a piece is a product of its own (fp32: 32 MB, a quarter of L2)
@@ -51,39 +51,47 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
     if any(t is not None and t.device != x.device for t in (head, targets, bias)):
         raise KernelError("token_logprobs: tensors on different devices")
     require_cuda(x, head, targets, bias)
-    with on_device(x):
-        logprob = x.new_empty(rows, dtype=torch.float32)
-        lse, mine = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
-        if rows == 0:
-            return logprob, lse
-        form = (ptr(bias), bias_code, float(scale), float(softcap))
-        if gemm_wide.takes(x, head) and _pairs() > 0:
-            shape = (ctypes.c_int * 4)()
-            if plain_function("sakv_logprob_shape")(rows, vocab, _pairs(), shape) != 0:
-                raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
-            full, pieces, rest_pieces = shape[0] * 256, shape[2], 2 * shape[3]
-            part = x.new_empty(2 * (pieces * full + rest_pieces * max(0, rows - full)), dtype=torch.float32)
-            call("sakv_logprob_pieces", ptr(x), x.stride(0), ptr(head), rows, vocab, k, shape, ptr(targets),
-                 ptr(part), ptr(mine), *form)
-        elif x.dtype == torch.float32:
-            full, pieces, rest_pieces = rows, -(-vocab // plain_function("sakv_logprob_f32_columns")()), 0
-            part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
-            call("sakv_logprob_f32", ptr(x), x.stride(0), ptr(head), rows, vocab, k, ptr(targets), ptr(part),
-                 ptr(mine), *form)
-        else:
-            columns = plain_function("sakv_logprob_fold_columns")()
-            most = max(1, PIECE_ELEMENTS // columns)
-            if rows > most:                # (the scratch of a piece stays as large as it is for these)
-                parts = [token_logprobs(x[i:i + most], head, targets[i:i + most], bias, scale=scale,
-                                        softcap=softcap) for i in range(0, rows, most)]
-                return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
-            piece = max(1, min(-(-vocab // columns), PIECE_ELEMENTS // (rows * columns))) * columns
-            full, pieces, rest_pieces = rows, -(-vocab // columns), 0
-            part = torch.empty((pieces, rows, 2), dtype=torch.float32, device=x.device)
-            for first in range(0, vocab, piece):
-                z = linear(x, head[first:first + piece], out_dtype=torch.float32)
-                call("sakv_logprob_fold", ptr(z), z.stride(0), rows, z.shape[1], first, vocab, ptr(targets),
-                     ptr(part[first // columns]), ptr(mine), *form)
-        call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, full, pieces,
-             rest_pieces)
+    form = (ptr(bias), bias_code, float(scale), float(softcap))
+    device = x.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _token_logprobs(x, head, targets, bias, form)
+    return _token_logprobs(x, head, targets, bias, form)
+
+
+def _token_logprobs(x, head, targets, bias, form):
+    rows, vocab, k = x.shape[0], head.shape[0], head.shape[1]
+    logprob = x.new_empty(rows, dtype=torch.float32)
+    lse, mine = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+    if rows == 0:
+        return logprob, lse
+    if gemm_wide.takes(x, head) and _pairs() > 0:
+        shape = (ctypes.c_int * 4)()
+        if plain_function("sakv_logprob_shape")(rows, vocab, _pairs(), shape) != 0:
+            raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
+        full, pieces, rest_pieces = shape[0] * 256, shape[2], 2 * shape[3]
+        part = x.new_empty(2 * (pieces * full + rest_pieces * max(0, rows - full)), dtype=torch.float32)
+        call("sakv_logprob_pieces", ptr(x), x.stride(0), ptr(head), rows, vocab, k, shape, ptr(targets),
+             ptr(part), ptr(mine), *form)
+    elif x.dtype == torch.float32:
+        full, pieces, rest_pieces = rows, -(-vocab // plain_function("sakv_logprob_f32_columns")()), 0
+        part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
+        call("sakv_logprob_f32", ptr(x), x.stride(0), ptr(head), rows, vocab, k, ptr(targets), ptr(part),
+             ptr(mine), *form)
+    else:
+        columns = plain_function("sakv_logprob_fold_columns")()
+        most = max(1, PIECE_ELEMENTS // columns)
+        if rows > most:                # (the scratch of a piece stays as large as it is for these)
+            parts = [_token_logprobs(x[i:i + most], head, targets[i:i + most], bias, form)
+                     for i in range(0, rows, most)]
+            return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+        piece = max(1, min(-(-vocab // columns), PIECE_ELEMENTS // (rows * columns))) * columns
+        full, pieces, rest_pieces = rows, -(-vocab // columns), 0
+        part = torch.empty((pieces, rows, 2), dtype=torch.float32, device=x.device)
+        for first in range(0, vocab, piece):
+            z = linear(x, head[first:first + piece], out_dtype=torch.float32)
+            call("sakv_logprob_fold", ptr(z), z.stride(0), rows, z.shape[1], first, vocab, ptr(targets),
+                 ptr(part[first // columns]), ptr(mine), *form)
+    call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, full, pieces,
+         rest_pieces)
     return logprob, lse

@@ -10,7 +10,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import CACHE_BLOCK, KernelError, call, on_device, require_cuda, sm_count
+from ._lib import CACHE_BLOCK, KernelError, call_on, require_cuda, sm_count
 from .attention import fast_path_takes, tensor_map
 
 UNIT_ROWS = 128           # most rows (sequences x query heads of one KV head) of a unit of work
@@ -208,10 +208,9 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if sequences == 0:
         return out
     part = qkv.new_empty(plan.partials * heads * (head_dim + 2), dtype=torch.float32)
-    with on_device(qkv):
-        call("sakv_shared_attention", tensor_map(k_cache), tensor_map(v_cache), qkv.data_ptr(), qkv.stride(0),
-             seq_lens.data_ptr(), block_table.data_ptr(), plan.words.data_ptr(), ctypes.addressof(plan.numbers), out.data_ptr(),
-             part.data_ptr(), head_dim, scale)
+    call_on(device, "sakv_shared_attention", tensor_map(k_cache), tensor_map(v_cache), qkv.data_ptr(),
+            qkv.stride(0), seq_lens.data_ptr(), block_table.data_ptr(), plan.words.data_ptr(),
+            ctypes.addressof(plan.numbers), out.data_ptr(), part.data_ptr(), head_dim, scale)
     if plan.unit_capacity:
         _lib.launches += 1          # the call launched the join too
     return out
