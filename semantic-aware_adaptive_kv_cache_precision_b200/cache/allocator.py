@@ -55,6 +55,13 @@ class Pool:
         self._free.extend(ids)
         self._free.sort(reverse=True)
 
+    def grow(self, size: int) -> None:
+        """More identifiers: the new ones are free."""
+        if size < self.size:
+            raise ValueError(f"a pool of {self.size} {self.what}s cannot grow to {size}")
+        self._free = list(range(size - 1, self.size - 1, -1)) + self._free
+        self.size = size
+
     def check(self) -> None:
         """Every id is either free or held, exactly once."""
         free = list(self._free)

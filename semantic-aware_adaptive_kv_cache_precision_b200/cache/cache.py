@@ -256,17 +256,18 @@ class SequenceCache:
 
     # -- another size ---------------------------------------------------------
 
-    def resize(self, max_tokens: int) -> None:
+    def resize(self, max_tokens: int, max_slots: int | None = None) -> None:
         """Give every pool room for `max_tokens` positions (rounded up to blocks) while sequences live:
         held blocks are moved into new storage, one behind the other in the order of their numbers, and the
-        old storage is given up. The number of slots stays. All or nothing: `CacheFull` where the held
-        blocks, or a sequence's length, do not fit; `OutOfDeviceMemory` where the device has no room for
-        old and new storage together."""
+        old storage is given up. `max_slots`: as many slots at least (they never become fewer). All or
+        nothing: `CacheFull` where the held blocks, or a sequence's length, do not fit; `OutOfDeviceMemory`
+        where the device has no room for old and new storage together."""
         if max_tokens <= 0:
             raise ValueError(f"max_tokens must be positive, got {max_tokens}")
         blocks = -(-max_tokens // BLOCK)
         longest = min(self.max_positions, blocks * BLOCK)
         width = -(-longest // BLOCK)
+        slots = max(self.max_slots, max_slots or 0)
         for group in self.groups:
             if group.pool.held > blocks:
                 raise CacheFull(f"{group.pool.held} cache blocks are held, {blocks} would not hold them; "
@@ -276,21 +277,37 @@ class SequenceCache:
                 raise CacheFull(f"a sequence of {int(self.lengths[s])} positions does not fit a cache of "
                                 f"{longest} per sequence; nothing was changed")
         storage = [group.storage(blocks) for group in self.groups]
+        states = self.states if slots == self.max_slots else {
+            key: allocate(lambda: torch.zeros((slots,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device),
+                          f"the per-sequence state of cache entry {key}", slots * t[0].numel() * t.element_size())
+            for key, t in self.states.items()}
+        for group, new in zip(self.groups, storage):
+            held = sorted(group.pool._held)
+            self._copy(group.tensors, held, list(range(len(held))), into=[t for t in new if t is not None])
+        if states is not self.states:
+            live = sorted(self.slots._held)
+            self._copy(list(self.states.values()), live, live, into=list(states.values()), axis=0)
+        # (from here on nothing can fail)
         for group, (keys, values) in zip(self.groups, storage):
             held = sorted(group.pool._held)
-            self._copy(group.tensors, held, list(range(len(held))),
-                       into=[t for t in (keys, values) if t is not None])
             place = np.full(group.pool.size + 1, -1, dtype=np.int32)       # (the last: -1 stays -1)
             place[held] = np.arange(len(held), dtype=np.int32)
-            tables = np.full((self.max_slots, width), -1, dtype=np.int32)
+            tables = np.full((slots, width), -1, dtype=np.int32)
             kept = min(width, group.max_blocks_per_seq)
-            tables[:, :kept] = place[group.tables[:, :kept]]
+            tables[:self.max_slots, :kept] = place[group.tables[:, :kept]]
             holders = np.zeros(blocks, dtype=np.int32)
             holders[:len(held)] = group.holders[held]
             group.pool = Pool(blocks, "cache block")
             group.pool.take(len(held))
             group.keys, group.values = keys, values
             group.tables, group.holders, group.max_blocks_per_seq = tables, holders, width
+        more = slots - self.max_slots
+        if more:
+            self.states = states
+            self.slots.grow(slots)
+            self.lengths = np.concatenate([self.lengths, np.zeros(more, dtype=np.int64)])
+            self._front = [np.concatenate([f, np.zeros(more, dtype=np.int64)]) for f in self._front]
+            self.max_slots = slots
         self.blocks, self.max_tokens = blocks, blocks * BLOCK
         self.max_seq_len, self.max_blocks_per_seq = longest, width
         self.sharing += 1

@@ -153,7 +153,7 @@ class Engine:
             # (`OutOfDeviceMemory`) the engine still has no cache and can be asked again
             cache = SequenceCache(self.model.cache_needs(), self.max_tokens,
                                   self.spec.max_positions, act, self.device,
-                                  max_slots=min(-(-self.max_tokens // BLOCK), 4096),
+                                  max_slots=_slots_for(self.max_tokens),
                                   poison_freed=self.poison_freed)
             self.model.prepare(cache.max_seq_len)
             self.cache = cache
@@ -221,14 +221,14 @@ class Engine:
     def resize_cache(self, max_tokens: int) -> None:
         """Give the cache room for `max_tokens` positions, more or fewer, while sequences live: what they
         hold is moved together into new storage and the old is given up (`SequenceCache.resize`; nothing
-        changes where it raises `CacheFull` or `OutOfDeviceMemory`). The number of slots stays. Steps
+        changes where it raises `CacheFull` or `OutOfDeviceMemory`). Steps
         captured over the old storage are captured again when their shape comes up."""
         if max_tokens <= 0:
             raise ValueError(f"max_tokens must be positive, got {max_tokens}")
         if self.cache is not None:
             old = [t for group in self.cache.groups for t in group.tensors]
             with torch.cuda.device(self.device):
-                self.cache.resize(max_tokens)
+                self.cache.resize(max_tokens, _slots_for(max_tokens))
                 self._forget_storage()
                 ops.forget_descriptors(*old)
                 self.model.prepare(self.cache.max_seq_len)
@@ -258,9 +258,11 @@ class Engine:
             for g, group in enumerate(cache.groups):
                 if group.need != need:
                     continue
+                block = sum(t.numel() // (t.shape[0] * t.shape[1]) * t.element_size() for t in group.tensors)
+                if int(np.maximum(group.holders - 1, 0).sum()) * block < self.shared_bytes_worth:
+                    continue         # (all that anyone shares is too little: no plan is worked out)
                 plan = ops.plan_shared(tables[g][:, :width], ends, heads, need.kv_heads, None, reach=reach,
                                        roomy=True, slots=2 * _lib.sm_count(self.device))
-                block = sum(t.numel() // (t.shape[0] * t.shape[1]) * t.element_size() for t in group.tensors)
                 if plan.saved * block < self.shared_bytes_worth:
                     continue
                 place = (g, heads, plan.layout)
@@ -401,8 +403,7 @@ class Engine:
             self._decode_ran_eagerly = True
             return run()
         key = (ctx.sequences, tuple(tuple(t.shape) for t in ctx.tables), self._stager.generation,
-               self._slots_in_key(ctx, cache), greedy,
-               tuple((k, plan.layout) for k, plan in sorted(ctx.shared.items())))
+               self._slots_in_key(ctx, cache), greedy, _plans_in_key(ctx))
         entry = self._graphs.get(key)
         if entry is None:
             if len(self._graphs) >= 64:                 # shapes come and go; keep the table small
@@ -443,7 +444,7 @@ class Engine:
         longer than a short prompt's kernels run; a replay takes what the kernels take.
         Requests of a shape never seen again cost nothing but a dictionary entry."""
         key = (shape, tuple(tuple(t.shape) for t in ctx.tables), self._stager.generation,
-               self._slots_in_key(ctx, cache))
+               self._slots_in_key(ctx, cache), _plans_in_key(ctx))
         entry = self._prefill_graphs.get(key)
         if entry is None:                                   # first time: eagerly
             if len(self._prefill_graphs) >= 256:
@@ -594,7 +595,8 @@ class Engine:
                 for i, scores in zip(todo, group):
                     parts[i].append(scores)
                 todo = todo[len(group):]
-            joined = [torch.cat(p) if p else torch.empty(0, device=self.device) for p in parts]
+            joined = [torch.cat(p) if p else torch.empty(0, dtype=torch.float32, device=self.device)
+                      for p in parts]
             flat = torch.cat(joined).cpu().numpy() if joined else np.empty(0, np.float32)
             at = np.cumsum([0] + [len(c) for c in rest])
             return [flat[a:z] for a, z in zip(at, at[1:])]
@@ -804,6 +806,17 @@ class Engine:
         tokens = chosen.host.tolist()
         sampling.check_chosen(tokens, self.spec.vocab_size)
         return tokens
+
+
+def _plans_in_key(ctx) -> tuple:
+    """What a captured step keeps of the plans for shared blocks: their layouts (what they say lies on the
+    device, at an address of the layout's own)."""
+    return tuple((place, plan.layout) for place, plan in sorted(ctx.shared.items()))
+
+
+def _slots_for(max_tokens: int) -> int:
+    """Sequences that may live at one time in a cache of `max_tokens` positions."""
+    return min(-(-int(max_tokens) // BLOCK), 4096)
 
 
 class _Chosen:

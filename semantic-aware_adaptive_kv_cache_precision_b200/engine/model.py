@@ -84,7 +84,9 @@ class DecoderModel:
 
     def kernel_libraries(self) -> list:
         """The kernel libraries this model's steps launch, as far as its parts name them."""
-        names = ["elementwise", "sampling"]
+        names = ["elementwise", "sampling", "copy_blocks", "logprobs"]
+        if self.shared_readers():
+            names.append("attention_shared")
         for block in list(self.blocks) + [self.final_norm]:
             names += list(getattr(block, "kernel_libraries", ()))
         return list(dict.fromkeys(names))

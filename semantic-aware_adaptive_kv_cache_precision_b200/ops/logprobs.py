@@ -38,9 +38,9 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
         raise KernelError(f"token_logprobs: x {tuple(x.shape)} {x.dtype} does not fit the head {tuple(head.shape)} "
                           f"{head.dtype}")
     dtype_code(x.dtype)
-    if x.stride(1) != 1 or not head.is_contiguous():
-        raise KernelError("token_logprobs: x rows and the head must be contiguous")
     rows, vocab, k = x.shape[0], head.shape[0], head.shape[1]
+    if x.stride(1) != 1 and k > 1 or rows > 1 and x.stride(0) < k or not head.is_contiguous():
+        raise KernelError("token_logprobs: x rows and the head must be contiguous, x rows apart")
     if targets.dtype != torch.int32 or targets.shape != (rows,) or not targets.is_contiguous():
         raise KernelError(f"token_logprobs: targets must be contiguous int32 [{rows}]")
     if bias is not None and (bias.shape != (vocab,) or not bias.is_contiguous()):
@@ -51,6 +51,8 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
     if any(t is not None and t.device != x.device for t in (head, targets, bias)):
         raise KernelError("token_logprobs: tensors on different devices")
     require_cuda(x, head, targets, bias)
+    if rows == 1 or k == 1:                      # (strides that nothing depends on may be any number)
+        x = x.as_strided((rows, k), (max(k, x.stride(0)) if rows > 1 else k, 1))
     form = (ptr(bias), bias_code, float(scale), float(softcap))
     device = x.get_device()
     if device != torch.cuda.current_device():

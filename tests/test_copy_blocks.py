@@ -171,6 +171,27 @@ def test_a_cache_of_another_size_has_the_same_sequences(device, size):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_a_larger_cache_may_have_more_slots(device):
+    cache = make(device, max_tokens=3 * BLOCK, max_slots=2, window=80)
+    a, b = cache.open(2)
+    fill(cache, a, 70, 1)
+    fill(cache, b, 10, 2)
+    before = [content(cache, s) for s in (a, b)]
+    cache.resize(30 * BLOCK, 7)
+    cache.check()
+    assert cache.max_slots == 7 and all(t.shape[0] == 7 for t in cache.states.values())
+    assert all(same(content(cache, s), x) for s, x in zip((a, b), before))
+    new = cache.fork(a, 5)
+    assert new == [2, 3, 4, 5, 6] and all(same(content(cache, s), before[0]) for s in new)
+    with pytest.raises(CacheFull):
+        cache.open(1)
+    cache.close(new + [a, b])
+    cache.resize(BLOCK, 1)                       # slots never become fewer
+    cache.check()
+    assert cache.max_slots == 7 and cache.slots.free == 7
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_size_that_does_not_hold_the_sequences_is_refused(device):
     cache = make(device)
     a, b = cache.open(2)

@@ -219,6 +219,35 @@ def test_a_captured_step_reads_the_plan_of_the_moment(varied_folders):
 
 
 @pytest_gpu
+def test_captured_steps_that_want_some_logits_ask_whether_blocks_are_shared(varied_folders):
+    """A step of one token a sequence that does not want every logit is captured by its counts and starts: with
+    the same ones and nothing shared it is another step."""
+    engine = engine_of(varied_folders("D", "bfloat16"), "bfloat16", max_tokens=8192)
+    engine.shared_bytes_worth = 0
+    rng = np.random.default_rng(8)
+    prompts = [rng.integers(0, 400, 200).tolist() for _ in range(3)]
+
+    def wanted(slots):
+        out = engine.step(slots, [[5], [6], [7]], [[0], [], [0]]).cpu()
+        engine.close(slots)
+        return out
+
+    def shared(prompt):
+        (a,) = engine.open(1)
+        engine.step([a], [prompt])
+        return [a] + engine.fork(a, 2)
+
+    def alone(prompt):
+        slots = engine.open(3)
+        engine.step(slots, [prompt] * 3)
+        return slots
+
+    for prompt in prompts:                  # (the second time the shape comes up it is captured, the third replayed)
+        a, b = wanted(shared(prompt)), wanted(alone(prompt))
+        assert ((a - b).abs() <= 0.06 * b.std(-1, keepdim=True)).all()
+
+
+@pytest_gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_a_cache_of_another_size_between_steps(varied_folders, dtype):
     engine = engine_of(varied_folders("A", dtype), dtype, max_tokens=1024)
@@ -249,6 +278,7 @@ def test_a_cache_of_another_size_between_steps(varied_folders, dtype):
         engine.resize_cache(BLOCK)
     assert engine.max_tokens == 8192
     engine.close([a])
+    assert all(len(g) == 3 for g in engine.generate([prompt] * 40, 3, stop_at_eos=False))     # slots grew too
     engine.resize_cache(BLOCK)
     assert engine.generate(prompt, 5, stop_at_eos=False).shape == (5,)
 

@@ -17,7 +17,8 @@ def test_refusals():
                       ((x, w, t, torch.zeros(49)), {}), ((x, w, t, torch.zeros(50).double()), {}),
                       ((x, w[:0], t), {}), ((x[:, :0], w[:, :0], t), {}), ((x, w, t), {"softcap": -1.0}),
                       ((x, w, t), {"softcap": math.inf}), ((x, w, t), {"softcap": math.nan}),
-                      ((x.double(), w.double(), t), {})):
+                      ((x.double(), w.double(), t), {}), ((x[:1].expand(3, 16), w, t), {}),
+                      ((torch.zeros(40).as_strided((3, 16), (4, 1)), w, t), {})):
         with pytest.raises(KernelError):
             call(*args, **how)
     with pytest.raises(KernelError, match="CUDA device only"):
@@ -105,6 +106,11 @@ def test_operands_that_the_copies_do_not_take():
     check(33, 64, 500, torch.bfloat16, x_pad=3)            # rows of x likewise
     check(33, 64, 500, torch.bfloat16, x_pad=24)           # rows a multiple of 16 bytes apart
     check(40, 64, 500, torch.float32, x_pad=3)
+    for dtype in (torch.bfloat16, torch.float32):
+        check(5, 1, 300, dtype)                            # one number a row
+        x, w, targets, got, lse = check(1, 64, 300, dtype)
+        again, _ = ops.token_logprobs(x.as_strided((1, 64), (0, 1)), w, targets)     # a row's own stride means nothing
+        assert torch.equal(again, got)
 
 
 @pytest.mark.gpu
