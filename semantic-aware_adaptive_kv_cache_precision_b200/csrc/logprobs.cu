@@ -60,6 +60,27 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint16_t kBoth = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// two floats in a register pair, and arithmetic on them (sm_100: one instruction for both)
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t both(float a) { return two(a, a); }
+__device__ __forceinline__ void apart_two(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // What becomes of a product x . w before the softmax.
 struct Shape {
   const void* bias;          // or null
@@ -73,36 +94,48 @@ __device__ __forceinline__ float bias_at(const Shape& f, int v) {
                      : reinterpret_cast<const float*>(f.bias)[v];
 }
 
-// c tanh(z / c). tanh(y) = 1 - 2 / (e^2y + 1), and below 1/4, where that difference would cancel, the series
-// y - y^3/3 + 2 y^5/15 - 17 y^7/315 + 62 y^9/2835 (the next term is below 2^-26 of y there).
+// The tensor-core kernel works on logits in a unit of its own, so that what shapes them costs little: with a cap a
+// logit is c tanh(y), y = (x . w + b) scale / c, and t = tanh(y) stands for it in maxima and exponents, whose factor
+// takes the cap up; without one it stands for itself.
+struct Unit {
+  float mul;             // y or z = mul (x . w) + mul b
+  float size;            // natural units in one (the cap, or 1)
+  float rate;            // log2(e) size
+};
+__device__ __forceinline__ Unit unit_of(const Shape& f) {
+  const float size = f.cap > 0.f ? f.cap : 1.f;
+  return Unit{f.cap > 0.f ? f.scale * f.over_cap : f.scale, size, kLog2e * size};
+}
+
+// tanh(y) = 1 - 2 / (e^2y + 1), and below 1/4, where that difference would cancel, the series y - y^3/3 + 2 y^5/15
+// - 17 y^7/315 + 62 y^9/2835 (the next term is below 2^-26 of y there). Logits are mostly all near zero or not: a
+// run of them takes the series alone where it may.
 constexpr float kNear = 0.25f;
-__device__ __forceinline__ float capped_near(const Shape& f, float z) {
-  const float y = z * f.over_cap, q = y * y;
-  return f.cap * fmaf(y * q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y);
-}
-__device__ __forceinline__ float capped(const Shape& f, float z) {
-  const float y = z * f.over_cap;
-  // (2 log2(e) y is kept below 2^7, where the quotient is still one; NaN stays)
-  const float e = y > 40.f ? 40.f : y;
-  const float far = 1.f - __fdividef(2.f, 1.f + mma::exp2_fast(e * (2.f * kLog2e)));
-  return fabsf(y) < kNear ? capped_near(f, z) : f.cap * far;
-}
-// The same for a run of logits, which are mostly all near zero or not.
 template <int N>
-__device__ __forceinline__ void cap_all(const Shape& f, float (&z)[N]) {
-  float big = 0.f;
-  bool odd = false;
+__device__ __forceinline__ void tanh_all(float (&y)[N]) {
+  float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    big = fmaxf(big, fabsf(z[i]));
-    odd |= z[i] != z[i];
-  }
-  if (__any_sync(0xffffffffu, odd || !(big * f.over_cap < kNear))) {
+  for (int i = 0; i < N; i += 8)
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = capped(f, z[i]);
+    for (int q = 0; q < 4; ++q) big[q] = mma::max3(big[q], fabsf(y[i + 2 * q]), fabsf(y[i + 2 * q + 1]));
+  const bool far = !(fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) < kNear);      // (NaN is itself in the series)
+  if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      // (2 log2(e) y is kept below 2^7, where the quotient is still one; NaN stays)
+      const float e = y[i] > 40.f ? 40.f : y[i], q = y[i] * y[i];
+      const float t = 1.f - __fdividef(2.f, 1.f + mma::exp2_fast(e * (2.f * kLog2e)));
+      const float s = fmaf(y[i] * q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y[i]);
+      y[i] = fabsf(y[i]) < kNear ? s : t;
+    }
   } else {
+    const uint64_t c9 = both(62.f / 2835.f), c7 = both(-17.f / 315.f), c5 = both(2.f / 15.f), c3 = both(-1.f / 3.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = capped_near(f, z[i]);
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t v = two(y[i], y[i + 1]), q = mul_two(v, v);
+      const uint64_t s = fma_two(q, fma_two(q, fma_two(q, c9, c7), c5), c3);
+      apart_two(fma_two(mul_two(v, q), s, v), y[i], y[i + 1]);
+    }
   }
 }
 
@@ -163,15 +196,16 @@ __device__ __forceinline__ void ld_32x32b_x32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// e^(z - top), right where the difference is; top may be -inf only beside z = -inf (0) or NaN (NaN)
-__device__ __forceinline__ float weight_of(float z, float top) {
-  return mma::exp2_fast((z - (top == -INFINITY ? 0.f : top)) * kLog2e);
+// e^(size (z - top)), rate = log2(e) size; right where the difference is: top may be -inf only beside z = -inf (0) or
+// NaN (NaN)
+__device__ __forceinline__ float weight_of(float z, float top, float rate) {
+  return mma::exp2_fast((z - (top == -INFINITY ? 0.f : top)) * rate);
 }
 // Below this a maximum's product with log2(e) leaves the type's range, or nearly.
 constexpr float kLow = -2e38f;
 
 // 64 columns of a row joined to the row's running (maximum, sum).
-__device__ __forceinline__ void take_up(const float (&z)[64], float& top, float& sum) {
+__device__ __forceinline__ void take_up(const float (&z)[64], float rate, float& top, float& sum) {
   float big4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 64; c += 8)
@@ -179,20 +213,20 @@ __device__ __forceinline__ void take_up(const float (&z)[64], float& top, float&
     for (int q = 0; q < 4; ++q) big4[q] = mma::max3(big4[q], z[c + 2 * q], z[c + 2 * q + 1]);
   const float big = fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3]));
   if (big > top) {
-    sum = sum == 0.f ? 0.f : sum * weight_of(top, big);
+    sum = sum == 0.f ? 0.f : sum * weight_of(top, big, rate);
     top = big;
   }
   if (top < kLow) {                    // nothing so far, or values that a mask made the type's lowest
 #pragma unroll
-    for (int c = 0; c < 64; ++c) sum += weight_of(z[c], top);
+    for (int c = 0; c < 64; ++c) sum += weight_of(z[c], top, rate);
     return;
   }
-  const float base = top * kLog2e;
+  const float base = top * rate;
   float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 64; c += 2) {
     float e0, e1;
-    mma::fma2(e0, e1, z[c], z[c + 1], kLog2e, -base);
+    mma::fma2(e0, e1, z[c], z[c + 1], rate, -base);
     mma::add2(s4[c & 2], s4[(c & 2) + 1], mma::exp2_fast(e0), mma::exp2_fast(e1));
   }
   sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
@@ -343,6 +377,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     const int thread = quarter * 32 + lane;                          // lane of tensor memory
     const int worker = half * BM + thread;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const Unit unit = kPlain ? Unit{1.f, 1.f, kLog2e} : unit_of(p.form);
     const int first_rest = p.full * kMaxTokens;
     float2* run = tail->run[quarter];        // (a warp's own columns of it)
     for (int c = worker; c < kMaxTokens; c += kEpilogueThreads)
@@ -367,7 +402,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         const float* biases = tail->bias[wide & 1];
         if (!kPlain && p.form.bias) {
           for (int c = worker; c < cols; c += kEpilogueThreads)
-            tail->bias[wide & 1][c] = n0 + c < p.N ? bias_at(p.form, n0 + c) : 0.f;
+            tail->bias[wide & 1][c] = n0 + c < p.N ? bias_at(p.form, n0 + c) * unit.mul : 0.f;
           asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
         }
         ++wide;
@@ -384,12 +419,14 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
 #pragma unroll
               for (int i = 0; i < 64; i += 4) {
                 const float4 b = *reinterpret_cast<const float4*>(biases + c + i);
-                z[i] += b.x; z[i + 1] += b.y; z[i + 2] += b.z; z[i + 3] += b.w;
+                apart_two(fma_two(two(z[i], z[i + 1]), both(unit.mul), two(b.x, b.y)), z[i], z[i + 1]);
+                apart_two(fma_two(two(z[i + 2], z[i + 3]), both(unit.mul), two(b.z, b.w)), z[i + 2], z[i + 3]);
               }
-            }
+            } else {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) z[i] *= p.form.scale;
-            if (kCap) cap_all(p.form, z);
+              for (int i = 0; i < 64; i += 2) mma::mul2(z[i], z[i + 1], unit.mul);
+            }
+            if (kCap) tanh_all(z);
           }
           const int real = min(cols, p.N - n0) - c;         // columns of the 64 that are tokens' of this tile
           if (real < 64) {
@@ -402,9 +439,9 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
             float found = 0.f;
 #pragma unroll
             for (int i = 0; i < 64; ++i) found = at == i ? z[i] : found;
-            if (here) p.mine[m] = found;       // (a row behind the last token has no target)
+            if (here) p.mine[m] = found * unit.size;       // (a row behind the last token has no target)
           }
-          take_up(z, top, sum);
+          take_up(z, unit.rate, top, sum);
         }
         // the second warp of the quarter hands its share to the first
         if (half) tail->share[thread] = make_float2(top, sum);
@@ -412,9 +449,9 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         if (!half) {
           const float2 other = tail->share[thread];
           const float big = fmaxf(top, other.x);
-          sum = (sum == 0.f ? 0.f : sum * weight_of(top, big)) +
-                (other.y == 0.f ? 0.f : other.y * weight_of(other.x, big));
-          if (ok && m < p.M) p.part[(long long)n_tile * first_rest + m] = make_float2(big, sum);
+          sum = (sum == 0.f ? 0.f : sum * weight_of(top, big, unit.rate)) +
+                (other.y == 0.f ? 0.f : other.y * weight_of(other.x, big, unit.rate));
+          if (ok && m < p.M) p.part[(long long)n_tile * first_rest + m] = make_float2(big * unit.size, sum);
         }
         asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
       }
@@ -422,7 +459,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         // rows of the head on the lanes: this thread's row against the rest of the tokens
         const int v = n0 + rank * p.w_rows + thread;
         const bool real = thread < p.w_rows && v < p.N;
-        const float bias = !kPlain && p.form.bias && real ? bias_at(p.form, v) : 0.f;
+        const float bias = !kPlain && p.form.bias && real ? bias_at(p.form, v) * unit.mul : 0.f;
         if (!p.both) {             // (else it has been waited for)
           ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 806);
           tc::fence_after_sync();
@@ -434,8 +471,8 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           ld_32x32b_x32(acc + c, z);
           if (!kPlain) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = (z[i] + bias) * p.form.scale;
-            if (kCap) cap_all(p.form, z);
+            for (int i = 0; i < 32; ++i) z[i] = fmaf(z[i], unit.mul, bias);
+            if (kCap) tanh_all(z);
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
@@ -443,7 +480,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
             const int of[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if (of[j] == v && real) p.mine[first_rest + c + i + j] = z[i + j];
+              if (of[j] == v && real) p.mine[first_rest + c + i + j] = z[i + j] * unit.size;
               z[i + j] = real ? z[i + j] : -INFINITY;
             }
           }
@@ -454,9 +491,9 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           const float top = fmaxf(old.x, over_lanes<true>(most, lane));
           const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = mma::exp2_fast((z[i] - __shfl_sync(0xffffffffu, base, i)) * kLog2e);
+          for (int i = 0; i < 32; ++i) z[i] = mma::exp2_fast((z[i] - __shfl_sync(0xffffffffu, base, i)) * unit.rate);
           const float sum = over_lanes<false>(z, lane);
-          run[c + lane] = make_float2(top, (old.y == 0.f ? 0.f : old.y * weight_of(old.x, top)) + sum);
+          run[c + lane] = make_float2(top, (old.y == 0.f ? 0.f : old.y * weight_of(old.x, top, unit.rate)) + sum);
         }
       }
       tc::fence_before_sync();
@@ -474,9 +511,9 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float2 v = tail->run[w][c];
-        sum += v.y == 0.f ? 0.f : v.y * weight_of(v.x, top);
+        sum += v.y == 0.f ? 0.f : v.y * weight_of(v.x, top, unit.rate);
       }
-      part[c] = make_float2(top, sum);
+      part[c] = make_float2(top * unit.size, sum);
     }
   }
   tc::fence_before_sync();
