@@ -706,6 +706,19 @@ join_kernel(const Plan plan, const float* __restrict__ part_o, const float2* __r
 
 __device__ int g_error;
 
+// Where the current device has it (asked once a device).
+int* error_word() {
+  static int* known[PerDeviceOnce::kDevices] = {};
+  const int device = PerDeviceOnce::current();
+  if (device < 0 || device >= PerDeviceOnce::kDevices) return nullptr;
+  if (!known[device]) {
+    void* at = nullptr;
+    if (cudaGetSymbolAddress(&at, g_error) != cudaSuccess) return nullptr;
+    known[device] = static_cast<int*>(at);
+  }
+  return known[device];
+}
+
 template <int D>
 int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_bfloat16* out, cudaStream_t stream) {
   static PerDeviceOnce configured;
@@ -732,9 +745,10 @@ struct SakvSharedPlan {
   int width, unit_at, unit_capacity, member_at, first_at, partials, sequences, heads, kv_heads;
 };
 
-// `plan`: int32 words on the device, laid out as the numbers `n` (on the host) say; `part`: scratch of
+// `keys`, `values`: the cache entry [blocks][kv_heads][64][head_dim]; `plan`: int32 words on the device, laid out as the numbers `n` (on the host) say; `part`: scratch of
 // partials x heads x (head_dim + 2) floats.
-SAKV_EXPORT int sakv_shared_attention(const void* k_map, const void* v_map, const void* q, long long q_stride,
+SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long long blocks, const void* q,
+                                      long long q_stride,
                                       const int32_t* seq_lens, const int32_t* block_table, const int32_t* plan,
                                       const SakvSharedPlan* n, void* out, float* part, int head_dim, float scale,
                                       cudaStream_t stream) {
@@ -755,14 +769,16 @@ SAKV_EXPORT int sakv_shared_attention(const void* k_map, const void* v_map, cons
   p.part_o = part;
   p.part_ml = reinterpret_cast<float2*>(part + (long long)n->partials * heads * head_dim);
   p.scale_log2e = scale * 1.4426950408889634f;
-  p.error = nullptr;
-  if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p.error), g_error) != cudaSuccess) return cudaErrorInvalidValue;
-  const CUtensorMap& km = *reinterpret_cast<const CUtensorMap*>(k_map);
-  const CUtensorMap& vm = *reinterpret_cast<const CUtensorMap*>(v_map);
+  p.error = error_word();
+  if (!p.error) return cudaErrorInvalidValue;
+  const long long rows = blocks * kv_heads * KT;
+  if (blocks <= 0 || rows > 0x7fffffffLL || (head_dim != 64 && head_dim != 128)) return cudaErrorInvalidValue;
+  CUtensorMap km, vm;
+  int bad = tma::make_map_bf16_2d(&km, keys, (uint64_t)rows, head_dim, (uint64_t)head_dim * 2, KT, 64);
+  if (!bad) bad = tma::make_map_bf16_2d(&vm, values, (uint64_t)rows, head_dim, (uint64_t)head_dim * 2, KT, 64);
+  if (bad) return bad;
   __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
-  if (head_dim == 64) return launch<64>(km, vm, p, o, stream);
-  if (head_dim == 128) return launch<128>(km, vm, p, o, stream);
-  return cudaErrorInvalidValue;
+  return head_dim == 64 ? launch<64>(km, vm, p, o, stream) : launch<128>(km, vm, p, o, stream);
 }
 
 SAKV_EXPORT int sakv_shared_attention_error(int* value) {

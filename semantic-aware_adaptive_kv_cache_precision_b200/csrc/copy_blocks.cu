@@ -10,7 +10,9 @@
 // transfer of its own and no memory on the device. Of a block whose last positions are not filled only
 // the filled rows of every head are copied: a "chunk" of the block, `chunk_bytes` of every `chunk_pitch`.
 //
-// The order of the pieces is free: targets are distinct, and none is a source (the caller has checked).
+// The order of the pieces is free: targets are distinct, and none is a source.
+#include <string.h>
+
 #include "common.cuh"
 
 namespace {
@@ -78,11 +80,30 @@ struct SakvCopyTensor {
   long long from_entry, to_entry, block, entries, chunks, chunk_bytes, chunk_pitch;
 };
 
-// `tensors` descriptors and `pairs` (source, target) pairs, both on the HOST and read before the call
-// returns. No pair's target may be another pair's target, nor lie in memory that is a source.
-SAKV_EXPORT int sakv_copy_blocks(const SakvCopyTensor* tensor, int tensors, const int* pair, int pairs,
-                                 cudaStream_t stream) {
-  if (tensors < 0 || pairs < 0) return cudaErrorInvalidValue;
+// `tensors` descriptors and `pairs` block numbers to copy from and to, all on the HOST and read before the call
+// returns. Numbers lie in [0, blocks) and [0, room), a target is named once and, where the targets lie in the sources'
+// own tensors (`within`), is no source: else nothing is copied and the call returns -1.
+SAKV_EXPORT int sakv_copy_blocks(const SakvCopyTensor* tensor, int tensors, const int* source, const int* target,
+                                 int pairs, int blocks, int room, int within, cudaStream_t stream) {
+  if (tensors < 0 || pairs < 0 || blocks < 0 || room < 0) return cudaErrorInvalidValue;
+  for (int i = 0; i < pairs; ++i)
+    if (source[i] < 0 || source[i] >= blocks || target[i] < 0 || target[i] >= room) return -1;
+  if (pairs > 1 || within) {
+    const size_t n = within && blocks > room ? blocks : room;       // a byte a block: whether it is taken
+    uint8_t few[4096];
+    uint8_t* taken = n <= sizeof(few) ? few : static_cast<uint8_t*>(malloc(n));
+    if (!taken) return cudaErrorMemoryAllocation;
+    memset(taken, 0, n);
+    bool good = true;
+    if (within)
+      for (int i = 0; i < pairs; ++i) taken[source[i]] = 1;
+    for (int i = 0; i < pairs && good; ++i) {
+      good = !taken[target[i]];
+      taken[target[i]] = 1;
+    }
+    if (taken != few) free(taken);
+    if (!good) return -1;
+  }
   for (int t0 = 0; t0 < tensors; t0 += kMaxTensors) {
     const int n = tensors - t0 < kMaxTensors ? tensors - t0 : kMaxTensors;
     // the widest vector that every address and size of these tensors is a multiple of
@@ -101,7 +122,7 @@ SAKV_EXPORT int sakv_copy_blocks(const SakvCopyTensor* tensor, int tensors, cons
     p.tensors = n;
     for (int first = 0; first < pairs; first += kMaxPairs) {
       p.pairs = pairs - first < kMaxPairs ? pairs - first : kMaxPairs;
-      for (int i = 0; i < p.pairs; ++i) p.pair[i] = make_int2(pair[2 * (first + i)], pair[2 * (first + i) + 1]);
+      for (int i = 0; i < p.pairs; ++i) p.pair[i] = make_int2(source[first + i], target[first + i]);
       long long blocks = 0;
       for (int i = 0; i < n; ++i) {
         const SakvCopyTensor& x = tensor[t0 + i];

@@ -769,6 +769,19 @@ join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, con
 
 __device__ int g_error;
 
+// Where the current device has it (asked once a device).
+int* error_word() {
+  static int* known[PerDeviceOnce::kDevices] = {};
+  const int device = PerDeviceOnce::current();
+  if (device < 0 || device >= PerDeviceOnce::kDevices) return nullptr;
+  if (!known[device]) {
+    void* at = nullptr;
+    if (cudaGetSymbolAddress(&at, g_error) != cudaSuccess) return nullptr;
+    known[device] = static_cast<int*>(at);
+  }
+  return known[device];
+}
+
 int resident_pairs() {
   static int known[64] = {};
   int device = 0;
@@ -800,6 +813,15 @@ int resident_pairs() {
 // Whether one tile takes the 256 tokens and the rest of M tokens.
 bool both_of(int M, int full) { return full == 1 && M > kMaxTokens; }
 
+// The join of `pieces` partials [pieces][full] of rows below `full` and `rest_pieces` [.][M - full] of the others, which
+// lie behind them (full: a multiple of 256, perhaps past M, or M).
+int join(const float* part, const float* mine, const int32_t* targets, float* logprob, float* lse, int M, int N,
+         int full, int pieces, int rest_pieces, cudaStream_t stream) {
+  return launch_overlapped(join_kernel, dim3((M + 31) / 32), dim3(32 * kJoinWarps), 0, stream, 1,
+                           reinterpret_cast<const float2*>(part), mine, targets, logprob, lse, M, N, full, pieces,
+                           rest_pieces);
+}
+
 Shape shape_of(const void* bias, int bias_bf16, float scale, float cap) {
   Shape f;
   f.bias = bias; f.bias_bf16 = bias_bf16; f.scale = scale; f.cap = cap;
@@ -814,23 +836,26 @@ SAKV_EXPORT int sakv_logprob_fold_columns() { return kFoldColumns; }
 // Rows of the head a piece of the 32-bit kernel has.
 SAKV_EXPORT int sakv_logprob_f32_columns() { return kCols; }
 
-// The partials of x [M, K] (rows `x_stride` apart) against the head [N, K] in float32: part [ceil(N / 128)][M].
+// The log-probabilities of x [M, K] (rows `x_stride` apart) against the head [N, K] in float32: scratch part
+// [ceil(N / 128)][M] pairs, mine [M].
 SAKV_EXPORT int sakv_logprob_f32(const float* x, long long x_stride, const float* head, int M, int N, int K,
                                  const int32_t* targets, float* part, float* mine, const void* bias, int bias_bf16,
-                                 float scale, float cap, cudaStream_t stream) {
+                                 float scale, float cap, float* logprob, float* lse, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || x_stride < K || M > 0x7fffffff - 64 || !(cap >= 0.f)) return cudaErrorInvalidValue;
   const Shape form = shape_of(bias, bias_bf16, scale, cap);
   float2* to = reinterpret_cast<float2*>(part);
   const bool wide = K % 4 == 0 && x_stride % 4 == 0 &&
                     !((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(head)) & 15);
-#define SAKV_F32(TM)                                                                                       \
-  return wide ? launch_f32<TM, true>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)           \
-              : launch_f32<TM, false>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
+#define SAKV_F32(TM)                                                                                      \
+  e = wide ? launch_f32<TM, true>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)             \
+           : launch_f32<TM, false>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
+  int e;
   if (M <= 8) SAKV_F32(1);
-  if (M <= 16) SAKV_F32(2);
-  if (M <= 32) SAKV_F32(4);
-  SAKV_F32(8);
+  else if (M <= 16) SAKV_F32(2);
+  else if (M <= 32) SAKV_F32(4);
+  else SAKV_F32(8);
 #undef SAKV_F32
+  return e ? e : join(part, mine, targets, logprob, lse, M, N, M, (N + kCols - 1) / kCols, 0, stream);
 }
 
 // Pairs of SMs that can hold the tensor-core kernel at one time (0: it cannot run here).
@@ -882,10 +907,12 @@ static int logprob_map(CUtensorMap* map, const void* base, long long rows, long 
 }
 
 // The partials of x [M, K] against the head [N, K] in bf16 (rows of x `x_stride` apart; 16-byte aligned), cut as
-// `shape` (sakv_logprob_shape) says: part [shape[2]][256 shape[0]] and, behind it, [2 shape[3]][M - 256 shape[0]].
+// `shape` (sakv_logprob_shape) says, joined: scratch part [shape[2]][256 shape[0]] and, behind it, [2 shape[3]][M - 256
+// shape[0]] pairs, mine [M].
 SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const void* head, int M, int N, int K,
                                     const int* shape, const int32_t* targets, float* part, float* mine,
-                                    const void* bias, int bias_bf16, float scale, float cap, cudaStream_t stream) {
+                                    const void* bias, int bias_bf16, float scale, float cap, float* logprob,
+                                    float* lse, cudaStream_t stream) {
   int expect[4];
   const int here = resident_pairs();
   if (K <= 0 || (K % 8) || !(cap >= 0.f)) return cudaErrorInvalidValue;
@@ -904,8 +931,8 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const voi
   p.stages = kRingMost / p.stage_bytes < kMaxStages ? kRingMost / p.stage_bytes : kMaxStages;
   p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;
   p.form = shape_of(bias, bias_bf16, scale, cap);
-  p.error = nullptr;
-  if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p.error), g_error) != cudaSuccess) return cudaErrorInvalidValue;
+  p.error = error_word();
+  if (!p.error) return cudaErrorInvalidValue;
   CUtensorMap x_map, rest_map, w_map;
   int e = logprob_map(&w_map, head, N, K, K, p.w_rows);
   if (!e) e = logprob_map(&x_map, x, M, K, x_stride, p.full ? BM : p.rest_cols / 2);
@@ -929,7 +956,8 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const voi
   config.attrs = attr;
   config.numAttrs = 2;
   const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, x_map, rest_map, w_map, p);
-  return launched != cudaSuccess ? static_cast<int>(launched) : launch_status();
+  if (launched != cudaSuccess) return static_cast<int>(launched);
+  return join(part, mine, targets, logprob, lse, M, N, p.full * kMaxTokens, p.n_tiles, 2 * shape[3], stream);
 }
 
 // The same partials of a piece of logits in memory: z [M, n], columns `first`, first + 1, ... of the vocabulary;
@@ -945,15 +973,11 @@ SAKV_EXPORT int sakv_logprob_fold(const float* z, long long ld, int M, int n, in
                         reinterpret_cast<float2*>(part), mine, shape_of(bias, bias_bf16, scale, cap));
 }
 
-// The join of `pieces` partials [pieces][full] of rows below `full` and `rest_pieces` [.][M - full] of the others, which
-// lie behind them (full: a multiple of 256, perhaps past M, or M).
+// The join of a fold's partials [pieces][M].
 SAKV_EXPORT int sakv_logprob_join(const float* part, const float* mine, const int32_t* targets, float* logprob,
-                                  float* lse, int M, int N, int full, int pieces, int rest_pieces,
-                                  cudaStream_t stream) {
-  if (M <= 0 || pieces < 0 || rest_pieces < 0 || full < 0 || (full % 32 && full != M)) return cudaErrorInvalidValue;
-  return launch_overlapped(join_kernel, dim3((M + 31) / 32), dim3(32 * kJoinWarps), 0, stream, 1,
-                           reinterpret_cast<const float2*>(part), mine, targets, logprob, lse, M, N, full, pieces,
-                           rest_pieces);
+                                  float* lse, int M, int N, int pieces, cudaStream_t stream) {
+  if (M <= 0 || pieces < 0) return cudaErrorInvalidValue;
+  return join(part, mine, targets, logprob, lse, M, N, M, pieces, 0, stream);
 }
 
 SAKV_EXPORT int sakv_logprob_error(int* value) {

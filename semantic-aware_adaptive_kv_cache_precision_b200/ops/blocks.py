@@ -22,13 +22,6 @@ def _span(t: torch.Tensor) -> tuple:
     return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
 
 
-def _ids(ids, size: int, what: str) -> list:
-    ids = list(map(int, ids))
-    if ids and (min(ids) < 0 or max(ids) >= size):
-        raise KernelError(f"copy_blocks: {what} must lie in [0, {size}), got [{min(ids)}, {max(ids)}]")
-    return ids
-
-
 def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: int = 1) -> None:
     """Block `src[n]` of every tensor becomes block `dst[n]`, all in one launch (up to 16 tensors and
     1,024 pairs; more take further launches).
@@ -65,26 +58,41 @@ def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: 
         a, z = t.data_ptr(), u.data_ptr()
         table[i] = (a, z) + geometry
         spans.append((z, z + (geometry[1] or room * geometry[2]) * geometry[3]))
-    src, dst = _ids(src, blocks, "sources"), _ids(dst, room, "targets")
-    count = len(src)
-    if count != len(dst):
-        raise KernelError(f"copy_blocks: {count} sources, {len(dst)} targets")
-    if len(set(dst)) != count:
-        raise KernelError("copy_blocks: a target is named twice")
-    if into is None:
-        if not set(dst).isdisjoint(src):
-            raise KernelError("copy_blocks: a target is a source too")
-        if _overlap(spans):
-            raise KernelError("copy_blocks: tensors overlap")
-    elif _overlap(spans, [_span(t) for t in tensors]):
-        raise KernelError("copy_blocks: a target tensor overlaps another one")
-    if device < 0:
+    try:
+        source, target = array.array("i", src), array.array("i", dst)
+    except (TypeError, OverflowError):                        # (numbers of other kinds)
+        source, target = array.array("q", map(int, src)), array.array("q", map(int, dst))
+        _check_numbers(source, target, blocks, room, into is None)
+        source, target = array.array("i", source), array.array("i", target)
+    count = len(source)
+    if count != len(target):
+        raise KernelError(f"copy_blocks: {count} sources, {len(target)} targets")
+    if into is not None:
+        if _overlap(spans, [_span(t) for t in tensors]):
+            raise KernelError("copy_blocks: a target tensor overlaps another one")
+    elif len(spans) > 1 and _overlap(spans):
+        raise KernelError("copy_blocks: tensors overlap")
+    if device < 0 or empty or not count:
+        _check_numbers(source, target, blocks, room, into is None)
         require_cuda(*tensors)
-    if not count or empty:
         return
-    pairs = array.array("i", bytes(8 * count))
-    pairs[0::2], pairs[1::2] = array.array("i", src), array.array("i", dst)
-    call_on(device, "sakv_copy_blocks", ctypes.addressof(table), len(tensors), pairs.buffer_info()[0], count)
+    try:
+        call_on(device, "sakv_copy_blocks", table, len(tensors), source.buffer_info()[0], target.buffer_info()[0],
+                count, blocks, room, into is None)
+    except KernelError:
+        _check_numbers(source, target, blocks, room, into is None)
+        raise
+
+
+def _check_numbers(source, target, blocks: int, room: int, within: bool) -> None:
+    """Says what is wrong with the numbers of a copy, if anything is."""
+    for ids, size, what in ((source, blocks, "sources"), (target, room, "targets")):
+        if len(ids) and (min(ids) < 0 or max(ids) >= size):
+            raise KernelError(f"copy_blocks: {what} must lie in [0, {size}), got [{min(ids)}, {max(ids)}]")
+    if len(set(target)) != len(target):
+        raise KernelError("copy_blocks: a target is named twice")
+    if within and not set(target).isdisjoint(source):
+        raise KernelError("copy_blocks: a target is a source too")
 
 
 def _geometry(t, u, rows, axis, blocks, room) -> tuple:

@@ -7,7 +7,7 @@ import ctypes
 
 import torch
 
-from . import gemm_wide
+from . import _lib
 from ._lib import F32, KernelError, call, dtype_code, plain_function, ptr, require_cuda
 from .linear import linear
 
@@ -33,6 +33,28 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
     softcap > 0. `x` [T, K] and `head` [vocab, K] of one type, float32 or bfloat16; `bias` [vocab] float32 or
     bfloat16. A negative target asks for nothing and gets 0; one past the vocabulary gets NaN. A row with a
     logit that is NaN or +inf has NaN; logits of -inf count for nothing."""
+    device, dtype = x.get_device(), x.dtype
+    # (one expression for the calls that are right; `_refuse` says what is wrong with the others)
+    if not (x.dim() == 2 and head.dim() == 2 and targets.dim() == 1 and dtype is head.dtype
+            and (dtype is torch.bfloat16 or dtype is torch.float32) and x.stride(1) == 1 and head.is_contiguous()
+            and 0 < x.shape[1] == head.shape[1] and head.shape[0] > 0
+            and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1)
+            and targets.dtype is torch.int32 and targets.shape[0] == x.shape[0] and targets.is_contiguous()
+            and 0.0 <= softcap < float("inf")
+            and device >= 0 and head.get_device() == device and targets.get_device() == device
+            and (bias is None or bias.dim() == 1 and bias.shape[0] == head.shape[0] and bias.is_contiguous()
+                 and bias.get_device() == device
+                 and (bias.dtype is torch.float32 or bias.dtype is torch.bfloat16))):
+        x = _refuse(x, head, targets, bias, softcap)
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _token_logprobs(x, head, targets, bias, scale, softcap)
+    return _token_logprobs(x, head, targets, bias, scale, softcap)
+
+
+def _refuse(x, head, targets, bias, softcap) -> torch.Tensor:
+    """Says what is wrong with a call of `token_logprobs`, or gives x with strides that mean something (of one
+    row, or one number a row, torch's may be any)."""
     if x.dim() != 2 or head.dim() != 2 or x.shape[1] != head.shape[1] or x.dtype != head.dtype \
             or head.shape[0] == 0 or x.shape[1] == 0:
         raise KernelError(f"token_logprobs: x {tuple(x.shape)} {x.dtype} does not fit the head {tuple(head.shape)} "
@@ -45,55 +67,73 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
         raise KernelError(f"token_logprobs: targets must be contiguous int32 [{rows}]")
     if bias is not None and (bias.shape != (vocab,) or not bias.is_contiguous()):
         raise KernelError(f"token_logprobs: bias must be contiguous [{vocab}]")
-    bias_code = F32 if bias is None else dtype_code(bias.dtype)
+    if bias is not None:
+        dtype_code(bias.dtype)
     if not softcap >= 0.0 or softcap == float("inf"):
         raise KernelError(f"token_logprobs: softcap must be a number >= 0, got {softcap}")
     if any(t is not None and t.device != x.device for t in (head, targets, bias)):
         raise KernelError("token_logprobs: tensors on different devices")
     require_cuda(x, head, targets, bias)
-    if rows == 1 or k == 1:                      # (strides that nothing depends on may be any number)
-        x = x.as_strided((rows, k), (max(k, x.stride(0)) if rows > 1 else k, 1))
-    form = (ptr(bias), bias_code, float(scale), float(softcap))
-    device = x.get_device()
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _token_logprobs(x, head, targets, bias, form)
-    return _token_logprobs(x, head, targets, bias, form)
+    return x.as_strided((rows, k), (max(k, x.stride(0)) if rows > 1 else k, 1))
 
 
-def _token_logprobs(x, head, targets, bias, form):
-    rows, vocab, k = x.shape[0], head.shape[0], head.shape[1]
-    logprob = x.new_empty(rows, dtype=torch.float32)
-    lse, mine = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+_shapes: dict = {}
+
+
+def _shape(rows: int, vocab: int):
+    """How the tensor-core kernel cuts so many rows and tokens on this device: (the numbers the launch takes, floats
+    of scratch)."""
+    pairs = _pairs()
+    hit = _shapes.get((rows, vocab, pairs))
+    if hit is None:
+        shape = (ctypes.c_int * 4)()
+        if plain_function("sakv_logprob_shape")(rows, vocab, pairs, shape) != 0:
+            raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
+        full = shape[0] * 256
+        if len(_shapes) >= 256:
+            _shapes.clear()
+        hit = _shapes[rows, vocab, pairs] = (shape, 2 * (shape[2] * full + 2 * shape[3] * max(0, rows - full)))
+    return hit
+
+
+def _token_logprobs(x, head, targets, bias, scale, softcap):
+    rows, k = x.shape
+    vocab, stride = head.shape[0], x.stride(0)
+    logprob, lse = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
     if rows == 0:
         return logprob, lse
-    if gemm_wide.takes(x, head) and _pairs() > 0:
-        shape = (ctypes.c_int * 4)()
-        if plain_function("sakv_logprob_shape")(rows, vocab, _pairs(), shape) != 0:
-            raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
-        full, pieces, rest_pieces = shape[0] * 256, shape[2], 2 * shape[3]
-        part = x.new_empty(2 * (pieces * full + rest_pieces * max(0, rows - full)), dtype=torch.float32)
-        call("sakv_logprob_pieces", ptr(x), x.stride(0), ptr(head), rows, vocab, k, shape, ptr(targets),
-             ptr(part), ptr(mine), *form)
-    elif x.dtype == torch.float32:
-        full, pieces, rest_pieces = rows, -(-vocab // plain_function("sakv_logprob_f32_columns")()), 0
-        part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
-        call("sakv_logprob_f32", ptr(x), x.stride(0), ptr(head), rows, vocab, k, ptr(targets), ptr(part),
-             ptr(mine), *form)
-    else:
+    if rows == 1:
+        stride = k
+    at, head_at = x.data_ptr(), head.data_ptr()
+    bias_at, bias_code = (None, F32) if bias is None else (bias.data_ptr(), dtype_code(bias.dtype))
+    if x.dtype is torch.bfloat16 and k % 8 == 0 and stride % 8 == 0 and (at | head_at) % 16 == 0 and _pairs() > 0:
+        shape, floats = _shape(rows, vocab)
+        part = x.new_empty(floats + rows, dtype=torch.float32)
+        scratch = part.data_ptr()
+        call("sakv_logprob_pieces", at, stride, head_at, rows, vocab, k, shape, targets.data_ptr(), scratch,
+             scratch + 4 * floats, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
+        _lib.launches += 1          # the call launched the join too
+    elif x.dtype is torch.float32:
+        floats = 2 * rows * -(-vocab // plain_function("sakv_logprob_f32_columns")())
+        part = x.new_empty(floats + rows, dtype=torch.float32)
+        scratch = part.data_ptr()
+        call("sakv_logprob_f32", at, stride, head_at, rows, vocab, k, targets.data_ptr(), scratch,
+             scratch + 4 * floats, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
+        _lib.launches += 1
+    else:                           # bfloat16 rows that TMA cannot take: logits a piece at a time
         columns = plain_function("sakv_logprob_fold_columns")()
         most = max(1, PIECE_ELEMENTS // columns)
         if rows > most:                # (the scratch of a piece stays as large as it is for these)
-            parts = [_token_logprobs(x[i:i + most], head, targets[i:i + most], bias, form)
+            parts = [_token_logprobs(x[i:i + most], head, targets[i:i + most], bias, scale, softcap)
                      for i in range(0, rows, most)]
             return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
         piece = max(1, min(-(-vocab // columns), PIECE_ELEMENTS // (rows * columns))) * columns
-        full, pieces, rest_pieces = rows, -(-vocab // columns), 0
-        part = torch.empty((pieces, rows, 2), dtype=torch.float32, device=x.device)
+        pieces = -(-vocab // columns)
+        part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
+        mine = x.new_empty(rows, dtype=torch.float32)
         for first in range(0, vocab, piece):
             z = linear(x, head[first:first + piece], out_dtype=torch.float32)
             call("sakv_logprob_fold", ptr(z), z.stride(0), rows, z.shape[1], first, vocab, ptr(targets),
-                 ptr(part[first // columns]), ptr(mine), *form)
-    call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, full, pieces,
-         rest_pieces)
+                 ptr(part[first // columns]), ptr(mine), bias_at, bias_code, scale, softcap)
+        call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, pieces)
     return logprob, lse

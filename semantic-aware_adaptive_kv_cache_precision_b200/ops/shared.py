@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from ._lib import CACHE_BLOCK, KernelError, call_on, require_cuda, sm_count
-from .attention import fast_path_takes, tensor_map
+from .attention import fast_path_takes
 
 UNIT_ROWS = 128           # most rows (sequences x query heads of one KV head) of a unit of work
 MOST_GROUP = 64           # most query heads of one KV head
@@ -190,10 +190,11 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     q_shape, k_shape, device = qkv.shape, k_cache.shape, qkv.get_device()
     # (one expression for the calls that are right: a decode step outside a captured graph is bound by the
     # host's work; `_refuse` says what is wrong with the others)
-    if not (qkv.dtype is torch.bfloat16 and (head_dim == 128 or head_dim == 64) and heads % kv_heads == 0
+    if not (qkv.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
+            and (head_dim == 128 or head_dim == 64) and heads % kv_heads == 0
             and heads <= 16 * kv_heads and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
             and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
-            and k_shape == v_cache.shape and len(k_shape) == 4 and k_shape[1] == kv_heads
+            and k_shape == v_cache.shape and len(k_shape) == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() and k_shape[1] == kv_heads
             and k_shape[2] == CACHE_BLOCK and k_shape[3] == head_dim
             and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32
             and seq_lens.dim() == 1 and block_table.dim() == 2
@@ -204,11 +205,12 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
             == block_table.get_device() == plan.words.get_device()):
         _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim)
     sequences = q_shape[0]
-    out = qkv.new_empty((sequences, heads * head_dim))
+    width = heads * head_dim
+    out = torch.empty_like(qkv) if q_shape[1] == width and qkv.is_contiguous() else qkv.new_empty((sequences, width))
     if sequences == 0:
         return out
-    part = qkv.new_empty(plan.partials * heads * (head_dim + 2), dtype=torch.float32)
-    call_on(device, "sakv_shared_attention", tensor_map(k_cache), tensor_map(v_cache), qkv.data_ptr(),
+    part = qkv.new_empty(2 * plan.partials * heads * (head_dim + 2))          # (as many floats)
+    call_on(device, "sakv_shared_attention", k_cache.data_ptr(), v_cache.data_ptr(), k_shape[0], qkv.data_ptr(),
             qkv.stride(0), seq_lens.data_ptr(), block_table.data_ptr(), plan.words.data_ptr(),
             ctypes.addressof(plan.numbers), out.data_ptr(), part.data_ptr(), head_dim, scale)
     if plan.unit_capacity:
@@ -225,9 +227,9 @@ def _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads,
         raise KernelError("shared_decode_attention: qkv must be [B, >= heads * head_dim], rows contiguous")
     for cache in (k_cache, v_cache):
         if cache.dim() != 4 or tuple(cache.shape[1:]) != (kv_heads, CACHE_BLOCK, head_dim) \
-                or cache.shape != k_cache.shape:
-            raise KernelError(f"shared_decode_attention: cache entries must be [blocks, {kv_heads}, {CACHE_BLOCK}, "
-                              f"{head_dim}]")
+                or cache.shape != k_cache.shape or not cache.is_contiguous() or cache.dtype != torch.bfloat16:
+            raise KernelError(f"shared_decode_attention: cache entries must be contiguous bf16 [blocks, {kv_heads}, "
+                              f"{CACHE_BLOCK}, {head_dim}]")
     sequences = qkv.shape[0]
     for t, shape in ((seq_lens, (sequences,)), (block_table, (sequences, plan.width))):
         if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
