@@ -306,6 +306,45 @@ def test_samples_that_end_and_a_full_cache(varied_folders):
 
 
 @pytest_gpu
+def test_targets_of_a_step(varied_folders):
+    engine = engine_of(varied_folders("A"))
+    a, b = engine.open(2)
+    got = engine.step([a, b], [[1, 2, 3], [4, 5]], [[0, 2, 2], []], targets=[[7, 8, 511], []])
+    assert got.shape == (3,) and got.dtype == torch.float32
+    z = torch.log_softmax(torch.from_numpy(engine.forward([1, 2, 3])).double(), -1)
+    np.testing.assert_allclose(got.cpu().numpy(), [z[0, 7], z[2, 8], z[2, 511]], rtol=0, atol=2e-4)
+    assert engine.step([a, b], [[1], [2]], [[], []], targets=[[], []]).shape == (0,)
+    lengths = engine.cache.lengths[[a, b]].tolist()
+    for how in (dict(targets=[[1, 2], [3]]), dict(targets=[[1]]), dict(targets=[[512], [3]]), dict(targets=[[-1], [3]]),
+                dict(targets=[[1], [3]], hidden_states=[])):
+        with pytest.raises(ValueError):
+            engine.step([a, b], [[1], [2]], **how)
+    assert engine.cache.lengths[[a, b]].tolist() == lengths
+    engine.close([a, b])
+
+
+@pytest_gpu
+def test_little_that_is_shared_is_read_by_everyone(varied_folders):
+    """Below the bytes that pay, no plan is made and the step is the one of sequences of their own, to the bit."""
+    engine = engine_of(varied_folders("D", "bfloat16"), "bfloat16")
+    rng = np.random.default_rng(9)
+    prompt = rng.integers(0, 400, 300).tolist()
+    (a,) = engine.open(1)
+    engine.step([a], [prompt])
+    slots = [a] + engine.fork(a, 3)
+    out = [engine.step(slots, [[t]] * 4).cpu() for t in (1, 2, 3)]
+    assert engine._shared_now[2] == {} and not engine._shared_buffers
+    assert all(torch.equal(o[0], row) for o in out for row in o)
+    engine.close(slots)
+    engine.shared_bytes_worth = None
+    (a,) = engine.open(1)
+    engine.step([a], [prompt])
+    slots = [a] + engine.fork(a, 3)
+    assert all(torch.equal(o, engine.step(slots, [[t]] * 4).cpu()) for o, t in zip(out, (1, 2, 3)))
+    engine.close(slots)
+
+
+@pytest_gpu
 def test_the_command_line(varied_folders, capsys):
     from semantic_aware_adaptive_kv_cache_precision_b200.cli import main
     folder = str(varied_folders("A"))
