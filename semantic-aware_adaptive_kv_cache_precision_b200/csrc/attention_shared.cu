@@ -5,7 +5,7 @@
 //
 // for the positions j of a sequence's length. The sum may be cut anywhere and joined: a piece with its own
 // (m, l, o = sum e^(s - m) v) enters with weight e^(m - max m). The host's plan cuts the block lists into
-// pieces that the same set of sequences lists (ops/shared.py); a unit of work is a piece, up to 64 rows of
+// pieces that the same set of sequences lists (ops/shared.py); a unit of work is a piece, up to 128 rows of
 // queries (sequences of the piece x query heads of one KV head) and that KV head.
 //
 //   grid  = units x KV heads, heaviest first; block = 6 warps, two blocks an SM

@@ -5,6 +5,7 @@ end, and serves every layer of every step until the next such change."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -42,10 +43,10 @@ def common_runs(tables: np.ndarray, lengths: np.ndarray, reach: np.ndarray) -> l
         at = np.maximum.accumulate(np.where(begins, np.arange(count)[:, None], 0), axis=0)
         lead = np.empty_like(order)
         np.put_along_axis(lead, order, np.take_along_axis(order, at, axis=0), axis=0)
-        alone = np.arange(count)[:, None] == lead
-        crowd = np.zeros_like(alone)                      # whether anyone else is in the sequence's group
-        np.logical_or.at(crowd, (lead, np.broadcast_to(np.arange(used), lead.shape)), ~alone)
-        crowd = np.take_along_axis(crowd, lead, axis=0)
+        several = ~begins                                 # whether anyone else is in the sequence's group
+        several[:-1] |= ~begins[1:]
+        crowd = np.empty_like(several)
+        np.put_along_axis(crowd, order, several, axis=0)
         changes = [0] + (1 + np.flatnonzero((lead[:, 1:] != lead[:, :-1]).any(axis=0))).tolist() + [used]
         open_runs = {}
         for c0, c1 in zip(changes, changes[1:]):
@@ -73,16 +74,54 @@ def common_runs(tables: np.ndarray, lengths: np.ndarray, reach: np.ndarray) -> l
     return runs
 
 
+# What a unit of work takes where an SM holds two, in us: to start and end, and a block of keys and values (measured
+# at head sizes of 64 and 128: 0.9 to 1.1), with more than NARROW_ROWS rows and with fewer; what a partial's
+# trip through memory takes, in us a (sequence, head), and its place in the sum over a sequence's partials.
+WIDE_US, NARROW_US, NARROW_ROWS, PARTIAL_US, JOIN_US = (6.0, 1.0), (4.0, 1.0), 32, 1.7e-4, 0.08
+
+
+def _unit_us(rows: np.ndarray) -> tuple:
+    wide = rows > NARROW_ROWS
+    return np.where(wide, WIDE_US[0], NARROW_US[0]), np.where(wide, WIDE_US[1], NARROW_US[1])
+
+
 def choose_piece(runs: list, group: int, kv_heads: int, slots: int) -> int:
-    """Into pieces of how many blocks the runs are cut: the fewest with which the units of work do not
-    outnumber `slots`, the thread blocks that run at one time."""
+    """Into pieces of how many blocks the runs are cut: of some twenty sizes the one whose units, dealt to `slots`
+    thread blocks the longest first, are done first. (Counting units alone, as many as there are slots, made
+    pieces as long as the prompts where many short tails took the slots: 40 heads over 8, 30 sequences of 5
+    prompts of 24,000 positions, 267 us a layer, now 49; 16 over 1, 8 of 2 prompts of 16,700: 19.5, now 14.4.)"""
+    rows_of = np.array([len(members) * group for members, _, _ in runs], dtype=np.int64)
     sizes = np.array([c1 - c0 for _, c0, c1 in runs], dtype=np.int64)
-    tiles = np.array([-(-len(m) * group // UNIT_ROWS) for m, _, _ in runs], dtype=np.int64) * kv_heads
+    # (a run's rows: whole units and, where some are left, one more)
+    rest = rows_of % UNIT_ROWS
+    rows = np.concatenate([np.full_like(rest, UNIT_ROWS), rest])
+    tiles = np.concatenate([rows_of // UNIT_ROWS, rest > 0])
+    kept = tiles > 0
+    rows, tiles, sizes = rows[kept], tiles[kept] * kv_heads, np.concatenate([sizes, sizes])[kept]
+    starts, slopes = _unit_us(rows)
+    rows = rows * tiles
     longest = int(sizes.max(initial=1))
-    piece = max(1, int((sizes * tiles).sum()) // max(1, slots))
-    while piece < longest and int((-(-sizes // piece) * tiles).sum()) > slots:
-        piece += max(1, piece // 16)
-    return min(piece, longest)
+    best, chosen, piece = math.inf, longest, max(1, int((sizes * tiles).sum() / (3 * slots)))
+    while True:
+        pieces = np.ceil(sizes / piece)
+        costs = starts + slopes * np.ceil(sizes / pieces)
+        counts = pieces * tiles
+        least = float(costs.max())
+        after = PARTIAL_US * float((pieces * rows).sum()) + JOIN_US * float(pieces.max())
+        if max(least, float((costs * counts).sum()) / slots) + after < best:
+            order = np.argsort(-costs)
+            todo = np.repeat(costs[order], counts[order].astype(np.int64))
+            done = np.zeros(slots)
+            for i in range(0, len(todo), slots):
+                some = todo[i:i + slots]
+                done.sort()
+                done[:len(some)] += some
+            took = float(done.max()) + after
+            if took < best:
+                best, chosen = took, piece
+        if piece >= longest or least >= best:
+            return chosen
+        piece = min(longest, piece + max(1, piece // 5))
 
 
 class _Numbers(ctypes.Structure):
@@ -112,6 +151,12 @@ class SharedPlan:
         return other
 
 
+def _spread(counts: np.ndarray) -> tuple:
+    """For `counts[i]` things each: the i of each thing, and its number among those of i."""
+    of = np.repeat(np.arange(len(counts)), counts)
+    return of, np.arange(len(of)) - (np.cumsum(counts) - counts)[of]
+
+
 def _round_up(n: int, to: int) -> int:
     return -(-n // to) * to
 
@@ -138,27 +183,37 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     group = heads // kv_heads
     runs = common_runs(tables, lengths, reach)
     piece = choose_piece(runs, group, kv_heads, slots or 2 * sm_count(device)) if runs else 1
-    pieces = []                                            # (members, first column, columns)
-    for members, c0, c1 in runs:
-        n = -(-(c1 - c0) // piece)
-        for i in range(n):                                 # (even pieces)
-            a, z = c0 + (c1 - c0) * i // n, c0 + (c1 - c0) * (i + 1) // n
-            pieces.append((members, a, z - a))
-    # a sequence's partials in the order of its positions
-    pieces.sort(key=lambda p: p[1])
-    counts = np.zeros(count, dtype=np.int64)
-    place = []
-    for members, _, _ in pieces:
-        place.append([int(counts[b]) for b in members])
-        counts[list(members)] += 1
-    first = np.concatenate([[0], np.cumsum(counts)])
-    units, pairs = [], []
-    for (members, c0, n), where in zip(pieces, place):
-        rows = len(members) * group
-        for r in range(0, rows, UNIT_ROWS):
-            units.append((members[0], c0, n, len(pairs) + r // group, r % group, min(UNIT_ROWS, rows - r), 0, 0))
-        pairs += [(b, int(first[b]) + w) for b, w in zip(members, where)]
-    units.sort(key=lambda u: -u[2] * (1 + u[5] // 16))                # the heaviest start first
+    counted = np.array([len(members) for members, _, _ in runs], dtype=np.int64)
+    ends = np.array([run[1:] for run in runs], dtype=np.int64).reshape(-1, 2)
+    listing = np.array([b for members, _, _ in runs for b in members], dtype=np.int64)
+    listed_at = np.cumsum(counted) - counted
+    # the runs in even pieces, in the order of their positions
+    sizes = ends[:, 1] - ends[:, 0]
+    many = -(-sizes // piece)
+    run, i = _spread(many)
+    begins = ends[run, 0] + sizes[run] * i // many[run]
+    columns = ends[run, 0] + sizes[run] * (i + 1) // many[run] - begins
+    order = np.argsort(begins, kind="stable")
+    run, begins, columns = run[order], begins[order], columns[order]
+    # each piece's members; a sequence's partials lie in the order of its positions
+    members = counted[run]
+    pairs_at = np.cumsum(members) - members
+    of, i = _spread(members)
+    sequence = listing[listed_at[run[of]] + i]
+    partial = np.empty_like(sequence)
+    partial[np.argsort(sequence, kind="stable")] = np.arange(len(sequence))
+    pairs = np.stack([sequence, partial], axis=1)
+    first = np.concatenate([[0], np.cumsum(np.bincount(sequence, minlength=count))])
+    # a piece's rows in units, those that take longest first
+    rows = members * group
+    of, i = _spread(-(-rows // UNIT_ROWS))
+    r = i * UNIT_ROWS
+    some = np.minimum(UNIT_ROWS, rows[of] - r)
+    nothing = np.zeros_like(of)
+    units = np.stack([listing[listed_at[run[of]]], begins[of], columns[of], pairs_at[of] + r // group, r % group,
+                      some, nothing, nothing], axis=1)
+    start, slope = _unit_us(some)
+    units = units[np.argsort(-(start + slope * columns[of]), kind="stable")]
     plan = SharedPlan()
     plan.sequences, plan.heads, plan.kv_heads, plan.width = count, heads, kv_heads, width
     plan.units, plan.reach = len(units), reach
@@ -168,13 +223,12 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     plan.unit_at = 8
     plan.member_at = plan.unit_at + UNIT_WORDS * plan.unit_capacity
     plan.first_at = plan.member_at + 2 * members_room
-    plan.saved = int(sum((len(m) - 1) * (c1 - c0) for m, c0, c1 in runs))
+    plan.saved = int(((counted - 1) * sizes).sum())
     words = np.zeros(_round_up(plan.first_at + count + 1, 4), dtype=np.int32)
     plan.numbers = _Numbers(*(getattr(plan, name) for name, _ in _Numbers._fields_))
     words[0], words[1] = len(units), count
-    if units:
-        words[8:8 + UNIT_WORDS * len(units)] = np.asarray(units, dtype=np.int32).reshape(-1)
-        words[plan.member_at:plan.member_at + 2 * len(pairs)] = np.asarray(pairs, dtype=np.int32).reshape(-1)
+    words[8:8 + UNIT_WORDS * len(units)] = units.reshape(-1)
+    words[plan.member_at:plan.member_at + 2 * len(pairs)] = pairs.reshape(-1)
     words[plan.first_at:plan.first_at + count + 1] = first
     plan.words = words if device is None else torch.from_numpy(words).to(device)
     return plan

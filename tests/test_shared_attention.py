@@ -112,8 +112,11 @@ def test_a_last_block_that_is_not_filled_is_nobody_elses():
 def test_pieces_fill_the_slots():
     runs = [(tuple(range(64)), 0, 500)] + [((b,), 500, 508) for b in range(64)]
     piece = choose_piece(runs, 6, 2, 296)
-    units = sum(-(-(z - a) // piece) * -(-len(m) * 6 // 128) * 2 for m, a, z in runs)
-    assert units <= 296 or piece == 500
+    assert 8 <= piece <= 40
+    # many short tails do not make the prompts' pieces long
+    runs = [(tuple(range(6 * p, 6 * p + 6)), 0, 374) for p in range(5)] + [((b,), 374, 380) for b in range(30)]
+    assert choose_piece(runs, 5, 8, 296) <= 100
+    assert choose_piece([((0,), 0, 1)], 6, 2, 296) == 1 and choose_piece([((0,), 0, 400)], 1, 1, 1) >= 100
 
 
 def test_refusals():
