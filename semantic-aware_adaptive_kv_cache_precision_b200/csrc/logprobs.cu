@@ -7,7 +7,7 @@
 // value, a common mask, times log2(e) would be -inf), and whoever meets the target's column leaves z_target; `join_kernel` merges the pieces. 2,048 tokens over 151,936 logits would be
 // 1.2 GB written and read again; the pieces are 10 MB.
 //
-// Two ways to a piece. bfloat16 operands: tcgen05 on PAIRS of SMs (`cta_group::2`), the softmax's sums in the
+// Ways to a piece. bfloat16 operands: tcgen05 on PAIRS of SMs (`cta_group::2`), the softmax's sums in the
 // epilogue. A pair takes a tile of the head's rows (up to 128 a block) against
 //   256 tokens   tokens on tensor memory's lanes, the head's rows its columns: thread = token row, so that no sum
 //                crosses a thread, or
@@ -25,9 +25,10 @@
 // Tiles of one piece of the head lie side by side in time, so the head comes from memory once. Up to some 256
 // tokens its bytes bound the kernel, above the tensor cores. The tile's height is chosen so that the last round
 // of tiles is not nearly empty (see the launcher).
-// float32 operands: plain multiply-adds, each sum over k and each row's sums over the vocabulary in one order
-// whatever rows are beside it, as in the other 32-bit products. bfloat16 rows that TMA cannot take: `fold_kernel`
-// reads a piece of logits that a product of its own left in a scratch.
+// float32 operands: each number as three of bfloat16 on the tensor cores (`split_logprob_kernel`), or plain multiply-adds
+// where the head's rows are not aligned; each sum over k and each row's sums over the vocabulary in one order whatever
+// rows are beside it, as in the other 32-bit products. bfloat16 rows that TMA cannot take: `fold_kernel` reads a piece
+// of logits that a product of its own left in a scratch.
 //
 // Sums and maxima are fp32. Every mbarrier wait is bounded, and a pair leaves together.
 // The reference keeps all logits (`src/microinfer/model.py:388-402`).
@@ -572,13 +573,13 @@ fold_kernel(const float* __restrict__ z, long long ld, int M, int n, int first, 
   part[(long long)blockIdx.y * M + m] = make_float2(top, sum);
 }
 
-// The product and its softmax in 32 bits. A block takes 8 TM rows of x and kCols rows of the head, K in steps of 16
+// The product and its softmax in 32 bits where the head's rows do not begin at multiples of 16 bytes, which TMA cannot
+// take: plain multiply-adds. A block takes 8 TM rows of x and kCols rows of the head, K in steps of 16
 // through a ring copied with cp.async; thread (ty, tx) of 8 x 16 has rows ty + 8 i and columns tx + 16 j, so that
 // the column's threads, and with them the order of a row's sums, are the same for every TM. Two multiply-adds an
 // instruction: a sum is one over the even k's and one over the odd ones, whose operands lie side by side as they
-// are read. Bound by reads of shared memory (16 bytes a lane take four cycles whatever the lanes share) beside
-// the multiply-adds: 64 rows of 1,024 over 32,768 take 131 us, 58 us at the multiply-adds' rate; one to eight
-// rows 54 us, 21 us at the memory's.
+// are read. Bound by reads of shared memory (16 bytes a lane take four cycles whatever the lanes share) and copies of
+// four bytes beside the multiply-adds: 64 rows of 1,023 over 32,768 take 142 us, 58 us at the multiply-adds' rate.
 constexpr int kCols = 128, kF32Threads = 128, kF32K = 16, kF32Stages = 4, kLd = kF32K + 4;
 
 // d += a * b in both halves
@@ -586,16 +587,11 @@ __device__ __forceinline__ void fma_pair(uint64_t& d, uint64_t a, uint64_t b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
 
-template <bool kWide>
 __device__ __forceinline__ void copy_f32(uint32_t dst, const float* src, bool real) {
-  if (kWide)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 
-// kWide: rows that begin at multiples of 16 bytes
-template <int TM, bool kWide>
+template <int TM>
 __global__ void __launch_bounds__(kF32Threads, TM == 8 ? 2 : 3)
 f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restrict__ head, int M, int N, int K,
            int m_tiles, const int32_t* __restrict__ targets, float2* __restrict__ part,
@@ -608,8 +604,8 @@ f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restr
   const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   const int steps = (K + kF32K - 1) / kF32K;
   // a thread copies one place of K (of a step) in rows kAt, kAt + kStep, ... of x and of the head
-  constexpr int kWidth = kWide ? 4 : 1, kPer = kF32K / kWidth, kStep = kF32Threads / kPer;
-  const int kc = threadIdx.x % kPer * kWidth, row = threadIdx.x / kPer;
+  constexpr int kStep = kF32Threads / kF32K;
+  const int kc = threadIdx.x % kF32K, row = threadIdx.x / kF32K;
   const float* from_x = x + (m0 + row) * x_stride + kc;
   const float* from_w = head + (n0 + row) * K + kc;
   const uint32_t to0 = base + (row * kLd + kc) * 4;
@@ -618,14 +614,13 @@ f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restr
     const bool in_k = step * kF32K + kc < K;
 #pragma unroll
     for (int r = 0; r < kRows; r += kStep) {
-      if (kRows % kStep && r + row >= kRows) break;
       const bool real = in_k && m0 + row + r < M;
-      copy_f32<kWide>(to + r * kLd * 4, real ? from_x + r * x_stride : head, real);
+      copy_f32(to + r * kLd * 4, real ? from_x + r * x_stride : head, real);
     }
 #pragma unroll
     for (int r = 0; r < kCols; r += kStep) {
       const bool real = in_k && n0 + row + r < N;
-      copy_f32<kWide>(to + (kRows + r) * kLd * 4, real ? from_w + (long long)r * K : head, real);
+      copy_f32(to + (kRows + r) * kLd * 4, real ? from_w + (long long)r * K : head, real);
     }
     from_x += kF32K;
     from_w += kF32K;
@@ -701,20 +696,372 @@ f32_kernel(const float* __restrict__ x, long long x_stride, const float* __restr
   }
 }
 
-template <int TM, bool kWide>
+template <int TM>
 int launch_f32(const float* x, long long x_stride, const float* head, int M, int N, int K, const int32_t* targets,
                float2* part, float* mine, const Shape& form, cudaStream_t stream) {
   constexpr int kSmem = kF32Stages * (8 * TM + kCols) * kLd * 4;
   static PerDeviceOnce configured;
   if (configured.needs()) {
-    const cudaError_t e = cudaFuncSetAttribute(f32_kernel<TM, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(f32_kernel<TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return (int)e;
     configured.done();
   }
   const long long m_tiles = (M + 8 * TM - 1) / (8 * TM), pieces = ((long long)N + kCols - 1) / kCols;
   if (m_tiles * pieces > 0x7fffffffLL) return cudaErrorInvalidValue;
-  return launch_ordered(f32_kernel<TM, kWide>, dim3((unsigned)(m_tiles * pieces)), dim3(kF32Threads), kSmem, stream, x,
+  return launch_ordered(f32_kernel<TM>, dim3((unsigned)(m_tiles * pieces)), dim3(kF32Threads), kSmem, stream, x,
                         x_stride, head, M, N, K, (int)m_tiles, targets, part, mine, form);
+}
+
+// ---- 32 bits on the tensor cores ----------------------------------------------------------------
+// A number of 24 bits is the sum of three bfloat16 numbers h + m + l, each the upper half of what the ones before
+// leave (exact: 8 bits each, cut off); a product is h h' + (h m' + m h') + (h l' + m m' + l h'), and what is left out
+// is below 2^-21 of it. The six are products on the tensor cores. These cut where they add, always the same way: sums
+// are taken off them every kChunk steps and added up in fp32 by the epilogue (over 64 tokens and K =
+// 1,536 the largest error is 3.0e-6 so, 1.2e-5 with one sum for all of K, 3.6e-6 with the library's product). A block takes a tile of `rows` rows of the head, on
+// the lanes of tensor memory, against up to 96 tokens, its columns:
+//   warp 0       TMA: the head as it is (boxes of 32 floats) into a ring,
+//   warp 1       tensor memory, and the products,
+//   warp 2       TMA: the tokens' numbers in three, which `split_kernel` has left in a scratch,
+//   warps 4-11   epilogue: two warps for every 32 lanes, each with every other 32 tokens. Sums stay in registers, so
+//                that the next tile's products run under the softmax,
+//   warps 12-15  the head's numbers in three: a thread reads 32 floats of a row and writes them to tensor memory, as
+//                the products' left operand (no second trip through shared memory, which their right one fills).
+// The right operand is h', m', l' side by side, or two of them (a product's width is 256 at most): three products or
+// four instead of six (issuing one takes some 60 cycles, a product with 32 tokens 16). The height of a tile depends on the vocabulary and the device alone and
+// every tile leaves a partial: a row's sums are the same to the bit whatever rows are beside it.
+constexpr int kSplitThreads = 512, kSplitTokens = 96, kSplitRaw = BM * BK * 4, kSplitRawMost = 6, kSplitXMost = 4;
+constexpr int kSplitConverters = 4, kSplitMerged = 64, kChunk = 2;
+constexpr uint32_t kSplitA = 3 * BK / 2;         // columns of tensor memory for a step's left operands
+constexpr uint32_t kSplitAcc = 2 * kSplitA;      // where the sums begin
+static_assert(kSplitAcc + 3 * kSplitTokens <= kTmemCols && 3 * kSplitMerged <= 256, "tensor memory, and a product's width");
+
+struct SplitParams {
+  int M, N, K;
+  int m_tiles, cols;         // tiles of `cols` tokens (a multiple of 32)
+  int rows, n_tiles;         // tiles of `rows` rows of the head
+  int raw_stages, x_stages;
+  const int32_t* targets;
+  float2* part;              // [n_tiles][M]
+  float* mine;
+  Shape form;
+  int* error;
+};
+
+struct SplitTail {
+  uint64_t raw_full[kSplitRawMost], raw_empty[kSplitRawMost], x_full[kSplitXMost], x_empty[kSplitXMost];
+  uint64_t a_full[2], a_empty[2], acc_full, acc_empty;
+  uint32_t tmem;
+  alignas(16) int32_t target[2][kSplitTokens];
+  float2 share[2][4][kSplitTokens];
+};
+
+// A place in a ring and the parity of its use.
+struct Place {
+  int at = 0, phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++at == stages) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// The upper halves of two numbers side by side, and what they leave.
+__device__ __forceinline__ uint32_t cut_two(float& a, float& b) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  mma::add2(a, b, -__uint_as_float(x & 0xffff0000u), -__uint_as_float(y & 0xffff0000u));
+  return __byte_perm(x, y, 0x7632);
+}
+
+// x [M, K] in three: out [3][rows][padded], zeros behind M and K; a thread takes four numbers.
+__global__ void __launch_bounds__(256)
+split_kernel(const float* __restrict__ x, long long x_stride, int M, int K, int rows, int padded, int wide,
+             uint2* __restrict__ out) {
+  let_next_kernel_start();
+  wait_for_previous_kernel();
+  const int per = padded / 4;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)rows * per;
+  if (i >= all) return;
+  const int k = static_cast<int>(i % per) * 4;
+  const long long m = i / per;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (k < K && m < M) {      // (K is a multiple of four)
+    const float* from = x + m * x_stride + k;
+    if (wide) {
+      read4(from, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = from[j];
+    }
+  }
+#pragma unroll
+  for (int piece = 0; piece < 3; ++piece) {
+    const uint32_t a = cut_two(v[0], v[1]);
+    out[piece * all + i] = make_uint2(a, cut_two(v[2], v[3]));
+  }
+}
+
+// 16 columns of this warp's 32 lanes are written (no wait).
+__device__ __forceinline__ void put_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+__global__ void __launch_bounds__(kSplitThreads, 1)
+split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                     const __grid_constant__ SplitParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* xs = raw + p.raw_stages * kSplitRaw;
+  const int x_piece = p.cols * BK * 2, x_bytes = 3 * x_piece;
+  SplitTail* tail = reinterpret_cast<SplitTail*>(xs + p.x_stages * x_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int total = p.m_tiles * p.n_tiles, n_kb = (p.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSplitRawMost; ++s) {
+      tma::mbar_init(&tail->raw_full[s], 1);
+      tma::mbar_init(&tail->raw_empty[s], kSplitConverters);
+    }
+    for (int s = 0; s < kSplitXMost; ++s) {
+      tma::mbar_init(&tail->x_full[s], 1);
+      tma::mbar_init(&tail->x_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tma::mbar_init(&tail->a_full[i], kSplitConverters);
+      tma::mbar_init(&tail->a_empty[i], 1);
+    }
+    tma::mbar_init(&tail->acc_full, 1);
+    tma::mbar_init(&tail->acc_empty, kEpilogueThreads);
+    tma::fence_barrier_init();
+  }
+  if (warp == 1) tc::tmem_alloc(&tail->tmem, kTmemCols);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tail->tmem;
+  let_next_kernel_start();       // (with its shared and tensor memory in hand)
+  wait_for_previous_kernel();
+
+  if (warp == 0 || warp == 2) {
+    // ---- TMA: the head's rows, or the tokens' -------------------------------------------------
+    if (lane == 0) {
+      const bool head = warp == 0;
+      const CUtensorMap* map = head ? &w_map : &x_map;
+      uint64_t *full = head ? tail->raw_full : tail->x_full, *empty = head ? tail->raw_empty : tail->x_empty;
+      const int stages = head ? p.raw_stages : p.x_stages;
+      tma::prefetch_map(map);
+      Place place;
+      long long issued = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+        const int row = head ? tile / p.m_tiles * p.rows : tile % p.m_tiles * p.cols;
+        for (int kb = 0; kb < n_kb; ++kb) {
+          ok = tma::mbar_wait(&empty[place.at], place.phase ^ 1, p.error, 811);
+          if (!ok) break;
+          uint64_t* bar = &full[place.at];
+          if (head) {
+            // (the floats as pairs of 16-bit numbers, 64 to a box)
+            uint8_t* dst = raw + place.at * kSplitRaw;
+            tma::mbar_expect_tx(bar, 2 * p.rows * BK * 2);
+            tma::load_2d(dst, map, kb * 2 * BK, row, bar);
+            tma::load_2d(dst + kSplitRaw / 2, map, kb * 2 * BK + BK, row, bar);
+          } else {
+            uint8_t* dst = xs + place.at * x_bytes;
+            tma::mbar_expect_tx(bar, x_bytes);
+            for (int piece = 0; piece < 3; ++piece)
+              tma::load_2d(dst + piece * x_piece, map, kb * BK, piece * p.m_tiles * p.cols + row, bar);
+          }
+          ++issued;
+          place.next(stages);
+        }
+      }
+      // before this block may leave: what was asked for has arrived
+      for (long long i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        if (!tma::mbar_wait(&full[i % stages], (i / stages) & 1, p.error, 812)) break;
+    }
+  } else if (warp == 1) {
+    // ---- products: the whole warp walks, one lane issues (the operands stay in uniform registers) -------
+    const uint32_t one = tc::idesc_bf16_f32(BM, p.cols), two = tc::idesc_bf16_f32(BM, 2 * p.cols);
+    const uint32_t three = tc::idesc_bf16_f32(BM, 3 * p.cols);
+    const bool merged = p.cols <= kSplitMerged;
+    // columns: h h' | h m' + m h' | h l' + m m' + l h'
+    const uint32_t s0 = tmem + kSplitAcc, s1 = s0 + p.cols, s2 = s1 + p.cols;
+    Place x, a, acc;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < n_kb; ++kb) {
+        ok = tma::mbar_wait(&tail->x_full[x.at], x.phase, p.error, 814) &&
+             tma::mbar_wait(&tail->a_full[a.at], a.phase, p.error, 815) &&
+             (kb % kChunk || tma::mbar_wait(&tail->acc_empty, acc.phase ^ 1, p.error, 813));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const uint32_t at = tma::smem_u32(xs + x.at * x_bytes), left = tmem + a.at * kSplitA;
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) {
+          const uint32_t h = left + k * 8, m = h + BK / 2, l = m + BK / 2;
+          const uint64_t xh = tc::smem_desc_k_major_sw128(at + k * 32);
+          const bool begun = kb % kChunk || k;
+          // (the order of what adds up in a column is the same either way)
+          if (merged) {
+            tc::mma_ts_warp(s0, h, xh, three, begun);
+          } else {
+            tc::mma_ts_warp(s0, h, xh, two, begun);
+            tc::mma_ts_warp(s2, h, tc::smem_desc_k_major_sw128(at + 2 * x_piece + k * 32), one, begun);
+          }
+          tc::mma_ts_warp(s1, m, xh, two, true);
+          tc::mma_ts_warp(s2, l, xh, one, true);
+        }
+        tc::commit_warp(&tail->a_empty[a.at]);
+        tc::commit_warp(&tail->x_empty[x.at]);
+        if (kb % kChunk == kChunk - 1 || kb + 1 == n_kb) {
+          tc::commit_warp(&tail->acc_full);
+          acc.next(1);
+        }
+        x.next(p.x_stages);
+        a.next(2);
+      }
+    }
+  } else if (warp >= 12) {
+    // ---- the head's numbers in three ------------------------------------------------------------
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    Place r, a;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < n_kb; ++kb) {
+        ok = tma::mbar_wait(&tail->raw_full[r.at], r.phase, p.error, 816) &&
+             tma::mbar_wait(&tail->a_empty[a.at], a.phase ^ 1, p.error, 817);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after_sync();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint8_t* from = raw + r.at * kSplitRaw + half * (kSplitRaw / 2) + row * 128;
+          float v[32];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float4 f = *reinterpret_cast<const float4*>(from + ((c ^ (row & 7)) << 4));
+            v[4 * c] = f.x; v[4 * c + 1] = f.y; v[4 * c + 2] = f.z; v[4 * c + 3] = f.w;
+          }
+          if (half) {
+            __syncwarp();
+            if (lane == 0) tma::mbar_arrive(&tail->raw_empty[r.at]);
+          }
+#pragma unroll
+          for (int piece = 0; piece < 3; ++piece) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = cut_two(v[2 * i], v[2 * i + 1]);
+            put_x16(to + a.at * kSplitA + piece * (BK / 2) + half * 16, w);
+          }
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tma::mbar_arrive(&tail->a_full[a.at]);
+        r.next(p.raw_stages);
+        a.next(2);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue -------------------------------------------------------------------------------
+    const int quarter = warp & 3, side = (warp - 4) >> 2, thread = quarter * 32 + lane, worker = side * BM + thread;
+    const uint32_t sums = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kSplitAcc;
+    Place acc, turn;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+      const int m0 = tile % p.m_tiles * p.cols, n_tile = tile / p.m_tiles;
+      const int v = n_tile * p.rows + thread;
+      const bool real = thread < p.rows && v < p.N;
+      const bool token = worker < p.cols && m0 + worker < p.M;
+      int32_t* target = tail->target[turn.at];
+      if (worker < kSplitTokens) target[worker] = token ? p.targets[m0 + worker] : -1;
+      const float bias = p.form.bias && real ? bias_at(p.form, v) : 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
+      float z[2][32];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) z[i >> 5][i & 31] = 0.f;
+      for (int kb = 0; kb < n_kb; kb += kChunk) {
+        ok = __all_sync(0xffffffffu, ok && tma::mbar_wait(&tail->acc_full, acc.phase, p.error, 818));
+        tc::fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = side * 32 + i * 64;
+          if (c < p.cols && ok) {
+#pragma unroll 1
+            for (int part = 2; part >= 0; --part) {      // (the largest last)
+              float some[32];
+              ld_32x32b_x32(sums + part * p.cols + c, some);
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) mma::add2(z[i][j], z[i][j + 1], some[j], some[j + 1]);
+            }
+          }
+        }
+        tc::fence_before_sync();
+        tma::mbar_arrive(&tail->acc_empty);
+        acc.next(1);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = side * 32 + i * 64;
+        if (c >= p.cols || !ok) continue;
+        if (p.form.bias) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[i][j] += bias;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[i][j] *= p.form.scale;
+        if (p.form.cap > 0.f) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[i][j] = p.form.cap * tanhf(z[i][j] * p.form.over_cap);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const int4 t = *reinterpret_cast<const int4*>(&target[c + j]);
+          const int of[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (of[q] == v && real) p.mine[m0 + c + j + q] = z[i][j + q];
+            z[i][j + q] = real ? z[i][j + q] : -INFINITY;
+          }
+        }
+        float most[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) most[j] = z[i][j];
+        const float top = over_lanes<true>(most, lane);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[i][j] = expf(z[i][j] - __shfl_sync(0xffffffffu, base, j));
+        tail->share[turn.at][quarter][c + lane] = make_float2(top, over_lanes<false>(z[i], lane));
+      }
+      // (what a tile leaves in shared memory stays until the one after the next, past the next one's barriers)
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
+      if (token && ok) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top = fmaxf(top, tail->share[turn.at][q][worker].x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 other = tail->share[turn.at][q][worker];
+          sum += other.y == 0.f ? 0.f : other.y * expf(other.x - top);
+        }
+        p.part[(long long)n_tile * p.M + m0 + worker] = make_float2(top, sum);
+      }
+      turn.next(2);
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
 }
 
 // lse and log-probability of every row from its partials: rows below `full` have `pieces` of them, [pieces][full],
@@ -844,16 +1191,8 @@ SAKV_EXPORT int sakv_logprob_f32(const float* x, long long x_stride, const float
   if (M <= 0 || N <= 0 || K <= 0 || x_stride < K || M > 0x7fffffff - 64 || !(cap >= 0.f)) return cudaErrorInvalidValue;
   const Shape form = shape_of(bias, bias_bf16, scale, cap);
   float2* to = reinterpret_cast<float2*>(part);
-  const bool wide = K % 4 == 0 && x_stride % 4 == 0 &&
-                    !((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(head)) & 15);
-#define SAKV_F32(TM)                                                                                      \
-  e = wide ? launch_f32<TM, true>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)             \
-           : launch_f32<TM, false>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
-  int e;
-  if (M <= 8) SAKV_F32(1);
-  else if (M <= 16) SAKV_F32(2);
-  else if (M <= 32) SAKV_F32(4);
-  else SAKV_F32(8);
+#define SAKV_F32(TM) launch_f32<TM>(x, x_stride, head, M, N, K, targets, to, mine, form, stream)
+  const int e = M <= 8 ? SAKV_F32(1) : M <= 16 ? SAKV_F32(2) : M <= 32 ? SAKV_F32(4) : SAKV_F32(8);
 #undef SAKV_F32
   return e ? e : join(part, mine, targets, logprob, lse, M, N, M, (N + kCols - 1) / kCols, 0, stream);
 }
@@ -904,6 +1243,82 @@ static int logprob_map(CUtensorMap* map, const void* base, long long rows, long 
     return cudaErrorInvalidValue;
   return tma::make_map_bf16_2d(map, base, (uint64_t)rows, (uint64_t)cols, (uint64_t)row_stride * 2,
                                (uint32_t)box_rows, BK);
+}
+
+// Rows of the head in a tile of the 32-bit tensor-core kernel for a vocabulary of N: the height that a device of so many
+// SMs gets through in the fewest rows, whatever the tokens.
+SAKV_EXPORT int sakv_logprob_split_rows(int N, int sms) {
+  if (N <= 0 || sms <= 0) return 0;
+  long long best = -1;
+  int rows = BM;
+  for (int r = BM; r >= 104; r -= 8) {
+    const long long tiles = ((long long)N + r - 1) / r, cost = (tiles + sms - 1) / sms * r;
+    if (best < 0 || cost < best) {
+      best = cost;
+      rows = r;
+    }
+  }
+  return rows;
+}
+
+// M tokens rounded up to whole tiles of it (0: too many): as few tiles as there can be, of equal width.
+SAKV_EXPORT int sakv_logprob_split_tokens(int M) {
+  if (M <= 0) return 0;
+  const long long tiles = ((long long)M + kSplitTokens - 1) / kSplitTokens;
+  const long long rows = ((M + tiles - 1) / tiles + 31) / 32 * 32 * tiles;
+  return rows <= 0x7fffffff / 3 ? (int)rows : 0;
+}
+
+// The same as sakv_logprob_f32 on the tensor cores, for heads whose rows begin at multiples of 16 bytes: tiles of `rows`
+// rows (sakv_logprob_split_rows), scratch part [ceil(N / rows)][M] pairs, mine [M], split [3][M rounded
+// up to sakv_logprob_split_tokens][K rounded up to 8] of 16 bits at a multiple of 16 bytes.
+SAKV_EXPORT int sakv_logprob_split(const float* x, long long x_stride, const float* head, int M, int N, int K, int rows,
+                                   const int32_t* targets, float* part, float* mine, void* split, const void* bias,
+                                   int bias_bf16, float scale, float cap, float* logprob, float* lse,
+                                   cudaStream_t stream) {
+  const int sms = sm_count();
+  if (M <= 0 || N <= 0 || K <= 0 || K % 4 || x_stride < K || !(cap >= 0.f) || !sakv_logprob_split_tokens(M) ||
+      N > 0x7fffffff - BM || K > 0x3fffffff - BK || rows != sakv_logprob_split_rows(N, sms) || rows <= 0)
+    return cudaErrorInvalidValue;
+  SplitParams p;
+  p.M = M; p.N = N; p.K = K;
+  const int padded_rows = sakv_logprob_split_tokens(M);
+  p.m_tiles = (M + kSplitTokens - 1) / kSplitTokens;
+  p.cols = padded_rows / p.m_tiles;
+  p.rows = rows;
+  p.n_tiles = (N + rows - 1) / rows;
+  if ((long long)p.m_tiles * p.n_tiles > 0x3fffffffLL) return cudaErrorInvalidValue;
+  // what is left of shared memory beside up to four steps of the tokens is the head's
+  const int x_bytes = 3 * p.cols * BK * 2, room = kSmemMost - 1024 - (int)sizeof(SplitTail);
+  p.x_stages = p.cols <= 32 ? 4 : p.cols <= 96 ? 3 : 2;
+  p.raw_stages = (room - p.x_stages * x_bytes) / kSplitRaw;
+  if (p.raw_stages > kSplitRawMost) p.raw_stages = kSplitRawMost;
+  p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;
+  p.form = shape_of(bias, bias_bf16, scale, cap);
+  p.error = error_word();
+  if (!p.error || p.raw_stages < 2) return cudaErrorInvalidValue;
+  const int padded = (K + 7) / 8 * 8;
+  CUtensorMap w_map, x_map;
+  int e = logprob_map(&w_map, head, N, 2LL * K, 2LL * K, rows);
+  if (!e) e = logprob_map(&x_map, split, 3LL * padded_rows, padded, padded, p.cols);
+  if (e) return e;
+  const int smem = p.raw_stages * kSplitRaw + p.x_stages * x_bytes + 1024 + (int)sizeof(SplitTail);
+  static PerDeviceOnce configured;
+  if (configured.needs()) {
+    const cudaError_t set =
+        cudaFuncSetAttribute(split_logprob_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (set != cudaSuccess) return (int)set;
+    configured.done();
+  }
+  const long long quads = (long long)padded_rows * (padded / 4), blocks = (quads + 255) / 256;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int wide = x_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(x) & 15);
+  e = launch_overlapped(split_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, 1, x, x_stride, M, K, padded_rows, padded,
+                        wide, reinterpret_cast<uint2*>(split));
+  const int tiles = p.m_tiles * p.n_tiles;
+  if (!e) e = launch_overlapped(split_logprob_kernel, dim3(tiles < sms ? tiles : sms), dim3(kSplitThreads), smem, stream, 1,
+                                w_map, x_map, p);
+  return e ? e : join(part, mine, targets, logprob, lse, M, N, M, p.n_tiles, 0, stream);
 }
 
 // The partials of x [M, K] against the head [N, K] in bf16 (rows of x `x_stride` apart; 16-byte aligned), cut as

@@ -8,11 +8,13 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import F32, KernelError, call, dtype_code, plain_function, ptr, require_cuda
+from ._lib import F32, KernelError, call, dtype_code, plain_function, ptr, require_cuda, sm_count
 from .linear import linear
 
 #: logits that lie in memory at one time where a piece is a product of its own (fp32: 32 MB, a quarter of L2)
 PIECE_ELEMENTS = 8 << 20
+#: numbers of x that are split at one time in 32 bits (six bytes each: 384 MB)
+SPLIT_ELEMENTS = 64 << 20
 
 
 _resident: dict = {}
@@ -96,6 +98,27 @@ def _shape(rows: int, vocab: int):
     return hit
 
 
+_heights: dict = {}
+
+
+def _split_rows(vocab: int) -> int:
+    """Rows of the head in a tile of the 32-bit tensor-core kernel on this device."""
+    sms = sm_count()
+    hit = _heights.get((vocab, sms))
+    if hit is None:
+        if len(_heights) >= 256:
+            _heights.clear()
+        hit = _heights[vocab, sms] = plain_function("sakv_logprob_split_rows")(vocab, sms)
+    return hit
+
+
+def _in_pieces(x, head, targets, bias, scale, softcap, most: int):
+    """So many rows at a time."""
+    parts = [_token_logprobs(x[i:i + most], head, targets[i:i + most], bias, scale, softcap)
+             for i in range(0, x.shape[0], most)]
+    return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+
+
 def _token_logprobs(x, head, targets, bias, scale, softcap):
     rows, k = x.shape
     vocab, stride = head.shape[0], x.stride(0)
@@ -113,6 +136,19 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
         call("sakv_logprob_pieces", at, stride, head_at, rows, vocab, k, shape, targets.data_ptr(), scratch,
              scratch + 4 * floats, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
         _lib.launches += 1          # the call launched the join too
+    elif x.dtype is torch.float32 and k % 4 == 0 and head_at % 16 == 0:
+        padded = -(-k // 8) * 8
+        most = max(1, SPLIT_ELEMENTS // padded)
+        if rows > most:
+            return _in_pieces(x, head, targets, bias, scale, softcap, most)
+        tile = _split_rows(vocab)
+        halves = 3 * plain_function("sakv_logprob_split_tokens")(rows) * padded // 2
+        floats = halves + 2 * rows * -(-vocab // tile)
+        part = x.new_empty(floats + rows, dtype=torch.float32)       # the split rows, the partials, the targets' logits
+        scratch = part.data_ptr()
+        call("sakv_logprob_split", at, stride, head_at, rows, vocab, k, tile, targets.data_ptr(), scratch + 4 * halves,
+             scratch + 4 * floats, scratch, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
+        _lib.launches += 2          # the call launched the split of x and the join too
     elif x.dtype is torch.float32:
         floats = 2 * rows * -(-vocab // plain_function("sakv_logprob_f32_columns")())
         part = x.new_empty(floats + rows, dtype=torch.float32)
@@ -124,9 +160,7 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
         columns = plain_function("sakv_logprob_fold_columns")()
         most = max(1, PIECE_ELEMENTS // columns)
         if rows > most:                # (the scratch of a piece stays as large as it is for these)
-            parts = [_token_logprobs(x[i:i + most], head, targets[i:i + most], bias, scale, softcap)
-                     for i in range(0, rows, most)]
-            return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+            return _in_pieces(x, head, targets, bias, scale, softcap, most)
         piece = max(1, min(-(-vocab // columns), PIECE_ELEMENTS // (rows * columns))) * columns
         pieces = -(-vocab // columns)
         part = x.new_empty((pieces, rows, 2), dtype=torch.float32)

@@ -193,3 +193,53 @@ def test_no_rows_rows_alone_streams_and_graphs():
     graph.replay()
     fresh, _ = ops.token_logprobs(x, w, targets)
     assert torch.equal(held, fresh) and not torch.equal(held, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [32, 33, 64, 65, 96, 97, 128, 129, 257])
+@pytest.mark.parametrize("k, vocab", [(4, 104), (60, 129), (68, 1000), (128, 127), (132, 15500), (260, 20000), (1028, 333)])
+def test_numbers_of_32_bits_in_three(rows, k, vocab):
+    check(rows, k, vocab, torch.float32, x_pad=(rows + k // 4) % 3, seed=rows + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [640, 4096])
+def test_long_sums_of_32_bits(k):
+    """Numbers of one sign, where what is cut off adds up."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.rand((40, k), generator=g, device="cuda") + 0.5
+    w = (torch.rand((700, k), generator=g, device="cuda") + 0.5) / k
+    targets = torch.randint(0, 700, (40,), generator=g, device="cuda", dtype=torch.int32)
+    got, lse = ops.token_logprobs(x, w, targets)
+    z = x.double() @ w.double().t()
+    want_lse = torch.logsumexp(z, 1)
+    want = z.gather(1, targets.long()[:, None])[:, 0] - want_lse
+    # the sums of 128 products are taken off the tensor cores, where each product and each of eight additions is cut
+    # by a step of the sum (2^-23) at most; what is left out of a product is 2^-21 of it; the k / 128 additions of
+    # those sums round by 2^-24; lse's own sum as above
+    dz = (136 + 4 + k / 256) * 2.0 ** -23 * z.amax()
+    assert ((lse.double() - want_lse).abs() <= dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (1 + want_lse)).all()
+    assert ((got.double() - want).abs() <= 2 * dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (2 + want_lse)).all()
+
+
+@pytest.mark.gpu
+def test_rows_of_32_bits_in_pieces(monkeypatch):
+    x, w, targets, got, lse = check(301, 132, 3001, torch.float32, seed=8)
+    monkeypatch.setattr(logprobs, "SPLIT_ELEMENTS", 70 * 136)
+    again, lse2 = ops.token_logprobs(x, w, targets)
+    assert torch.equal(again, got) and torch.equal(lse, lse2)
+
+
+def test_heights_and_widths_of_32_bit_tiles():
+    """Host code of the launcher. (Needs nvcc, not a GPU.)"""
+    from semantic_aware_adaptive_kv_cache_precision_b200.ops._lib import plain_function
+    for vocab in (1, 103, 18944, 18945, 50257, 151936):
+        for sms in (1, 148):
+            rows = plain_function("sakv_logprob_split_rows")(vocab, sms)
+            assert 104 <= rows <= 128 and rows % 8 == 0
+    for rows in (1, 32, 33, 128, 129, 185, 2047, 4097):
+        padded = plain_function("sakv_logprob_split_tokens")(rows)
+        tiles = -(-rows // 96)
+        assert rows <= padded < rows + 32 * tiles and padded % (32 * tiles) == 0 and padded // tiles <= 96
+    assert plain_function("sakv_logprob_split_tokens")(0) == 0
+    assert plain_function("sakv_logprob_split_tokens")(2 ** 31 - 1) == 0 == plain_function("sakv_logprob_split_rows")(0, 1)
