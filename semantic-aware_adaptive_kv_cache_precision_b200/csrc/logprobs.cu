@@ -716,21 +716,29 @@ int launch_f32(const float* x, long long x_stride, const float* head, int M, int
 // A number of 24 bits is the sum of three bfloat16 numbers h + m + l, each the upper half of what the ones before
 // leave (exact: 8 bits each, cut off); a product is h h' + (h m' + m h') + (h l' + m m' + l h'), and what is left out
 // is below 2^-21 of it. The six are products on the tensor cores. These cut where they add, always the same way: sums
-// are taken off them every kChunk steps and added up in fp32 by the epilogue (over 64 tokens and K =
-// 1,536 the largest error is 3.0e-6 so, 1.2e-5 with one sum for all of K, 3.6e-6 with the library's product). A block takes a tile of `rows` rows of the head, on
-// the lanes of tensor memory, against up to 96 tokens, its columns:
+// of h h' are taken off them every kChunk steps and added up in fp32 by the epilogue. The largest error over 64 tokens
+// and K = 1,536 is 1.6e-6 to 2.6e-6 so (every second step; every fourth: 3.1e-6 and 4 % less time), 1.2e-5 with one
+// sum for all of K, 3.5e-6 to 6.9e-6 with the library's product. A number that is not finite makes its products NaN.
+// A block takes a tile of `rows` rows of the head, on the lanes of tensor memory, against up to 96 tokens, its columns:
 //   warp 0       TMA: the head as it is (boxes of 32 floats) into a ring,
 //   warp 1       tensor memory, and the products,
 //   warp 2       TMA: the tokens' numbers in three, which `split_kernel` has left in a scratch,
-//   warps 4-11   epilogue: two warps for every 32 lanes, each with every other 32 tokens. Sums stay in registers, so
-//                that the next tile's products run under the softmax,
-//   warps 12-15  the head's numbers in three: a thread reads 32 floats of a row and writes them to tensor memory, as
-//                the products' left operand (no second trip through shared memory, which their right one fills).
+//   warp 3       has waited for those before the warp that issues looks,
+//   warps 4-15   epilogue: for every 32 lanes a warp for each 32 tokens. Sums stay in registers, so that the next
+//                tile's products run under the softmax,
+//   warps 16-23  the head's numbers in three, four warps a step in turns: a thread takes a row's floats and writes them
+//                to tensor memory, as the products' left operand (no second trip through shared memory, which their
+//                right one fills).
 // The right operand is h', m', l' side by side, or two of them (a product's width is 256 at most): three products or
-// four instead of six (issuing one takes some 60 cycles, a product with 32 tokens 16). The height of a tile depends on the vocabulary and the device alone and
-// every tile leaves a partial: a row's sums are the same to the bit whatever rows are beside it.
-constexpr int kSplitThreads = 512, kSplitTokens = 96, kSplitRaw = BM * BK * 4, kSplitRawMost = 6, kSplitXMost = 4;
-constexpr int kSplitConverters = 4, kSplitMerged = 64, kChunk = 2;
+// four a 16 of K instead of six, since issuing one takes some 55 cycles whatever its width. The height of a tile
+// depends on the vocabulary and the device alone and every tile leaves a partial: a row's sums are the same to the bit
+// whatever rows are beside it.
+// Measured: 64 tokens, K 1,024, 32,768 rows 44 us (21 at the memory's rate, 15 the products at the tensor cores'; the
+// multiply-adds below took 131); 64, 1,536, 151,936 253 us (145, 107); 185, 1,704, 94,657 344 us (100, 214; 1,480). A
+// step of 64 takes 0.9 to 1.2 us, of which the floats' arrival is 0.7: cutting them in three and the products, each a
+// chain of waits, share what is left (without the products 0.86, without the cutting 0.9).
+constexpr int kSplitThreads = 768, kSplitTokens = 96, kSplitEpilogue = 4 * kSplitTokens, kSplitRaw = BM * BK * 4;
+constexpr int kSplitRawMost = 6, kSplitXMost = 4, kSplitConverters = 4, kSplitMerged = 64, kChunk = 2;
 constexpr uint32_t kSplitA = 3 * BK / 2;         // columns of tensor memory for a step's left operands
 constexpr uint32_t kSplitAcc = 2 * kSplitA;      // where the sums begin
 static_assert(kSplitAcc + 3 * kSplitTokens <= kTmemCols && 3 * kSplitMerged <= 256, "tensor memory, and a product's width");
@@ -748,8 +756,8 @@ struct SplitParams {
 };
 
 struct SplitTail {
-  uint64_t raw_full[kSplitRawMost], raw_empty[kSplitRawMost], x_full[kSplitXMost], x_empty[kSplitXMost];
-  uint64_t a_full[2], a_empty[2], acc_full, acc_empty;
+  uint64_t raw_full[kSplitRawMost], raw_empty[kSplitRawMost], x_full[kSplitXMost];
+  uint64_t a_full[2], done[kSplitXMost], acc_full, acc_empty;
   uint32_t tmem;
   alignas(16) int32_t target[2][kSplitTokens];
   float2 share[2][4][kSplitTokens];
@@ -768,9 +776,9 @@ struct Place {
 
 // The upper halves of two numbers side by side, and what they leave.
 __device__ __forceinline__ uint32_t cut_two(float& a, float& b) {
-  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-  mma::add2(a, b, -__uint_as_float(x & 0xffff0000u), -__uint_as_float(y & 0xffff0000u));
-  return __byte_perm(x, y, 0x7632);
+  const uint32_t upper = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+  mma::add2(a, b, -__uint_as_float(upper << 16), -__uint_as_float(upper & 0xffff0000u));
+  return upper;
 }
 
 // x [M, K] in three: out [3][rows][padded], zeros behind M and K; a thread takes four numbers.
@@ -821,6 +829,7 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   SplitTail* tail = reinterpret_cast<SplitTail*>(xs + p.x_stages * x_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int total = p.m_tiles * p.n_tiles, n_kb = (p.K + BK - 1) / BK;
+  const long long steps = ((long long)total - blockIdx.x + gridDim.x - 1) / gridDim.x * n_kb;   // of this block
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSplitRawMost; ++s) {
@@ -829,14 +838,11 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     }
     for (int s = 0; s < kSplitXMost; ++s) {
       tma::mbar_init(&tail->x_full[s], 1);
-      tma::mbar_init(&tail->x_empty[s], 1);
+      tma::mbar_init(&tail->done[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      tma::mbar_init(&tail->a_full[i], kSplitConverters);
-      tma::mbar_init(&tail->a_empty[i], 1);
-    }
+    for (int i = 0; i < 2; ++i) tma::mbar_init(&tail->a_full[i], kSplitConverters + 1);
     tma::mbar_init(&tail->acc_full, 1);
-    tma::mbar_init(&tail->acc_empty, kEpilogueThreads);
+    tma::mbar_init(&tail->acc_empty, kSplitEpilogue);
     tma::fence_barrier_init();
   }
   if (warp == 1) tc::tmem_alloc(&tail->tmem, kTmemCols);
@@ -852,7 +858,7 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     if (lane == 0) {
       const bool head = warp == 0;
       const CUtensorMap* map = head ? &w_map : &x_map;
-      uint64_t *full = head ? tail->raw_full : tail->x_full, *empty = head ? tail->raw_empty : tail->x_empty;
+      uint64_t *full = head ? tail->raw_full : tail->x_full, *empty = head ? tail->raw_empty : tail->done;
       const int stages = head ? p.raw_stages : p.x_stages;
       tma::prefetch_map(map);
       Place place;
@@ -885,94 +891,119 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
         if (!tma::mbar_wait(&full[i % stages], (i / stages) & 1, p.error, 812)) break;
     }
   } else if (warp == 1) {
-    // ---- products: the whole warp walks, one lane issues (the operands stay in uniform registers) -------
+    // ---- products: the whole warp walks and one lane issues, and no turn of the loops depends on what a lane saw, so
+    // that the operands stay in uniform registers, which the instruction reads --------------------------------
     const uint32_t one = tc::idesc_bf16_f32(BM, p.cols), two = tc::idesc_bf16_f32(BM, 2 * p.cols);
     const uint32_t three = tc::idesc_bf16_f32(BM, 3 * p.cols);
     const bool merged = p.cols <= kSplitMerged;
+    const uint32_t elected = tc::elect_lane();
     // columns: h h' | h m' + m h' | h l' + m m' + l h'
     const uint32_t s0 = tmem + kSplitAcc, s1 = s0 + p.cols, s2 = s1 + p.cols;
+    const uint64_t x0 = tc::smem_desc_k_major_sw128(tma::smem_u32(xs));
     Place x, a, acc;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+    for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
       for (int kb = 0; kb < n_kb; ++kb) {
-        ok = tma::mbar_wait(&tail->x_full[x.at], x.phase, p.error, 814) &&
-             tma::mbar_wait(&tail->a_full[a.at], a.phase, p.error, 815) &&
+        ok = ok && tma::mbar_wait(&tail->a_full[a.at], a.phase, p.error, 815) &&
              (kb % kChunk || tma::mbar_wait(&tail->acc_empty, acc.phase ^ 1, p.error, 813));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        __syncwarp();
         tc::fence_after_sync();
-        const uint32_t at = tma::smem_u32(xs + x.at * x_bytes), left = tmem + a.at * kSplitA;
+        const uint32_t go = elected && ok;
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
-          const uint32_t h = left + k * 8, m = h + BK / 2, l = m + BK / 2;
-          const uint64_t xh = tc::smem_desc_k_major_sw128(at + k * 32);
-          const bool begun = kb % kChunk || k;
+          const uint32_t h = tmem + a.at * kSplitA + k * 8, m = h + BK / 2, l = m + BK / 2;
+          // (descriptors count 16 bytes)
+          const uint64_t xh = x0 + ((x.at * x_bytes + k * 32) >> 4), xm = xh + (x_piece >> 4);
+          const bool begun = kb % kChunk || k, others = kb || k;      // h h' so far, and the others
           // (the order of what adds up in a column is the same either way)
-          if (merged) {
-            tc::mma_ts_warp(s0, h, xh, three, begun);
+          if (merged && begun == others) {
+            tc::mma_ts_if(go, s0, h, xh, three, begun);
           } else {
-            tc::mma_ts_warp(s0, h, xh, two, begun);
-            tc::mma_ts_warp(s2, h, tc::smem_desc_k_major_sw128(at + 2 * x_piece + k * 32), one, begun);
+            tc::mma_ts_if(go, s0, h, xh, one, begun);
+            tc::mma_ts_if(go, s1, h, xm, two, others);
           }
-          tc::mma_ts_warp(s1, m, xh, two, true);
-          tc::mma_ts_warp(s2, l, xh, one, true);
+          tc::mma_ts_if(go, s1, m, xh, two, true);
+          tc::mma_ts_if(go, s2, l, xh, one, true);
         }
-        tc::commit_warp(&tail->a_empty[a.at]);
-        tc::commit_warp(&tail->x_empty[x.at]);
+        tc::commit_if(go, &tail->done[x.at]);
         if (kb % kChunk == kChunk - 1 || kb + 1 == n_kb) {
-          tc::commit_warp(&tail->acc_full);
+          tc::commit_if(go, &tail->acc_full);
           acc.next(1);
         }
         x.next(p.x_stages);
         a.next(2);
       }
     }
-  } else if (warp >= 12) {
-    // ---- the head's numbers in three ------------------------------------------------------------
-    const int quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    Place r, a;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-      for (int kb = 0; kb < n_kb; ++kb) {
-        ok = tma::mbar_wait(&tail->raw_full[r.at], r.phase, p.error, 816) &&
-             tma::mbar_wait(&tail->a_empty[a.at], a.phase ^ 1, p.error, 817);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc::fence_after_sync();
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint8_t* from = raw + r.at * kSplitRaw + half * (kSplitRaw / 2) + row * 128;
-          float v[32];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float4 f = *reinterpret_cast<const float4*>(from + ((c ^ (row & 7)) << 4));
-            v[4 * c] = f.x; v[4 * c + 1] = f.y; v[4 * c + 2] = f.z; v[4 * c + 3] = f.w;
-          }
-          if (half) {
-            __syncwarp();
-            if (lane == 0) tma::mbar_arrive(&tail->raw_empty[r.at]);
-          }
-#pragma unroll
-          for (int piece = 0; piece < 3; ++piece) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = cut_two(v[2 * i], v[2 * i + 1]);
-            put_x16(to + a.at * kSplitA + piece * (BK / 2) + half * 16, w);
-          }
+  } else if (warp == 3) {
+    // ---- the tokens' numbers have arrived (the warp that issues has no time to wait for more than one barrier) ------
+    if (lane == 0) {
+      Place x, a, free;          // free: the step before the last one's, whose place in `a` a step takes
+      bool ok = true;
+      for (long long step = 0; step < steps && ok; ++step) {
+        if (step >= 2) {
+          ok = tma::mbar_wait(&tail->done[free.at], free.phase, p.error, 819);
+          free.next(p.x_stages);
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tma::mbar_arrive(&tail->a_full[a.at]);
-        r.next(p.raw_stages);
+        ok = ok && tma::mbar_wait(&tail->x_full[x.at], x.phase, p.error, 814);
+        if (ok) tma::mbar_arrive(&tail->a_full[a.at]);
+        x.next(p.x_stages);
         a.next(2);
       }
     }
+  } else if (warp >= 16) {
+    // ---- the head's numbers in three ------------------------------------------------------------
+    const int quarter = warp & 3, row = quarter * 32 + lane, turn = (warp - 16) >> 2;
+    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + turn * kSplitA;
+    Place r, free;
+    if (turn) {
+      r.next(p.raw_stages);
+      free.next(p.x_stages);
+    }
+    bool ok = true;
+    for (long long step = turn; step < steps; step += 2) {
+      ok = __all_sync(0xffffffffu, tma::mbar_wait(&tail->raw_full[r.at], r.phase, p.error, 816));
+      if (!ok) break;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t* from = raw + r.at * kSplitRaw + half * (kSplitRaw / 2) + row * 128;
+        float v[32];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float4 f = *reinterpret_cast<const float4*>(from + ((c ^ (row & 7)) << 4));
+          v[4 * c] = f.x; v[4 * c + 1] = f.y; v[4 * c + 2] = f.z; v[4 * c + 3] = f.w;
+        }
+        if (half) {
+          __syncwarp();
+          if (lane == 0) tma::mbar_arrive(&tail->raw_empty[r.at]);
+        } else if (step >= 2) {
+          ok = __all_sync(0xffffffffu, tma::mbar_wait(&tail->done[free.at], free.phase, p.error, 817));
+          if (!ok) break;
+          free.next(p.x_stages);
+          free.next(p.x_stages);
+          tc::fence_after_sync();
+        }
+#pragma unroll
+        for (int piece = 0; piece < 3; ++piece) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = cut_two(v[2 * i], v[2 * i + 1]);
+          put_x16(to + piece * (BK / 2) + half * 16, w);
+        }
+      }
+      if (!ok) break;
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::mbar_arrive(&tail->a_full[turn]);
+      r.next(p.raw_stages);
+      r.next(p.raw_stages);
+    }
   } else if (warp >= 4) {
     // ---- epilogue -------------------------------------------------------------------------------
-    const int quarter = warp & 3, side = (warp - 4) >> 2, thread = quarter * 32 + lane, worker = side * BM + thread;
-    const uint32_t sums = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kSplitAcc;
+    const int quarter = warp & 3, thread = quarter * 32 + lane, worker = threadIdx.x - 4 * 32;
+    const int c = (warp - 4) / 4 * 32;         // this warp's tokens of a tile
+    const bool mine = c < p.cols;
+    const uint32_t sums = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kSplitAcc + c;
     Place acc, turn;
     bool ok = true;
     for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
@@ -983,43 +1014,36 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       int32_t* target = tail->target[turn.at];
       if (worker < kSplitTokens) target[worker] = token ? p.targets[m0 + worker] : -1;
       const float bias = p.form.bias && real ? bias_at(p.form, v) : 0.f;
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
-      float z[2][32];
+      asm volatile("bar.sync 1, %0;" ::"n"(kSplitEpilogue) : "memory");
+      float z[32];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) z[i >> 5][i & 31] = 0.f;
+      for (int j = 0; j < 32; ++j) z[j] = 0.f;
       for (int kb = 0; kb < n_kb; kb += kChunk) {
         ok = __all_sync(0xffffffffu, ok && tma::mbar_wait(&tail->acc_full, acc.phase, p.error, 818));
         tc::fence_after_sync();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = side * 32 + i * 64;
-          if (c < p.cols && ok) {
+        if (mine && ok) {
 #pragma unroll 1
-            for (int part = 2; part >= 0; --part) {      // (the largest last)
-              float some[32];
-              ld_32x32b_x32(sums + part * p.cols + c, some);
+          for (int part = kb + kChunk < n_kb ? 0 : 2; part >= 0; --part) {      // (the largest last)
+            float some[32];
+            ld_32x32b_x32(sums + part * p.cols, some);
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) mma::add2(z[i][j], z[i][j + 1], some[j], some[j + 1]);
-            }
+            for (int j = 0; j < 32; j += 2) mma::add2(z[j], z[j + 1], some[j], some[j + 1]);
           }
         }
         tc::fence_before_sync();
         tma::mbar_arrive(&tail->acc_empty);
         acc.next(1);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = side * 32 + i * 64;
-        if (c >= p.cols || !ok) continue;
+      if (mine && ok) {
         if (p.form.bias) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[i][j] += bias;
+          for (int j = 0; j < 32; ++j) z[j] += bias;
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z[i][j] *= p.form.scale;
+        for (int j = 0; j < 32; ++j) z[j] *= p.form.scale;
         if (p.form.cap > 0.f) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[i][j] = p.form.cap * tanhf(z[i][j] * p.form.over_cap);
+          for (int j = 0; j < 32; ++j) z[j] = p.form.cap * tanhf(z[j] * p.form.over_cap);
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -1027,21 +1051,21 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
           const int of[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            if (of[q] == v && real) p.mine[m0 + c + j + q] = z[i][j + q];
-            z[i][j + q] = real ? z[i][j + q] : -INFINITY;
+            if (of[q] == v && real) p.mine[m0 + c + j + q] = z[j + q];
+            z[j + q] = real ? z[j + q] : -INFINITY;
           }
         }
         float most[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) most[j] = z[i][j];
+        for (int j = 0; j < 32; ++j) most[j] = z[j];
         const float top = over_lanes<true>(most, lane);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z[i][j] = expf(z[i][j] - __shfl_sync(0xffffffffu, base, j));
-        tail->share[turn.at][quarter][c + lane] = make_float2(top, over_lanes<false>(z[i], lane));
+        for (int j = 0; j < 32; ++j) z[j] = expf(z[j] - __shfl_sync(0xffffffffu, base, j));
+        tail->share[turn.at][quarter][c + lane] = make_float2(top, over_lanes<false>(z, lane));
       }
       // (what a tile leaves in shared memory stays until the one after the next, past the next one's barriers)
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(kSplitEpilogue) : "memory");
       if (token && ok) {
         float top = -INFINITY, sum = 0.f;
 #pragma unroll

@@ -116,26 +116,37 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
       : "memory");
 }
 
-// The same and `commit`, called by a whole warp, for which the hardware's elected lane (always the same) issues:
-// operands that the warp's lanes agree on stay in uniform registers, which the instruction reads. Many small
-// products are issued in half the time (48 to 60 cycles each for some 100).
-__device__ __forceinline__ void mma_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                            uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "elect.sync _|q, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
-      : "memory");
-}
-
-__device__ __forceinline__ void commit_warp(uint64_t* bar) {
+// 1 in the one lane that the hardware elects, 0 in the others; all lanes call.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t is;
   asm volatile(
       "{\n\t.reg .pred q;\n\t"
       "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(is));
+  return is;
+}
+
+// The same and `commit`, walked through by a whole warp, in the lane whose `go` is not 0: what the warp's lanes
+// agree on stays in uniform registers, which the instruction reads. Many small products are issued sooner so.
+__device__ __forceinline__ void mma_ts_if(uint32_t go, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                          uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(go)
+      : "memory");
+}
+
+__device__ __forceinline__ void commit_if(uint32_t go, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
-          static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
+          static_cast<uint32_t>(__cvta_generic_to_shared(bar))),
+      "r"(go)
       : "memory");
 }
 
