@@ -51,10 +51,15 @@ constexpr int kMaxTokens = 256;                  // tokens of a tile
 // 54 / 52, 37 / 33, 232 / 218; 65 behind 512 tokens 291 / 263, 110 / 114, 52 / 51, 560 / 599; 140 behind them
 // 280 / 268, 118 / 116, 60 / 51, 658 / 645.
 constexpr int kRestMost = 96;
-// Tokens behind 256 up to which one tile takes both. Measured likewise (both / two tiles of 256): 32 170 / 178,
+// Tokens behind 256 up to which one tile takes both, where K is at most kLongK. Measured likewise (both / two tiles of 256): 32 170 / 178,
 // 70 / 84, 39 / 40, 375 / 394; 77 172 / 177, 76 / 84, 44 / 41, 380 / 394; 128 180 / 181, 79 / 85, 46 / 41, 367 /
 // 408; 160 189 / 182, 83 / 86, 49 / 41, 435 / 409.
 constexpr int kBothMost = 128;
+// The tensor cores cut where they add, always the same way: K is taken in chunks of at most kLongK, added up in fp32 by
+// the epilogue (512 tokens and K = 4,096: relative error 5.9e-7, in one sum 2.7e-6; 64 and 1,536: 2.1e-7, 4.5e-7; the
+// time is the same). 257 to 384 tokens in one tile have no registers left for that: above kLongK they are two tiles
+// (333 tokens, K = 2,048, 50,257 rows: 102 us; in one tile 103 to 106, error 8e-7 instead of 3e-7).
+constexpr int kLongK = 1024;
 constexpr int kEpilogueThreads = 256;            // two warps a quarter of tensor memory's lanes, each half the columns
 constexpr int kThreads = 64 + kEpilogueThreads;
 constexpr uint32_t kTmemCols = 512;
@@ -144,6 +149,7 @@ struct Params {
   int M, N, K;               // tokens, vocabulary, inner size
   int full, rest, rest_cols; // tiles of 256 tokens; tokens behind them, and those rounded up to 32
   int both;                  // one tile takes 256 tokens AND the rest (full is 1)
+  int chunk;                 // steps of BK that go into one sum
   int w_rows;                // rows of the head a block takes of a tile
   int n_tiles;               // tiles of 2 w_rows rows of the head
   int stages, stage_bytes;
@@ -250,8 +256,8 @@ __device__ __forceinline__ float over_lanes(float (&v)[32], int lane) {
   return v[0];
 }
 
-// kPlain: no bias, no scale, no cap
-template <bool kPlain, bool kCap>
+// kPlain: no bias, no scale, no cap; kLong: K in several chunks
+template <bool kPlain, bool kCap, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1)
 logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap rest_map,
                const __grid_constant__ CUtensorMap w_map, const __grid_constant__ Params p) {
@@ -281,7 +287,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
   __syncthreads();
   tma::cluster_sync_all();
   tc::fence_after_sync();
-  const uint32_t tmem = bar->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bar->tmem, 0);      // (known to be the warp's own)
   let_next_kernel_start();       // (with its shared and tensor memory in hand)
   wait_for_previous_kernel();
 
@@ -328,48 +334,51 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       }
     }
   } else if (warp == 1) {
-    // ---- MMA issue: one lane of the pair's first block ----------------------------------------
-    if (rank == 0 && lane == 0) {
+    // ---- products, issued in the pair's first block: the whole warp walks and one lane issues, and no turn of the loops
+    // depends on what a lane saw, so that the operands stay in uniform registers (5 to 10 % of the kernel's time) ----
+    if (rank == 0) {
+      const uint32_t elected = tc::elect_lane();
+      const uint64_t first = tc::smem_desc_k_major_sw128(tma::smem_u32(smem));      // (descriptors count 16 bytes)
+      const uint32_t wide_desc = tc::idesc_bf16_f32(2 * BM, 2 * p.w_rows);
+      const uint32_t rest_desc = tc::idesc_bf16_f32(2 * BM, p.rest_cols);
       int stage = 0, phase = 0, count = 0;
       bool ok = true;
-      for (int round = 0; round * pairs < tiles.total && ok; ++round) {
+      for (int round = 0; round * pairs < tiles.total; ++round) {
         const int tile = tiles.at(round, pair, pairs);
         if (tile >= tiles.total) continue;
         const bool wide = tile % tiles.per < p.full, rest = !wide || p.both;
-        const uint32_t wide_desc = tc::idesc_bf16_f32(2 * BM, 2 * p.w_rows);
-        const uint32_t rest_desc = tc::idesc_bf16_f32(2 * BM, p.rest_cols);
-        // (both: 256 tokens in the first half of tensor memory, the rest in the second, one tile at a time)
-        const int buf = p.both ? 0 : count & 1, use = p.both ? count : count >> 1;
-        const uint32_t wide_acc = tmem + buf * kMaxTokens, rest_acc = tmem + (p.both ? 1 : buf) * kMaxTokens;
-        if (use >= 1 && !tma::mbar_wait(&bar->acc_empty[buf], (use - 1) & 1, p.error, 802)) break;
-        for (int kb = 0; kb < n_kb && ok; ++kb) {
-          if (!tma::mbar_wait(&bar->full[stage], phase, p.error, 803)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after_sync();
-          const uint32_t w = tma::smem_u32(smem + stage * p.stage_bytes), x = w + kWBytes;
-          const uint32_t xr = x + (wide ? kXBytes : 0);
-          if (wide) {
+        for (int chunk = 0; chunk < n_kb; chunk += p.chunk) {
+          // (both: 256 tokens in the first half of tensor memory, the rest in the second, one sum at a time)
+          const int buf = p.both ? 0 : count & 1, use = p.both ? count : count >> 1;
+          const uint32_t wide_acc = tmem + buf * kMaxTokens, rest_acc = tmem + (p.both ? 1 : buf) * kMaxTokens;
+          ok = ok && (use < 1 || tma::mbar_wait(&bar->acc_empty[buf], (use - 1) & 1, p.error, 802));
+          const int end = min(chunk + p.chunk, n_kb);
+          for (int kb = chunk; kb < end; ++kb) {
+            ok = ok && tma::mbar_wait(&bar->full[stage], phase, p.error, 803);
+            __syncwarp();
+            tc::fence_after_sync();
+            const uint32_t go = elected && ok;
+            const uint64_t w = first + stage * (p.stage_bytes >> 4), x = w + (kWBytes >> 4);
+            const uint64_t xr = x + (wide ? kXBytes >> 4 : 0);
+            if (wide) {
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              tc::mma_ss_pair(wide_acc, tc::smem_desc_k_major_sw128(x + k * 32),
-                              tc::smem_desc_k_major_sw128(w + k * 32), wide_desc, kb > 0 || k > 0);
-          }
-          if (rest) {
+              for (int k = 0; k < BK / 16; ++k)
+                tc::mma_ss_pair_if(go, wide_acc, x + 2 * k, w + 2 * k, wide_desc, kb > chunk || k > 0);
+            }
+            if (rest) {
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              tc::mma_ss_pair(rest_acc, tc::smem_desc_k_major_sw128(w + k * 32),
-                              tc::smem_desc_k_major_sw128(xr + k * 32), rest_desc, kb > 0 || k > 0);
+              for (int k = 0; k < BK / 16; ++k)
+                tc::mma_ss_pair_if(go, rest_acc, w + 2 * k, xr + 2 * k, rest_desc, kb > chunk || k > 0);
+            }
+            tc::commit_pair_if(go, &bar->empty[stage], kBoth);
+            if (++stage == p.stages) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          tc::commit_pair(&bar->empty[stage], kBoth);
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          tc::commit_pair_if(elected && ok, &bar->acc_full[buf], kBoth);
+          ++count;
         }
-        if (ok) tc::commit_pair(&bar->acc_full[buf], kBoth);
-        ++count;
       }
     }
   } else {
@@ -385,8 +394,38 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       tail->target[c] = c < p.rest ? p.targets[first_rest + c] : -1;
     for (int c = half * 32 + lane; c < kMaxTokens; c += 64) run[c] = make_float2(-INFINITY, 0.f);
     asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
-    int count = 0, wide = 0;       // tiles so far, and those of 256 tokens among them
+    int count = 0, wide = 0;       // sums so far, and tiles of 256 tokens among theirs
     bool ok = true;
+    // the sums of all chunks of K, `width` columns a run, this thread's runs from half `width` on, every other one
+    auto add_up = [&](auto& sums, int cols, int real) {
+      constexpr int kRuns = sizeof(sums) / sizeof(sums[0]), kWidth = sizeof(sums[0]) / sizeof(float);
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) sums[r][i] = 0.f;
+      for (int kb = 0; kb < n_kb; kb += p.chunk) {
+        const int buf = count & 1;
+        ok = ok && tma::mbar_wait(&bar->acc_full[buf], (count >> 1) & 1, p.error, 804);
+        ok = __all_sync(0xffffffffu, ok);
+        tc::fence_after_sync();
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r) {
+          const int c = (2 * r + half) * kWidth;
+          if (c < cols && c < real && ok) {
+#pragma unroll
+            for (int i = 0; i < kWidth; i += 16) {
+              float some[16];
+              tc::ld_32x32b_x16(lane_base + buf * kMaxTokens + c + i, some);
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) mma::add2(sums[r][i + j], sums[r][i + j + 1], some[j], some[j + 1]);
+            }
+          }
+        }
+        tc::fence_before_sync();
+        tma::mbar_arrive_cluster(tma::cluster_address(tma::smem_u32(&bar->acc_empty[buf]), 0));
+        ++count;
+      }
+    };
     for (int round = 0; round * pairs < tiles.total; ++round) {
       const int tile = tiles.at(round, pair, pairs);
       if (tile >= tiles.total) continue;
@@ -407,14 +446,8 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
         }
         ++wide;
-        ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 804);
-        tc::fence_after_sync();
-        const uint32_t acc = lane_base + buf * kMaxTokens;
         float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-        for (int c = half * 64; c < cols && ok && n0 + c < p.N; c += 128) {
-          float z[64];
-          tc::ld_32x32b_x64(acc + c, z);
+        auto take = [&](float (&z)[64], int c) {
           if (!kPlain) {
             if (p.form.bias) {
 #pragma unroll
@@ -443,6 +476,25 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
             if (here) p.mine[m] = found * unit.size;       // (a row behind the last token has no target)
           }
           take_up(z, unit.rate, top, sum);
+        };
+        if (kLong) {
+          float sums[2][64];
+          add_up(sums, cols, p.N - n0);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int c = (2 * r + half) * 64;
+            if (c < cols && ok && n0 + c < p.N) take(sums[r], c);
+          }
+        } else {
+          ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 804);
+          tc::fence_after_sync();
+          const uint32_t acc = lane_base + buf * kMaxTokens;
+#pragma unroll 1
+          for (int c = half * 64; c < cols && ok && n0 + c < p.N; c += 128) {
+            float z[64];
+            tc::ld_32x32b_x64(acc + c, z);
+            take(z, c);
+          }
         }
         // the second warp of the quarter hands its share to the first
         if (half) tail->share[thread] = make_float2(top, sum);
@@ -461,15 +513,7 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         const int v = n0 + rank * p.w_rows + thread;
         const bool real = thread < p.w_rows && v < p.N;
         const float bias = !kPlain && p.form.bias && real ? bias_at(p.form, v) * unit.mul : 0.f;
-        if (!p.both) {             // (else it has been waited for)
-          ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 806);
-          tc::fence_after_sync();
-        }
-        const uint32_t acc = lane_base + (p.both ? 1 : buf) * kMaxTokens;
-#pragma unroll 1
-        for (int c = half * 32; c < p.rest_cols && ok; c += 64) {
-          float z[32];
-          ld_32x32b_x32(acc + c, z);
+        auto take = [&](float (&z)[32], int c) {
           if (!kPlain) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) z[i] = fmaf(z[i], unit.mul, bias);
@@ -495,8 +539,30 @@ logprob_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
           for (int i = 0; i < 32; ++i) z[i] = mma::exp2_fast((z[i] - __shfl_sync(0xffffffffu, base, i)) * unit.rate);
           const float sum = over_lanes<false>(z, lane);
           run[c + lane] = make_float2(top, (old.y == 0.f ? 0.f : old.y * weight_of(old.x, top, unit.rate)) + sum);
+        };
+        if (kLong) {
+          float sums[kBothMost / 64][32];
+          add_up(sums, p.rest_cols, p.rest_cols);
+#pragma unroll
+          for (int r = 0; r < kBothMost / 64; ++r) {
+            const int c = (2 * r + half) * 32;
+            if (c < p.rest_cols && ok) take(sums[r], c);
+          }
+        } else {
+          if (!p.both) {           // (else it has been waited for)
+            ok = ok && tma::mbar_wait(&bar->acc_full[buf], use & 1, p.error, 806);
+            tc::fence_after_sync();
+          }
+          const uint32_t acc = lane_base + (p.both ? 1 : buf) * kMaxTokens;
+#pragma unroll 1
+          for (int c = half * 32; c < p.rest_cols && ok; c += 64) {
+            float z[32];
+            ld_32x32b_x32(acc + c, z);
+            take(z, c);
+          }
         }
       }
+      if (kLong) continue;         // (given back chunk by chunk)
       tc::fence_before_sync();
       // (given back whatever happened: the issuing lane counts 256 arrivals a tile)
       tma::mbar_arrive_cluster(tma::cluster_address(tma::smem_u32(&bar->acc_empty[buf]), 0));
@@ -849,7 +915,7 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tail->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tail->tmem, 0);     // (known to be the warp's own)
   let_next_kernel_start();       // (with its shared and tensor memory in hand)
   wait_for_previous_kernel();
 
@@ -1162,7 +1228,9 @@ int resident_pairs() {
   auto allow = [](auto kernel) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost) == cudaSuccess;
   };
-  if (allow(logprob_kernel<true, false>) && allow(logprob_kernel<false, false>) && allow(logprob_kernel<false, true>)) {
+  if (allow(logprob_kernel<true, false, false>) && allow(logprob_kernel<false, false, false>) &&
+      allow(logprob_kernel<false, true, false>) && allow(logprob_kernel<true, false, true>) &&
+      allow(logprob_kernel<false, false, true>) && allow(logprob_kernel<false, true, true>)) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * sm_count());
     config.blockDim = dim3(kThreads);
@@ -1174,7 +1242,7 @@ int resident_pairs() {
     attr[0].val.clusterDim.z = 1;
     config.attrs = attr;
     config.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&clusters, logprob_kernel<true, false>, &config) != cudaSuccess) clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, logprob_kernel<true, false, true>, &config) != cudaSuccess) clusters = 0;
     cudaGetLastError();
   }
   known[device] = clusters + 1;
@@ -1182,7 +1250,7 @@ int resident_pairs() {
 }
 
 // Whether one tile takes the 256 tokens and the rest of M tokens.
-bool both_of(int M, int full) { return full == 1 && M > kMaxTokens; }
+bool both_of(int M, int K, int full) { return full == 1 && M > kMaxTokens && K <= kLongK; }
 
 // The join of `pieces` partials [pieces][full] of rows below `full` and `rest_pieces` [.][M - full] of the others, which
 // lie behind them (full: a multiple of 256, perhaps past M, or M).
@@ -1224,23 +1292,23 @@ SAKV_EXPORT int sakv_logprob_f32(const float* x, long long x_stride, const float
 // Pairs of SMs that can hold the tensor-core kernel at one time (0: it cannot run here).
 SAKV_EXPORT int sakv_logprob_resident() { return resident_pairs(); }
 
-// How M tokens against N rows of the head are cut, for `pairs` pairs of SMs:
+// How M tokens against N rows of K numbers of the head are cut, for `pairs` pairs of SMs:
 // shape = {tiles of 256 tokens, rows of the head a block takes of a tile, tiles of the head, pairs launched}.
 // A block takes 128 rows of the head, or fewer where that makes the last round of tiles fuller. A few tokens: bound
 // by the head's bytes, so any height serves, the one that gives every block the same number of rows in all. More:
 // the height is a multiple of 16 (the products' width, two blocks' rows, is one of 32), and a round of tiles costs
 // what its operands' rows take from L2.
-SAKV_EXPORT int sakv_logprob_shape(int M, int N, int pairs, int* shape) {
-  if (M <= 0 || N <= 0 || pairs <= 0 || N > 0x7fffffff - 512 || M > 0x7fffffff - 512) return cudaErrorInvalidValue;
-  const int most = M > kMaxTokens && M < 2 * kMaxTokens ? kBothMost : kRestMost;
+SAKV_EXPORT int sakv_logprob_shape(int M, int N, int K, int pairs, int* shape) {
+  if (M <= 0 || N <= 0 || K <= 0 || pairs <= 0 || N > 0x7fffffff - 512 || M > 0x7fffffff - 512) return cudaErrorInvalidValue;
+  const int most = M > kMaxTokens && M < 2 * kMaxTokens && K <= kLongK ? kBothMost : kRestMost;
   const int full = M / kMaxTokens + (M % kMaxTokens > most ? 1 : 0);
-  const int per = both_of(M, full) ? 1 : full + (M > full * kMaxTokens);
+  const int per = both_of(M, K, full) ? 1 : full + (M > full * kMaxTokens);
   int rows = BM;
   if (full == 0) {
     const int rounds = (N + 2 * BM * pairs - 1) / (2 * BM * pairs);
     rows = (N + 2 * pairs * rounds - 1) / (2 * pairs * rounds);
   } else {
-    const int beside = both_of(M, full) ? (M - kMaxTokens + 31) / 32 * 16 : 0;
+    const int beside = both_of(M, K, full) ? (M - kMaxTokens + 31) / 32 * 16 : 0;
     long long best = -1;
     for (int r = BM; r >= 96; r -= 16) {
       const long long tiles = (N + 2 * r - 1) / (2 * r) * (long long)per;
@@ -1356,7 +1424,7 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const voi
   const int here = resident_pairs();
   if (K <= 0 || (K % 8) || !(cap >= 0.f)) return cudaErrorInvalidValue;
   if (here <= 0) return cudaErrorNotSupported;
-  const int bad = sakv_logprob_shape(M, N, here, expect);
+  const int bad = sakv_logprob_shape(M, N, K, here, expect);
   if (bad) return bad;
   for (int i = 0; i < 4; ++i)
     if (shape[i] != expect[i]) return cudaErrorInvalidValue;
@@ -1365,7 +1433,7 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const voi
   p.full = shape[0]; p.w_rows = shape[1]; p.n_tiles = shape[2];
   p.rest = M > p.full * kMaxTokens ? M - p.full * kMaxTokens : 0;
   p.rest_cols = (p.rest + 31) / 32 * 32;
-  p.both = both_of(M, p.full);
+  p.both = both_of(M, K, p.full);
   p.stage_bytes = kWBytes + (p.full ? kXBytes : 0) + (p.full == 0 || p.both ? p.rest_cols / 2 * BK * 2 : 0);
   p.stages = kRingMost / p.stage_bytes < kMaxStages ? kRingMost / p.stage_bytes : kMaxStages;
   p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;
@@ -1378,8 +1446,13 @@ SAKV_EXPORT int sakv_logprob_pieces(const void* x, long long x_stride, const voi
   if (!e && p.full && p.rest) e = logprob_map(&rest_map, x, M, K, x_stride, p.rest_cols / 2);
   else rest_map = x_map;
   if (e) return e;
-  auto kernel = cap > 0.f ? logprob_kernel<false, true>
-                          : bias || scale != 1.f ? logprob_kernel<false, false> : logprob_kernel<true, false>;
+  const int steps = (K + BK - 1) / BK, chunks = (K + kLongK - 1) / kLongK;
+  p.chunk = (steps + chunks - 1) / chunks;
+  auto kernel = chunks > 1
+      ? cap > 0.f ? logprob_kernel<false, true, true>
+                  : bias || scale != 1.f ? logprob_kernel<false, false, true> : logprob_kernel<true, false, true>
+      : cap > 0.f ? logprob_kernel<false, true, false>
+                  : bias || scale != 1.f ? logprob_kernel<false, false, false> : logprob_kernel<true, false, false>;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(2 * shape[3]);
   config.blockDim = dim3(kThreads);

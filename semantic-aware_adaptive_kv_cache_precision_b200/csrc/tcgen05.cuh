@@ -127,7 +127,7 @@ __device__ __forceinline__ uint32_t elect_lane() {
   return is;
 }
 
-// The same and `commit`, walked through by a whole warp, in the lane whose `go` is not 0: what the warp's lanes
+// The products and `commit`, walked through by a whole warp, in the lane whose `go` is not 0: what the warp's lanes
 // agree on stays in uniform registers, which the instruction reads. Many small products are issued sooner so.
 __device__ __forceinline__ void mma_ts_if(uint32_t go, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                           uint32_t idesc, bool accumulate) {
@@ -137,6 +137,17 @@ __device__ __forceinline__ void mma_ts_if(uint32_t go, uint32_t d_tmem, uint32_t
       "setp.ne.b32 p, %4, 0;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(go)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_ss_if(uint32_t go, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(go)
       : "memory");
 }
 
@@ -210,6 +221,28 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar, uint16_t mask) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%0], %1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar))),
       "h"(mask)
+      : "memory");
+}
+
+// Both again, for a warp that walks and a lane that issues (see `mma_ts_if`).
+__device__ __forceinline__ void mma_ss_pair_if(uint32_t go, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(go)
+      : "memory");
+}
+
+__device__ __forceinline__ void commit_pair_if(uint32_t go, uint64_t* bar, uint16_t mask) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;\n\t}" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar))),
+      "h"(mask), "r"(go)
       : "memory");
 }
 

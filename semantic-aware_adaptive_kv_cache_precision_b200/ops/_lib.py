@@ -117,7 +117,7 @@ PLAIN_SIGNATURES = {
     "sakv_decode_attention_map": ("attention_decode", [P, P, L, I, I]),
     "sakv_decode_attention_error": ("attention_decode", [P]),
     "sakv_decode_attention_max_cluster": ("attention_decode", [I]),
-    "sakv_logprob_shape": ("logprobs", [I, I, I, P]),
+    "sakv_logprob_shape": ("logprobs", [I, I, I, I, P]),
     "sakv_logprob_split_rows": ("logprobs", [I, I]),
     "sakv_logprob_split_tokens": ("logprobs", [I]),
     "sakv_logprob_fold_columns": ("logprobs", []),

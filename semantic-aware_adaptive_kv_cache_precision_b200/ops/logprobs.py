@@ -83,19 +83,19 @@ def _refuse(x, head, targets, bias, softcap) -> torch.Tensor:
 _shapes: dict = {}
 
 
-def _shape(rows: int, vocab: int):
+def _shape(rows: int, vocab: int, k: int):
     """How the tensor-core kernel cuts so many rows and tokens on this device: (the numbers the launch takes, floats
     of scratch)."""
     pairs = _pairs()
-    hit = _shapes.get((rows, vocab, pairs))
+    hit = _shapes.get((rows, vocab, k, pairs))
     if hit is None:
         shape = (ctypes.c_int * 4)()
-        if plain_function("sakv_logprob_shape")(rows, vocab, pairs, shape) != 0:
+        if plain_function("sakv_logprob_shape")(rows, vocab, k, pairs, shape) != 0:
             raise KernelError(f"token_logprobs: {rows} rows over {vocab} tokens are too many")
         full = shape[0] * 256
         if len(_shapes) >= 256:
             _shapes.clear()
-        hit = _shapes[rows, vocab, pairs] = (shape, 2 * (shape[2] * full + 2 * shape[3] * max(0, rows - full)))
+        hit = _shapes[rows, vocab, k, pairs] = (shape, 2 * (shape[2] * full + 2 * shape[3] * max(0, rows - full)))
     return hit
 
 
@@ -131,7 +131,7 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
     at, head_at = x.data_ptr(), head.data_ptr()
     bias_at, bias_code = (None, F32) if bias is None else (bias.data_ptr(), dtype_code(bias.dtype))
     if x.dtype is torch.bfloat16 and k % 8 == 0 and stride % 8 == 0 and (at | head_at) % 16 == 0 and _pairs() > 0:
-        shape, floats = _shape(rows, vocab)
+        shape, floats = _shape(rows, vocab, k)
         part = x.new_empty(floats + rows, dtype=torch.float32)
         scratch = part.data_ptr()
         call("sakv_logprob_pieces", at, stride, head_at, rows, vocab, k, shape, targets.data_ptr(), scratch,

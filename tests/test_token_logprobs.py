@@ -85,17 +85,18 @@ def test_tiles_cover_the_vocabulary(pairs):
     from semantic_aware_adaptive_kv_cache_precision_b200.ops._lib import plain_function
     shape = (ctypes.c_int * 4)()
     for rows in (1, 31, 96, 97, 255, 256, 257, 333, 384, 385, 511, 513, 608, 609, 2047, 2048):
-        for vocab in (1, 2, 300, 4097, 50257, 151936):
-            assert plain_function("sakv_logprob_shape")(rows, vocab, pairs, shape) == 0
+        for vocab, k in ((v, k) for v in (1, 2, 300, 4097, 50257, 151936) for k in (64, 1024, 1032)):
+            assert plain_function("sakv_logprob_shape")(rows, vocab, k, pairs, shape) == 0
             full, height, tiles, launched = shape
             rest = rows - 256 * full
-            per = 1 if full == 1 and rest > 0 else full + (rest > 0)
-            assert rest <= 128 and rest > -256 and 1 <= height <= 128 and (not full or height % 16 == 0)
+            per = 1 if full == 1 and rest > 0 and k <= 1024 else full + (rest > 0)
+            assert rest <= (128 if k <= 1024 else 96)
+            assert rest > -256 and 1 <= height <= 128 and (not full or height % 16 == 0)
             assert (tiles - 1) * 2 * height < vocab <= tiles * 2 * height
             assert launched == min(pairs, tiles * per)
             if not full:                      # every block has the same number of rows in all, but for the last ones
                 assert -(-tiles // launched) * 2 * height * launched - vocab < 2 * launched * -(-tiles // launched)
-    for bad in ((0, 5, 1), (5, 0, 1), (5, 5, 0), (2 ** 31 - 1, 5, 1)):
+    for bad in ((0, 5, 64, 1), (5, 0, 64, 1), (5, 5, 0, 1), (5, 5, 64, 0), (2 ** 31 - 1, 5, 64, 1)):
         assert plain_function("sakv_logprob_shape")(*bad, shape) != 0
 
 
@@ -243,3 +244,31 @@ def test_heights_and_widths_of_32_bit_tiles():
         assert rows <= padded < rows + 32 * tiles and padded % (32 * tiles) == 0 and padded // tiles <= 96
     assert plain_function("sakv_logprob_split_tokens")(0) == 0
     assert plain_function("sakv_logprob_split_tokens")(2 ** 31 - 1) == 0 == plain_function("sakv_logprob_split_rows")(0, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [1024, 1032, 2056, 3136])
+@pytest.mark.parametrize("rows", [5, 40, 96, 97, 256, 300, 352, 353, 520, 610])
+def test_sums_in_several_chunks(rows, k):
+    check(rows, k, 1333, torch.bfloat16, torch.float32 if rows % 2 else None, 0.5 if rows % 3 else 1.0,
+          20.0 if rows % 5 == 0 else 0.0, seed=rows + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [40, 256])
+def test_long_sums_of_16_bits(rows):
+    """Numbers of one sign, where what is cut off adds up."""
+    k = 4096
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.rand((rows, k), generator=g, device="cuda") + 0.5).to(torch.bfloat16)
+    w = ((torch.rand((700, k), generator=g, device="cuda") + 0.5) / k).to(torch.bfloat16)
+    targets = torch.randint(0, 700, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    got, lse = ops.token_logprobs(x, w, targets)
+    z = x.double() @ w.double().t()
+    want_lse = torch.logsumexp(z, 1)
+    want = z.gather(1, targets.long()[:, None])[:, 0] - want_lse
+    # 1,024 products and 64 additions on the tensor cores, each cut by a step of the sum (2^-23) at most, then three
+    # additions that round by 2^-24; lse's own sum as above
+    dz = (1024 + 64 + 2) * 2.0 ** -23 * z.amax()
+    assert ((lse.double() - want_lse).abs() <= dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (1 + want_lse)).all()
+    assert ((got.double() - want).abs() <= 2 * dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (2 + want_lse)).all()
