@@ -367,44 +367,49 @@ attend_wide(const Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
         tma::mbar_wait(&bar->v_full[i % kWideStages], (i / kWideStages) & 1, p.error, 164);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kWideRows, KT);                   // K-major both
-      constexpr uint32_t idesc_pv = tc::idesc_bf16_f32(kWideRows, D) | (1u << 16);      // B MN-major
-      bool ok = tma::mbar_wait(&bar->q_full, 0, p.error, 165);
-      const uint32_t q_addr = tma::smem_u32(q_s);
-      auto issue_pv = [&](int i) {
-        const int stage = i % kWideStages;
-        if (!tma::mbar_wait(&bar->p_full, i & 1, p.error, 166)) return false;
-        if (!tma::mbar_wait(&bar->v_full[stage], (i / kWideStages) & 1, p.error, 167)) return false;
-        tc::fence_after_sync();
-        const uint32_t v_addr = tma::smem_u32(kv_s + stage * S::kStageBytes + S::kTileBytes);
+    // the whole warp walks and one lane issues, and no turn of the loop depends on what a lane saw, so that the operands
+    // stay in uniform registers
+    constexpr uint32_t idesc_s = tc::idesc_bf16_f32(kWideRows, KT);                   // K-major both
+    constexpr uint32_t idesc_pv = tc::idesc_bf16_f32(kWideRows, D) | (1u << 16);      // B MN-major
+    const uint32_t elected = tc::elect_lane();
+    const int tiles = __shfl_sync(0xffffffffu, n, 0);
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t queries = tc::smem_desc_k_major_sw128(tma::smem_u32(q_s));         // (descriptors count 16 bytes)
+    const uint64_t keys = tc::smem_desc_k_major_sw128(tma::smem_u32(kv_s));
+    const uint64_t values = desc_values(tma::smem_u32(kv_s + S::kTileBytes));
+    bool ok = tma::mbar_wait(&bar->q_full, 0, p.error, 165);
+    auto issue_pv = [&](int i) {
+      const int stage = i % kWideStages;
+      ok = ok && tma::mbar_wait(&bar->p_full, i & 1, p.error, 166) &&
+           tma::mbar_wait(&bar->v_full[stage], (i / kWideStages) & 1, p.error, 167);
+      __syncwarp();
+      tc::fence_after_sync();
+      const uint32_t go = elected && ok;
+      const uint64_t v = values + stage * (S::kStageBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < KT / 16; ++k)
-          tc::mma_ts(tmem + kOCol, tmem + (i & 1) * KT + k * 8, desc_values(v_addr + k * 2048), idesc_pv,
-                     i > 0 || k > 0);
-        tc::commit(&bar->pv_done);
-        tc::commit(&bar->v_empty[stage]);
-        return true;
-      };
-      for (int j = 0; j < n && ok; ++j) {
-        const int stage = j % kWideStages;
-        // (S_j goes where S_{j-2} and then P_{j-2} lay: P_{j-2} V_{j-2} was issued before this, and one
-        // thread's products run in the order it issued them)
-        ok = tma::mbar_wait(&bar->k_full[stage], (j / kWideStages) & 1, p.error, 168);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint32_t k_addr = tma::smem_u32(kv_s + stage * S::kStageBytes);
+      for (int k = 0; k < KT / 16; ++k)
+        tc::mma_ts_if(go, base + kOCol, base + (i & 1) * KT + k * 8, v + k * (2048 >> 4), idesc_pv, i > 0 || k > 0);
+      tc::commit_if(go, &bar->pv_done);
+      tc::commit_if(go, &bar->v_empty[stage]);
+    };
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j % kWideStages;
+      // (S_j goes where S_{j-2} and then P_{j-2} lay: P_{j-2} V_{j-2} was issued before this, and one
+      // thread's products run in the order it issued them)
+      ok = ok && tma::mbar_wait(&bar->k_full[stage], (j / kWideStages) & 1, p.error, 168);
+      __syncwarp();
+      tc::fence_after_sync();
+      const uint32_t go = elected && ok;
+      const uint64_t k_at = keys + stage * (S::kStageBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc::mma_ss(tmem + (j & 1) * KT,
-                     tc::smem_desc_k_major_sw128(q_addr + (k >> 2) * (kWideRows * 128) + (k & 3) * 32),
-                     tc::smem_desc_k_major_sw128(k_addr + (k >> 2) * (KT * 128) + (k & 3) * 32), idesc_s, k > 0);
-        tc::commit(&bar->s_full[j & 1]);
-        tc::commit(&bar->k_empty[stage]);
-        if (j >= 1) ok = issue_pv(j - 1);
-      }
-      if (ok && n > 0) issue_pv(n - 1);
+      for (int k = 0; k < D / 16; ++k)
+        tc::mma_ss_if(go, base + (j & 1) * KT, queries + ((k >> 2) * (kWideRows * 128) + (k & 3) * 32) / 16,
+                      k_at + ((k >> 2) * (KT * 128) + (k & 3) * 32) / 16, idesc_s, k > 0);
+      tc::commit_if(go, &bar->s_full[j & 1]);
+      tc::commit_if(go, &bar->k_empty[stage]);
+      if (j >= 1) issue_pv(j - 1);
     }
+    if (tiles > 0) issue_pv(tiles - 1);
   } else {
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;                         // row of the unit = tensor-memory lane
