@@ -15,6 +15,8 @@ from .linear import linear
 PIECE_ELEMENTS = 8 << 20
 #: numbers of x that are split at one time in 32 bits (six bytes each: 384 MB)
 SPLIT_ELEMENTS = 64 << 20
+#: (maximum, sum) pairs of tiles that they leave at one time (512 MB)
+SPLIT_PAIRS = 64 << 20
 
 
 _resident: dict = {}
@@ -138,11 +140,10 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
              scratch + 4 * floats, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
         _lib.launches += 1          # the call launched the join too
     elif x.dtype is torch.float32 and k % 4 == 0 and head_at % 16 == 0:
-        padded = -(-k // 8) * 8
-        most = max(1, SPLIT_ELEMENTS // padded)
+        padded, tile = -(-k // 8) * 8, _split_rows(vocab)
+        most = max(1, min(SPLIT_ELEMENTS // padded, SPLIT_PAIRS // -(-vocab // tile)))
         if rows > most:
             return _in_pieces(x, head, targets, bias, scale, softcap, most)
-        tile = _split_rows(vocab)
         halves = 3 * plain_function("sakv_logprob_split_tokens")(rows) * padded // 2
         floats = halves + 2 * rows * -(-vocab // tile)
         part = x.new_empty(floats + rows, dtype=torch.float32)       # the split rows, the partials, the targets' logits

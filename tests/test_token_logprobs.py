@@ -224,9 +224,10 @@ def test_long_sums_of_32_bits(k):
 
 
 @pytest.mark.gpu
-def test_rows_of_32_bits_in_pieces(monkeypatch):
+@pytest.mark.parametrize("name, value", [("SPLIT_ELEMENTS", 70 * 136), ("SPLIT_PAIRS", 29 * 101)])
+def test_rows_of_32_bits_in_pieces(monkeypatch, name, value):
     x, w, targets, got, lse = check(301, 132, 3001, torch.float32, seed=8)
-    monkeypatch.setattr(logprobs, "SPLIT_ELEMENTS", 70 * 136)
+    monkeypatch.setattr(logprobs, name, value)
     again, lse2 = ops.token_logprobs(x, w, targets)
     assert torch.equal(again, got) and torch.equal(lse, lse2)
 
