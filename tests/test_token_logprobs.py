@@ -273,3 +273,42 @@ def test_long_sums_of_16_bits(rows):
     dz = (1024 + 64 + 2) * 2.0 ** -23 * z.amax()
     assert ((lse.double() - want_lse).abs() <= dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (1 + want_lse)).all()
     assert ((got.double() - want).abs() <= 2 * dz + 512 * 2.0 ** -23 + 2.0 ** -21 * (2 + want_lse)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, k", [(torch.float32, 260), (torch.float32, 1028), (torch.bfloat16, 2056)])
+def test_two_streams_and_graphs_at_once(dtype, k):
+    """Calls side by side, and two captured calls replayed side by side, share nothing."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    sides = []
+    for rows, vocab in ((70, 30000), (130, 9000)):
+        x = torch.randn((rows, k), generator=g, device="cuda").to(dtype)
+        w = (torch.randn((vocab, k), generator=g, device="cuda") / math.sqrt(k)).to(dtype)
+        targets = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+        sides.append((x, w, targets, torch.cuda.Stream()))
+    alone = [ops.token_logprobs(x, w, t)[0].clone() for x, w, t, _ in sides]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (x, w, t, stream) in enumerate(sides):
+            with torch.cuda.stream(stream):
+                got[i].append(ops.token_logprobs(x, w, t)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, many in zip(alone, got) for b in many)
+    graphs = []
+    for x, w, t, _ in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = ops.token_logprobs(x, w, t)[0]
+        graphs.append((graph, held))
+    for x, _, _, _ in sides:
+        x.copy_(x.flip(0))
+    fresh = [ops.token_logprobs(x, w, t)[0] for x, w, t, _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for (graph, _), (_, _, _, stream) in zip(graphs, sides):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(held, want) for (_, held), want in zip(graphs, fresh))
+    assert not torch.equal(fresh[0], alone[0])
