@@ -800,7 +800,7 @@ int launch_f32(const float* x, long long x_stride, const float* head, int M, int
 // depends on the vocabulary and the device alone and every tile leaves a partial: a row's sums are the same to the bit
 // whatever rows are beside it.
 // Measured: 64 tokens, K 1,024, 32,768 rows 44 us (21 at the memory's rate, 15 the products at the tensor cores'; the
-// multiply-adds below took 131); 64, 1,536, 151,936 253 us (145, 107); 185, 1,704, 94,657 344 us (100, 214; 1,480). A
+// multiply-adds below took 131); 64, 1,536, 151,936 240 us (145, 107); 185, 1,704, 94,657 334 us (100, 214; 1,480). A
 // step of 64 takes 0.9 to 1.2 us, of which the floats' arrival is 0.7: cutting them in three and the products, each a
 // chain of waits, share what is left (without the products 0.86, without the cutting 0.9).
 constexpr int kSplitThreads = 768, kSplitTokens = 96, kSplitEpilogue = 4 * kSplitTokens, kSplitRaw = BM * BK * 4;
@@ -851,8 +851,8 @@ __device__ __forceinline__ uint32_t cut_two(float& a, float& b) {
 __global__ void __launch_bounds__(256)
 split_kernel(const float* __restrict__ x, long long x_stride, int M, int K, int rows, int padded, int wide,
              uint2* __restrict__ out) {
-  let_next_kernel_start();
   wait_for_previous_kernel();
+  let_next_kernel_start();       // (in this order: the next one reads the head before it waits for this one)
   const int per = padded / 4;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)rows * per;
   if (i >= all) return;
@@ -917,7 +917,8 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tail->tmem, 0);     // (known to be the warp's own)
   let_next_kernel_start();       // (with its shared and tensor memory in hand)
-  wait_for_previous_kernel();
+  // (what comes before `split_kernel` is done once that one lets this one start; only the warp that reads what it
+  // writes waits for it, and all others wait for that warp before they write)
 
   if (warp == 0 || warp == 2) {
     // ---- TMA: the head's rows, or the tokens' -------------------------------------------------
@@ -927,6 +928,7 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       uint64_t *full = head ? tail->raw_full : tail->x_full, *empty = head ? tail->raw_empty : tail->done;
       const int stages = head ? p.raw_stages : p.x_stages;
       tma::prefetch_map(map);
+      if (!head) wait_for_previous_kernel();
       Place place;
       long long issued = 0;
       bool ok = true;
