@@ -36,6 +36,8 @@ DEFAULT_MAX_STEP_TOKENS = 16384
 # 8 sequences 1.242 / 1.320 (59), 1.539 / 1.485 (115); 14 layers of 28 over 4, 64 sequences 1.617 / 1.731 (66),
 # 1.730 / 1.744 (132), 1.964 / 1.838 (264); 8 sequences 1.372 / 1.412 (29), 1.511 / 1.471 (59).
 SHARED_BYTES_WORTH = 80 << 20
+# Layouts of plans whose words are kept on the device for captured steps to read.
+MOST_PLAN_BUFFERS = 64
 
 
 class Engine:
@@ -247,8 +249,12 @@ class Engine:
             known, reach, plans = self._shared_now
             if known == key and all(e <= r for e, r in zip(ends, reach)):
                 return plans
-        if len(self._shared_buffers) >= 64:       # layouts come and go; captured steps go with them
+        if len(self._shared_buffers) >= MOST_PLAN_BUFFERS:
+            # layouts come and go; every captured step goes with them, whichever way it was captured: a graph
+            # reads its plan at the buffer's address, and a later plan of the same layout lies elsewhere
             self._graphs.clear()
+            self._prefill_graphs.clear()
+            self._shared_now = None
             self._shared_buffers.clear()
         # (eight blocks further: a decode loop asks again after 512 steps at the earliest)
         reach = [min(width * BLOCK, e + 8 * BLOCK) for e in ends]

@@ -359,3 +359,44 @@ def test_the_command_line(varied_folders, capsys):
     assert main(["score", "--model", folder, "--dtype", "float32", "--prompt-ids", "1,2,3"]) == 0
     line = json.loads(capsys.readouterr().out)
     assert line["prompt"] == 0 and line["tokens"] == 2
+
+
+def engine_without_a_gpu(monkeypatch, cache, readers):
+    """An engine's bookkeeping of plans over a cache on the host, with nothing that launches."""
+    from types import SimpleNamespace
+    from semantic_aware_adaptive_kv_cache_precision_b200.engine import engine as module
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    monkeypatch.setattr(module._lib, "sm_count", lambda device=None: 148)
+    e = Engine.__new__(Engine)
+    e.device, e.cache, e.model = torch.device("cpu"), None, SimpleNamespace(shared_readers=lambda: readers, arena=None)
+    e.shared_bytes_worth, e._shared_now, e._shared_buffers = 0, None, {}
+    e._graphs, e._prefill_graphs = {}, {}
+    return e
+
+
+def test_captured_steps_go_with_the_plans_they_read(monkeypatch):
+    """A captured step reads its plan at a device address. When the buffers of plans are given up, every captured
+    step whose key has a plan is, however it was captured: the next plan of that layout lies elsewhere."""
+    from types import SimpleNamespace
+    from semantic_aware_adaptive_kv_cache_precision_b200.cache import KVNeed, SequenceCache
+    from semantic_aware_adaptive_kv_cache_precision_b200.engine import engine as module
+    monkeypatch.setattr(module, "MOST_PLAN_BUFFERS", 3, raising=False)
+    need = KVNeed(1, 64)
+    cache = SequenceCache([need], 64 * BLOCK, 64 * BLOCK, torch.bfloat16, "cpu", max_slots=90)
+    e = engine_without_a_gpu(monkeypatch, cache, [(need, 2)])
+    (a,) = cache.open(1)
+    cache.reserve([a], [2 * BLOCK])
+    cache.advance([a], [2 * BLOCK])
+    slots = [a] + cache.fork(a, 80)
+    for n in list(range(2, 75)) + [2, 40]:
+        plans = e._shared_plans(slots[:n], [2 * BLOCK] * n, cache)
+        assert plans
+        key = ("step", n, module._plans_in_key(SimpleNamespace(shared=plans)))
+        at = [plan.words.data_ptr() for plan in plans.values()]
+        for table in (e._graphs, e._prefill_graphs):
+            if key in table:           # (it would be replayed)
+                assert table[key] == at
+            table[key] = at
+        assert len(e._shared_buffers) <= 64
+        held = {b.data_ptr() for b in e._shared_buffers.values()}
+        assert all(set(x) <= held for table in (e._graphs, e._prefill_graphs) for x in table.values())
