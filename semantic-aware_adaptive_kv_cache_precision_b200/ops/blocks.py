@@ -42,21 +42,23 @@ def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: 
         return
     table = (_Tensor * len(tensors))()
     device = tensors[0].get_device()
-    known, blocks, room, empty = None, -1, -1, False
+    known, blocks, room, some = None, -1, -1, 0
     spans = []
-    for i, (t, u) in enumerate(zip(tensors, targets)):
+    for t, u in zip(tensors, targets):
         shape = t.shape
         alike = (shape, t.dtype, None if u is t else u.shape)
         if alike != known:                 # (the keys' pool and the values' are mostly alike)
             known = alike
             geometry, blocks, room = _geometry(t, u, rows, axis, blocks, room)
-            empty = empty or t.numel() == 0
         if not t.is_contiguous() or t.get_device() != device or u is not t and (
                 not u.is_contiguous() or u.get_device() != device or u.dtype != t.dtype):
             raise KernelError(f"copy_blocks: {tuple(shape)} {t.dtype} into {tuple(u.shape)} {u.dtype}: contiguous "
                               "tensors of one type on one device")
+        if t.numel() == 0:                 # (state of no size beside other state: nothing of it to copy)
+            continue
         a, z = t.data_ptr(), u.data_ptr()
-        table[i] = (a, z) + geometry
+        table[some] = (a, z) + geometry
+        some += 1
         spans.append((z, z + (geometry[1] or room * geometry[2]) * geometry[3]))
     try:
         source, target = array.array("i", src), array.array("i", dst)
@@ -72,12 +74,12 @@ def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: 
             raise KernelError("copy_blocks: a target tensor overlaps another one")
     elif len(spans) > 1 and _overlap(spans):
         raise KernelError("copy_blocks: tensors overlap")
-    if device < 0 or empty or not count:
+    if device < 0 or not some or not count:
         _check_numbers(source, target, blocks, room, into is None)
         require_cuda(*tensors)
         return
     try:
-        call_on(device, "sakv_copy_blocks", table, len(tensors), source.buffer_info()[0], target.buffer_info()[0],
+        call_on(device, "sakv_copy_blocks", table, some, source.buffer_info()[0], target.buffer_info()[0],
                 count, blocks, room, into is None)
     except KernelError:
         _check_numbers(source, target, blocks, room, into is None)

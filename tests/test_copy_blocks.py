@@ -285,3 +285,39 @@ def test_copies_past_four_gigabytes_and_captured():
     t[0, 4999] += 1
     graph.replay()
     assert torch.equal(t[0, 17, :, :5], t[0, 4999, :, :5]) and not t[0, 17, :, 5:].any()
+
+
+@pytest.mark.gpu
+def test_tensors_of_no_size_beside_others():
+    g = torch.Generator().manual_seed(6)
+    states = [torch.randn((8,) + s, generator=g).cuda() for s in ((0, 7), (3, 4), (2, 0), (5,))]
+    want = [s.clone() for s in states]
+    for w in want:
+        w[[1, 6]] = w[[0, 3]]
+    ops.copy_blocks(states, [0, 3], [1, 6], axis=0)
+    assert all(torch.equal(a, b) for a, b in zip(states, want))
+    pools = [torch.randn(s, generator=g).cuda() for s in ((0, 8, 2, 64, 4), (3, 8, 2, 64, 4), (1, 8, 2, 64, 0))]
+    want = [p.clone() for p in pools]
+    want[1][:, 2, :, :9] = want[1][:, 5, :, :9]
+    ops.copy_blocks(pools, [5], [2], rows=9)
+    assert all(torch.equal(a, b) for a, b in zip(pools, want))
+    ops.copy_blocks([pools[0], pools[2]], [5], [2])                # nothing at all to copy
+    for bad in (lambda: ops.copy_blocks(pools, [8], [2]), lambda: ops.copy_blocks([pools[0]], [0], [8]),
+                lambda: ops.copy_blocks([pools[0], states[0]], [0], [1])):
+        with pytest.raises(KernelError):
+            bad()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_state_of_no_size_keeps_no_other_state_from_moving(device):
+    """A mixer whose convolution has one tap keeps no inputs beside its recurrent state."""
+    needs = [KVNeed(2, 16), MultiNeed((StateNeed((0, 6), "float32"), StateNeed((2, 3), "float32"))), StateNeed((4,), "int32")]
+    cache = SequenceCache(needs, 6 * BLOCK, 1024, torch.float32, device, max_slots=3)
+    (a,) = cache.open(1)
+    fill(cache, a, 70, 1)
+    want = content(cache, a)
+    (b,) = cache.fork(a)
+    assert same(content(cache, b), want)
+    cache.resize(12 * BLOCK, 9)
+    cache.check()
+    assert same(content(cache, a), want) and same(content(cache, b), want)
