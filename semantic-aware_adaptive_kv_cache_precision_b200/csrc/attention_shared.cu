@@ -566,8 +566,8 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   // First of all, and in narrow units too: until a block has given up its right to tensor memory, the SM starts no
   // second block of a kernel that may ask for it (measured: the second ones started 8 to 15 us late).
   if ((threadIdx.x >> 5) == 1) tc::tmem_alloc(&tmem_at, kTmemCols);
-  // (the plan, the block lists and the lengths are the step's inputs: they were written before the kernel
-  // before this one began; what that one wrote, queries, keys and values, is read behind the wait)
+  // (the plan, the block lists and the lengths were written before the kernel before this one began, or this one was
+  // launched behind all that came before it; what else that one wrote, queries, keys and values, is read behind the wait)
   const int unit = blockIdx.x / p.kv_heads, g = blockIdx.x - unit * p.kv_heads;
   const int group = p.heads / p.kv_heads;
   // (the grid is as large as the plan has room for; a unit behind its last one reads words of no meaning, and
@@ -724,8 +724,11 @@ int* error_word() {
   return known[device];
 }
 
+// `settled`: the plan, the lengths and the block lists were written before the kernel before this one began, as a
+// step's inputs are, and may be read while it runs. Else the first kernel starts behind all that came before it.
 template <int D>
-int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_bfloat16* out, cudaStream_t stream) {
+int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_bfloat16* out, bool settled,
+           cudaStream_t stream) {
   static PerDeviceOnce configured;
   if (configured.needs()) {
     const cudaError_t e = cudaFuncSetAttribute(shared_attention_kernel<D>,
@@ -733,13 +736,17 @@ int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_b
     if (e != cudaSuccess) return (int)e;
     configured.done();
   }
+  const dim3 units((unsigned)(p.plan.unit_capacity * p.kv_heads)), rows((unsigned)(p.sequences * p.heads));
+  auto join = join_kernel<D>;
   if (p.plan.unit_capacity > 0) {
-    const int e = launch_overlapped(shared_attention_kernel<D>, dim3((unsigned)(p.plan.unit_capacity * p.kv_heads)),
-                                    dim3(kThreads), Smem<D>::kBytes, stream, 1, k_map, v_map, p);
+    auto attend = shared_attention_kernel<D>;
+    const int e = settled ? launch_overlapped(attend, units, dim3(kThreads), Smem<D>::kBytes, stream, 1, k_map, v_map, p)
+                          : launch_ordered(attend, units, dim3(kThreads), Smem<D>::kBytes, stream, k_map, v_map, p);
     if (e) return e;
+  } else if (!settled) {
+    return launch_ordered(join, rows, dim3(kNarrowThreads), 0, stream, p.plan, p.part_o, p.part_ml, out, p.heads);
   }
-  return launch_overlapped(join_kernel<D>, dim3((unsigned)(p.sequences * p.heads)), dim3(kNarrowThreads), 0, stream, 1,
-                           p.plan, p.part_o, p.part_ml, out, p.heads);
+  return launch_overlapped(join, rows, dim3(kNarrowThreads), 0, stream, 1, p.plan, p.part_o, p.part_ml, out, p.heads);
 }
 
 }  // namespace
@@ -750,13 +757,13 @@ struct SakvSharedPlan {
   int width, unit_at, unit_capacity, member_at, first_at, partials, sequences, heads, kv_heads;
 };
 
-// `keys`, `values`: the cache entry [blocks][kv_heads][64][head_dim]; `plan`: int32 words on the device, laid out as the numbers `n` (on the host) say; `part`: scratch of
-// partials x heads x (head_dim + 2) floats.
+// `keys`, `values`: the cache entry [blocks][kv_heads][64][head_dim]; `plan`: int32 words on the device, laid out as the
+// numbers `n` (on the host) say; `part`: scratch of partials x heads x (head_dim + 2) floats; `settled`: see `launch`.
 SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long long blocks, const void* q,
                                       long long q_stride,
                                       const int32_t* seq_lens, const int32_t* block_table, const int32_t* plan,
                                       const SakvSharedPlan* n, void* out, float* part, int head_dim, float scale,
-                                      cudaStream_t stream) {
+                                      int settled, cudaStream_t stream) {
   const int sequences = n->sequences, heads = n->heads, kv_heads = n->kv_heads, max_blocks = n->width;
   if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kMostGroup ||
       max_blocks <= 0 || max_blocks > (1 << 24) || n->unit_capacity < 0 || n->partials < 0 || (q_stride & 1) ||
@@ -783,7 +790,7 @@ SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long
   if (!bad) bad = tma::make_map_bf16_2d(&vm, values, (uint64_t)rows, head_dim, (uint64_t)head_dim * 2, KT, 64);
   if (bad) return bad;
   __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
-  return head_dim == 64 ? launch<64>(km, vm, p, o, stream) : launch<128>(km, vm, p, o, stream);
+  return head_dim == 64 ? launch<64>(km, vm, p, o, settled != 0, stream) : launch<128>(km, vm, p, o, settled != 0, stream);
 }
 
 SAKV_EXPORT int sakv_shared_attention_error(int* value) {

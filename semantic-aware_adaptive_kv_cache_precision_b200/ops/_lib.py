@@ -99,7 +99,7 @@ SIGNATURES = {
     "sakv_gemm_wide": ("gemm_wide", [P, P, I, I, I, I, P, L, P]),
     "sakv_gemm_pair": ("gemm_pair", [P, P, I, I, I, I, P, L, I, F, F, F, P]),
     "sakv_copy_blocks": ("copy_blocks", [P, I, P, P, I, I, I, I, P]),
-    "sakv_shared_attention": ("attention_shared", [P, P, L, P, L, P, P, P, P, P, P, I, F, P]),
+    "sakv_shared_attention": ("attention_shared", [P, P, L, P, L, P, P, P, P, P, P, I, F, I, P]),
     "sakv_logprob_pieces": ("logprobs", [P, L, P, I, I, I, P, P, P, P, P, I, F, F, P, P, P]),
     "sakv_logprob_f32": ("logprobs", [P, L, P, I, I, I, P, P, P, P, I, F, F, P, P, P]),
     "sakv_logprob_split": ("logprobs", [P, L, P, I, I, I, I, P, P, P, P, P, I, F, F, P, P, P]),

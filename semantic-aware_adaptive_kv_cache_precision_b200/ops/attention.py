@@ -83,6 +83,10 @@ def attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                      in_cluster: bool | None = None) -> torch.Tensor:
     """One query token per sequence (row b of `qkv` belongs to sequence b).
 
+    Lengths, block lists, rotary tables and every cached key and value but the newest are a step's inputs: the kernel
+    reads them while the kernel before it on the stream may still be running, so that one must not have written them
+    (the one before that may, or a copy). What it has written of `qkv` and of the newest position is waited for.
+
     `rotary`: None, or `(cos, sin)` (fp32 [positions, head_dim / 2], rotation over the whole
     head): `qkv` is then the projection's output as it came, [q | k | v] unrotated, and the
     kernel rotates the queries on its way and (`write_cache`) puts the newest position's

@@ -236,11 +236,13 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
 
 def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                             seq_lens: torch.Tensor, block_table: torch.Tensor, plan: SharedPlan, heads: int,
-                            kv_heads: int, head_dim: int, scale: float) -> torch.Tensor:
+                            kv_heads: int, head_dim: int, scale: float, *, settled: bool = False) -> torch.Tensor:
     """One query token per sequence over its cached keys and values, like `attention_decode` (bfloat16,
     head sizes 64 and 128, no window; `qkv`'s rows begin with the rotated queries, the newest key and value
     are in the cache), reading a block that `plan` found in several sequences' lists once for all of them.
-    `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros."""
+    `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros. `settled`: the plan's words, the
+    lengths and the block lists were written before the kernel before this one on the stream began, as a step's
+    inputs are; they are then read while that one still runs (else the call starts when all before it is done)."""
     q_shape, k_shape, device = qkv.shape, k_cache.shape, qkv.get_device()
     # (one expression for the calls that are right: a decode step outside a captured graph is bound by the
     # host's work; `_refuse` says what is wrong with the others)
@@ -266,7 +268,8 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     part = qkv.new_empty(2 * plan.partials * heads * (head_dim + 2))          # (as many floats)
     call_on(device, "sakv_shared_attention", k_cache.data_ptr(), v_cache.data_ptr(), k_shape[0], qkv.data_ptr(),
             qkv.stride(0), seq_lens.data_ptr(), block_table.data_ptr(), plan.words.data_ptr(),
-            ctypes.addressof(plan.numbers), out.data_ptr(), part.data_ptr(), head_dim, scale)
+            ctypes.addressof(plan.numbers), out.data_ptr(), part.data_ptr(), head_dim, scale,
+            bool(settled))
     if plan.unit_capacity:
         _lib.launches += 1          # the call launched the join too
     return out

@@ -99,7 +99,7 @@ class GQAAttention(Part):
         if shared is not None:       # sequences forked from one another: common blocks are read once
             attended = ops.shared_decode_attention(qkv, view.keys, view.values, step.seq_lens,
                                                    view.block_table, shared, s.heads, s.kv_heads,
-                                                   s.head_dim, s.scale)
+                                                   s.head_dim, s.scale, settled=True)
         else:
             attended = self.attend(qkv, step, view, rotary, write_cache)
         out = ops.linear(attended, self.w_o, self.b_o, accumulate_into=residual, may_defer=defer)

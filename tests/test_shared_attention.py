@@ -264,3 +264,36 @@ def test_equal_queries_get_equal_bits_and_captured_calls_repeat():
     graph.replay()
     ops_out = call()
     assert torch.equal(held, ops_out) and torch.equal(held[1], first[1]) and not torch.equal(held[2], first[2])
+
+
+@pytest.mark.gpu
+def test_lengths_that_the_kernel_before_has_written():
+    """A call right behind a kernel that lets its successor start early and then writes the lengths reads them as that
+    one leaves them."""
+    heads, kv_heads, d = 12, 2, 128
+    tables, lengths, blocks = lists_of([(1000, [(0, 30), (0, 200), (0, 131)])])
+    k = torch.randn(blocks, kv_heads, BLOCK, d, device="cuda").to(torch.bfloat16)
+    v = torch.randn_like(k)
+    q = torch.randn(3, heads * d, device="cuda").to(torch.bfloat16)
+    plan = ops.plan_shared(tables, lengths, heads, kv_heads, device="cuda")
+    table = torch.tensor(tables, dtype=torch.int32, device="cuda")
+    call = lambda lens: ops.shared_decode_attention(q, k, v, lens, table, plan, heads, kv_heads, d, d ** -0.5)
+    want = {}
+    for n in (0, 25):
+        want[n] = call(torch.tensor(lengths - n, dtype=torch.int32, device="cuda"))
+    assert not torch.equal(want[0], want[25])
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    graphs = {}
+    for n in want:                  # (captured, so that no time passes between the two; the largest score names the length)
+        scores = torch.zeros(3, 2000000, device="cuda")
+        scores[range(3), (lengths - n).tolist()] = 1.0
+        ops.choose(scores, out=lens), call(lens)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.choose(scores, out=lens)
+            out = call(lens)
+        graphs[n] = graph, out, scores
+    for i in range(20):
+        graph, out, _ = graphs[25 * (i % 2)]
+        graph.replay()
+        assert torch.equal(out, want[25 * (i % 2)])
