@@ -59,6 +59,7 @@ struct Smem {
 struct Plan {
   const int32_t* words;
   int unit_at, member_at, first_at;    // units (8 words each), members (2 each), a sequence's first partial
+  int span_at;                         // the shortest and the longest length of a sequence that the plan covers
   int unit_capacity;
 };
 
@@ -78,10 +79,11 @@ struct Params {
 };
 
 // Words 0-1 of the plan: units, sequences. A unit's words: the sequence whose block list is read, its first
-// block, blocks, first member, first row of that member, rows, 0, 0; rows are (member, query head of the KV
-// head), heads fastest. A member: (sequence, its partial).
+// block, blocks, first member, first row of that member, rows, whether several sequences list its blocks, 0; rows are
+// (member, query head of the KV head), heads fastest. A member: (sequence, its partial). Blocks that several list are
+// filled in all of them; lengths that say otherwise are outside the plan, and the unit and the join answer NaN.
 struct Unit {
-  int sequence, column, columns, member, row, rows, pad0, pad1;
+  int sequence, column, columns, member, row, rows, shared, pad;
 };
 
 // Row r of the unit: its query, and where its partial goes.
@@ -578,10 +580,11 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   Unit u{};
   int n_tiles = 0, kv_len = 0;
   if (live) {
-    u = Unit{a.x, a.y, a.z, a.w, b.x, b.y, 0, 0};
+    u = Unit{a.x, a.y, a.z, a.w, b.x, b.y, b.z, 0};
     const int given = p.seq_lens[u.sequence];
     kv_len = given < 0 || given > p.max_blocks * KT ? 0 : given;
     n_tiles = min((kv_len + KT - 1) / KT - u.column, u.columns);
+    if (u.shared && kv_len / KT < u.column + u.columns) n_tiles = 0;
     const int members = (u.row + u.rows + group - 1) / group;
     if (threadIdx.x < members)
       member[threadIdx.x] = *reinterpret_cast<const int2*>(p.plan.words + p.plan.member_at +
@@ -620,7 +623,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   wait_for_previous_kernel();
   if (n_tiles <= 0) {            // a piece that the sequence has not reached yet: it counts for nothing
     for (int r = threadIdx.x; r < u.rows; r += kThreads)
-      p.part_ml[row_at(p, member, u, g, r, D).slot] = make_float2(-INFINITY, 0.f);
+      p.part_ml[row_at(p, member, u, g, r, D).slot] = make_float2(-INFINITY, u.shared ? NAN : 0.f);
   } else if (is_wide) {
     attend_wide<D>(p, &k_map, &v_map, smem, wide, tmem_at, listed, g, u, n_tiles, kv_len, member);
   } else if (threadIdx.x < kNarrowThreads) {
@@ -644,11 +647,13 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 template <int D>
 __global__ void __launch_bounds__(kNarrowThreads)
 join_kernel(const Plan plan, const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-            __nv_bfloat16* __restrict__ out, int heads) {
+            __nv_bfloat16* __restrict__ out, const int32_t* __restrict__ seq_lens, int heads) {
   constexpr int kLanes = D / 4, kGroups = kNarrowThreads / kLanes, kRound = 4;
   let_next_kernel_start();
   const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
   const int first = plan.words[plan.first_at + b], end = plan.words[plan.first_at + b + 1];
+  const int least = plan.words[plan.span_at + 2 * b], most = plan.words[plan.span_at + 2 * b + 1];
+  const int len = seq_lens[b];
   const int group = threadIdx.x / kLanes, c = threadIdx.x % kLanes * 4;
   wait_for_previous_kernel();
   float big = -INFINITY, total = 0.f;
@@ -704,7 +709,9 @@ join_kernel(const Plan plan, const float* __restrict__ part_o, const float2* __r
     total += w * sm_l[i];
     acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;      // no key at all: zeros
+  // (no key at all: zeros; a length that the plan does not cover: not a number, rather than a part of the answer)
+  const float inv = len <= 0 || total == 0.f ? 0.f : len < least || len > most ? NAN : 1.f / total;
+  if (len <= 0) acc = make_float4(0.f, 0.f, 0.f, 0.f);
   *reinterpret_cast<uint2*>(out + (long long)blockIdx.x * D + c) =
       make_uint2(mma::pack_bf16(acc.x * inv, acc.y * inv), mma::pack_bf16(acc.z * inv, acc.w * inv));
 }
@@ -744,17 +751,19 @@ int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_b
                           : launch_ordered(attend, units, dim3(kThreads), Smem<D>::kBytes, stream, k_map, v_map, p);
     if (e) return e;
   } else if (!settled) {
-    return launch_ordered(join, rows, dim3(kNarrowThreads), 0, stream, p.plan, p.part_o, p.part_ml, out, p.heads);
+    return launch_ordered(join, rows, dim3(kNarrowThreads), 0, stream, p.plan, p.part_o, p.part_ml, out, p.seq_lens,
+                          p.heads);
   }
-  return launch_overlapped(join, rows, dim3(kNarrowThreads), 0, stream, 1, p.plan, p.part_o, p.part_ml, out, p.heads);
+  return launch_overlapped(join, rows, dim3(kNarrowThreads), 0, stream, 1, p.plan, p.part_o, p.part_ml, out, p.seq_lens,
+                          p.heads);
 }
 
 }  // namespace
 
-// A plan's numbers (ops/shared.py): width of the block lists, words where units, members and the sequences'
-// first partials begin, units, partials that the scratch holds.
+// A plan's numbers (ops/shared.py): width of the block lists, words where units, members, the sequences' first
+// partials and the lengths covered begin, units, partials that the scratch holds.
 struct SakvSharedPlan {
-  int width, unit_at, unit_capacity, member_at, first_at, partials, sequences, heads, kv_heads;
+  int width, unit_at, unit_capacity, member_at, first_at, span_at, partials, sequences, heads, kv_heads;
 };
 
 // `keys`, `values`: the cache entry [blocks][kv_heads][64][head_dim]; `plan`: int32 words on the device, laid out as the
@@ -773,7 +782,7 @@ SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long
     return cudaErrorInvalidValue;
   if (sequences == 0) return 0;
   Params p;
-  p.plan = Plan{plan, n->unit_at, n->member_at, n->first_at, n->unit_capacity};
+  p.plan = Plan{plan, n->unit_at, n->member_at, n->first_at, n->span_at, n->unit_capacity};
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.q_stride = q_stride;
   p.q_aligned = q_stride % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   p.seq_lens = seq_lens; p.block_table = block_table; p.max_blocks = max_blocks; p.sequences = sequences;

@@ -127,15 +127,16 @@ def choose_piece(runs: list, group: int, kv_heads: int, slots: int) -> int:
 class _Numbers(ctypes.Structure):
     """A plan's numbers as the launch takes them."""
     _fields_ = [(name, ctypes.c_int) for name in ("width", "unit_at", "unit_capacity", "member_at", "first_at",
-                                                  "partials", "sequences", "heads", "kv_heads")]
+                                                  "span_at", "partials", "sequences", "heads", "kv_heads")]
 
 
 class SharedPlan:
     """Which pieces of the block lists are read for which sequences: int32 words on the device, and their
-    layout. Right for every step until `lengths` pass `reach` or the sharing changes."""
+    layout. Right for every step until lengths pass `reach` (rounded up to whole blocks), fall below what is shared,
+    or the sharing changes."""
 
     __slots__ = ("words", "sequences", "heads", "kv_heads", "units", "unit_at", "unit_capacity", "member_at",
-                 "first_at", "partials", "reach", "width", "saved", "numbers")
+                 "first_at", "span_at", "partials", "reach", "width", "saved", "numbers")
 
     @property
     def layout(self) -> tuple:
@@ -209,11 +210,16 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     of, i = _spread(-(-rows // UNIT_ROWS))
     r = i * UNIT_ROWS
     some = np.minimum(UNIT_ROWS, rows[of] - r)
-    nothing = np.zeros_like(of)
+    several = counted > 1
     units = np.stack([listing[listed_at[run[of]]], begins[of], columns[of], pairs_at[of] + r // group, r % group,
-                      some, nothing, nothing], axis=1)
+                      some, several[run[of]], np.zeros_like(of)], axis=1)
     start, slope = _unit_us(some)
     units = units[np.argsort(-(start + slope * columns[of]), kind="stable")]
+    # the lengths that this holds for: what a sequence shares is filled, and its columns go no further
+    spans = np.zeros((count, 2), dtype=np.int64)
+    spans[:, 1] = -(-reach // CACHE_BLOCK) * CACHE_BLOCK
+    shared = several[np.repeat(np.arange(len(counted)), counted)]
+    np.maximum.at(spans[:, 0], listing[shared], np.repeat(ends[:, 1] * CACHE_BLOCK, counted)[shared])
     plan = SharedPlan()
     plan.sequences, plan.heads, plan.kv_heads, plan.width = count, heads, kv_heads, width
     plan.units, plan.reach = len(units), reach
@@ -224,12 +230,14 @@ def plan_shared(tables, lengths, heads: int, kv_heads: int, device=None, *, reac
     plan.member_at = plan.unit_at + UNIT_WORDS * plan.unit_capacity
     plan.first_at = plan.member_at + 2 * members_room
     plan.saved = int(((counted - 1) * sizes).sum())
-    words = np.zeros(_round_up(plan.first_at + count + 1, 4), dtype=np.int32)
+    plan.span_at = plan.first_at + count + 1
+    words = np.zeros(_round_up(plan.span_at + 2 * count, 4), dtype=np.int32)
     plan.numbers = _Numbers(*(getattr(plan, name) for name, _ in _Numbers._fields_))
     words[0], words[1] = len(units), count
     words[8:8 + UNIT_WORDS * len(units)] = units.reshape(-1)
     words[plan.member_at:plan.member_at + 2 * len(pairs)] = pairs.reshape(-1)
     words[plan.first_at:plan.first_at + count + 1] = first
+    words[plan.span_at:plan.span_at + 2 * count] = spans.reshape(-1)
     plan.words = words if device is None else torch.from_numpy(words).to(device)
     return plan
 
@@ -240,7 +248,9 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     """One query token per sequence over its cached keys and values, like `attention_decode` (bfloat16,
     head sizes 64 and 128, no window; `qkv`'s rows begin with the rotated queries, the newest key and value
     are in the cache), reading a block that `plan` found in several sequences' lists once for all of them.
-    `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros. `settled`: the plan's words, the
+    `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros; one whose length the plan does not
+    cover (past its reach, or below the blocks it shares) gets NaN, and so do those that the plan lets read those
+    blocks through its list. `settled`: the plan's words, the
     lengths and the block lists were written before the kernel before this one on the stream began, as a step's
     inputs are; they are then read while that one still runs (else the call starts when all before it is done)."""
     q_shape, k_shape, device = qkv.shape, k_cache.shape, qkv.get_device()

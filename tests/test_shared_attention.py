@@ -297,3 +297,57 @@ def test_lengths_that_the_kernel_before_has_written():
         graph, out, _ = graphs[25 * (i % 2)]
         graph.replay()
         assert torch.equal(out, want[25 * (i % 2)])
+
+
+def test_a_plan_says_which_lengths_it_is_right_for():
+    tables, lengths, _ = lists_of(CASES["tree"] + CASES["empty"])
+    reach = np.minimum(lengths + 70, tables.shape[1] * BLOCK)
+    plan = ops.plan_shared(tables, lengths, 4, 2, slots=20, reach=reach)
+    spans = plan.words[plan.span_at:plan.span_at + 2 * len(lengths)].reshape(-1, 2)
+    assert (spans[:, 1] == -(-reach // BLOCK) * BLOCK).all()
+    for b, row in enumerate(tables):         # the last filled block that another list has in the same place
+        shared = [c + 1 for c in range(lengths[b] // BLOCK)
+                  if any(o != b and lengths[o] // BLOCK > c and tables[o, c] == row[c] for o in range(len(tables)))]
+        assert spans[b, 0] == BLOCK * max(shared, default=0) <= lengths[b]
+    assert plan.span_at + 2 * len(lengths) <= len(plan.words)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads, d", [(12, 2, 128), (8, 8, 64)])
+@pytest.mark.parametrize("forks", [4, 30])
+def test_lengths_that_the_plan_does_not_cover(heads, kv_heads, d, forks):
+    """No part of an answer: NaN, in the sequence itself and where another's list is read for it; zeros for a
+    sequence of no length; all others as they were."""
+    tables, lengths, blocks = lists_of([(640, [(0, 30 + i) for i in range(forks)]), (0, [(0, 100)])])
+    k = torch.randn(blocks, kv_heads, BLOCK, d, device="cuda").to(torch.bfloat16)
+    v = torch.randn_like(k)
+    b = len(lengths)
+    q = torch.randn(b, heads * d, device="cuda").to(torch.bfloat16)
+    plan = ops.plan_shared(tables, lengths, heads, kv_heads, device="cuda", slots=12)
+    table = torch.tensor(tables, dtype=torch.int32, device="cuda")
+
+    def call(changed):
+        n = lengths.copy()
+        for i, to in changed.items():
+            n[i] = to
+        return ops.shared_decode_attention(q, k, v, torch.tensor(n, dtype=torch.int32, device="cuda"), table, plan,
+                                           heads, kv_heads, d, d ** -0.5)
+
+    want = call({})
+    assert torch.isfinite(want).all()
+    last, alone = forks - 1, forks               # one whose list is read for nobody else, and one that shares nothing
+    for length, nan in ((704, False), (640, False), (639, True), (1, True), (705, True), (tables.shape[1] * BLOCK, True),
+                        (10 ** 9, True)):
+        out = call({last: length})
+        assert out[last].isnan().all() if nan else torch.isfinite(out[last]).all()
+        rest = [i for i in range(b) if i != last]
+        assert torch.equal(out[rest], want[rest])
+    for length, nan in ((1, False), (128, False), (129, True)):
+        out = call({alone: length})
+        assert out[alone].isnan().all() if nan else torch.isfinite(out[alone]).all()
+        assert torch.equal(out[:alone], want[:alone])
+    for length in (0, -5):
+        out = call({last: length, alone: length})
+        assert not out[last].any() and not out[alone].any() and torch.equal(out[:last], want[:last])
+    first = call({0: 0})                         # the list that is read for all
+    assert not first[0].any() and first[1:alone].isnan().all() and torch.equal(first[alone], want[alone])
