@@ -43,6 +43,8 @@ constexpr int kMembers = kWideRows + 2;
 constexpr uint32_t kTmemCols = 256;  // wide: S 2 x 64 (P over the first 32 of each), O from 128 on
 constexpr uint32_t kOCol = 128;
 constexpr float kLazy = 8.f;         // O is rescaled when a row's maximum has grown by 2^8
+// A wide unit takes maxima before it scales them, and scales -inf: right for scales above 0 alone.
+constexpr float kLeastScale = 1e-30f;
 
 template <int D>
 struct Smem {
@@ -775,10 +777,11 @@ SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long
                                       int settled, cudaStream_t stream) {
   const int sequences = n->sequences, heads = n->heads, kv_heads = n->kv_heads, max_blocks = n->width;
   if (sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kMostGroup ||
-      max_blocks <= 0 || max_blocks > (1 << 24) || n->unit_capacity < 0 || n->partials < 0 || (q_stride & 1) ||
+      max_blocks < 0 || max_blocks > (1 << 24) || n->unit_capacity < 0 || n->partials < 0 || (q_stride & 1) ||
       (n->unit_at & 7) || (n->member_at & 1) || (reinterpret_cast<uintptr_t>(q) & 3) ||
       (reinterpret_cast<uintptr_t>(plan) & 15) || (reinterpret_cast<uintptr_t>(part) & 15) ||
-      (long long)n->unit_capacity * kv_heads > 0x7fffffffLL || (long long)sequences * heads > 0x7fffffffLL)
+      (long long)n->unit_capacity * kv_heads > 0x7fffffffLL || (long long)sequences * heads > 0x7fffffffLL ||
+      !(scale >= kLeastScale && scale <= 1.f / kLeastScale))
     return cudaErrorInvalidValue;
   if (sequences == 0) return 0;
   Params p;

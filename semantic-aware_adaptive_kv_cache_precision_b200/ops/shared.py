@@ -16,6 +16,7 @@ from .attention import fast_path_takes
 
 UNIT_ROWS = 128           # most rows (sequences x query heads of one KV head) of a unit of work
 MOST_GROUP = 64           # most query heads of one KV head
+LEAST_SCALE = 1e-30       # scales from here to its reciprocal
 UNIT_WORDS = 8
 
 
@@ -144,7 +145,11 @@ class SharedPlan:
         return (self.sequences, self.width, self.unit_capacity, self.member_at, self.first_at, self.partials)
 
     def on(self, words: torch.Tensor) -> "SharedPlan":
-        """The same plan with its words at `words` (int32, on the device)."""
+        """The same plan with its words at `words` (contiguous int32, on the device, at a multiple of 16 bytes)."""
+        if words.dtype != torch.int32 or words.dim() != 1 or not words.is_contiguous() \
+                or words.shape[0] < self.span_at + 2 * self.sequences or words.data_ptr() % 16:
+            raise KernelError(f"SharedPlan: words must be contiguous int32 [{self.span_at + 2 * self.sequences} or more] "
+                              f"at a multiple of 16 bytes, got {tuple(words.shape)} {words.dtype}")
         other = SharedPlan()
         for name in SharedPlan.__slots__:
             setattr(other, name, getattr(self, name))
@@ -257,8 +262,8 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     # (one expression for the calls that are right: a decode step outside a captured graph is bound by the
     # host's work; `_refuse` says what is wrong with the others)
     if not (qkv.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
-            and (head_dim == 128 or head_dim == 64) and heads % kv_heads == 0
-            and heads <= 16 * kv_heads and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
+            and (head_dim == 128 or head_dim == 64) and 0 < kv_heads and heads % kv_heads == 0
+            and heads <= 16 * kv_heads and LEAST_SCALE <= scale <= 1 / LEAST_SCALE and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
             and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
             and k_shape == v_cache.shape and len(k_shape) == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() and k_shape[1] == kv_heads
             and k_shape[2] == CACHE_BLOCK and k_shape[3] == head_dim
@@ -267,9 +272,9 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
             and seq_lens.shape[0] == q_shape[0] and block_table.shape[0] == q_shape[0]
             and block_table.shape[1] == plan.width and seq_lens.is_contiguous() and block_table.is_contiguous()
             and plan.sequences == q_shape[0] and plan.heads == heads and plan.kv_heads == kv_heads
-            and device >= 0 and device == k_cache.get_device() == v_cache.get_device() == seq_lens.get_device()
+            and plan.words.__class__ is torch.Tensor and device >= 0 and device == k_cache.get_device() == v_cache.get_device() == seq_lens.get_device()
             == block_table.get_device() == plan.words.get_device()):
-        _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim)
+        _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim, scale)
     sequences = q_shape[0]
     width = heads * head_dim
     out = torch.empty_like(qkv) if q_shape[1] == width and qkv.is_contiguous() else qkv.new_empty((sequences, width))
@@ -285,9 +290,9 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     return out
 
 
-def _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim) -> None:
+def _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim, scale) -> None:
     """Says what is wrong with a call of `shared_decode_attention`."""
-    if not fast_path_takes(qkv.dtype, heads, kv_heads, head_dim):
+    if kv_heads <= 0 or not fast_path_takes(qkv.dtype, heads, kv_heads, head_dim):
         raise KernelError("shared_decode_attention: sizes not taken; use the plain kernel")
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < heads * head_dim or qkv.stride(0) % 2 \
             or qkv.data_ptr() % 4:
@@ -304,5 +309,10 @@ def _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads,
     if (plan.sequences, plan.heads, plan.kv_heads) != (sequences, heads, kv_heads):
         raise KernelError(f"shared_decode_attention: the plan is for {plan.sequences} sequences, {plan.heads} heads "
                           f"over {plan.kv_heads}")
+    if not LEAST_SCALE <= scale <= 1 / LEAST_SCALE:
+        raise KernelError(f"shared_decode_attention: scale must be a number from {LEAST_SCALE} to {1 / LEAST_SCALE}, "
+                          f"got {scale}")
+    if not isinstance(plan.words, torch.Tensor):
+        raise KernelError("shared_decode_attention: the plan's words are on the host; `plan.on` takes them to the device")
     require_cuda(qkv, k_cache, v_cache, seq_lens, block_table, plan.words)
     raise KernelError("shared_decode_attention: tensors on different devices")

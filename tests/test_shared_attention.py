@@ -351,3 +351,43 @@ def test_lengths_that_the_plan_does_not_cover(heads, kv_heads, d, forks):
         assert not out[last].any() and not out[alone].any() and torch.equal(out[:last], want[:last])
     first = call({0: 0})                         # the list that is read for all
     assert not first[0].any() and first[1:alone].isnan().all() and torch.equal(first[alone], want[alone])
+
+
+def test_refusals_of_scales_and_of_plans_that_are_not_there():
+    tables, lengths, _ = lists_of(CASES["forks"])
+    host = ops.plan_shared(tables, lengths, 12, 2, slots=8)
+    plan = host.on(torch.from_numpy(host.words))
+    for words in (host.words[:-8], host.words.astype(np.int64), np.repeat(host.words, 2)[::2], host.words[None],
+                  np.concatenate([[0], host.words]).astype(np.int32)[1:]):
+        with pytest.raises(KernelError, match="words must be"):
+            host.on(torch.from_numpy(words))
+    b, width = tables.shape
+    good = dict(qkv=torch.zeros(b, 12 * 64, dtype=torch.bfloat16), k_cache=torch.zeros(99, 2, 64, 64, dtype=torch.bfloat16),
+                v_cache=torch.zeros(99, 2, 64, 64, dtype=torch.bfloat16),
+                seq_lens=torch.zeros(b, dtype=torch.int32), block_table=torch.zeros(b, width, dtype=torch.int32),
+                plan=plan, heads=12, kv_heads=2, head_dim=64, scale=1.0)
+    for scale in (0.0, -0.5, math.nan, math.inf, 1e39, 1e-60):
+        with pytest.raises(KernelError, match="scale must be"):
+            ops.shared_decode_attention(**{**good, "scale": scale})
+    with pytest.raises(KernelError, match="on the host"):
+        ops.shared_decode_attention(**{**good, "plan": host})
+    for kv_heads in (0, -2):
+        with pytest.raises(KernelError):
+            ops.shared_decode_attention(**{**good, "kv_heads": kv_heads})
+    with pytest.raises(KernelError, match="CUDA device only"):
+        ops.shared_decode_attention(**good)
+
+
+def test_a_plan_of_lists_without_columns():
+    plan = ops.plan_shared(np.zeros((3, 0), int), [0, 0, 0], 4, 2, slots=8, roomy=True)
+    assert plan.units == plan.unit_capacity == 0 and plan.width == 0
+
+
+@pytest.mark.gpu
+def test_lists_without_columns():
+    plan = ops.plan_shared(np.zeros((3, 0), int), [0, 0, 0], 4, 2, device="cuda")
+    k = torch.full((2, 2, BLOCK, 64), math.nan, device="cuda", dtype=torch.bfloat16)
+    out = ops.shared_decode_attention(torch.ones(3, 256, device="cuda", dtype=torch.bfloat16), k, k,
+                                      torch.zeros(3, dtype=torch.int32, device="cuda"),
+                                      torch.zeros(3, 0, dtype=torch.int32, device="cuda"), plan, 4, 2, 64, 0.125)
+    assert out.shape == (3, 256) and not out.any()
