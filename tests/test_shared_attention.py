@@ -391,3 +391,44 @@ def test_lists_without_columns():
                                       torch.zeros(3, dtype=torch.int32, device="cuda"),
                                       torch.zeros(3, 0, dtype=torch.int32, device="cuda"), plan, 4, 2, 64, 0.125)
     assert out.shape == (3, 256) and not out.any()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_and_graphs_at_once():
+    """Calls side by side, and two captured calls replayed side by side, share nothing."""
+    sides = []
+    for heads, kv_heads, d, forks in ((12, 2, 128, 9), (8, 4, 64, 40)):
+        tables, lengths, blocks = lists_of([(3000, [(0, 5 + 11 * i) for i in range(forks)])])
+        k = torch.randn(blocks, kv_heads, BLOCK, d, device="cuda").to(torch.bfloat16)
+        v = torch.randn_like(k)
+        q = torch.randn(forks, heads * d, device="cuda").to(torch.bfloat16)
+        plan = ops.plan_shared(tables, lengths, heads, kv_heads, device="cuda")
+        args = (q, k, v, torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                torch.tensor(tables, dtype=torch.int32, device="cuda"), plan, heads, kv_heads, d, d ** -0.5)
+        sides.append((args, torch.cuda.Stream()))
+    alone = [ops.shared_decode_attention(*args) for args, _ in sides]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for turn in range(10):
+        for i, (args, stream) in enumerate(sides):
+            with torch.cuda.stream(stream):
+                got[i].append(ops.shared_decode_attention(*args, settled=turn % 2 == 1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, many in zip(alone, got) for b in many)
+    graphs = []
+    for args, _ in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = [ops.shared_decode_attention(*args, settled=s) for s in (False, True, True)]
+        graphs.append((graph, held))
+    for args, _ in sides:
+        args[0].copy_(args[0].flip(0))
+    fresh = [ops.shared_decode_attention(*args) for args, _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (graph, _), (_, stream) in zip(graphs, sides):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(h, want) for (_, held), want in zip(graphs, fresh) for h in held)
+    assert not torch.equal(fresh[0], alone[0])
