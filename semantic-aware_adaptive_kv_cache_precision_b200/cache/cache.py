@@ -256,18 +256,14 @@ class SequenceCache:
 
     # -- another size ---------------------------------------------------------
 
-    def resize(self, max_tokens: int, max_slots: int | None = None) -> None:
-        """Give every pool room for `max_tokens` positions (rounded up to blocks) while sequences live:
-        held blocks are moved into new storage, one behind the other in the order of their numbers, and the
-        old storage is given up. `max_slots`: as many slots at least (they never become fewer). All or
-        nothing: `CacheFull` where the held blocks, or a sequence's length, do not fit; `OutOfDeviceMemory`
-        where the device has no room for old and new storage together."""
+    def sizes_for(self, max_tokens: int) -> tuple:
+        """(blocks of every pool, longest sequence) of a cache of `max_tokens` positions; `CacheFull` where what is
+        held now would not fit it."""
         if max_tokens <= 0:
             raise ValueError(f"max_tokens must be positive, got {max_tokens}")
         blocks = -(-max_tokens // BLOCK)
         longest = min(self.max_positions, blocks * BLOCK)
         width = -(-longest // BLOCK)
-        slots = max(self.max_slots, max_slots or 0)
         for group in self.groups:
             if group.pool.held > blocks:
                 raise CacheFull(f"{group.pool.held} cache blocks are held, {blocks} would not hold them; "
@@ -276,6 +272,17 @@ class SequenceCache:
             if self.lengths[s] > longest or any((group.tables[s, width:] >= 0).any() for group in self.groups):
                 raise CacheFull(f"a sequence of {int(self.lengths[s])} positions does not fit a cache of "
                                 f"{longest} per sequence; nothing was changed")
+        return blocks, longest
+
+    def resize(self, max_tokens: int, max_slots: int | None = None) -> None:
+        """Give every pool room for `max_tokens` positions (rounded up to blocks) while sequences live:
+        held blocks are moved into new storage, one behind the other in the order of their numbers, and the
+        old storage is given up. `max_slots`: as many slots at least (they never become fewer). All or
+        nothing: `CacheFull` where the held blocks, or a sequence's length, do not fit; `OutOfDeviceMemory`
+        where the device has no room for old and new storage together."""
+        blocks, longest = self.sizes_for(max_tokens)
+        width = -(-longest // BLOCK)
+        slots = max(self.max_slots, max_slots or 0)
         storage = [group.storage(blocks) for group in self.groups]
         states = self.states if slots == self.max_slots else {
             key: allocate(lambda: torch.zeros((slots,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device),

@@ -20,6 +20,7 @@ from .. import ops, sampling
 from ..ops import _lib
 from ..cache import BLOCK, CacheFull, SequenceCache
 from ..config import config_from_dict, config_from_folder
+from ..errors import OutOfDeviceMemory
 from .generate import (decode_ahead, COMPLETE, DECODING, EXHAUSTED, PREFILLING, Ending, RequestState,
                        check_prompt, check_window, plan_batches, plan_prefill, plan_samples, positions_needed,
                        stop_ids_of_folder)
@@ -228,12 +229,18 @@ class Engine:
         if max_tokens <= 0:
             raise ValueError(f"max_tokens must be positive, got {max_tokens}")
         if self.cache is not None:
-            old = [t for group in self.cache.groups for t in group.tensors]
+            _, longest = self.cache.sizes_for(max_tokens)
             with torch.cuda.device(self.device):
-                self.cache.resize(max_tokens, _slots_for(max_tokens))
+                # what can fail comes before what changes: tables of positions that reach further serve the cache as
+                # it is too, but steps captured over those that they replace must not run again
                 self._forget_storage()
-                ops.forget_descriptors(*old)
-                self.model.prepare(self.cache.max_seq_len)
+                longest = max(longest, self.cache.max_seq_len)
+                try:
+                    self.model.prepare(longest)
+                except torch.OutOfMemoryError as exc:
+                    raise OutOfDeviceMemory(f"the device has no room for the tables of {longest} positions; "
+                                            "the cache is as it was") from exc
+                self.cache.resize(max_tokens, _slots_for(max_tokens))
         self.max_tokens = int(max_tokens)
 
     def _shared_plans(self, slots, ends, cache) -> dict:

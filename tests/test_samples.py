@@ -400,3 +400,41 @@ def test_captured_steps_go_with_the_plans_they_read(monkeypatch):
         assert len(e._shared_buffers) <= 64
         held = {b.data_ptr() for b in e._shared_buffers.values()}
         assert all(set(x) <= held for table in (e._graphs, e._prefill_graphs) for x in table.values())
+
+
+def test_a_size_whose_tables_find_no_room_changes_nothing(monkeypatch):
+    """The tables of positions are made before the cache changes, and never for fewer positions than it takes."""
+    import contextlib
+    from semantic_aware_adaptive_kv_cache_precision_b200.cache import KVNeed, SequenceCache
+    from semantic_aware_adaptive_kv_cache_precision_b200.errors import OutOfDeviceMemory
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    cache = SequenceCache([KVNeed(1, 64)], 8 * BLOCK, 64 * BLOCK, torch.bfloat16, "cpu")
+    e = engine_without_a_gpu(monkeypatch, cache, [])
+    e.cache, e.max_tokens, asked = cache, 8 * BLOCK, []
+
+    def prepare(n):
+        asked.append(n)
+        if n > 30 * BLOCK:
+            raise torch.OutOfMemoryError("no room")
+
+    e.model.prepare = prepare
+    (a,) = cache.open(1)
+    cache.reserve([a], [100])
+    cache.advance([a], [100])
+    keys, table = cache.groups[0].keys, cache.groups[0].tables.copy()
+    e._graphs["step"] = e._prefill_graphs["step"] = object()
+    with pytest.raises(OutOfDeviceMemory):
+        e.resize_cache(40 * BLOCK)
+    cache.check()
+    assert cache.max_seq_len == e.max_tokens == 8 * BLOCK and cache.groups[0].keys is keys
+    assert (cache.groups[0].tables == table).all()
+    assert not e._graphs and not e._prefill_graphs         # (tables of some layers may be new ones)
+    e._graphs["step"] = object()
+    with pytest.raises(CacheFull):
+        e.resize_cache(BLOCK)                              # refused before anything is made or dropped
+    assert asked == [40 * BLOCK] and e._graphs and e.max_tokens == 8 * BLOCK
+    e.resize_cache(20 * BLOCK)
+    assert cache.max_seq_len == e.max_tokens == 20 * BLOCK and not e._graphs
+    e.resize_cache(4 * BLOCK)
+    assert cache.max_seq_len == 4 * BLOCK and asked[1:] == [20 * BLOCK, 20 * BLOCK]
+    cache.check()
