@@ -33,8 +33,8 @@ class RotaryHalf(Part):
             return
         inv_freq, magnitude = self.frequencies()
         angle = np.arange(n, dtype=np.float64)[:, None] * inv_freq[None, :]
-        self.cos = torch.from_numpy((np.cos(angle) * magnitude).astype(np.float32)).to(device)
-        self.sin = torch.from_numpy((np.sin(angle) * magnitude).astype(np.float32)).to(device)
+        cos, sin = (torch.from_numpy((f(angle) * magnitude).astype(np.float32)).to(device) for f in (np.cos, np.sin))
+        self.cos, self.sin = cos, sin          # (both or, where the device has no room for one, neither)
 
     def frequencies(self):
         """(float64 [rotary_dim / 2], magnitude): pair i turns by `position * f_i`, f_i =

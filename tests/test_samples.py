@@ -438,3 +438,25 @@ def test_a_size_whose_tables_find_no_room_changes_nothing(monkeypatch):
     e.resize_cache(4 * BLOCK)
     assert cache.max_seq_len == 4 * BLOCK and asked[1:] == [20 * BLOCK, 20 * BLOCK]
     cache.check()
+
+
+def test_rotary_tables_are_made_both_or_neither(monkeypatch):
+    from types import SimpleNamespace
+    from semantic_aware_adaptive_kv_cache_precision_b200.parts.rotary import RotaryHalf
+    part = RotaryHalf(SimpleNamespace(rotary_dim=8, head_dim=8, max_positions=100, theta=1e4, scaling=None), "", None)
+    part.prepare("cpu", 10)
+    moved, to = [], torch.Tensor.to
+
+    def full(t, *args, **how):
+        moved.append(t)
+        if len(moved) == 2:
+            raise torch.OutOfMemoryError("no room")
+        return to(t, *args, **how)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "to", full)
+        with pytest.raises(torch.OutOfMemoryError):
+            part.prepare("cpu", 50)
+    assert part.cos.shape == part.sin.shape == (10, 4)
+    part.prepare("cpu", 50)
+    assert part.cos.shape == part.sin.shape == (50, 4)
