@@ -15,7 +15,7 @@ from .linear import linear
 PIECE_ELEMENTS = 8 << 20
 #: numbers of x that are split at one time in 32 bits (six bytes each: 384 MB)
 SPLIT_ELEMENTS = 64 << 20
-#: (maximum, sum) pairs of tiles that they leave at one time (512 MB)
+#: (maximum, sum) pairs that rows leave at one time, one a tile of the head (512 MB)
 SPLIT_PAIRS = 64 << 20
 
 
@@ -134,6 +134,10 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
     bias_at, bias_code = (None, F32) if bias is None else (bias.data_ptr(), dtype_code(bias.dtype))
     if x.dtype is torch.bfloat16 and k % 8 == 0 and stride % 8 == 0 and (at | head_at) % 16 == 0 and _pairs() > 0:
         shape, floats = _shape(rows, vocab, k)
+        if floats > 2 * SPLIT_PAIRS and rows > 256:
+            # (whole tiles of 256 rows; the heads' tiles of fewer rows may be lower ones, so a piece is looked at again)
+            return _in_pieces(x, head, targets, bias, scale, softcap,
+                              max(256, min(rows - 1, rows * 2 * SPLIT_PAIRS // floats) // 256 * 256))
         part = x.new_empty(floats + rows, dtype=torch.float32)
         scratch = part.data_ptr()
         call("sakv_logprob_pieces", at, stride, head_at, rows, vocab, k, shape, targets.data_ptr(), scratch,
@@ -152,7 +156,11 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
              scratch + 4 * floats, scratch, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
         _lib.launches += 2          # the call launched the split of x and the join too
     elif x.dtype is torch.float32:
-        floats = 2 * rows * -(-vocab // plain_function("sakv_logprob_f32_columns")())
+        pieces = -(-vocab // plain_function("sakv_logprob_f32_columns")())
+        most = max(1, SPLIT_PAIRS // pieces)
+        if rows > most:
+            return _in_pieces(x, head, targets, bias, scale, softcap, most)
+        floats = 2 * rows * pieces
         part = x.new_empty(floats + rows, dtype=torch.float32)
         scratch = part.data_ptr()
         call("sakv_logprob_f32", at, stride, head_at, rows, vocab, k, targets.data_ptr(), scratch,

@@ -312,3 +312,26 @@ def test_two_streams_and_graphs_at_once(dtype, k):
     torch.cuda.synchronize()
     assert all(torch.equal(held, want) for (_, held), want in zip(graphs, fresh))
     assert not torch.equal(fresh[0], alone[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, k, most", [(torch.bfloat16, 136, 256), (torch.bfloat16, 136, 512), (torch.float32, 131, 29),
+                                            (torch.float32, 132, 29)])
+def test_scratch_has_a_bound(monkeypatch, dtype, k, most):
+    """Many rows are taken some at a time, so that what tiles leave stays below a bound, whichever way they go."""
+    x, w, targets, got, lse = check(1301, k, 3001, dtype, seed=8)
+    launches = []
+    real = logprobs.call
+    monkeypatch.setattr(logprobs, "call", lambda name, *args: (launches.append((name, args[3])), real(name, *args)))
+    ops.token_logprobs(x, w, targets)
+    assert len(launches) == 1
+    # (tiles of the head: 16 of 192 rows, 24 of 128, 29 of 104)
+    monkeypatch.setattr(logprobs, "SPLIT_PAIRS", most * (16 if dtype == torch.bfloat16 else 24 if k % 4 else 29))
+    del launches[:]
+    again, lse2 = ops.token_logprobs(x, w, targets)
+    assert len(launches) >= 1301 // most and all(rows <= most for _, rows in launches), launches
+    assert sum(rows for _, rows in launches) == 1301
+    want, want_lse, bound = reference(x, w, targets, None, 1.0, 0.0)
+    assert ((again.double() - want).abs() <= bound).all() and ((lse2.double() - want_lse).abs() <= bound).all()
+    if dtype == torch.float32:
+        assert torch.equal(again, got) and torch.equal(lse, lse2)
