@@ -1301,19 +1301,22 @@ SAKV_EXPORT int sakv_logprob_resident() { return resident_pairs(); }
 // the height is a multiple of 16 (the products' width, two blocks' rows, is one of 32), and a round of tiles costs
 // what its operands' rows take from L2.
 SAKV_EXPORT int sakv_logprob_shape(int M, int N, int K, int pairs, int* shape) {
-  if (M <= 0 || N <= 0 || K <= 0 || pairs <= 0 || N > 0x7fffffff - 512 || M > 0x7fffffff - 512) return cudaErrorInvalidValue;
+  // (row numbers of tiles that reach past the head are 32-bit numbers)
+  if (M <= 0 || N <= 0 || K <= 0 || pairs <= 0 || pairs > (1 << 16) || N > 0x7fffffff - 4 * BM * pairs ||
+      M > 0x7fffffff - 512)
+    return cudaErrorInvalidValue;
   const int most = M > kMaxTokens && M < 2 * kMaxTokens && K <= kLongK ? kBothMost : kRestMost;
   const int full = M / kMaxTokens + (M % kMaxTokens > most ? 1 : 0);
   const int per = both_of(M, K, full) ? 1 : full + (M > full * kMaxTokens);
   int rows = BM;
   if (full == 0) {
-    const int rounds = (N + 2 * BM * pairs - 1) / (2 * BM * pairs);
-    rows = (N + 2 * pairs * rounds - 1) / (2 * pairs * rounds);
+    const long long rounds = (N + 2LL * BM * pairs - 1) / (2 * BM * pairs);
+    rows = (int)((N + 2 * pairs * rounds - 1) / (2 * pairs * rounds));
   } else {
     const int beside = both_of(M, K, full) ? (M - kMaxTokens + 31) / 32 * 16 : 0;
     long long best = -1;
     for (int r = BM; r >= 96; r -= 16) {
-      const long long tiles = (N + 2 * r - 1) / (2 * r) * (long long)per;
+      const long long tiles = (N + 2LL * r - 1) / (2 * r) * per;
       const long long cost = (tiles + pairs - 1) / pairs * (r + BM + beside);
       if (best < 0 || cost < best) {
         best = cost;
@@ -1384,7 +1387,7 @@ SAKV_EXPORT int sakv_logprob_split(const float* x, long long x_stride, const flo
   if ((long long)p.m_tiles * p.n_tiles > 0x3fffffffLL) return cudaErrorInvalidValue;
   // what is left of shared memory beside up to four steps of the tokens is the head's
   const int x_bytes = 3 * p.cols * BK * 2, room = kSmemMost - 1024 - (int)sizeof(SplitTail);
-  p.x_stages = p.cols <= 32 ? 4 : p.cols <= 96 ? 3 : 2;
+  p.x_stages = p.cols <= 32 ? 4 : 3;
   p.raw_stages = (room - p.x_stages * x_bytes) / kSplitRaw;
   if (p.raw_stages > kSplitRawMost) p.raw_stages = kSplitRawMost;
   p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;

@@ -335,3 +335,18 @@ def test_scratch_has_a_bound(monkeypatch, dtype, k, most):
     assert ((again.double() - want).abs() <= bound).all() and ((lse2.double() - want_lse).abs() <= bound).all()
     if dtype == torch.float32:
         assert torch.equal(again, got) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_tiles_of_heads_as_long_as_numbers_go(rows):
+    """Host code of the launcher: right up to where row numbers would leave 32 bits, refused from there on."""
+    import ctypes
+    from semantic_aware_adaptive_kv_cache_precision_b200.ops._lib import plain_function
+    shape = (ctypes.c_int * 4)()
+    for pairs in (1, 74, 1000):
+        most = 2 ** 31 - 1 - 512 * pairs
+        assert plain_function("sakv_logprob_shape")(rows, most, 64, pairs, shape) == 0
+        full, height, tiles, launched = shape
+        assert 1 <= height <= 128 and launched == pairs and (tiles - 1) * 2 * height < most <= tiles * 2 * height
+        assert plain_function("sakv_logprob_shape")(rows, most + 1, 64, pairs, shape) != 0
+    assert plain_function("sakv_logprob_shape")(rows, 1000, 64, 2 ** 20, shape) != 0
