@@ -17,6 +17,8 @@ PIECE_ELEMENTS = 8 << 20
 SPLIT_ELEMENTS = 64 << 20
 #: (maximum, sum) pairs that rows leave at one time, one a tile of the head (512 MB)
 SPLIT_PAIRS = 64 << 20
+#: the largest scale and cap: they and a cap's reciprocal stay 32-bit numbers, also times log2(e)
+MOST_SHAPE = 1e30
 
 
 _resident: dict = {}
@@ -45,19 +47,19 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
             and 0 < x.shape[1] == head.shape[1] and head.shape[0] > 0
             and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1)
             and targets.dtype is torch.int32 and targets.shape[0] == x.shape[0] and targets.is_contiguous()
-            and 0.0 <= softcap < float("inf")
+            and (softcap == 0.0 or 1 / MOST_SHAPE <= softcap <= MOST_SHAPE) and -MOST_SHAPE <= scale <= MOST_SHAPE
             and device >= 0 and head.get_device() == device and targets.get_device() == device
             and (bias is None or bias.dim() == 1 and bias.shape[0] == head.shape[0] and bias.is_contiguous()
                  and bias.get_device() == device
                  and (bias.dtype is torch.float32 or bias.dtype is torch.bfloat16))):
-        x = _refuse(x, head, targets, bias, softcap)
+        x = _refuse(x, head, targets, bias, scale, softcap)
     if device != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _token_logprobs(x, head, targets, bias, scale, softcap)
     return _token_logprobs(x, head, targets, bias, scale, softcap)
 
 
-def _refuse(x, head, targets, bias, softcap) -> torch.Tensor:
+def _refuse(x, head, targets, bias, scale, softcap) -> torch.Tensor:
     """Says what is wrong with a call of `token_logprobs`, or gives x with strides that mean something (of one
     row, or one number a row, torch's may be any)."""
     if x.dim() != 2 or head.dim() != 2 or x.shape[1] != head.shape[1] or x.dtype != head.dtype \
@@ -74,8 +76,9 @@ def _refuse(x, head, targets, bias, softcap) -> torch.Tensor:
         raise KernelError(f"token_logprobs: bias must be contiguous [{vocab}]")
     if bias is not None:
         dtype_code(bias.dtype)
-    if not softcap >= 0.0 or softcap == float("inf"):
-        raise KernelError(f"token_logprobs: softcap must be a number >= 0, got {softcap}")
+    if not (softcap == 0.0 or 1 / MOST_SHAPE <= softcap <= MOST_SHAPE) or not -MOST_SHAPE <= scale <= MOST_SHAPE:
+        raise KernelError(f"token_logprobs: softcap must be 0 or a number from {1 / MOST_SHAPE} to {MOST_SHAPE}, scale one "
+                          f"of at most {MOST_SHAPE}, got {softcap} and {scale}")
     if any(t is not None and t.device != x.device for t in (head, targets, bias)):
         raise KernelError("token_logprobs: tensors on different devices")
     require_cuda(x, head, targets, bias)

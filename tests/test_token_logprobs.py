@@ -350,3 +350,29 @@ def test_tiles_of_heads_as_long_as_numbers_go(rows):
         assert 1 <= height <= 128 and launched == pairs and (tiles - 1) * 2 * height < most <= tiles * 2 * height
         assert plain_function("sakv_logprob_shape")(rows, most + 1, 64, pairs, shape) != 0
     assert plain_function("sakv_logprob_shape")(rows, 1000, 64, 2 ** 20, shape) != 0
+
+
+def test_caps_and_scales_that_32_bits_do_not_hold_are_refused():
+    x, w, t = torch.zeros(3, 16), torch.zeros(50, 16), torch.zeros(3, dtype=torch.int32)
+    for how in ({"softcap": 1e39}, {"softcap": 1e-39}, {"softcap": 1e-50}, {"scale": 1e39}, {"scale": -math.inf},
+                {"scale": math.nan}):
+        with pytest.raises(KernelError, match="softcap must be 0 or"):
+            ops.token_logprobs(x, w, t, **how)
+    for how in ({"softcap": 1e30}, {"softcap": 1e-30}, {"scale": -1e30}, {"scale": 0.0}):
+        with pytest.raises(KernelError, match="CUDA device only"):
+            ops.token_logprobs(x, w, t, **how)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_largest_and_smallest_caps(dtype):
+    for rows in (5, 300):
+        check(rows, 64, 700, dtype, softcap=1e4)
+        x, w, targets, got, lse = check(rows, 64, 700, dtype)
+        again, lse2 = ops.token_logprobs(x, w, targets, softcap=1e30)
+        # (a cap that far away changes a logit by its last digit: two roundings of 2^-24, as near the cap as far from it)
+        assert ((again - got).abs() <= 2.0 ** -19 * (1 + lse.abs() + got.abs())).all()
+        low, lse3 = ops.token_logprobs(x, w, targets, softcap=1e-30)
+        assert ((lse3 - math.log(700)).abs() <= 1e-5).all() and ((low + math.log(700)).abs() <= 1e-5).all()
+        flat, _ = ops.token_logprobs(x, w, targets, scale=0.0)
+        assert ((flat + math.log(700)).abs() <= 1e-5).all()
