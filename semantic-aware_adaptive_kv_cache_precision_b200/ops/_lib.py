@@ -103,7 +103,7 @@ SIGNATURES = {
     "sakv_logprob_pieces": ("logprobs", [P, L, P, I, I, I, P, P, P, P, P, I, F, F, P, P, P]),
     "sakv_logprob_f32": ("logprobs", [P, L, P, I, I, I, P, P, P, P, I, F, F, P, P, P]),
     "sakv_logprob_split": ("logprobs", [P, L, P, I, I, I, I, P, P, P, P, P, I, F, F, P, P, P]),
-    "sakv_logprob_fold": ("logprobs", [P, L, I, I, I, I, P, P, P, P, I, F, F, P]),
+    "sakv_logprob_pad": ("logprobs", [P, L, L, I, I, P, P]),
     "sakv_logprob_join": ("logprobs", [P, P, P, P, P, I, I, I, P]),
     "sakv_lib_accumulate": ("gemm_lib", [P, L, P, P, L, I, I, I, P, L, P]),
 }
@@ -120,7 +120,6 @@ PLAIN_SIGNATURES = {
     "sakv_logprob_shape": ("logprobs", [I, I, I, I, P]),
     "sakv_logprob_split_rows": ("logprobs", [I, I]),
     "sakv_logprob_split_tokens": ("logprobs", [I]),
-    "sakv_logprob_fold_columns": ("logprobs", []),
     "sakv_logprob_f32_columns": ("logprobs", []),
     "sakv_logprob_resident": ("logprobs", []),
     "sakv_logprob_error": ("logprobs", [P]),

@@ -9,10 +9,11 @@ import torch
 
 from . import _lib
 from ._lib import F32, KernelError, call, dtype_code, plain_function, ptr, require_cuda, sm_count
-from .linear import linear
 
-#: logits that lie in memory at one time where a piece is a product of its own (fp32: 32 MB, a quarter of L2)
-PIECE_ELEMENTS = 8 << 20
+#: numbers of the head that lie in memory a second time where it is copied to rows that TMA takes (512 MB), and its
+#: rows among them (which bound what tiles of many rows of x leave)
+PIECE_ELEMENTS = 256 << 20
+PIECE_ROWS = 1 << 18
 #: numbers of x that are split at one time in 32 bits (six bytes each: 384 MB)
 SPLIT_ELEMENTS = 64 << 20
 #: (maximum, sum) pairs that rows leave at one time, one a tile of the head (512 MB)
@@ -125,7 +126,8 @@ def _in_pieces(x, head, targets, bias, scale, softcap, most: int):
     return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
 
 
-def _token_logprobs(x, head, targets, bias, scale, softcap):
+def _token_logprobs(x, head, targets, bias, scale, softcap, found=None):
+    """`found` (rows of 16 bits that TMA takes, few enough for one launch): gets the targets' logits."""
     rows, k = x.shape
     vocab, stride = head.shape[0], x.stride(0)
     logprob, lse = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
@@ -146,6 +148,8 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
         call("sakv_logprob_pieces", at, stride, head_at, rows, vocab, k, shape, targets.data_ptr(), scratch,
              scratch + 4 * floats, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
         _lib.launches += 1          # the call launched the join too
+        if found is not None:
+            found.copy_(part[floats:])
     elif x.dtype is torch.float32 and k % 4 == 0 and head_at % 16 == 0:
         padded, tile = -(-k // 8) * 8, _split_rows(vocab)
         most = max(1, min(SPLIT_ELEMENTS // padded, SPLIT_PAIRS // -(-vocab // tile)))
@@ -169,18 +173,47 @@ def _token_logprobs(x, head, targets, bias, scale, softcap):
         call("sakv_logprob_f32", at, stride, head_at, rows, vocab, k, targets.data_ptr(), scratch,
              scratch + 4 * floats, bias_at, bias_code, scale, softcap, logprob.data_ptr(), lse.data_ptr())
         _lib.launches += 1
-    else:                           # bfloat16 rows that TMA cannot take: logits a piece at a time
-        columns = plain_function("sakv_logprob_fold_columns")()
-        most = max(1, PIECE_ELEMENTS // columns)
-        if rows > most:                # (the scratch of a piece stays as large as it is for these)
-            return _in_pieces(x, head, targets, bias, scale, softcap, most)
-        piece = max(1, min(-(-vocab // columns), PIECE_ELEMENTS // (rows * columns))) * columns
-        pieces = -(-vocab // columns)
-        part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
-        mine = x.new_empty(rows, dtype=torch.float32)
-        for first in range(0, vocab, piece):
-            z = linear(x, head[first:first + piece], out_dtype=torch.float32)
-            call("sakv_logprob_fold", ptr(z), z.stride(0), rows, z.shape[1], first, vocab, ptr(targets),
-                 ptr(part[first // columns]), ptr(mine), bias_at, bias_code, scale, softcap)
-        call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, pieces)
+    else:                           # bfloat16 rows that TMA cannot take
+        return _copied(x, head, targets, bias, scale, softcap)
     return logprob, lse
+
+
+def _copied(x, head, targets, bias, scale, softcap):
+    """bfloat16 rows whose size is no multiple of 8, or that do not begin at multiples of 16 bytes: from copies that are
+    and do, of x and, where it takes one, of the head, a piece of it at a time. (A piece's partial is its log of the sum of
+    exponentials: it stands for one maximum beside a sum of 1.) 64 rows of 1,535 over 151,936: 267 us, of which the copy
+    takes 177; 2,047 rows 745."""
+    if _pairs() <= 0:
+        raise KernelError("token_logprobs: no pair of this device's SMs holds the kernel")
+    rows, k = x.shape
+    vocab, padded = head.shape[0], -(-k // 8) * 8
+    if k == padded and head.data_ptr() % 16 == 0:
+        return _token_logprobs(_padded(x, x.new_empty((rows, k))), head, targets, bias, scale, softcap)
+    piece = min(vocab, max(1, min(PIECE_ELEMENTS // padded, PIECE_ROWS)))
+    most = max(256, SPLIT_PAIRS // -(-piece // 192) // 256 * 256)        # (tiles of the head have 192 rows at least)
+    if rows > most:
+        return _in_pieces(x, head, targets, bias, scale, softcap, most)
+    x, room = _padded(x, x.new_empty((rows, padded))), x.new_empty((piece, padded))
+    if piece == vocab:
+        return _token_logprobs(x, _padded(head, room), targets, bias, scale, softcap)
+    pieces = -(-vocab // piece)
+    part = x.new_empty((pieces, rows, 2), dtype=torch.float32)
+    mine, found = x.new_zeros(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+    for i, first in enumerate(range(0, vocab, piece)):
+        n = min(piece, vocab - first)
+        here = (targets >= first) & (targets < first + n)
+        _, lse = _token_logprobs(x, _padded(head[first:first + n], room[:n]), torch.where(here, targets - first, -1),
+                                 None if bias is None else bias[first:first + n], scale, softcap, found)
+        part[i, :, 0] = lse
+        part[i, :, 1] = lse != -float("inf")
+        mine = torch.where(here, found, mine)
+    logprob, lse = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+    call("sakv_logprob_join", ptr(part), ptr(mine), ptr(targets), ptr(logprob), ptr(lse), rows, vocab, pieces)
+    return logprob, lse
+
+
+def _padded(rows: torch.Tensor, into: torch.Tensor) -> torch.Tensor:
+    """`rows` at the front of the rows of `into`, zeros behind them."""
+    count, k = rows.shape
+    call("sakv_logprob_pad", rows.data_ptr(), k if count == 1 else rows.stride(0), count, k, into.shape[1], into.data_ptr())
+    return into

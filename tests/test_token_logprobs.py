@@ -376,3 +376,49 @@ def test_the_largest_and_smallest_caps(dtype):
         assert ((lse3 - math.log(700)).abs() <= 1e-5).all() and ((low + math.log(700)).abs() <= 1e-5).all()
         flat, _ = ops.token_logprobs(x, w, targets, scale=0.0)
         assert ((flat + math.log(700)).abs() <= 1e-5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 70, 300, 700])
+@pytest.mark.parametrize("k, x_pad, head_at", [(37, 0, 0), (64, 3, 0), (64, 0, 1), (40, 24, 4), (1, 0, 0), (1031, 2, 3)])
+def test_rows_that_are_copied_use_the_kernel(monkeypatch, rows, k, x_pad, head_at):
+    """bfloat16 rows that TMA cannot take: no product of a library, whole and in pieces of the head and of the rows."""
+    def none(*args, **how):
+        raise AssertionError("a library's product")
+
+    vocab = 1777
+    g = torch.Generator(device="cuda").manual_seed(k + rows)
+    x = torch.randn((rows, k + x_pad), generator=g, device="cuda").to(torch.bfloat16)[:, :k]
+    flat = (torch.randn(vocab * k + head_at, generator=g, device="cuda") * 2 / math.sqrt(k)).to(torch.bfloat16)
+    w = flat[head_at:].view(vocab, k)
+    bias = torch.randn(vocab, generator=g, device="cuda")
+    bias[:500] = -math.inf                                       # whole pieces of the head
+    targets = torch.randint(500, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    targets[0], targets[1], targets[2] = 499, -1, vocab
+    with monkeypatch.context() as m:
+        for name in ("mm", "addmm", "matmul", "bmm"):
+            m.setattr(torch, name, none)
+        calls = [ops.token_logprobs(x, w, targets, bias, scale=0.5)]
+        m.setattr(logprobs, "PIECE_ELEMENTS", 500 * (-(-k // 8) * 8))
+        calls.append(ops.token_logprobs(x, w, targets, bias, scale=0.5))
+        m.setattr(logprobs, "PIECE_ROWS", 250)
+        m.setattr(logprobs, "SPLIT_PAIRS", 256 * 2)
+        calls.append(ops.token_logprobs(x, w, targets, bias, scale=0.5))
+    want, want_lse, bound = reference(x, w, targets, bias, 0.5, 0.0)
+    bound = bound + 2.0 ** -21 * (1 + want_lse.abs())           # (pieces' sums are joined through a second logarithm)
+    for got, lse in calls:
+        assert ((lse.double() - want_lse).abs() <= bound).all(), ((lse.double() - want_lse).abs() / bound).max()
+        assert ((got.double() - want).abs() <= bound)[3:].all()
+        assert got[0] == -math.inf and got[1] == 0 and got[2].isnan()
+    bias[:] = -math.inf
+    monkeypatch.setattr(logprobs, "PIECE_ELEMENTS", 500 * (-(-k // 8) * 8))
+    got, lse = ops.token_logprobs(x, w, targets, bias)
+    assert (lse == -math.inf).all() and got[1] == 0 and got[[0] + list(range(2, rows))].isnan().all()
+    x[1], bias[:] = math.nan, 0.0
+    got, lse = ops.token_logprobs(x, w, targets, bias)
+    assert lse[1].isnan() and torch.isfinite(lse[2:]).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, _ = ops.token_logprobs(x, w, targets, bias)
+    graph.replay()
+    assert torch.equal(held[3:], got[3:])
