@@ -753,7 +753,8 @@ int launch_f32(const float* x, long long x_stride, const float* head, int M, int
 // is below 2^-21 of it. The six are products on the tensor cores. These cut where they add, always the same way: sums
 // of h h' are taken off them every kChunk steps and added up in fp32 by the epilogue. The largest error over 64 tokens
 // and K = 1,536 is 1.6e-6 to 2.6e-6 so (every second step; every fourth: 3.1e-6 and 4 % less time), 1.2e-5 with one
-// sum for all of K, 3.5e-6 to 6.9e-6 with the library's product. A number that is not finite makes its products NaN.
+// sum for all of K, 3.5e-6 to 6.9e-6 with the library's product. Sums that are NaN are taken again with
+// plain multiply-adds: the parts of an infinity are infinity and NaN.
 // A block takes a tile of `rows` rows of the head, on the lanes of tensor memory, against up to 96 tokens, its columns:
 //   warp 0       TMA: the head as it is (boxes of 32 floats) into a ring,
 //   warp 1       tensor memory, and the products,
@@ -783,6 +784,8 @@ struct SplitParams {
   int m_tiles, cols;         // tiles of `cols` tokens (a multiple of 32)
   int rows, n_tiles;         // tiles of `rows` rows of the head
   int raw_stages, x_stages;
+  const float *x, *head;     // as they are, for sums that are NaN in three parts
+  long long x_stride;
   const int32_t* targets;
   float2* part;              // [n_tiles][M]
   float* mine;
@@ -842,6 +845,28 @@ split_kernel(const float* __restrict__ x, long long x_stride, int M, int K, int 
     const uint32_t a = cut_two(v[0], v[1]);
     out[piece * all + i] = make_uint2(a, cut_two(v[2], v[3]));
   }
+}
+
+// A row's (maximum, sum) over a warp's rows of the head, from plain multiply-adds: for sums that came out NaN, since the
+// three parts of an infinity are infinity and NaN. A row that has a NaN of its own, which all lanes look for together,
+// keeps it. `target`: the row's; `v`: the lane's token, of those that are `real`.
+__device__ __noinline__ float2 plain_row(const SplitParams* p, int m, int target, int v, bool real) {
+  const float* x = p->x + m * p->x_stride;
+  bool none = true;
+  for (int k = threadIdx.x & 31; k < p->K; k += 32) none &= x[k] == x[k];
+  if (!__all_sync(0xffffffffu, none)) return make_float2(-INFINITY, NAN);
+  float z = -INFINITY;
+  if (real) {
+    const float* w = p->head + (long long)v * p->K;
+    z = 0.f;
+    for (int k = 0; k < p->K; ++k) z = fmaf(x[k], w[k], z);
+    if (p->form.bias) z += bias_at(p->form, v);
+    z *= p->form.scale;
+    if (p->form.cap > 0.f) z = p->form.cap * tanhf(z * p->form.over_cap);
+    if (v == target) p->mine[m] = z;
+  }
+  const float top = warp_max(z);
+  return make_float2(top, warp_sum(expf(z - (top == -INFINITY ? 0.f : top))));
 }
 
 // 16 columns of this warp's 32 lanes are written (no wait).
@@ -1099,7 +1124,14 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int j = 0; j < 32; ++j) z[j] = expf(z[j] - __shfl_sync(0xffffffffu, base, j));
-        tail->share[turn.at][quarter][c + lane] = make_float2(top, over_lanes<false>(z, lane));
+        float2 share = make_float2(top, over_lanes<false>(z, lane));
+        for (unsigned odd = __ballot_sync(0xffffffffu, share.y != share.y); odd; odd &= odd - 1) {
+          const int j = __ffs(odd) - 1;
+          if (m0 + c + j >= p.M) continue;
+          const float2 plain = plain_row(&p, m0 + c + j, target[c + j], v, real);
+          if (lane == j) share = plain;
+        }
+        tail->share[turn.at][quarter][c + lane] = share;
       }
       // (what a tile leaves in shared memory stays until the one after the next, past the next one's barriers)
       asm volatile("bar.sync 1, %0;" ::"n"(kSplitEpilogue) : "memory");
@@ -1357,6 +1389,7 @@ SAKV_EXPORT int sakv_logprob_split(const float* x, long long x_stride, const flo
   p.x_stages = p.cols <= 32 ? 4 : 3;
   p.raw_stages = (room - p.x_stages * x_bytes) / kSplitRaw;
   if (p.raw_stages > kSplitRawMost) p.raw_stages = kSplitRawMost;
+  p.x = x; p.head = head; p.x_stride = x_stride;
   p.targets = targets; p.part = reinterpret_cast<float2*>(part); p.mine = mine;
   p.form = shape_of(bias, bias_bf16, scale, cap);
   p.error = error_word();

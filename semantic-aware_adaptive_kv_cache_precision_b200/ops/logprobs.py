@@ -39,8 +39,7 @@ def token_logprobs(x: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, b
     [T]) under the logits `cap(scale * (x head^T + bias))`, cap(z) = softcap * tanh(z / softcap) where
     softcap > 0. `x` [T, K] and `head` [vocab, K] of one type, float32 or bfloat16; `bias` [vocab] float32 or
     bfloat16. A negative target asks for nothing and gets 0; one past the vocabulary gets NaN. A row with a
-    logit that is NaN or +inf has NaN; logits of -inf, which a bias makes, count for nothing (numbers of `x` or
-    `head` that are not finite make NaN in float32)."""
+    logit that is NaN or +inf has NaN; logits of -inf count for nothing."""
     device, dtype = x.get_device(), x.dtype
     # (one expression for the calls that are right; `_refuse` says what is wrong with the others)
     if not (x.dim() == 2 and head.dim() == 2 and targets.dim() == 1 and dtype is head.dtype

@@ -422,3 +422,36 @@ def test_rows_that_are_copied_use_the_kernel(monkeypatch, rows, k, x_pad, head_a
         held, _ = ops.token_logprobs(x, w, targets, bias)
     graph.replay()
     assert torch.equal(held[3:], got[3:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("k", [64, 63, 1100, 1101])
+@pytest.mark.parametrize("rows", [7, 300])
+def test_infinities_in_rows_and_in_the_head(dtype, k, rows):
+    """As the formula has them, whichever way the rows go: a logit of -inf counts for nothing, one that is +inf or NaN makes
+    its row NaN."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn((rows, k), generator=g, device="cuda").to(dtype)
+    w = torch.randn((700, k), generator=g, device="cuda").div_(math.sqrt(k)).to(dtype)
+    x[:, 3] = x[:, 3].abs() + 0.5
+    x[3, 3] = -1.0                           # its logit of the head's third row is +inf
+    x[4, 3] = 0.0                            # and of this row NaN
+    w[2, 3] = w[650, 3] = -math.inf
+    x[5, 9], w[:, 9] = -math.inf, w[:, 9].abs() + 0.25          # every logit of this row is -inf, but for one
+    w[77, 9] = -1.0                                             # that is +inf
+    x[6, 1] = math.nan
+    targets = torch.arange(rows, dtype=torch.int32, device="cuda")
+    targets[1] = 650
+    got, lse = ops.token_logprobs(x, w, targets)
+    good = [0, 1, 2] + list(range(7, rows))
+    assert got[3:7].isnan().all() and lse[3:7].isnan().all()
+    kept = torch.ones(700, dtype=torch.bool, device="cuda")
+    kept[[2, 650]] = False
+    near = targets.clone()
+    near[1], near[2] = 0, 0
+    place = torch.cumsum(kept, 0).int() - 1                      # of a token among those that count
+    want, want_lse, bound = reference(x[good], w[kept], place[near.long().clamp(max=699)][good], None, 1.0, 0.0)
+    assert ((lse[good].double() - want_lse).abs() <= bound).all()
+    assert got[1] == -math.inf and got[2] == -math.inf
+    assert ((got[good].double() - want).abs() <= bound)[[0] + list(range(3, len(good)))].all()
