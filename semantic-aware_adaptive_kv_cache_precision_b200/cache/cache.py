@@ -57,6 +57,8 @@ class KVGroup:
         self.need, self.entries = need, entries
         self.pool = Pool(blocks, "cache block")
         self.holders = np.zeros(blocks, dtype=np.int32)     # sequences that list each block
+        # moves whenever the sequences that share blocks of this group may have changed
+        self.sharing = 0
         if need.dtype is not None:
             if need.dtype not in _DTYPES:
                 raise TypeError(f"{need!r}: dtype must be one of {sorted(_DTYPES)} or None")
@@ -131,10 +133,8 @@ class SequenceCache:
                                        self.max_slots, dtype, device))
             for i, entry in enumerate(entries):
                 self.entry_group[entry] = (g, i)
-        # holders beyond the first, over all blocks (0: no block is listed twice), and a number that
-        # moves whenever the sequences that share blocks may have changed
+        # holders beyond the first, over all blocks (0: no block is listed twice)
         self._shared = 0
-        self.sharing = 0
         # first position whose block a window group still holds, per (group, slot)
         self._front = [np.zeros(self.max_slots, dtype=np.int64) for _ in self.groups]
 
@@ -186,7 +186,7 @@ class SequenceCache:
             blocks = [b for b in blocks if group.holders[b] == 0]
             kept -= len(blocks)
             self._shared -= kept
-            self.sharing += kept > 0
+            group.sharing += kept > 0
             if not blocks:
                 return
         if self.poison_freed and group.keys.is_floating_point():
@@ -238,6 +238,7 @@ class SequenceCache:
             common = row[:full]
             listed = common[common >= 0]
             group.holders[listed] += count
+            group.sharing += 1
             self._shared += count * len(listed)
             group.tables[new] = -1
             group.tables[new, :full] = common
@@ -248,7 +249,6 @@ class SequenceCache:
                 group.tables[new, full] = own
                 self._copy(group.tensors, [int(row[full])] * count, own, rows=rows)
         self.lengths[new] = length
-        self.sharing += 1
         if self.states:
             by_type = list(self.states.values())
             self._copy(by_type, [slot] * count, new, axis=0)
@@ -308,6 +308,7 @@ class SequenceCache:
             group.pool.take(len(held))
             group.keys, group.values = keys, values
             group.tables, group.holders, group.max_blocks_per_seq = tables, holders, width
+            group.sharing += 1
         more = slots - self.max_slots
         if more:
             self.states = states
@@ -317,7 +318,6 @@ class SequenceCache:
             self.max_slots = slots
         self.blocks, self.max_tokens = blocks, blocks * BLOCK
         self.max_seq_len, self.max_blocks_per_seq = longest, width
-        self.sharing += 1
 
     # -- growth -------------------------------------------------------------
 

@@ -89,6 +89,7 @@ class Engine:
         self.shared_bytes_worth = SHARED_BYTES_WORTH
         self._shared_now = None        # (what the plans below are right for, how far, the plans)
         self._shared_buffers: dict = {}
+        self._shared_readers = None    # [(cache group, query heads)] that plans are made for
         #: steps of up to this many tokens are captured when their shape repeats (0: never);
         #: at most `prefill_graph_count` of them are kept
         self.prefill_graph_tokens = 8192
@@ -127,7 +128,7 @@ class Engine:
         from .. import ops
         self._graphs.clear()
         self._prefill_graphs.clear()
-        self._shared_now = None
+        self._shared_now = self._shared_readers = None
         self._shared_buffers.clear()
         held = [] if self.model.arena is None else [self.model.arena.buffer]
         if self.cache is not None:
@@ -251,7 +252,10 @@ class Engine:
         if self.shared_bytes_worth is None or not cache.shares_blocks:
             return {}
         width = min(table_width(ends), cache.max_blocks_per_seq)
-        key = (tuple(slots), cache.sharing, width)
+        if self._shared_readers is None:
+            self._shared_readers = [(g, heads) for need, heads in self.model.shared_readers()
+                                    for g, group in enumerate(cache.groups) if group.need == need]
+        key = (tuple(slots), tuple(cache.groups[g].sharing for g, _ in self._shared_readers), width)
         if self._shared_now is not None:
             known, reach, plans = self._shared_now
             if known == key and all(e <= r for e, r in zip(ends, reach)):
@@ -267,25 +271,23 @@ class Engine:
         reach = [min(width * BLOCK, e + 8 * BLOCK) for e in ends]
         tables = cache.tables_for(slots)
         plans = {}
-        for need, heads in self.model.shared_readers():
-            for g, group in enumerate(cache.groups):
-                if group.need != need:
-                    continue
-                block = sum(t.numel() // (t.shape[0] * t.shape[1]) * t.element_size() for t in group.tensors)
-                if int(np.maximum(group.holders - 1, 0).sum()) * block < self.shared_bytes_worth:
-                    continue         # (all that anyone shares is too little: no plan is worked out)
-                plan = ops.plan_shared(tables[g][:, :width], ends, heads, need.kv_heads, None, reach=reach,
-                                       roomy=True, slots=2 * _lib.sm_count(self.device))
-                if plan.saved * block < self.shared_bytes_worth:
-                    continue
-                place = (g, heads, plan.layout)
-                buffer = self._shared_buffers.get(place)
-                words = torch.from_numpy(plan.words)
-                if buffer is None:
-                    buffer = self._shared_buffers[place] = torch.empty(words.shape, dtype=torch.int32,
-                                                                       device=self.device)
-                buffer.copy_(words.pin_memory(), non_blocking=True)
-                plans[g, heads] = plan.on(buffer)
+        for g, heads in self._shared_readers:
+            group = cache.groups[g]
+            block = sum(t.numel() // (t.shape[0] * t.shape[1]) * t.element_size() for t in group.tensors)
+            if int(np.maximum(group.holders - 1, 0).sum()) * block < self.shared_bytes_worth:
+                continue             # (all that anyone shares is too little: no plan is worked out)
+            plan = ops.plan_shared(tables[g][:, :width], ends, heads, group.need.kv_heads, None, reach=reach,
+                                   roomy=True, slots=2 * _lib.sm_count(self.device))
+            if plan.saved * block < self.shared_bytes_worth:
+                continue
+            place = (g, heads, plan.layout)
+            buffer = self._shared_buffers.get(place)
+            words = torch.from_numpy(plan.words)
+            if buffer is None:
+                buffer = self._shared_buffers[place] = torch.empty(words.shape, dtype=torch.int32,
+                                                                   device=self.device)
+            buffer.copy_(words.pin_memory(), non_blocking=True)
+            plans[g, heads] = plan.on(buffer)
         self._shared_now = (key, reach, plans)
         return plans
 

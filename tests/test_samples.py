@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from semantic_aware_adaptive_kv_cache_precision_b200 import Engine, write_random_model
+from semantic_aware_adaptive_kv_cache_precision_b200 import Engine, ops, write_random_model
 from semantic_aware_adaptive_kv_cache_precision_b200.cache import BLOCK, CacheFull
 from semantic_aware_adaptive_kv_cache_precision_b200.engine.generate import plan_samples
 
@@ -369,7 +369,7 @@ def engine_without_a_gpu(monkeypatch, cache, readers):
     monkeypatch.setattr(module._lib, "sm_count", lambda device=None: 148)
     e = Engine.__new__(Engine)
     e.device, e.cache, e.model = torch.device("cpu"), None, SimpleNamespace(shared_readers=lambda: readers, arena=None)
-    e.shared_bytes_worth, e._shared_now, e._shared_buffers = 0, None, {}
+    e.shared_bytes_worth, e._shared_now, e._shared_buffers, e._shared_readers = 0, None, {}, None
     e._graphs, e._prefill_graphs = {}, {}
     return e
 
@@ -460,3 +460,32 @@ def test_rotary_tables_are_made_both_or_neither(monkeypatch):
     assert part.cos.shape == part.sin.shape == (10, 4)
     part.prepare("cpu", 50)
     assert part.cos.shape == part.sin.shape == (50, 4)
+
+
+def test_a_window_that_slides_leaves_the_plans_of_other_groups(monkeypatch):
+    """Blocks that a window's group gives back are none that a plan speaks of."""
+    from semantic_aware_adaptive_kv_cache_precision_b200.cache import KVNeed, SequenceCache
+    whole, window = KVNeed(1, 64), KVNeed(2, 64, window=100)
+    cache = SequenceCache([whole, window], 40 * BLOCK, 40 * BLOCK, torch.bfloat16, "cpu", max_slots=9)
+    e = engine_without_a_gpu(monkeypatch, cache, [(whole, 2)])
+    made = []
+    plan_shared = ops.plan_shared
+    monkeypatch.setattr(ops, "plan_shared", lambda *args, **how: (made.append(args[1]), plan_shared(*args, **how))[1])
+
+    def grow(slots, n):
+        cache.reserve(slots, [n] * len(slots))
+        plans = e._shared_plans(slots, [n] * len(slots), cache)
+        cache.advance(slots, [n] * len(slots))
+        return plans
+
+    (a,) = cache.open(1)
+    grow([a], 4 * BLOCK)
+    slots = [a] + cache.fork(a, 3)
+    for n in range(4 * BLOCK + 1, 8 * BLOCK):        # the window leaves every block that the four share behind
+        assert grow(slots, n)
+    cache.check()
+    assert len(made) == 1 and cache.groups[1].sharing > cache.groups[0].sharing
+    b = cache.fork(a, 1)
+    assert grow(slots + b, 8 * BLOCK) and len(made) == 2
+    cache.close(b)
+    assert grow(slots, 8 * BLOCK + 1) and len(made) == 3
