@@ -39,6 +39,8 @@ DEFAULT_MAX_STEP_TOKENS = 16384
 SHARED_BYTES_WORTH = 80 << 20
 # Layouts of plans whose words are kept on the device for captured steps to read.
 MOST_PLAN_BUFFERS = 64
+# Batches whose plans are kept on the host, for when they step again.
+KNOWN_PLANS = 8
 
 
 class Engine:
@@ -88,7 +90,8 @@ class Engine:
         #: at least this many bytes a layer (None: never)
         self.shared_bytes_worth = SHARED_BYTES_WORTH
         self._shared_now = None        # (what the plans below are right for, how far, the plans)
-        self._shared_buffers: dict = {}
+        self._shared_known: dict = {}  # the plans of the batches of late: what they are right for -> (how far, plans)
+        self._shared_buffers: dict = {}    # place -> (words on the device, the plan that they are)
         self._shared_readers = None    # [(cache group, query heads)] that plans are made for
         #: steps of up to this many tokens are captured when their shape repeats (0: never);
         #: at most `prefill_graph_count` of them are kept
@@ -129,6 +132,7 @@ class Engine:
         self._graphs.clear()
         self._prefill_graphs.clear()
         self._shared_now = self._shared_readers = None
+        self._shared_known.clear()
         self._shared_buffers.clear()
         held = [] if self.model.arena is None else [self.model.arena.buffer]
         if self.cache is not None:
@@ -255,7 +259,8 @@ class Engine:
         if self._shared_readers is None:
             self._shared_readers = [(g, heads) for need, heads in self.model.shared_readers()
                                     for g, group in enumerate(cache.groups) if group.need == need]
-        key = (tuple(slots), tuple(cache.groups[g].sharing for g, _ in self._shared_readers), width)
+        key = (tuple(slots), tuple(cache.groups[g].sharing for g, _ in self._shared_readers), width,
+               self.shared_bytes_worth)
         if self._shared_now is not None:
             known, reach, plans = self._shared_now
             if known == key and all(e <= r for e, r in zip(ends, reach)):
@@ -267,29 +272,44 @@ class Engine:
             self._prefill_graphs.clear()
             self._shared_now = None
             self._shared_buffers.clear()
+        # (batches that step in turn each find their own again)
+        reach, made = self._shared_known.pop(key, (None, None))
+        if reach is None or any(e > r for e, r in zip(ends, reach)):
+            reach, made = self._plans_for(slots, ends, cache, width)
+        self._shared_known[key] = reach, made
+        if len(self._shared_known) > KNOWN_PLANS:
+            del self._shared_known[next(iter(self._shared_known))]
+        plans = {}
+        for (g, heads), plan in made.items():
+            place = (g, heads, plan.layout)
+            buffer, holds = self._shared_buffers.get(place, (None, None))
+            words = torch.from_numpy(plan.words)
+            if buffer is None:
+                buffer = torch.empty(words.shape, dtype=torch.int32, device=self.device)
+            if holds is not plan:
+                buffer.copy_(words.pin_memory(), non_blocking=True)
+                self._shared_buffers[place] = buffer, plan
+            plans[g, heads] = plan.on(buffer)
+        self._shared_now = (key, reach, plans)
+        return plans
+
+    def _plans_for(self, slots, ends, cache, width) -> tuple:
+        """(how far they reach, the plans worth making, their words on the host) of `_shared_plans`."""
         # (eight blocks further: a decode loop asks again after 512 steps at the earliest)
         reach = [min(width * BLOCK, e + 8 * BLOCK) for e in ends]
         tables = cache.tables_for(slots)
         plans = {}
         for g, heads in self._shared_readers:
-            group = cache.groups[g]
+            group, table = cache.groups[g], tables[g][:, :width]
             block = sum(t.numel() // (t.shape[0] * t.shape[1]) * t.element_size() for t in group.tensors)
-            if int(np.maximum(group.holders - 1, 0).sum()) * block < self.shared_bytes_worth:
-                continue             # (all that anyone shares is too little: no plan is worked out)
-            plan = ops.plan_shared(tables[g][:, :width], ends, heads, group.need.kv_heads, None, reach=reach,
-                                   roomy=True, slots=2 * _lib.sm_count(self.device))
-            if plan.saved * block < self.shared_bytes_worth:
-                continue
-            place = (g, heads, plan.layout)
-            buffer = self._shared_buffers.get(place)
-            words = torch.from_numpy(plan.words)
-            if buffer is None:
-                buffer = self._shared_buffers[place] = torch.empty(words.shape, dtype=torch.int32,
-                                                                   device=self.device)
-            buffer.copy_(words.pin_memory(), non_blocking=True)
-            plans[g, heads] = plan.on(buffer)
-        self._shared_now = (key, reach, plans)
-        return plans
+            listed = table[table >= 0]
+            if (len(listed) - np.count_nonzero(np.bincount(listed))) * block < self.shared_bytes_worth:
+                continue             # (all that these sequences list twice is too little: no plan is worked out)
+            plan = ops.plan_shared(table, ends, heads, group.need.kv_heads, None, reach=reach, roomy=True,
+                                   slots=2 * _lib.sm_count(self.device))
+            if plan.saved * block >= self.shared_bytes_worth:
+                plans[g, heads] = plan
+        return reach, plans
 
     def next_tokens(self, slots: list, device_tokens: torch.Tensor) -> torch.Tensor:
         """One greedy decode step: feed `device_tokens[i]` (int32 [len(slots)], on the device)

@@ -370,6 +370,7 @@ def engine_without_a_gpu(monkeypatch, cache, readers):
     e = Engine.__new__(Engine)
     e.device, e.cache, e.model = torch.device("cpu"), None, SimpleNamespace(shared_readers=lambda: readers, arena=None)
     e.shared_bytes_worth, e._shared_now, e._shared_buffers, e._shared_readers = 0, None, {}, None
+    e._shared_known = {}
     e._graphs, e._prefill_graphs = {}, {}
     return e
 
@@ -398,7 +399,7 @@ def test_captured_steps_go_with_the_plans_they_read(monkeypatch):
                 assert table[key] == at
             table[key] = at
         assert len(e._shared_buffers) <= 64
-        held = {b.data_ptr() for b in e._shared_buffers.values()}
+        held = {b.data_ptr() for b, _ in e._shared_buffers.values()}
         assert all(set(x) <= held for table in (e._graphs, e._prefill_graphs) for x in table.values())
 
 
@@ -489,3 +490,50 @@ def test_a_window_that_slides_leaves_the_plans_of_other_groups(monkeypatch):
     assert grow(slots + b, 8 * BLOCK) and len(made) == 2
     cache.close(b)
     assert grow(slots, 8 * BLOCK + 1) and len(made) == 3
+
+
+def counted_plans(monkeypatch):
+    made, plan_shared = [], ops.plan_shared
+    monkeypatch.setattr(ops, "plan_shared", lambda *args, **how: (made.append(len(args[1])), plan_shared(*args, **how))[1])
+    return made
+
+
+def test_batches_that_step_in_turn_keep_their_plans(monkeypatch):
+    """And each reads its own, also where two lie at one address; a batch that shares nothing asks for no plan."""
+    from semantic_aware_adaptive_kv_cache_precision_b200.cache import KVNeed, SequenceCache
+    from semantic_aware_adaptive_kv_cache_precision_b200.engine import engine as module
+    need = KVNeed(1, 64)
+    cache = SequenceCache([need], 64 * BLOCK, 64 * BLOCK, torch.bfloat16, "cpu", max_slots=60)
+    e = engine_without_a_gpu(monkeypatch, cache, [(need, 2)])
+    e.shared_bytes_worth = 4 * 2 * 64 * 64 * 2           # four blocks of keys and values
+    made = counted_plans(monkeypatch)
+    heads = cache.open(4)
+    cache.reserve(heads, [4 * BLOCK, 4 * BLOCK, 3 * BLOCK, 2 * BLOCK])
+    cache.advance(heads, [4 * BLOCK, 4 * BLOCK, 3 * BLOCK, 2 * BLOCK])
+    first, second = ([h] + cache.fork(h, 3) for h in heads[:2])
+    alone = heads[2:]
+    mixed = [first[0], second[0], heads[2], heads[3]]    # as many sequences, nothing shared among them
+    lists = {}
+    for turn in range(20):
+        for name, slots in (("first", first), ("second", second), ("mixed", mixed), ("alone", alone)):
+            now = [int(cache.lengths[s]) + 1 for s in slots]
+            cache.reserve(slots, now)
+            plans = e._shared_plans(slots, now, cache)
+            assert bool(plans) == (name in ("first", "second"))
+            if plans:
+                plan = plans[0, 2]
+                fresh = ops.plan_shared(cache.tables_for(slots)[0][:, :plan.width], now, 2, 1, None, reach=plan.reach,
+                                        roomy=True, slots=296)
+                made.pop()
+                lists.setdefault(name, plan.words.data_ptr())
+                assert lists[name] == plan.words.data_ptr() and np.array_equal(plan.words.numpy(), fresh.words)
+    assert lists["first"] == lists["second"]             # (one layout)
+    assert made == [4, 4]
+    for i in range(20):                                  # batches come and go: no more than some are kept
+        slots = first[:2 + i % 3] + alone[:i % 2]
+        e._shared_plans(slots, [int(cache.lengths[s]) + 1 for s in slots], cache)
+        assert len(e._shared_known) <= module.KNOWN_PLANS
+    e.shared_bytes_worth = 10 ** 12                      # what pays is asked anew
+    assert e._shared_plans(first, [4 * BLOCK + 2] * 4, cache) == {}
+    e.shared_bytes_worth = 0
+    assert e._shared_plans(first, [4 * BLOCK + 2] * 4, cache)
