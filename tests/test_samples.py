@@ -537,3 +537,32 @@ def test_batches_that_step_in_turn_keep_their_plans(monkeypatch):
     assert e._shared_plans(first, [4 * BLOCK + 2] * 4, cache) == {}
     e.shared_bytes_worth = 0
     assert e._shared_plans(first, [4 * BLOCK + 2] * 4, cache)
+
+
+@pytest_gpu
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("worth", [0, None])
+def test_chosen_tokens_over_shared_blocks_are_the_logits_best(varied_folders, graphs, worth):
+    """`next_tokens` chooses inside the step, captured or not: its tokens have the largest logits that `step` gives equal
+    forks that are fed the same, and lead to the same places."""
+    engine = engine_of(varied_folders("D", "bfloat16"), "bfloat16", cuda_graphs=graphs, max_tokens=16384)
+    engine.shared_bytes_worth = worth
+    rng = np.random.default_rng(11)
+    (a,) = engine.open(1)
+    engine.step([a], [rng.integers(0, engine.vocab_size, 450).tolist()])
+    slots = engine.fork(a, 4)
+    fed = torch.tensor([3, 77, 150, 399], dtype=torch.int32, device="cuda")
+    twins = engine.fork(a, 4)
+    seen = set()
+    for _ in range(12):
+        logits = engine.step(twins, device_tokens=fed.clone())
+        if worth == 0:
+            assert engine._shared_now[2]
+        fed = engine.next_tokens(slots, fed).clone()
+        best, mine = logits.amax(1), logits.gather(1, fed.long()[:, None])[:, 0]
+        # (both steps are bfloat16 steps of the same sequences: as far apart as such steps are)
+        assert ((best - mine) <= 0.06 * logits.std(1)).all()
+        seen.update(fed.tolist())
+    assert len(seen) > 4
+    engine.close([a] + slots + twins)
+    engine.cache.check()
