@@ -37,7 +37,7 @@ constexpr int kNarrowThreads = kWarps * 32;
 constexpr int kStages = 3;           // of a narrow unit
 // Rows up to which a unit is narrow. Measured, us of the kernel over 32,000 shared positions, two KV heads of 6
 // query heads: 12 rows 11.5 narrow; 24 rows 14.3 narrow, 14.1 wide; 60 rows 20.2 narrow, 14.1 wide.
-constexpr int kWideRows = 128, kNarrowRows = 32, kMostGroup = 64;
+constexpr int kWideRows = 128, kNarrowRows = 32, kMostGroup = 16;
 constexpr int kWideStages = 2;
 constexpr int kMembers = kWideRows + 2;
 constexpr uint32_t kTmemCols = 256;  // wide: S 2 x 64 (P over the first 32 of each), O from 128 on

@@ -15,7 +15,7 @@ from ._lib import CACHE_BLOCK, KernelError, call_on, require_cuda, sm_count
 from .attention import fast_path_takes
 
 UNIT_ROWS = 128           # most rows (sequences x query heads of one KV head) of a unit of work
-MOST_GROUP = 64           # most query heads of one KV head
+MOST_GROUP = 16           # most query heads of one KV head, as in the other tensor-core kernels
 LEAST_SCALE = 1e-30       # scales from here to its reciprocal
 UNIT_WORDS = 8
 
@@ -263,7 +263,7 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     # host's work; `_refuse` says what is wrong with the others)
     if not (qkv.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
             and (head_dim == 128 or head_dim == 64) and 0 < kv_heads and heads % kv_heads == 0
-            and heads <= 16 * kv_heads and LEAST_SCALE <= scale <= 1 / LEAST_SCALE and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
+            and heads <= MOST_GROUP * kv_heads and LEAST_SCALE <= scale <= 1 / LEAST_SCALE and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
             and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
             and k_shape == v_cache.shape and len(k_shape) == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() and k_shape[1] == kv_heads
             and k_shape[2] == CACHE_BLOCK and k_shape[3] == head_dim

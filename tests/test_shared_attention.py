@@ -432,3 +432,11 @@ def test_calls_on_two_streams_and_graphs_at_once():
     torch.cuda.synchronize()
     assert all(torch.equal(h, want) for (_, held), want in zip(graphs, fresh) for h in held)
     assert not torch.equal(fresh[0], alone[0])
+
+
+def test_a_plan_that_no_call_takes_is_refused():
+    tables, lengths, _ = lists_of(CASES["forks"])
+    assert ops.plan_shared(tables, lengths, 16, 1, slots=8).units
+    for heads, kv_heads in ((17, 1), (48, 2), (64, 1)):
+        with pytest.raises(KernelError, match="at most 16"):
+            ops.plan_shared(tables, lengths, heads, kv_heads, slots=8)
