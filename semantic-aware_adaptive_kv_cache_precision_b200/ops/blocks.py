@@ -6,6 +6,7 @@ from __future__ import annotations
 import array
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -60,10 +61,14 @@ def copy_blocks(tensors, src, dst, *, into=None, rows: int | None = None, axis: 
         table[some] = (a, z) + geometry
         some += 1
         spans.append((z, z + (geometry[1] or room * geometry[2]) * geometry[3]))
+    src, dst = (ids if hasattr(ids, "__len__") else list(ids) for ids in (src, dst))     # (each is read twice, perhaps)
     try:
         source, target = array.array("i", src), array.array("i", dst)
-    except (TypeError, OverflowError):                        # (numbers of other kinds)
-        source, target = array.array("q", map(int, src)), array.array("q", map(int, dst))
+    except (TypeError, OverflowError):                        # (numbers of other kinds, or past 32 bits)
+        try:
+            source, target = (array.array("q", map(operator.index, ids)) for ids in (src, dst))
+        except (TypeError, OverflowError):
+            raise KernelError("copy_blocks: sources and targets must be whole numbers") from None
         _check_numbers(source, target, blocks, room, into is None)
         source, target = array.array("i", source), array.array("i", target)
     count = len(source)

@@ -321,3 +321,18 @@ def test_state_of_no_size_keeps_no_other_state_from_moving(device):
     cache.resize(12 * BLOCK, 9)
     cache.check()
     assert same(content(cache, a), want) and same(content(cache, b), want)
+
+
+def test_block_numbers_are_whole_and_read_as_often_as_needed():
+    t = torch.zeros(2, 6, 1, 8, 4)
+    for src, dst in (([1.7], [2]), ([1], [2.0]), (["1"], [2]), ([1], [None]), ([2 ** 70], [1]),
+                     (np.array([1.0]), np.array([2])), (torch.tensor([1.5]), [2])):
+        with pytest.raises(KernelError, match="whole numbers"):
+            ops.copy_blocks([t], src, dst)
+    for src, dst in ((iter([1]), iter([2 ** 40])), (iter([-1]), [2]), (np.array([1]), np.array([6])),
+                     (torch.tensor([7]), [2])):
+        with pytest.raises(KernelError, match="must lie in"):
+            ops.copy_blocks([t], src, dst)
+    for src, dst in ((iter([1]), iter([2])), (np.array([1]), np.array([2], dtype=np.int16)), (torch.tensor([1]), range(2, 3))):
+        with pytest.raises(KernelError, match="CUDA device only"):
+            ops.copy_blocks([t], src, dst)
