@@ -74,6 +74,7 @@ struct Params {
   const int32_t* block_table;
   int max_blocks, sequences;
   int heads, kv_heads;
+  int settled;                         // whether plan, lengths and block lists may be read before the wait (see `launch`)
   float* part_o;                       // [partials][heads][D]
   float2* part_ml;                     // [partials][heads]: (maximum in base 2, sum)
   float scale_log2e;
@@ -570,8 +571,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   // First of all, and in narrow units too: until a block has given up its right to tensor memory, the SM starts no
   // second block of a kernel that may ask for it (measured: the second ones started 8 to 15 us late).
   if ((threadIdx.x >> 5) == 1) tc::tmem_alloc(&tmem_at, kTmemCols);
-  // (the plan, the block lists and the lengths were written before the kernel before this one began, or this one was
-  // launched behind all that came before it; what else that one wrote, queries, keys and values, is read behind the wait)
+  // (settled: the plan, the block lists and the lengths were written before the kernel before this one began; what that
+  // one wrote, queries, keys and values, is read behind the wait below. Else all of it is.)
+  if (!p.settled) wait_for_previous_kernel();
   const int unit = blockIdx.x / p.kv_heads, g = blockIdx.x - unit * p.kv_heads;
   const int group = p.heads / p.kv_heads;
   // (the grid is as large as the plan has room for; a unit behind its last one reads words of no meaning, and
@@ -649,9 +651,10 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 template <int D>
 __global__ void __launch_bounds__(kNarrowThreads)
 join_kernel(const Plan plan, const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-            __nv_bfloat16* __restrict__ out, const int32_t* __restrict__ seq_lens, int heads) {
+            __nv_bfloat16* __restrict__ out, const int32_t* __restrict__ seq_lens, int heads, int settled) {
   constexpr int kLanes = D / 4, kGroups = kNarrowThreads / kLanes, kRound = 4;
   let_next_kernel_start();
+  if (!settled) wait_for_previous_kernel();
   const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
   const int first = plan.words[plan.first_at + b], end = plan.words[plan.first_at + b + 1];
   const int least = plan.words[plan.span_at + 2 * b], most = plan.words[plan.span_at + 2 * b + 1];
@@ -733,11 +736,11 @@ int* error_word() {
   return known[device];
 }
 
-// `settled`: the plan, the lengths and the block lists were written before the kernel before this one began, as a
-// step's inputs are, and may be read while it runs. Else the first kernel starts behind all that came before it.
+// `p.settled`: the plan, the lengths and the block lists were written before the kernel before this one began, as a
+// step's inputs are, and may be read while it runs. Else they are read behind the wait for it, which takes 1 us of 27 a
+// layer (64 sequences of 32,000 positions; 5 if the kernel were launched behind all that came before).
 template <int D>
-int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_bfloat16* out, bool settled,
-           cudaStream_t stream) {
+int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_bfloat16* out, cudaStream_t stream) {
   static PerDeviceOnce configured;
   if (configured.needs()) {
     const cudaError_t e = cudaFuncSetAttribute(shared_attention_kernel<D>,
@@ -745,19 +748,13 @@ int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, Params& p, __nv_b
     if (e != cudaSuccess) return (int)e;
     configured.done();
   }
-  const dim3 units((unsigned)(p.plan.unit_capacity * p.kv_heads)), rows((unsigned)(p.sequences * p.heads));
-  auto join = join_kernel<D>;
   if (p.plan.unit_capacity > 0) {
-    auto attend = shared_attention_kernel<D>;
-    const int e = settled ? launch_overlapped(attend, units, dim3(kThreads), Smem<D>::kBytes, stream, 1, k_map, v_map, p)
-                          : launch_ordered(attend, units, dim3(kThreads), Smem<D>::kBytes, stream, k_map, v_map, p);
+    const int e = launch_overlapped(shared_attention_kernel<D>, dim3((unsigned)(p.plan.unit_capacity * p.kv_heads)),
+                                    dim3(kThreads), Smem<D>::kBytes, stream, 1, k_map, v_map, p);
     if (e) return e;
-  } else if (!settled) {
-    return launch_ordered(join, rows, dim3(kNarrowThreads), 0, stream, p.plan, p.part_o, p.part_ml, out, p.seq_lens,
-                          p.heads);
   }
-  return launch_overlapped(join, rows, dim3(kNarrowThreads), 0, stream, 1, p.plan, p.part_o, p.part_ml, out, p.seq_lens,
-                          p.heads);
+  return launch_overlapped(join_kernel<D>, dim3((unsigned)(p.sequences * p.heads)), dim3(kNarrowThreads), 0, stream, 1,
+                           p.plan, p.part_o, p.part_ml, out, p.seq_lens, p.heads, p.settled);
 }
 
 }  // namespace
@@ -789,7 +786,7 @@ SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.q_stride = q_stride;
   p.q_aligned = q_stride % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   p.seq_lens = seq_lens; p.block_table = block_table; p.max_blocks = max_blocks; p.sequences = sequences;
-  p.heads = heads; p.kv_heads = kv_heads;
+  p.heads = heads; p.kv_heads = kv_heads; p.settled = settled != 0;
   p.part_o = part;
   p.part_ml = reinterpret_cast<float2*>(part + (long long)n->partials * heads * head_dim);
   p.scale_log2e = scale * 1.4426950408889634f;
@@ -802,7 +799,7 @@ SAKV_EXPORT int sakv_shared_attention(const void* keys, const void* values, long
   if (!bad) bad = tma::make_map_bf16_2d(&vm, values, (uint64_t)rows, head_dim, (uint64_t)head_dim * 2, KT, 64);
   if (bad) return bad;
   __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
-  return head_dim == 64 ? launch<64>(km, vm, p, o, settled != 0, stream) : launch<128>(km, vm, p, o, settled != 0, stream);
+  return head_dim == 64 ? launch<64>(km, vm, p, o, stream) : launch<128>(km, vm, p, o, stream);
 }
 
 SAKV_EXPORT int sakv_shared_attention_error(int* value) {

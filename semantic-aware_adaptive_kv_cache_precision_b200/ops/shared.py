@@ -255,9 +255,9 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     are in the cache), reading a block that `plan` found in several sequences' lists once for all of them.
     `plan`: `plan_shared` of these block lists. A sequence of length 0 gets zeros; one whose length the plan does not
     cover (past its reach, or below the blocks it shares) gets NaN, and so do those that the plan lets read those
-    blocks through its list. `settled`: the plan's words, the
-    lengths and the block lists were written before the kernel before this one on the stream began, as a step's
-    inputs are; they are then read while that one still runs (else the call starts when all before it is done)."""
+    blocks through its list. `settled`: the plan's words, the lengths and the block lists were written before the kernel
+    before this one on the stream began, as a step's inputs are; they are then read while that one still runs (else
+    when it is done)."""
     q_shape, k_shape, device = qkv.shape, k_cache.shape, qkv.get_device()
     # (one expression for the calls that are right: a decode step outside a captured graph is bound by the
     # host's work; `_refuse` says what is wrong with the others)
