@@ -335,7 +335,7 @@ def kernel_case(name: str) -> int:
         lens = torch.full((batch,), CONTEXT + 5, dtype=torch.int32, device=dev)
         qkv = torch.randn(batch, (A + 2 * G) * d, device=dev, dtype=torch.bfloat16)
         run = lambda i: ops.attention_decode(qkv, k, v, lens, table, A, G, d, d ** -0.5, None,
-                                             CONTEXT + 5)
+                                             CONTEXT + 5, settled=True)       # (as in a step)
     elif name == "attention_prefill_2048":
         n = PREFILL_TOKENS
         k = torch.randn(n // 64, G, 64, d, device=dev, dtype=torch.bfloat16)

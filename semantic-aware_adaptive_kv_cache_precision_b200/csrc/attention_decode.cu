@@ -73,14 +73,13 @@ __global__ void __launch_bounds__(kThreads)
 decode_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                         const __grid_constant__ CUtensorMap v_map,
                         const __nv_bfloat16* __restrict__ q, long long q_stride,
-                        const int32_t* __restrict__ seq_lens,
-                        const int32_t* __restrict__ block_table, int max_blocks,
+                        const int32_t* seq_lens, const int32_t* block_table, int max_blocks,
                         __nv_bfloat16* __restrict__ out, float* __restrict__ part_o,
                         float* __restrict__ part_ml, int heads, int kv_heads, int splits,
                         float scale_log2e, int window, int* __restrict__ error,
                         const float* __restrict__ cos_t, const float* __restrict__ sin_t,
                         int rotary_rows, __nv_bfloat16* __restrict__ k_out,
-                        __nv_bfloat16* __restrict__ v_out) {
+                        __nv_bfloat16* __restrict__ v_out, int settled) {
   // With `cos_t`/`sin_t` (rotary tables [positions, D / 2], rotation over the whole head) the
   // queries, keys and values in `q`'s rows are as the projection left them: this kernel
   // rotates its queries as it loads them, and the one block of a (sequence, KV head) whose
@@ -109,10 +108,13 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap k_map,
     tma::prefetch_map(&k_map);
     tma::prefetch_map(&v_map);
   }
-  // The lengths and block lists are the step's inputs, written before its first kernel
-  // started, and every cached key but the newest was written by an earlier step: all of
+  // `settled`: the lengths and block lists are the step's inputs, written before its first
+  // kernel started, and every cached key but the newest was written by an earlier step: all of
   // that is read, and those tiles are on their way, before this kernel waits for the one
-  // before it, which wrote the queries and the newest key and value.
+  // before it, which wrote the queries and the newest key and value. A caller who cannot say
+  // so has the wait first. (Their pointers are not `__restrict__`: reads of what a kernel may
+  // take for constant were moved above the wait.)
+  if (!settled) wait_for_previous_kernel();
   // (a length outside [0, max_blocks * 64] cannot come from the engine; a caller of the
   // exported function that passes one gets zeros for that sequence, not a wild read)
   const int given_len = seq_lens[b];
@@ -638,7 +640,7 @@ int launch(const CUtensorMap* k_map, const CUtensorMap* v_map, const __nv_bfloat
            __nv_bfloat16* out, float* part_o, float* part_ml, int sequences, int heads,
            int kv_heads, int splits, float scale, int window, const float* cos_t,
            const float* sin_t, int rotary_rows, __nv_bfloat16* k_out, __nv_bfloat16* v_out,
-           cudaStream_t stream) {
+           int settled, cudaStream_t stream) {
   static PerDeviceOnce configured;      // (attributes are per device)
   int* error = nullptr;
   if (cudaGetSymbolAddress(reinterpret_cast<void**>(&error), g_error) != cudaSuccess)
@@ -665,13 +667,13 @@ int launch(const CUtensorMap* k_map, const CUtensorMap* v_map, const __nv_bfloat
                                      q, q_stride, seq_lens, block_table, max_blocks, out, part_o,
                                      part_ml, heads, kv_heads, splits,
                                      scale * 1.4426950408889634f, window, error, cos_t, sin_t,
-                                     rotary_rows, k_out, v_out);
+                                     rotary_rows, k_out, v_out, settled);
   }
   int status = launch_overlapped(decode_attention_kernel<D, false>, grid, dim3(kThreads),
                                  Smem<D>::kBytes, stream, 1, *k_map, *v_map, q, q_stride,
                                  seq_lens, block_table, max_blocks, out, part_o, part_ml, heads,
                                  kv_heads, splits, scale * 1.4426950408889634f, window, error,
-                                 cos_t, sin_t, rotary_rows, k_out, v_out);
+                                 cos_t, sin_t, rotary_rows, k_out, v_out, settled);
   const int fold_groups = min(kFoldGroups, (splits + 15) / 16);
   if (status == 0 && splits > 1 && fold_groups == 1)
     status = launch_overlapped(combine_kernel, dim3(sequences * heads), dim3(D <= 128 ? D : 128),
@@ -704,11 +706,12 @@ SAKV_EXPORT int sakv_decode_attention(const void* k_map, const void* v_map, cons
                                       int kv_heads, int head_dim, int splits, float scale,
                                       int window, const float* cos_table, const float* sin_table,
                                       int rotary_rows, void* k_cache, void* v_cache,
-                                      cudaStream_t stream) {
+                                      int settled, cudaStream_t stream) {
   // `cos_table`, `sin_table` (fp32 [rotary_rows, head_dim / 2], both or neither): `q`'s rows are
   // then the projection's whole output [q | k | v], unrotated, and the kernel rotates the
   // queries and, into the cache entry `k_cache`, `v_cache` (or nowhere if those are null),
-  // writes the newest position's rotated key and its value.
+  // writes the newest position's rotated key and its value. `settled`: the lengths, block lists, tables and
+  // every cached position but the newest were written before the kernel before this one began.
   if ((cos_table == nullptr) != (sin_table == nullptr) || (k_cache == nullptr) != (v_cache == nullptr) ||
       (k_cache && !cos_table) || (cos_table && rotary_rows <= 0) || ((uintptr_t)cos_table & 7) || ((uintptr_t)sin_table & 7) ||
       ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) ||
@@ -725,7 +728,7 @@ SAKV_EXPORT int sakv_decode_attention(const void* k_map, const void* v_map, cons
                    (const __nv_bfloat16*)q, q_stride, seq_lens, block_table, max_blocks,      \
                    (__nv_bfloat16*)out, part_o, part_ml, sequences, heads, kv_heads, splits,  \
                    scale, window, cos_table, sin_table, rotary_rows, (__nv_bfloat16*)k_cache, \
-                   (__nv_bfloat16*)v_cache, stream)
+                   (__nv_bfloat16*)v_cache, settled, stream)
   if (head_dim == 64) GO(64);
   if (head_dim == 128) GO(128);
 #undef GO
@@ -809,9 +812,9 @@ SAKV_EXPORT int sakv_decode_attention_static_scratch(
     return launch<64>((const CUtensorMap*)k_map, (const CUtensorMap*)v_map,
                       (const __nv_bfloat16*)q, q_stride, seq_lens, block_table, max_blocks,
                       (__nv_bfloat16*)out, part_o, part_ml, sequences, heads, kv_heads, splits,
-                      scale, window, nullptr, nullptr, 0, nullptr, nullptr, stream);
+                      scale, window, nullptr, nullptr, 0, nullptr, nullptr, 0, stream);
   return launch<128>((const CUtensorMap*)k_map, (const CUtensorMap*)v_map,
                      (const __nv_bfloat16*)q, q_stride, seq_lens, block_table, max_blocks,
                      (__nv_bfloat16*)out, part_o, part_ml, sequences, heads, kv_heads, splits,
-                     scale, window, nullptr, nullptr, 0, nullptr, nullptr, stream);
+                     scale, window, nullptr, nullptr, 0, nullptr, nullptr, 0, stream);
 }

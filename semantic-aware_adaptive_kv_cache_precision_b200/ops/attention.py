@@ -80,12 +80,12 @@ def attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                      seq_lens: torch.Tensor, block_table: torch.Tensor, heads: int, kv_heads: int,
                      head_dim: int, scale: float, window, max_len: int,
                      splits: int | None = None, rotary=None, write_cache: bool = True,
-                     in_cluster: bool | None = None) -> torch.Tensor:
+                     in_cluster: bool | None = None, settled: bool = False) -> torch.Tensor:
     """One query token per sequence (row b of `qkv` belongs to sequence b).
 
-    Lengths, block lists, rotary tables and every cached key and value but the newest are a step's inputs: the kernel
-    reads them while the kernel before it on the stream may still be running, so that one must not have written them
-    (the one before that may, or a copy). What it has written of `qkv` and of the newest position is waited for.
+    `settled`: the lengths, block lists, rotary tables and every cached position but the newest were written before
+    the kernel before this one on the stream began, as a step's inputs are; they are then read while that one still runs
+    (else when it is done).
 
     `rotary`: None, or `(cos, sin)` (fp32 [positions, head_dim / 2], rotation over the whole
     head): `qkv` is then the projection's output as it came, [q | k | v] unrotated, and the
@@ -119,7 +119,7 @@ def attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
          qkv.stride(0), ptr(seq_lens), ptr(block_table), block_table.shape[1], ptr(out),
          ptr(part_o), ptr(part_ml), sequences, heads, kv_heads, head_dim, splits, float(scale),
          int(window) if window else 0, *_rotary_arguments(rotary, write_cache, qkv, k_cache, v_cache,
-                                                         heads, kv_heads, head_dim, max_len))
+                                                         heads, kv_heads, head_dim, max_len), bool(settled))
     if part_o is not None:
         _lib.launches += 1          # the call launched the fold kernel too
     return out

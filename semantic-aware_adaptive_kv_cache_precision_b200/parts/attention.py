@@ -117,7 +117,7 @@ class GQAAttention(Part):
                 return ops.attention_decode(qkv, view.keys, view.values, step.seq_lens,
                                             view.block_table, s.heads, s.kv_heads, s.head_dim,
                                             s.scale, s.window, step.max_len_bound or step.max_len,
-                                            rotary=rotary, write_cache=write_cache)
+                                            rotary=rotary, write_cache=write_cache, settled=True)
             if ops.tc_prefill_takes(qkv.dtype, s.heads, s.kv_heads, s.head_dim) and step.starts:
                 key = ("wide_tiles", s.heads, s.window)
                 plan = step.plans.get(key)

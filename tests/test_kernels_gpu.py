@@ -982,3 +982,32 @@ def test_attention_prefill_tcgen05_kernel(heads, kv_heads, window, slots):
                                  dev(lengths, torch.int32), dev(table, torch.int32), heads,
                                  kv_heads, d, scale, window)
     np.testing.assert_allclose(host(got), host(twin), rtol=0, atol=2e-2)
+
+
+@pytest.mark.parametrize("splits, in_cluster", [(1, False), (2, True), (4, True), (6, False)])
+def test_decode_attention_behind_a_kernel_that_writes_its_inputs(splits, in_cluster):
+    """A kernel that lets its successor start early and then writes the lengths: a call right behind it (captured, so that
+    no time passes between the two) reads them as it leaves them."""
+    heads, kv_heads, d = 12, 2, 128
+    rng = np.random.default_rng(3)
+    lengths = np.array([2040, 700, 1300])
+    k_cache, v_cache, table = paged_case(rng, lengths.tolist(), kv_heads, d, poison=False)
+    qkv, table = dev(rng.standard_normal((3, heads * d)), torch.bfloat16), dev(table, torch.int32)
+    call = lambda lens: ops.attention_decode(qkv, k_cache, v_cache, lens, table, heads, kv_heads, d, d ** -0.5, None, 2040,
+                                             splits=splits, in_cluster=in_cluster)
+    want = {n: call(dev(lengths - n, torch.int32)) for n in (0, 300)}
+    assert not torch.equal(want[0], want[300])
+    lens, graphs = torch.zeros(3, dtype=torch.int32, device=DEV), {}
+    for n in want:
+        scores = torch.zeros(3, 2000000, device=DEV)         # (the largest names the length)
+        scores[range(3), (lengths - n).tolist()] = 1.0
+        ops.choose(scores, out=lens), call(lens)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.choose(scores, out=lens)
+            out = call(lens)
+        graphs[n] = graph, out, scores
+    for i in range(10):
+        graph, out, _ = graphs[300 * (i % 2)]
+        graph.replay()
+        assert torch.equal(out, want[300 * (i % 2)])
