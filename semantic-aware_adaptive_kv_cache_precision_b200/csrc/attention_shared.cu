@@ -650,8 +650,8 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 // ... with kRound reads in flight, and are merged through shared memory in their order.
 template <int D>
 __global__ void __launch_bounds__(kNarrowThreads)
-join_kernel(const Plan plan, const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-            __nv_bfloat16* __restrict__ out, const int32_t* __restrict__ seq_lens, int heads, int settled) {
+join_kernel(const Plan plan, const float* part_o, const float2* part_ml, __nv_bfloat16* __restrict__ out,
+            const int32_t* seq_lens, int heads, int settled) {
   constexpr int kLanes = D / 4, kGroups = kNarrowThreads / kLanes, kRound = 4;
   let_next_kernel_start();
   if (!settled) wait_for_previous_kernel();

@@ -97,6 +97,9 @@ static inline int launch_status() { return static_cast<int>(cudaGetLastError());
 // it on the stream is still running. It must call `wait_for_previous_kernel()` before it
 // reads anything that kernel wrote and before it writes global memory at all; it calls
 // `let_next_kernel_start()` at its top so that its own successor can do the same.
+// What that kernel may have written is not reached through a `const __restrict__` pointer whose
+// read stands beside the wait: the compiler takes such memory for constant and has moved the
+// read above the wait.
 __device__ __forceinline__ void wait_for_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

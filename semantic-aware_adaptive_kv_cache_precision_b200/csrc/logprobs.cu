@@ -821,7 +821,7 @@ __device__ __forceinline__ uint32_t cut_two(float& a, float& b) {
 
 // x [M, K] in three: out [3][rows][padded], zeros behind M and K; a thread takes four numbers.
 __global__ void __launch_bounds__(256)
-split_kernel(const float* __restrict__ x, long long x_stride, int M, int K, int rows, int padded, int wide,
+split_kernel(const float* x, long long x_stride, int M, int K, int rows, int padded, int wide,
              uint2* __restrict__ out) {
   wait_for_previous_kernel();
   let_next_kernel_start();       // (in this order: the next one reads the head before it waits for this one)
@@ -1162,7 +1162,7 @@ split_logprob_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
 // every 32nd piece of all of them (lane = row: neighbouring rows' partials are neighbours in memory).
 constexpr int kJoinWarps = 32;
 __global__ void __launch_bounds__(32 * kJoinWarps)
-join_kernel(const float2* __restrict__ part, const float* __restrict__ mine, const int32_t* __restrict__ targets,
+join_kernel(const float2* part, const float* mine, const int32_t* targets,
             float* __restrict__ logprob, float* __restrict__ lse, int M, int N, int full, int pieces,
             int rest_pieces) {
   constexpr int kRound = 8;
