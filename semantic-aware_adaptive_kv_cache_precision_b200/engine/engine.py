@@ -423,6 +423,13 @@ class Engine:
         the next: a part whose launches depend on them is not `graph_safe`.)"""
         return tuple(ctx.host_slots) if cache.states else ()
 
+    def _pool_for_capture(self):
+        """The memory that all captured steps of this engine share; another when none is left, since the allocator does
+        not take a pool again whose last graph has gone while something in it is still held."""
+        if not self._graphs and not any(isinstance(e, tuple) for e in self._prefill_graphs.values()):
+            self._graph_pool = torch.cuda.graph_pool_handle()
+        return self._graph_pool
+
     def _decode_by_graph(self, ctx, cache, greedy: bool = False) -> torch.Tensor:
         """Run a decode step through the CUDA graph of its shape (batch size and width of
         the block lists), capturing it the first time the shape comes up after one
@@ -444,12 +451,11 @@ class Engine:
             if len(self._graphs) >= 64:                 # shapes come and go; keep the table small
                 self._graphs.clear()
             graph = torch.cuda.CUDAGraph()
-            if self._graph_pool is None:
-                self._graph_pool = torch.cuda.graph_pool_handle()
+            pool = self._pool_for_capture()
             torch.cuda.synchronize(self.device)
             before = _lib.launches
             try:
-                with torch.cuda.graph(graph, pool=self._graph_pool):
+                with torch.cuda.graph(graph, pool=pool):
                     out = run()
             except Exception as exc:
                 self.graph_failure = repr(exc)      # kept for whoever wants to know why
@@ -494,12 +500,11 @@ class Engine:
                 return self.model.logits(self.model.hidden(ctx, cache), ctx.want)
             ctx.plans = entry                               # nothing is uploaded while capturing
             graph = torch.cuda.CUDAGraph()
-            if self._graph_pool is None:
-                self._graph_pool = torch.cuda.graph_pool_handle()
+            pool = self._pool_for_capture()
             torch.cuda.synchronize(self.device)
             before = _lib.launches
             try:
-                with torch.cuda.graph(graph, pool=self._graph_pool):
+                with torch.cuda.graph(graph, pool=pool):
                     out = self.model.logits(self.model.hidden(ctx, cache), ctx.want)
             except Exception as exc:
                 self.graph_failure = repr(exc)

@@ -566,3 +566,33 @@ def test_chosen_tokens_over_shared_blocks_are_the_logits_best(varied_folders, gr
     assert len(seen) > 4
     engine.close([a] + slots + twins)
     engine.cache.check()
+
+
+@pytest_gpu
+@pytest.mark.parametrize("what", ["resize", "many shapes", "many plans"])
+def test_steps_are_captured_again_after_all_captured_ones_have_gone(varied_folders, monkeypatch, what):
+    """Also where something that lies in their memory is still held, as scratch that a capture made may be."""
+    from semantic_aware_adaptive_kv_cache_precision_b200.engine import engine as module
+    engine = engine_of(varied_folders("D", "bfloat16"), "bfloat16", max_tokens=16384)
+    engine.shared_bytes_worth = 0
+    (a,) = engine.open(1)
+    engine.step([a], [list(range(200))])
+    slots = [a] + engine.fork(a, 4)
+    for _ in range(3):
+        engine.step(slots, [[7]] * 5)
+    assert len(engine._graphs) == 1 and engine._shared_buffers
+    held = [entry[1] for entry in engine._graphs.values()]
+    if what == "resize":
+        engine.resize_cache(20000)
+    elif what == "many shapes":
+        graph = next(iter(engine._graphs.values()))
+        engine._graphs.update({i: graph for i in range(63)})
+        del graph
+    else:
+        monkeypatch.setattr(module, "MOST_PLAN_BUFFERS", 1)
+    for n in (4, 5, 4, 5):
+        engine.step(slots[:n], [[7]] * n)
+    assert engine.cuda_graphs and engine.graph_failure is None and engine._graphs
+    assert held[0].shape[0] == 5
+    engine.close(slots)
+    engine.cache.check()
