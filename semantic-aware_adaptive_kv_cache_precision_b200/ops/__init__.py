@@ -615,9 +615,14 @@ def choose(logits: torch.Tensor, temperature: float = 0.0, seed: int = 0,
     chunks = plain_function("sakv_choose_chunks")(vocab)
     scratch = _choose_scratch.get(logits.device)
     if scratch is None or scratch[0].numel() < rows * chunks or scratch[1].numel() < rows:
-        scratch = (torch.empty(max(rows * chunks, 4096), dtype=torch.int64, device=logits.device),
-                   torch.zeros(max(rows, 1024), dtype=torch.int32, device=logits.device))
-        _choose_scratch[logits.device] = scratch
+        capturing = torch.cuda.is_current_stream_capturing()
+        room = 1 if capturing else 2
+        scratch = (torch.empty(max(room * rows * chunks, 4096), dtype=torch.int64, device=logits.device),
+                   torch.zeros(max(room * rows, 1024), dtype=torch.int32, device=logits.device))
+        if not capturing:       # (what a capture makes is the graph's: its zeros are written when it is replayed)
+            # graphs captured over a smaller one go on using it: it is kept
+            _choose_replaced.append(_choose_scratch.get(logits.device))
+            _choose_scratch[logits.device] = scratch
     call("sakv_choose", ptr(logits), logits.stride(0) if rows else vocab, rows, vocab,
          float(temperature), int(seed) & 0xFFFFFFFFFFFFFFFF, ptr(request), ptr(step), ptr(out),
          ptr(scratch[0]), ptr(scratch[1]))
@@ -625,3 +630,4 @@ def choose(logits: torch.Tensor, temperature: float = 0.0, seed: int = 0,
 
 
 _choose_scratch: dict = {}
+_choose_replaced: list = []

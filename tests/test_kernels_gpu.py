@@ -1011,3 +1011,31 @@ def test_decode_attention_behind_a_kernel_that_writes_its_inputs(splits, in_clus
         graph, out, _ = graphs[300 * (i % 2)]
         graph.replay()
         assert torch.equal(out, want[300 * (i % 2)])
+
+
+def test_scratch_of_choices_outlives_the_graphs_that_use_it():
+    """A captured choice goes on working over its scratch when a larger choice has taken another, and one that is captured
+    first leaves its own to its graph."""
+    z = torch.randn(3, 20000, device=DEV)
+    ops.choose(z)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        small = ops.choose(z)
+    kept = ops._choose_scratch[z.device]
+    span = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in kept]
+    most = max(kept[0].numel(), kept[1].numel()) + 1
+    del kept
+    large = torch.randn(most, 300, device=DEV)
+    captured = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(captured):
+        best = ops.choose(large)
+    assert ops._choose_scratch[z.device][0].data_ptr() == span[0][0]
+    assert torch.equal(ops.choose(large).long(), large.argmax(1))         # (eagerly, before the graph has run)
+    others = [torch.empty((hi - lo) // 4, dtype=torch.int32, device=DEV) for lo, hi in span for _ in range(20)]
+    for t in others:
+        at = t.data_ptr()
+        assert not any(lo < at + t.numel() * 4 and at < hi for lo, hi in span)
+    for _ in range(3):
+        z.normal_(), large.normal_()
+        graph.replay(), captured.replay()
+        assert torch.equal(small.long(), z.argmax(1)) and torch.equal(best.long(), large.argmax(1))
