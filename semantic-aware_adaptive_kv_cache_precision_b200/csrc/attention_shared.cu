@@ -21,7 +21,7 @@
 // Every unit leaves a partial (m, l, o) for each of its (sequence, head); a sequence's partials lie side by
 // side, in the order of its positions, and `join_kernel` merges them. Scores, maxima, exponentials and sums
 // are fp32; probabilities are rounded to bf16 for the product with the values, as values are stored (an error
-// of half a step, 2^-9 of a probability, as in the other attention kernels). Every wait on a copy is bounded.
+// of half a step, up to 2^-8 of a probability, as in the other attention kernels). Every wait on a copy is bounded.
 // The reference reads a sequence's cache for every sequence (`src/core_kernels/attention.cu:754-815`).
 #include "common.cuh"
 #include "mma.cuh"

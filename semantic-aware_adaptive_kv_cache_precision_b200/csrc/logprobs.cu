@@ -4,8 +4,9 @@
 //   lse = m + log sum_v e^(z_v - m),  m = max_v z_v;    logprob = z_target - lse
 //
 // The vocabulary is taken in pieces: a piece leaves (m, sum e^(z - m)) a row (m in natural units: the type's lowest
-// value, a common mask, times log2(e) would be -inf), and whoever meets the target's column leaves z_target; `join_kernel` merges the pieces. 2,048 tokens over 151,936 logits would be
-// 1.2 GB written and read again; the pieces are 10 MB.
+// value, a common mask, times log2(e) would be -inf), and whoever meets the target's column leaves z_target;
+// `join_kernel` merges the pieces. 2,048 tokens over 151,936 logits would be 1.2 GB written and read again; the pieces
+// are 10 MB.
 //
 // Ways to a piece. bfloat16 operands: tcgen05 on PAIRS of SMs (`cta_group::2`), the softmax's sums in the
 // epilogue. A pair takes a tile of the head's rows (up to 128 a block) against
@@ -27,7 +28,8 @@
 // of tiles is not nearly empty (see the launcher).
 // float32 operands: each number as three of bfloat16 on the tensor cores (`split_logprob_kernel`), or plain multiply-adds
 // where the head's rows are not aligned; each sum over k and each row's sums over the vocabulary in one order whatever
-// rows are beside it, as in the other 32-bit products. bfloat16 rows that TMA cannot take come here as copies that it can.
+// rows are beside it, as in the other 32-bit products. bfloat16 rows that TMA cannot take come as copies that it can
+// (`pad_kernel`).
 //
 // Sums and maxima are fp32. Every mbarrier wait is bounded, and a pair leaves together.
 // The reference keeps all logits (`src/microinfer/model.py:388-402`).
@@ -50,14 +52,14 @@ constexpr int kMaxTokens = 256;                  // tokens of a tile
 // 54 / 52, 37 / 33, 232 / 218; 65 behind 512 tokens 291 / 263, 110 / 114, 52 / 51, 560 / 599; 140 behind them
 // 280 / 268, 118 / 116, 60 / 51, 658 / 645.
 constexpr int kRestMost = 96;
-// Tokens behind 256 up to which one tile takes both, where K is at most kLongK. Measured likewise (both / two tiles of 256): 32 170 / 178,
-// 70 / 84, 39 / 40, 375 / 394; 77 172 / 177, 76 / 84, 44 / 41, 380 / 394; 128 180 / 181, 79 / 85, 46 / 41, 367 /
+// Tokens behind 256 up to which one tile takes both, where K is at most kLongK. Measured likewise (both / two tiles of
+// 256): 32 170 / 178, 70 / 84, 39 / 40, 375 / 394; 77 172 / 177, 76 / 84, 44 / 41, 380 / 394; 128 180 / 181, 79 / 85, 46 / 41, 367 /
 // 408; 160 189 / 182, 83 / 86, 49 / 41, 435 / 409.
 constexpr int kBothMost = 128;
 // The tensor cores cut where they add, always the same way: K is taken in chunks of at most kLongK, added up in fp32 by
 // the epilogue (512 tokens and K = 4,096: relative error 5.9e-7, in one sum 2.7e-6; 64 and 1,536: 2.1e-7, 4.5e-7; the
 // time is the same). 257 to 384 tokens in one tile have no registers left for that: above kLongK they are two tiles
-// (333 tokens, K = 2,048, 50,257 rows: 102 us; in one tile 103 to 106, error 8e-7 instead of 3e-7).
+// (333 tokens, K = 2,048, 50,257 rows: 85 us; one tile took 1 to 4 % more, with an error of 8e-7 instead of 3e-7).
 constexpr int kLongK = 1024;
 constexpr int kEpilogueThreads = 256;            // two warps a quarter of tensor memory's lanes, each half the columns
 constexpr int kThreads = 64 + kEpilogueThreads;

@@ -36,6 +36,9 @@ DEFAULT_MAX_STEP_TOKENS = 16384
 # 1.548 / 1.647 (33), 1.665 / 1.673 (66), 1.894 / 1.723 (132); 16 sequences 1.336 / 1.353 (63), 1.538 / 1.487 (126);
 # 8 sequences 1.242 / 1.320 (59), 1.539 / 1.485 (115); 14 layers of 28 over 4, 64 sequences 1.617 / 1.731 (66),
 # 1.730 / 1.744 (132), 1.964 / 1.838 (264); 8 sequences 1.372 / 1.412 (29), 1.511 / 1.471 (59).
+# The plan, 0.4 to 1.5 ms of the host when a batch or what it shares changes, is not in these. Whole calls of `generate`
+# (64 samples, 200 tokens at a temperature; ms, each for itself / shared): without an end before, 2,048 positions 402 / 364,
+# 4,096 491 / 382; with 1 % of the tokens stops, so that a sequence ends every few steps, 347 / 360 and 403 / 393.
 SHARED_BYTES_WORTH = 80 << 20
 # Layouts of plans whose words are kept on the device for captured steps to read.
 MOST_PLAN_BUFFERS = 64

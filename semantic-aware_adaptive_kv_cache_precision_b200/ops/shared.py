@@ -263,16 +263,18 @@ def shared_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     # host's work; `_refuse` says what is wrong with the others)
     if not (qkv.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
             and (head_dim == 128 or head_dim == 64) and 0 < kv_heads and heads % kv_heads == 0
-            and heads <= MOST_GROUP * kv_heads and LEAST_SCALE <= scale <= 1 / LEAST_SCALE and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
+            and heads <= MOST_GROUP * kv_heads and LEAST_SCALE <= scale <= 1 / LEAST_SCALE
+            and len(q_shape) == 2 and q_shape[1] >= heads * head_dim
             and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
-            and k_shape == v_cache.shape and len(k_shape) == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() and k_shape[1] == kv_heads
-            and k_shape[2] == CACHE_BLOCK and k_shape[3] == head_dim
+            and k_shape == v_cache.shape and len(k_shape) == 4 and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_shape[1] == kv_heads and k_shape[2] == CACHE_BLOCK and k_shape[3] == head_dim
             and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32
             and seq_lens.dim() == 1 and block_table.dim() == 2
             and seq_lens.shape[0] == q_shape[0] and block_table.shape[0] == q_shape[0]
             and block_table.shape[1] == plan.width and seq_lens.is_contiguous() and block_table.is_contiguous()
             and plan.sequences == q_shape[0] and plan.heads == heads and plan.kv_heads == kv_heads
-            and plan.words.__class__ is torch.Tensor and device >= 0 and device == k_cache.get_device() == v_cache.get_device() == seq_lens.get_device()
+            and plan.words.__class__ is torch.Tensor
+            and device >= 0 and device == k_cache.get_device() == v_cache.get_device() == seq_lens.get_device()
             == block_table.get_device() == plan.words.get_device()):
         _refuse(qkv, k_cache, v_cache, seq_lens, block_table, plan, heads, kv_heads, head_dim, scale)
     sequences = q_shape[0]
