@@ -126,7 +126,7 @@ def _in_pieces(x, head, targets, bias, scale, softcap, most: int):
 
 
 def _token_logprobs(x, head, targets, bias, scale, softcap, found=None):
-    """`found` (rows of 16 bits that TMA takes, few enough for one launch): gets the targets' logits."""
+    """`found` (rows of 16 bits that TMA takes, as many as one launch may have): gets the targets' logits."""
     rows, k = x.shape
     vocab, stride = head.shape[0], x.stride(0)
     logprob, lse = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
@@ -138,7 +138,7 @@ def _token_logprobs(x, head, targets, bias, scale, softcap, found=None):
     bias_at, bias_code = (None, F32) if bias is None else (bias.data_ptr(), dtype_code(bias.dtype))
     if x.dtype is torch.bfloat16 and k % 8 == 0 and stride % 8 == 0 and (at | head_at) % 16 == 0 and _pairs() > 0:
         shape, floats = _shape(rows, vocab, k)
-        if floats > 2 * SPLIT_PAIRS and rows > 256:
+        if floats > 2 * SPLIT_PAIRS and rows > 256 and found is None:
             # (whole tiles of 256 rows; the heads' tiles of fewer rows may be lower ones, so a piece is looked at again)
             return _in_pieces(x, head, targets, bias, scale, softcap,
                               max(256, min(rows - 1, rows * 2 * SPLIT_PAIRS // floats) // 256 * 256))

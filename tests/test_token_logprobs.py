@@ -455,3 +455,11 @@ def test_infinities_in_rows_and_in_the_head(dtype, k, rows):
     assert ((lse[good].double() - want_lse).abs() <= bound).all()
     assert got[1] == -math.inf and got[2] == -math.inf
     assert ((got[good].double() - want).abs() <= bound)[[0] + list(range(3, len(good)))].all()
+
+
+@pytest.mark.gpu
+def test_pieces_of_the_head_take_their_rows_in_one_launch(monkeypatch):
+    """Where what the last rows leave takes a piece's scratch past its bound by some pairs."""
+    monkeypatch.setattr(logprobs, "PIECE_ROWS", 250)
+    monkeypatch.setattr(logprobs, "SPLIT_PAIRS", 2048)
+    check(864, 37, 900, torch.bfloat16, torch.float32)
