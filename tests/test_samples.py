@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 import torch
 
-from semantic_aware_adaptive_kv_cache_precision_b200 import Engine, ops, write_random_model
+from semantic_aware_adaptive_kv_cache_precision_b200 import Engine, write_random_model
+from semantic_aware_adaptive_kv_cache_precision_b200 import ops
 from semantic_aware_adaptive_kv_cache_precision_b200.cache import BLOCK, CacheFull
 from semantic_aware_adaptive_kv_cache_precision_b200.engine.generate import plan_samples
 
